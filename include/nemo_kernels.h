@@ -298,6 +298,74 @@ int nk_joint_partial(gpu_t *g, const float *enc, const float *pred, const uint16
 /* out[2 r], out[2 r + 1] = index and value bits of the best of row r's n partials (lowest index on ties) */
 int nk_argmax_reduce(gpu_t *g, const float *part_v, const int *part_i, int *out, uint32_t n, uint32_t rows);
 
+/* ---- 4-bit rows and weights --------------------------------------------------------------------
+ * Microscaled 4-bit floating point (no counterpart in the reference).  A row of K values is blocks of
+ * 32 that share a scale byte s (the power of two 2^(s - 127); 255: every value of the block is NaN), each
+ * value a 4-bit code: a sign bit over the magnitudes 0, 0.5, 1, 1.5, 2, 3, 4, 6.  Code k of a row is in byte
+ * k / 2, the low half first.  Rows are padded with zero codes and scales to whole groups of 128 values:
+ * NK_FP4_ROW(K) bytes of codes and NK_FP4_SCALES(K) bytes of scales; nk_fp4_quant writes the padding and
+ * the products read it.  Codes 16-byte aligned with strides % 16 == 0, scales 4-byte aligned with
+ * strides % 4 == 0.  One matrix is at most 2^32 runs of 8 values. */
+#define NK_FP4_ROW(K) (((uint32_t)(K) / 128u + ((uint32_t)(K) % 128u != 0)) * 64u)
+#define NK_FP4_SCALES(K) (((uint32_t)(K) / 128u + ((uint32_t)(K) % 128u != 0)) * 4u)
+enum { NK_F32 = 0, NK_BF16 = 1 }; /* the type of a row operand */
+/* M rows of K values to 4 bits.  s is the exponent of the block's largest magnitude less 2 (0 where that is
+ * below 2^-125), values are rounded to the nearest magnitude of x / 2^(s - 127), ties to the even code, and
+ * those above 6 become 6.  A block that holds an infinity or a NaN becomes NaN. */
+int nk_fp4_quant(gpu_t *g, const void *X, int type, uint32_t ldx, uint8_t *Q, uint32_t ldq, uint8_t *S, uint32_t lds,
+                 uint32_t M, uint32_t K);
+/* The values back, exact in either type (f32 overflows to infinity where 6 * 2^127 does). */
+int nk_fp4_dequant(gpu_t *g, const uint8_t *Q, uint32_t ldq, const uint8_t *S, uint32_t lds, void *X, int type,
+                   uint32_t ldx, uint32_t M, uint32_t K);
+/* nk_gemm with 4-bit weights: C[m][n] (= or +=) alpha * act(sum_k A[m][k] W[n][k] + bias[n]), the same
+ * activations, any M, N and K; sums in f32.  nk_gemm_fp4: A in 4 bits too (the products are exact).
+ * nk_gemm_w4: A f32 rows, 16-byte aligned with lda % 4 == 0, which enter as 16 significant bits
+ * (bf16 hi + lo) as in nk_gemm.  lda, ldas, ldw and ldws are strides in bytes (lda of nk_gemm_w4 in floats).
+ * C must not overlap the operands. */
+int nk_gemm_fp4(gpu_t *g, const uint8_t *Aq, uint32_t lda, const uint8_t *As, uint32_t ldas, const uint8_t *Wq,
+                uint32_t ldw, const uint8_t *Ws, uint32_t ldws, const float *bias, float *C, uint32_t ldc, uint32_t M,
+                uint32_t N, uint32_t K, int act, int accumulate, float alpha);
+int nk_gemm_w4(gpu_t *g, const float *A, uint32_t lda, const uint8_t *Wq, uint32_t ldw, const uint8_t *Ws,
+               uint32_t ldws, const float *bias, float *C, uint32_t ldc, uint32_t M, uint32_t N, uint32_t K, int act,
+               int accumulate, float alpha);
+
+/* ---- selective state space scan ------------------------------------------------------------------
+ * The two operators of a selective-scan block over the sequences of a batch (no counterpart in the
+ * reference).  seqs (device, 16-byte aligned) has four ints per sequence: { first row, rows, the slot whose
+ * state it goes on from or -1 for zeros, the slot that takes the state behind its last row or -1 for
+ * none }.  The slots may be the same; no slot is written by two sequences, or by one and read by another.
+ * A sequence of no rows hands its state on.  Rows that no sequence has are not written.  The rows of a
+ * sequence are below M and its slots below `slots`; max_rows is at least the longest sequence: a
+ * sequence that breaks these is left out (nothing of it is written).
+ *
+ * nk_causal_conv: Y[t][d] = act(bias[d] + sum_j W[d][j] X[t - (taps - 1) + j][d]) for D channels, with X before
+ * the sequence's first row from the slot: state is [slots][taps - 1][D] f32, the last inputs, oldest
+ * first.  W [D][taps], bias may be NULL, taps 2, 3 or 4, act none, SiLU or ReLU; X and Y of one type. */
+int nk_causal_conv(gpu_t *g, const void *X, int type, uint32_t ldx, const float *W, const float *bias, float *state,
+                   uint32_t slots, const int *seqs, uint32_t nseq, uint32_t max_rows, void *Y, uint32_t ldy, uint32_t M,
+                   uint32_t D, uint32_t taps, int act);
+/* nk_ssm_scan: per channel d of D and state n of N (1..64), over the rows t of a sequence,
+ *   s = dt[t][d] + dt_bias[d], then log(1 + e^s) where softplus is set
+ *   h[n] = exp(s A[d][n]) h[n] + s B[t][g][n] x[t][d]          g = d / (D / groups)
+ *   y[t][d] = (sum_n C[t][g][n] h[n] + skip[d] x[t][d]) * SiLU(z[t][d])
+ * x, dt, B, C, z, y are rows of one type; B and C rows have the stride ldbc and [groups][N] values (two
+ * parts of one projection's rows, say); A [D][N], skip, dt_bias and the state [slots][D][N] are f32.  skip,
+ * dt_bias and z (no gate) may be NULL.  y must not overlap the inputs.  Long sequences of few channels are
+ * split along their rows: the pieces' states lie in the context's scratch (no residual update may be
+ * pending; a capture needs the scratch sized by a call before it). */
+typedef struct {
+    int type;
+    uint32_t ldx, lddt, ldbc, ldz, ldy;
+    const void *x, *dt, *B, *C, *z;
+    void *y;
+    const float *A, *skip, *dt_bias;
+    float *state;
+    const int *seqs;
+    uint32_t slots, nseq, max_rows, M, D, N, groups;
+    int softplus;
+} nk_scan_t;
+int nk_ssm_scan(gpu_t *g, const nk_scan_t *a);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,66 @@
+/* Launchers of the selective-scan block's operators (include/nemo_kernels.h): arguments are checked before any
+ * launch; the sequences' table lies on the device and is checked by the kernels. */
+#include "nemo_kernels.h"
+#include "gpu.h"
+#include "../kernel_params.h"
+#include <stdio.h>
+
+static int bad(gpu_t *g, const char *what) { return gpu_fail(g, what); }
+static int aligned(const void *p, uintptr_t n) { return ((uintptr_t)p & (n - 1)) == 0; }
+
+#define CCONV_ROWS 32 /* as in the kernel */
+
+/* what both operators ask of the batch */
+static const char *batch_bad(const float *state, uint32_t slots, const int *seqs, uint32_t nseq, uint32_t max_rows, uint32_t D) {
+    if (!seqs || !aligned(seqs, 16)) return "sequences: a 16-byte aligned table";
+    if (nseq > 65535) return "sequences: at most 65535 in a call";
+    if (D > 1u << 28) return "sequences: at most 2^28 channels";
+    if (slots > 0x7fffffffu || (slots && (!state || !aligned(state, 4)))) return "sequences: slots without a state";
+    if (max_rows > 1u << 30) return "sequences: at most 2^30 rows each";
+    return NULL;
+}
+
+int nk_causal_conv(gpu_t *g, const void *X, int type, uint32_t ldx, const float *W, const float *bias, float *state,
+                   uint32_t slots, const int *seqs, uint32_t nseq, uint32_t max_rows, void *Y, uint32_t ldy, uint32_t M,
+                   uint32_t D, uint32_t taps, int act) {
+    if (!nseq || !D) return 0;
+    const char *why = batch_bad(state, slots, seqs, nseq, max_rows, D);
+    if (why) return bad(g, why);
+    if (type != NK_F32 && type != NK_BF16) return bad(g, "causal_conv: rows are f32 or bf16");
+    const uintptr_t size = type == NK_F32 ? 4 : 2;
+    if (taps < 2 || taps > 4 || act < NK_ACT_NONE || act > NK_ACT_RELU)
+        return bad(g, "causal_conv: 2 to 4 taps, no activation, SiLU or ReLU");
+    if (!X || !Y || !W || !aligned(X, size) || !aligned(Y, size) || !aligned(W, 4) || !aligned(bias, 4) || ldx < D || ldy < D)
+        return bad(g, "causal_conv: aligned rows of at least D values");
+    const uint32_t tiles = max_rows ? (max_rows + CCONV_ROWS - 1) / CCONV_ROWS : 1;
+    if (tiles > 65535) return bad(g, "causal_conv: a sequence of more than 65535 * 32 rows");
+    NkCconvArgs a = { X, W, bias, state, seqs, Y, ldx, ldy, slots, nseq, max_rows, M, D, taps, (u32)act, 0 };
+    char name[24];
+    snprintf(name, sizeof name, "cconv_%s_%u", type == NK_F32 ? "f32" : "bf16", taps);
+    gpu_next_bytes(g, 2.0 * size * M * D + 8.0 * nseq * (taps - 1) * D + 4.0 * D * (taps + 1));
+    return gpu_launch(g, name, &a, sizeof a, (D + 255) / 256, tiles, nseq, 256, 1, 1);
+}
+
+int nk_ssm_scan(gpu_t *g, const nk_scan_t *p) {
+    if (!p) return bad(g, "ssm_scan: no arguments");
+    if (!p->nseq || !p->D) return 0;
+    const char *why = batch_bad(p->state, p->slots, p->seqs, p->nseq, p->max_rows, p->D);
+    if (why) return bad(g, why);
+    if (p->type != NK_F32 && p->type != NK_BF16) return bad(g, "ssm_scan: rows are f32 or bf16");
+    const uintptr_t size = p->type == NK_F32 ? 4 : 2;
+    if (!p->N || p->N > 64 || !p->groups || p->D % p->groups) return bad(g, "ssm_scan: 1 to 64 states, groups that divide the channels");
+    if (!p->x || !p->dt || !p->B || !p->C || !p->y || !p->A || !aligned(p->x, size) || !aligned(p->dt, size) ||
+        !aligned(p->B, size) || !aligned(p->C, size) || !aligned(p->z, size) || !aligned(p->y, size) || !aligned(p->A, 4) ||
+        !aligned(p->skip, 4) || !aligned(p->dt_bias, 4))
+        return bad(g, "ssm_scan: x, dt, B, C, y and A aligned to their values");
+    if (p->ldx < p->D || p->lddt < p->D || p->ldy < p->D || (p->z && p->ldz < p->D) || p->ldbc < (uint64_t)p->groups * p->N)
+        return bad(g, "ssm_scan: rows of at least D values, B and C of groups * N");
+    NkScanArgs a = { p->x, p->dt, p->B, p->C, p->z, p->y, p->A, p->skip, p->dt_bias, p->state, p->seqs,
+                     p->ldx, p->lddt, p->ldbc, p->ldz, p->ldy, p->slots, p->nseq, p->max_rows, p->M, p->D, p->N,
+                     p->groups, p->softplus != 0 };
+    char name[24];
+    snprintf(name, sizeof name, "scan_%s_%u", p->type == NK_F32 ? "f32" : "bf16", p->N <= 8 ? 8u : p->N <= 16 ? 16u : p->N <= 32 ? 32u : 64u);
+    gpu_next_bytes(g, (double)size * p->M * (4.0 * p->D + 2.0 * p->groups * p->N) + 8.0 * p->nseq * p->D * p->N);
+    gpu_next_flops(g, (double)p->M * p->D * (7.0 * p->N + 12));
+    return gpu_launch(g, name, &a, sizeof a, (p->D + 255) / 256, p->nseq, 1, 256, 1, 1);
+}

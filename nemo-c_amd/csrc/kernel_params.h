@@ -487,4 +487,53 @@ typedef struct {
     float eps, scale;
 } NkChainArgs;
 
+/* ---- 4-bit rows (32 values share a power of two) ---------------------------------------------- */
+/* X [M][ldx] f32 or bf16 <-> codes Q (bytes, two codes each, rows of ldq) and scales S (bytes, rows of lds);
+ * both padded to groups of 128 values (g8: runs of 8 values in a padded row). */
+typedef struct {
+    void *X;
+    unsigned char *Q, *S;
+    u32 ldx, ldq, lds, M, K, g8, vec; /* vec: rows of X are read and written 16 bytes at a time */
+} NkFp4Args;
+
+/* C = alpha * act(A W^T + bias) (+ C): W 4-bit rows (Wq, Ws); A 4-bit rows (Aq, As) or f32 rows (A). */
+typedef struct {
+    const float *A;
+    const unsigned char *Aq, *As, *Wq, *Ws;
+    const float *bias;
+    float *C;
+    u32 lda, ldas, ldw, ldws, ldc; /* lda: floats of A, or bytes of Aq */
+    u32 M, N, K, act, accumulate, vec; /* vec: four consecutive outputs are stored at once */
+    float alpha;
+} NkGemm4Args;
+
+/* ---- sequences of a batch: seqs[i] = { first row, rows, slot read (-1: zeros), slot written (-1: none) } - */
+/* Whether a table entry fits: rows below M and at most max_rows of them, slots below `slots`.  The kernels
+ * leave out a sequence whose entry does not (nothing of it is read or written). */
+#ifdef __HIPCC__
+__host__ __device__
+#endif
+static inline int nk_seq_ok(int first, int rows, int from, int to, u32 M, u32 max_rows, u32 slots) {
+    return first >= 0 && rows >= 0 && (u32)first <= M && (u32)rows <= M - (u32)first && (u32)rows <= max_rows && from >= -1 &&
+           to >= -1 && (from < 0 || (u32)from < slots) && (to < 0 || (u32)to < slots);
+}
+
+typedef struct {
+    const void *X;
+    const float *W, *bias;
+    float *state;     /* [slots][taps - 1][D] */
+    const int *seqs;
+    void *Y;
+    u32 ldx, ldy, slots, nseq, max_rows, M, D, taps, act, vec;
+} NkCconvArgs;
+
+typedef struct {
+    const void *x, *dt, *B, *C, *z;
+    void *y;
+    const float *A, *skip, *dt_bias;
+    float *state;     /* [slots][D][N] */
+    const int *seqs;
+    u32 ldx, lddt, ldbc, ldz, ldy, slots, nseq, max_rows, M, D, N, groups, softplus;
+} NkScanArgs;
+
 #endif

@@ -170,6 +170,15 @@ API = {
     "nk_lstm_cell": (C.c_int, [_vp, _vp, _vp, _vp, _vp, _u32]),
     "nk_joint_partial": (C.c_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _u32, _u32, _u32, _u32, _u32, _u32]),
     "nk_argmax_reduce": (C.c_int, [_vp, _vp, _vp, _vp, _u32, _u32]),
+    "nk_fp4_quant": (C.c_int, [_vp, _vp, C.c_int, _u32, _vp, _u32, _vp, _u32, _u32, _u32]),
+    "nk_fp4_dequant": (C.c_int, [_vp, _vp, _u32, _vp, _u32, _vp, C.c_int, _u32, _u32, _u32]),
+    "nk_gemm_fp4": (C.c_int, [_vp, _vp, _u32, _vp, _u32, _vp, _u32, _vp, _u32, _vp, _vp, _u32, _u32, _u32, _u32, C.c_int,
+                              C.c_int, C.c_float]),
+    "nk_gemm_w4": (C.c_int, [_vp, _vp, _u32, _vp, _u32, _vp, _u32, _vp, _vp, _u32, _u32, _u32, _u32, C.c_int, C.c_int,
+                             C.c_float]),
+    "nk_causal_conv": (C.c_int, [_vp, _vp, C.c_int, _u32, _vp, _vp, _vp, _u32, _vp, _u32, _u32, _vp, _u32, _u32, _u32,
+                                 _u32, C.c_int]),
+    "nk_ssm_scan": (C.c_int, [_vp, _vp]),
     # include/nemo_gpu.h (the reference's runtime interface; gpu_arg_t arrays are GpuArg below)
     "gpu_buf_ptr": (_vp, [_vp]),
     "gpu_dispatch": (C.c_int, [_vp, C.c_char_p, _vp, C.c_int] + [_u32] * 6),
@@ -231,6 +240,18 @@ def gpu_args(*items):
 class Resid(C.Structure):
     """nk_resid_t: a pending residual update (partial rows in the context's scratch)."""
     _fields_ = [("parts", C.c_void_p), ("nparts", C.c_uint32), ("alpha", C.c_float)]
+
+
+class Scan(C.Structure):
+    """nk_scan_t: the operands of nk_ssm_scan (device addresses; lengths in elements)."""
+    _fields_ = ([("type", C.c_int)] + [(n, _u32) for n in ("ldx", "lddt", "ldbc", "ldz", "ldy")] +
+                [(n, _vp) for n in ("x", "dt", "B", "C", "z", "y", "A", "skip", "dt_bias", "state", "seqs")] +
+                [(n, _u32) for n in ("slots", "nseq", "max_rows", "M", "D", "N", "groups")] + [("softplus", C.c_int)])
+
+
+def fp4_row(k: int) -> int:
+    """Bytes of the codes of a 4-bit row of k values (NK_FP4_ROW); its scales take a sixteenth of that."""
+    return -(-k // 128) * 64
 
 
 class Gpu:
