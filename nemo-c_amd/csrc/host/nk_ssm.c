@@ -14,7 +14,7 @@ static int aligned(const void *p, uintptr_t n) { return ((uintptr_t)p & (n - 1))
 static const char *batch_bad(const float *state, uint32_t slots, const int *seqs, uint32_t nseq, uint32_t max_rows, uint32_t D) {
     if (!seqs || !aligned(seqs, 16)) return "sequences: a 16-byte aligned table";
     if (nseq > 65535) return "sequences: at most 65535 in a call";
-    if (D > 1u << 28) return "sequences: at most 2^28 channels";
+    if (D > 1u << 27) return "sequences: at most 2^27 channels";
     if (slots > 0x7fffffffu || (slots && (!state || !aligned(state, 4)))) return "sequences: slots without a state";
     if (max_rows > 1u << 30) return "sequences: at most 2^30 rows each";
     return NULL;
@@ -55,12 +55,38 @@ int nk_ssm_scan(gpu_t *g, const nk_scan_t *p) {
         return bad(g, "ssm_scan: x, dt, B, C, y and A aligned to their values");
     if (p->ldx < p->D || p->lddt < p->D || p->ldy < p->D || (p->z && p->ldz < p->D) || p->ldbc < (uint64_t)p->groups * p->N)
         return bad(g, "ssm_scan: rows of at least D values, B and C of groups * N");
-    NkScanArgs a = { p->x, p->dt, p->B, p->C, p->z, p->y, p->A, p->skip, p->dt_bias, p->state, p->seqs,
+    const uint32_t per = p->D / p->groups, block = per >= 256 ? 256 : (per + 63) / 64 * 64;
+    const uint32_t tiles = p->groups * ((per + block - 1) / block), waves = p->nseq * tiles * (block / 64);
+    NkScanArgs a = { p->x, p->dt, p->B, p->C, p->z, p->y, p->A, p->skip, p->dt_bias, p->state, p->seqs, NULL,
                      p->ldx, p->lddt, p->ldbc, p->ldz, p->ldy, p->slots, p->nseq, p->max_rows, p->M, p->D, p->N,
-                     p->groups, p->softplus != 0 };
-    char name[24];
-    snprintf(name, sizeof name, "scan_%s_%u", p->type == NK_F32 ? "f32" : "bf16", p->N <= 8 ? 8u : p->N <= 16 ? 16u : p->N <= 32 ? 32u : 64u);
+                     p->groups, p->softplus != 0, 0, 0,
+                     p->N % 4 == 0 && aligned(p->A, 16) && aligned(p->state, 16) };
+    const uint32_t ns = p->N <= 8 ? 8 : p->N <= 16 ? 16 : p->N <= 32 ? 32 : 64;
+    const char *type = p->type == NK_F32 ? "f32" : "bf16";
+    char name[32];
     gpu_next_bytes(g, (double)size * p->M * (4.0 * p->D + 2.0 * p->groups * p->N) + 8.0 * p->nseq * p->D * p->N);
     gpu_next_flops(g, (double)p->M * p->D * (7.0 * p->N + 12));
-    return gpu_launch(g, name, &a, sizeof a, (p->D + 255) / 256, p->nseq, 1, 256, 1, 1);
+    if (p->max_rows <= 4) {
+        uint32_t q = 1;
+        while (4 * q < p->N) q *= 2;
+        snprintf(name, sizeof name, "scan_few_%s_%u", type, q);
+        return gpu_launch(g, name, &a, sizeof a, (uint32_t)(((uint64_t)p->D * q + 255) / 256), p->nseq, 1, 256, 1, 1);
+    }
+    if (waves < 512 && p->max_rows > 64) {
+        const uint32_t want = (4096 + waves - 1) / waves;
+        uint32_t piece = (p->max_rows + want - 1) / want;
+        piece = piece < 32 ? 32 : (piece + 31) / 32 * 32;
+        const uint32_t pieces = (p->max_rows + piece - 1) / piece;
+        a.ws = gpu_scratch_ws(g, (size_t)p->nseq * pieces * (p->N + 1) * p->D);
+        if (!a.ws) return bad(g, "ssm_scan: scratch unavailable (size it before capture)");
+        a.piece = piece;
+        a.pieces = pieces;
+        snprintf(name, sizeof name, "scan_ends_%s_%u", type, ns);
+        if (gpu_launch(g, name, &a, sizeof a, tiles, p->nseq, pieces, block, 1, 1)) return -1;
+        if (gpu_launch(g, "scan_join", &a, sizeof a, (p->D + 255) / 256, p->N, p->nseq, 256, 1, 1)) return -1;
+        snprintf(name, sizeof name, "scan_from_%s_%u", type, ns);
+        return gpu_launch(g, name, &a, sizeof a, tiles, p->nseq, pieces, block, 1, 1);
+    }
+    snprintf(name, sizeof name, "scan_%s_%u", type, ns);
+    return gpu_launch(g, name, &a, sizeof a, tiles, p->nseq, 1, block, 1, 1);
 }

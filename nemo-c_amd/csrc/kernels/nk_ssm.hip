@@ -71,50 +71,232 @@ template <typename T, int TAPS> __device__ __forceinline__ void cconv_impl(const
 CCONV(float, f32, 2) CCONV(float, f32, 3) CCONV(float, f32, 4)
 CCONV(u16, bf16, 2) CCONV(u16, bf16, 3) CCONV(u16, bf16, 4)
 
-/* log(1 + e^v), without a threshold */
-__device__ __forceinline__ float softplus_f(float v) { return fmaxf(v, 0.0f) + log1pf(expf(-fabsf(v))); }
+/* e^v for v <= 0 to about two steps: 2^(v log2 e) with the product's rounding put back (the hardware's
+ * exponential gives 0 below 2^-126) */
+__device__ __forceinline__ float exp_neg(float v) {
+    const float t = v * 1.44269504f, r = fmaf(v, 1.44269504f, -t) + v * 1.92596299e-8f;
+    const float e = __builtin_amdgcn_exp2f(t);
+    return v < -104.0f ? 0.0f : fmaf(e, r * 0.693147181f, e); /* r is NaN where v is infinite */
+}
+/* log(1 + e^v) = max(v, 0) + 2 atanh(e / (2 + e)) with e = e^-|v|: the series in q^2 <= 1/9 to q^15 leaves 1.5e-9 */
+__device__ __forceinline__ float softplus_f(float v) {
+    const float e = exp_neg(-fabsf(v)), q = e * __builtin_amdgcn_rcpf(2.0f + e), w = q * q;
+    float s = 1.0f / 15;
+    s = fmaf(s, w, 1.0f / 13);
+    s = fmaf(s, w, 1.0f / 11);
+    s = fmaf(s, w, 1.0f / 9);
+    s = fmaf(s, w, 1.0f / 7);
+    s = fmaf(s, w, 1.0f / 5);
+    s = fmaf(s, w, 1.0f / 3);
+    s = fmaf(s * w, q, q);
+    return v != v ? v : fmaxf(v, 0.0f) + 2.0f * s;
+}
 
-/* One thread per channel with its NS >= N states in registers, row after row.  e^(s A) is 2^(s A log2 e) by
- * the hardware's exponential (results below 2^-126 come out as 0). */
-template <typename T, int NS> __device__ __forceinline__ void scan_impl(const NkScanArgs &a) {
-    const seq_t s = seq_load(a.seqs, blockIdx.y, a.M, a.max_rows, a.slots);
-    const u32 d = blockIdx.x * 256 + threadIdx.x;
-    if (!s.ok || d >= a.D) return;
-    const u32 g = d / (a.D / a.groups);
+#define SCAN_TILE 32 /* rows whose B and C are in LDS at a time */
+
+/* Rows t0 .. t1 - 1 of a sequence, one thread per channel with its NS >= N states in registers.
+ * e^(s A) is 2^(s A log2 e) by the hardware's exponential (results below 2^-126 come out as 0).  B and C are the
+ * same for every channel of the workgroup's group: a tile of their rows lies in LDS as f32, padded
+ * with zeros to NS, and is read by all lanes at one address.  ENDS: only the states (from zero) and the
+ * sum of the steps are wanted, no rows are written. */
+template <typename T, int NS, bool ENDS>
+__device__ __forceinline__ void scan_rows(const NkScanArgs &a, const seq_t &s, u32 t0, u32 t1, u32 g, u32 d, bool live,
+                                          float (&h)[NS], float &sum, float *lds) {
     const T *x = (const T *)a.x + (u64)s.first * a.ldx + d, *dt = (const T *)a.dt + (u64)s.first * a.lddt + d;
     const T *B = (const T *)a.B + (u64)s.first * a.ldbc + (u64)g * a.N, *C = (const T *)a.C + (u64)s.first * a.ldbc + (u64)g * a.N;
     const T *z = a.z ? (const T *)a.z + (u64)s.first * a.ldz + d : nullptr;
     T *y = (T *)a.y + (u64)s.first * a.ldy + d;
     const float skip = a.skip ? a.skip[d] : 0.0f, db = a.dt_bias ? a.dt_bias[d] : 0.0f;
-    float A[NS], h[NS];
+    constexpr u32 W = ENDS ? NS : 2 * NS;
+    float A[NS];
 #pragma unroll
     for (int n = 0; n < NS; ++n) {
-        A[n] = (u32)n < a.N ? a.A[(u64)d * a.N + n] * 1.44269504f : 0.0f;
-        h[n] = (u32)n < a.N && s.from >= 0 ? a.state[((u64)s.from * a.D + d) * a.N + n] : 0.0f;
+        const float v = a.A[(u64)d * a.N + min((u32)n, a.N - 1)];
+        A[n] = (u32)n < a.N ? v * 1.44269504f : 0.0f;
     }
-    for (u32 t = 0; t < s.rows; ++t) {
-        const float v = ld_row(x + (u64)t * a.ldx);
-        float p = ld_row(dt + (u64)t * a.lddt) + db;
-        if (a.softplus) p = softplus_f(p);
-        float o = 0.0f;
+    for (u32 u = t0; u < t1; u += SCAN_TILE) {
+        const u32 rows = min(t1 - u, (u32)SCAN_TILE);
+        __syncthreads();
+        for (u32 i = threadIdx.x; i < (rows + 3) / 4 * 4 * W; i += blockDim.x) {
+            const u32 r = i / W, n = i % W, m = n % NS;
+            lds[i] = r < rows && m < a.N ? ld_row((n < NS ? B : C) + (u64)(u + r) * a.ldbc + m) : 0.0f;
+        }
+        __syncthreads();
+        /* four rows' loads at a time; past the end a step of zero, which leaves the states as they are */
+#pragma unroll 1
+        for (u32 r0 = 0; r0 < rows; r0 += 4) {
+            float xv[4], pv[4], zv[4];
 #pragma unroll
-        for (int n = 0; n < NS; ++n) {
-            if ((u32)n < a.N) {
-                const float b = ld_row(B + (u64)t * a.ldbc + n), c = ld_row(C + (u64)t * a.ldbc + n);
-                h[n] = fmaf(__builtin_amdgcn_exp2f(p * A[n]), h[n], p * v * b);
-                o = fmaf(c, h[n], o);
+            for (int k = 0; k < 4; ++k) {
+                const u64 t = u + min(r0 + k, rows - 1);
+                xv[k] = ld_row(x + t * a.ldx);
+                pv[k] = ld_row(dt + t * a.lddt);
+                if constexpr (!ENDS) zv[k] = z ? ld_row(z + t * a.ldz) : 0.0f;
+            }
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const bool in = r0 + k < rows;
+                float p = a.softplus ? softplus_f(pv[k] + db) : pv[k] + db, v = p * xv[k];
+                p = in ? p : 0.0f;
+                v = in ? v : 0.0f;
+                if constexpr (ENDS) sum += p;
+                float o = 0.0f;
+                const floatx4 *bc = (const floatx4 *)(lds + (r0 + k) * W);
+#pragma unroll
+                for (int n = 0; n < NS; n += 4) {
+                    const floatx4 b = bc[n / 4];
+                    floatx4 c;
+                    if constexpr (!ENDS) c = bc[(NS + n) / 4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        h[n + e] = fmaf(__builtin_amdgcn_exp2f(p * A[n + e]), h[n + e], v * b[e]);
+                        if constexpr (!ENDS) o = fmaf(c[e], h[n + e], o);
+                    }
+                }
+                if constexpr (!ENDS) {
+                    o = fmaf(skip, xv[k], o);
+                    if (z) o *= silu_f(zv[k]);
+                    if (live && in) st_row(y + (u64)(u + r0 + k) * a.ldy, o);
+                }
             }
         }
-        if (a.skip) o = fmaf(skip, v, o);
-        if (z) o *= silu_f(ld_row(z + (u64)t * a.ldz));
-        st_row(y + (u64)t * a.ldy, o);
     }
-    if (s.to >= 0)
-#pragma unroll
-        for (int n = 0; n < NS; ++n)
-            if ((u32)n < a.N) a.state[((u64)s.to * a.D + d) * a.N + n] = h[n];
 }
-#define SCAN(T, NAME, NS) \
-    extern "C" __global__ __launch_bounds__(256) void scan_##NAME##_##NS(const NkScanArgs a) { scan_impl<T, NS>(a); }
+
+/* channel of this thread: workgroups of blockDim channels inside one group */
+struct chan_t {
+    u32 g, d;
+    bool live;
+};
+__device__ __forceinline__ chan_t scan_channel(const NkScanArgs &a) {
+    const u32 per = a.D / a.groups, tiles = (per + blockDim.x - 1) / blockDim.x, g = blockIdx.x / tiles;
+    const u32 c = (blockIdx.x - g * tiles) * blockDim.x + threadIdx.x;
+    return (chan_t){ g, g * per + min(c, per - 1), c < per };
+}
+
+/* PART 0: whole sequences.  PART 1: the states that the pieces of a.piece rows end in from zero, and their
+ * sums of steps.  PART 2: the pieces again from the states that scan_join has put in their place. */
+template <typename T, int NS, int PART> __device__ __forceinline__ void scan_impl(const NkScanArgs &a) {
+    __shared__ float lds[SCAN_TILE * NS * (PART == 1 ? 1 : 2)];
+    const seq_t s = seq_load(a.seqs, blockIdx.y, a.M, a.max_rows, a.slots);
+    const chan_t c = scan_channel(a);
+    const u32 t0 = PART ? blockIdx.z * a.piece : 0, t1 = PART ? min(t0 + a.piece, s.rows) : s.rows;
+    if (!s.ok || (PART && t0 >= s.rows)) return;
+    float h[NS], sum = 0.0f;
+    /* scratch: per piece N states of D channels, then the sums */
+    float *ws = PART ? a.ws + ((u64)blockIdx.y * a.pieces + blockIdx.z) * (a.N + 1) * a.D + c.d : nullptr;
+#pragma unroll
+    for (int n = 0; n < NS; ++n) h[n] = 0.0f;
+    if (PART == 2 || (PART == 0 && s.from >= 0)) {
+        const float *from = PART ? ws : a.state + ((u64)s.from * a.D + c.d) * a.N;
+#pragma unroll
+        for (int n = 0; n < NS; ++n) {
+            const float v = from[min((u32)n, a.N - 1) * (PART ? (u64)a.D : 1)];
+            h[n] = (u32)n < a.N ? v : 0.0f;
+        }
+    }
+    scan_rows<T, NS, PART == 1>(a, s, t0, t1, c.g, c.d, c.live, h, sum, lds);
+    if (!c.live || PART == 2 || (PART == 0 && s.to < 0)) return;
+    float *to = PART ? ws : a.state + ((u64)s.to * a.D + c.d) * a.N;
+#pragma unroll
+    for (int n = 0; n < NS; ++n)
+        if ((u32)n < a.N) to[n * (PART ? (u64)a.D : 1)] = h[n];
+    if (PART == 1) ws[(u64)a.N * a.D] = sum;
+}
+#define SCAN(T, NAME, NS)                                                                                              \
+    extern "C" __global__ __launch_bounds__(256) void scan_##NAME##_##NS(const NkScanArgs a) { scan_impl<T, NS, 0>(a); } \
+    extern "C" __global__ __launch_bounds__(256) void scan_ends_##NAME##_##NS(const NkScanArgs a) { scan_impl<T, NS, 1>(a); } \
+    extern "C" __global__ __launch_bounds__(256) void scan_from_##NAME##_##NS(const NkScanArgs a) { scan_impl<T, NS, 2>(a); }
 SCAN(float, f32, 8) SCAN(float, f32, 16) SCAN(float, f32, 32) SCAN(float, f32, 64)
 SCAN(u16, bf16, 8) SCAN(u16, bf16, 16) SCAN(u16, bf16, 32) SCAN(u16, bf16, 64)
+
+/* The pieces of a sequence one after another: the state a piece starts from takes the place of the one it
+ * ends in from zero, H <- e^(A sum) H + end.  One thread per state. */
+extern "C" __global__ __launch_bounds__(256) void scan_join(const NkScanArgs a) {
+    const seq_t s = seq_load(a.seqs, blockIdx.z, a.M, a.max_rows, a.slots);
+    const u32 d = blockIdx.x * 256 + threadIdx.x, n = blockIdx.y;
+    if (!s.ok || d >= a.D) return;
+    const float A = a.A[(u64)d * a.N + n] * 1.44269504f;
+    float h = s.from >= 0 ? a.state[((u64)s.from * a.D + d) * a.N + n] : 0.0f;
+    const u32 pieces = (s.rows + a.piece - 1) / a.piece;
+    const u64 step = (u64)(a.N + 1) * a.D;
+    float *w = a.ws + (u64)blockIdx.z * a.pieces * step + d;
+    for (u32 i = 0; i < pieces; ++i, w += step) {
+        const float end = w[(u64)n * a.D], sum = w[(u64)a.N * a.D];
+        w[(u64)n * a.D] = h;
+        h = fmaf(__builtin_amdgcn_exp2f(sum * A), h, end);
+    }
+    if (s.to >= 0) a.state[((u64)s.to * a.D + d) * a.N + n] = h;
+}
+
+/* Few rows (tokens): every state row is read and written once and the rows are nothing beside them, so the
+ * states are spread over lanes: Q lanes per channel with four consecutive states each, a row's output
+ * summed over the Q lanes. */
+template <typename T, int Q> __device__ __forceinline__ void scan_few_impl(const NkScanArgs &a) {
+    const seq_t s = seq_load(a.seqs, blockIdx.y, a.M, a.max_rows, a.slots);
+    const u32 i = blockIdx.x * 256 + threadIdx.x, n0 = 4 * (i % Q);
+    const bool live = i / Q < a.D;
+    const u32 d = min(i / Q, a.D - 1), g = d / (a.D / a.groups);
+    if (!s.ok) return;
+    /* the four states' places in a row of N (a place past the end counts as the last and is masked) */
+    u32 at[4];
+    float A[4], h[4] = { 0.f, 0.f, 0.f, 0.f };
+#pragma unroll
+    for (int e = 0; e < 4; ++e) at[e] = min(n0 + e, a.N - 1);
+    const float *ar = a.A + (u64)d * a.N, *hr = a.state + ((u64)max(s.from, 0) * a.D + d) * a.N;
+    if (a.vec && n0 < a.N) {
+        const floatx4 v = *(const floatx4 *)(ar + n0);
+        A[0] = v[0]; A[1] = v[1]; A[2] = v[2]; A[3] = v[3];
+    } else
+#pragma unroll
+        for (int e = 0; e < 4; ++e) A[e] = ar[at[e]];
+    if (s.from >= 0) {
+        if (a.vec && n0 < a.N) {
+            const floatx4 v = *(const floatx4 *)(hr + n0);
+            h[0] = v[0]; h[1] = v[1]; h[2] = v[2]; h[3] = v[3];
+        } else
+#pragma unroll
+            for (int e = 0; e < 4; ++e) h[e] = hr[at[e]];
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        A[e] = n0 + e < a.N ? A[e] * 1.44269504f : 0.0f;
+        h[e] = n0 + e < a.N ? h[e] : 0.0f;
+    }
+    const float skip = a.skip ? a.skip[d] : 0.0f, db = a.dt_bias ? a.dt_bias[d] : 0.0f;
+    for (u32 t = s.first; t < s.first + s.rows; ++t) {
+        const float v = ld_row((const T *)a.x + (u64)t * a.ldx + d);
+        float p = ld_row((const T *)a.dt + (u64)t * a.lddt + d) + db;
+        const T *B = (const T *)a.B + (u64)t * a.ldbc + (u64)g * a.N, *C = (const T *)a.C + (u64)t * a.ldbc + (u64)g * a.N;
+        float b[4], c[4], o = 0.0f;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            b[e] = ld_row(B + at[e]);
+            c[e] = ld_row(C + at[e]);
+        }
+        const float z = a.z ? ld_row((const T *)a.z + (u64)t * a.ldz + d) : 0.0f;
+        if (a.softplus) p = softplus_f(p);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const bool in = n0 + e < a.N;
+            h[e] = fmaf(__builtin_amdgcn_exp2f(p * A[e]), h[e], p * v * b[e]);
+            o = in ? fmaf(c[e], h[e], o) : o;
+        }
+#pragma unroll
+        for (int w = Q / 2; w > 0; w >>= 1) o += __shfl_xor(o, w, 64);
+        o = fmaf(skip, v, o);
+        if (a.z) o *= silu_f(z);
+        if (live && n0 == 0) st_row((T *)a.y + (u64)t * a.ldy + d, o);
+    }
+    if (s.to < 0 || !live) return;
+    float *to = a.state + ((u64)s.to * a.D + d) * a.N;
+    if (a.vec && n0 < a.N) *(floatx4 *)(to + n0) = (floatx4){ h[0], h[1], h[2], h[3] };
+    else
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (n0 + e < a.N) to[n0 + e] = h[e];
+}
+#define SCAN_FEW(Q)                                                                                                    \
+    extern "C" __global__ __launch_bounds__(256) void scan_few_f32_##Q(const NkScanArgs a) { scan_few_impl<float, Q>(a); } \
+    extern "C" __global__ __launch_bounds__(256) void scan_few_bf16_##Q(const NkScanArgs a) { scan_few_impl<u16, Q>(a); }
+SCAN_FEW(1) SCAN_FEW(2) SCAN_FEW(4) SCAN_FEW(8) SCAN_FEW(16)
