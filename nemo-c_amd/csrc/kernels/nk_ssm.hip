@@ -102,10 +102,10 @@ __device__ __forceinline__ float softplus_f(float v) {
 template <typename T, int NS, bool ENDS>
 __device__ __forceinline__ void scan_rows(const NkScanArgs &a, const seq_t &s, u32 t0, u32 t1, u32 g, u32 d, bool live,
                                           float (&h)[NS], float &sum, float *lds) {
-    const T *x = (const T *)a.x + (u64)s.first * a.ldx + d, *dt = (const T *)a.dt + (u64)s.first * a.lddt + d;
+    const T *x = (const T *)a.x + (u64)s.first * a.ldx, *dt = (const T *)a.dt + (u64)s.first * a.lddt;
     const T *B = (const T *)a.B + (u64)s.first * a.ldbc + (u64)g * a.N, *C = (const T *)a.C + (u64)s.first * a.ldbc + (u64)g * a.N;
-    const T *z = a.z ? (const T *)a.z + (u64)s.first * a.ldz + d : nullptr;
-    T *y = (T *)a.y + (u64)s.first * a.ldy + d;
+    const T *z = a.z ? (const T *)a.z + (u64)s.first * a.ldz : nullptr;
+    T *y = (T *)a.y + (u64)s.first * a.ldy;
     const float skip = a.skip ? a.skip[d] : 0.0f, db = a.dt_bias ? a.dt_bias[d] : 0.0f;
     constexpr u32 W = ENDS ? NS : 2 * NS;
     float A[NS];
@@ -129,9 +129,9 @@ __device__ __forceinline__ void scan_rows(const NkScanArgs &a, const seq_t &s, u
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
                 const u64 t = u + min(r0 + k, rows - 1);
-                xv[k] = ld_row(x + t * a.ldx);
-                pv[k] = ld_row(dt + t * a.lddt);
-                if constexpr (!ENDS) zv[k] = z ? ld_row(z + t * a.ldz) : 0.0f;
+                xv[k] = ld_row(x + t * a.ldx + d);
+                pv[k] = ld_row(dt + t * a.lddt + d);
+                if constexpr (!ENDS) zv[k] = z ? ld_row(z + t * a.ldz + d) : 0.0f;
             }
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
@@ -156,7 +156,7 @@ __device__ __forceinline__ void scan_rows(const NkScanArgs &a, const seq_t &s, u
                 if constexpr (!ENDS) {
                     o = fmaf(skip, xv[k], o);
                     if (z) o *= silu_f(zv[k]);
-                    if (live && in) st_row(y + (u64)(u + r0 + k) * a.ldy, o);
+                    if (live && in) st_row(y + (u64)(u + r0 + k) * a.ldy + d, o);
                 }
             }
         }
@@ -175,32 +175,34 @@ __device__ __forceinline__ chan_t scan_channel(const NkScanArgs &a) {
 }
 
 /* PART 0: whole sequences.  PART 1: the states that the pieces of a.piece rows end in from zero, and their
- * sums of steps.  PART 2: the pieces again from the states that scan_join has put in their place. */
+ * sums of steps (of all but a sequence's last, which nothing follows).  PART 2: the pieces again from the
+ * states that scan_join has put in their predecessors' places. */
 template <typename T, int NS, int PART> __device__ __forceinline__ void scan_impl(const NkScanArgs &a) {
     __shared__ float lds[SCAN_TILE * NS * (PART == 1 ? 1 : 2)];
     const seq_t s = seq_load(a.seqs, blockIdx.y, a.M, a.max_rows, a.slots);
     const chan_t c = scan_channel(a);
     const u32 t0 = PART ? blockIdx.z * a.piece : 0, t1 = PART ? min(t0 + a.piece, s.rows) : s.rows;
-    if (!s.ok || (PART && t0 >= s.rows)) return;
+    if (!s.ok || (PART == 1 ? t0 + a.piece >= s.rows : PART == 2 && t0 && t0 >= s.rows)) return;
     float h[NS], sum = 0.0f;
     /* scratch: per piece N states of D channels, then the sums */
     float *ws = PART ? a.ws + ((u64)blockIdx.y * a.pieces + blockIdx.z) * (a.N + 1) * a.D + c.d : nullptr;
 #pragma unroll
     for (int n = 0; n < NS; ++n) h[n] = 0.0f;
-    if (PART == 2 || (PART == 0 && s.from >= 0)) {
-        const float *from = PART ? ws : a.state + ((u64)s.from * a.D + c.d) * a.N;
+    const bool joined = PART == 2 && t0;
+    if (joined || (PART != 1 && !t0 && s.from >= 0)) {
+        const float *from = joined ? ws - (u64)(a.N + 1) * a.D : a.state + ((u64)s.from * a.D + c.d) * a.N;
 #pragma unroll
         for (int n = 0; n < NS; ++n) {
-            const float v = from[min((u32)n, a.N - 1) * (PART ? (u64)a.D : 1)];
+            const float v = from[min((u32)n, a.N - 1) * (joined ? (u64)a.D : 1)];
             h[n] = (u32)n < a.N ? v : 0.0f;
         }
     }
     scan_rows<T, NS, PART == 1>(a, s, t0, t1, c.g, c.d, c.live, h, sum, lds);
-    if (!c.live || PART == 2 || (PART == 0 && s.to < 0)) return;
-    float *to = PART ? ws : a.state + ((u64)s.to * a.D + c.d) * a.N;
+    if (!c.live || (PART != 1 && (s.to < 0 || t1 < s.rows))) return;
+    float *to = PART == 1 ? ws : a.state + ((u64)s.to * a.D + c.d) * a.N;
 #pragma unroll
     for (int n = 0; n < NS; ++n)
-        if ((u32)n < a.N) to[n * (PART ? (u64)a.D : 1)] = h[n];
+        if ((u32)n < a.N) to[n * (PART == 1 ? (u64)a.D : 1)] = h[n];
     if (PART == 1) ws[(u64)a.N * a.D] = sum;
 }
 #define SCAN(T, NAME, NS)                                                                                              \
@@ -210,23 +212,34 @@ template <typename T, int NS, int PART> __device__ __forceinline__ void scan_imp
 SCAN(float, f32, 8) SCAN(float, f32, 16) SCAN(float, f32, 32) SCAN(float, f32, 64)
 SCAN(u16, bf16, 8) SCAN(u16, bf16, 16) SCAN(u16, bf16, 32) SCAN(u16, bf16, 64)
 
-/* The pieces of a sequence one after another: the state a piece starts from takes the place of the one it
- * ends in from zero, H <- e^(A sum) H + end.  One thread per state. */
+/* The pieces of a sequence one after another: H <- e^(A sum) H + end, the state that the next piece starts from,
+ * takes the place of the piece's own end.  One thread per state; the loads of JOIN pieces are in flight at a time
+ * (one at a time 36 us for 128 pieces of 2048 channels, a memory round trip each). */
+#define JOIN 16
 extern "C" __global__ __launch_bounds__(256) void scan_join(const NkScanArgs a) {
     const seq_t s = seq_load(a.seqs, blockIdx.z, a.M, a.max_rows, a.slots);
     const u32 d = blockIdx.x * 256 + threadIdx.x, n = blockIdx.y;
-    if (!s.ok || d >= a.D) return;
+    if (!s.ok || d >= a.D || s.rows <= a.piece) return;
     const float A = a.A[(u64)d * a.N + n] * 1.44269504f;
     float h = s.from >= 0 ? a.state[((u64)s.from * a.D + d) * a.N + n] : 0.0f;
-    const u32 pieces = (s.rows + a.piece - 1) / a.piece;
+    const u32 ends = (s.rows - 1) / a.piece; /* pieces that another follows */
     const u64 step = (u64)(a.N + 1) * a.D;
     float *w = a.ws + (u64)blockIdx.z * a.pieces * step + d;
-    for (u32 i = 0; i < pieces; ++i, w += step) {
-        const float end = w[(u64)n * a.D], sum = w[(u64)a.N * a.D];
-        w[(u64)n * a.D] = h;
-        h = fmaf(__builtin_amdgcn_exp2f(sum * A), h, end);
+    for (u32 i = 0; i < ends; i += JOIN) {
+        float end[JOIN], sum[JOIN];
+#pragma unroll
+        for (u32 k = 0; k < JOIN; ++k) {
+            const float *p = w + min(i + k, ends - 1) * step;
+            end[k] = p[(u64)n * a.D];
+            sum[k] = p[(u64)a.N * a.D];
+        }
+#pragma unroll
+        for (u32 k = 0; k < JOIN; ++k) {
+            if (i + k >= ends) break;
+            h = fmaf(__builtin_amdgcn_exp2f(sum[k] * A), h, end[k]);
+            w[(i + k) * step + (u64)n * a.D] = h;
+        }
     }
-    if (s.to >= 0) a.state[((u64)s.to * a.D + d) * a.N + n] = h;
 }
 
 /* Few rows (tokens): every state row is read and written once and the rows are nothing beside them, so the
