@@ -72,10 +72,16 @@ int nk_ssm_scan(gpu_t *g, const nk_scan_t *p) {
         snprintf(name, sizeof name, "scan_few_%s_%u", type, q);
         return gpu_launch(g, name, &a, sizeof a, (uint32_t)(((uint64_t)p->D * q + 255) / 256), p->nseq, 1, 256, 1, 1);
     }
-    if (waves < 512 && p->max_rows > 64) {
-        const uint32_t want = (4096 + waves - 1) / waves;
-        uint32_t piece = (p->max_rows + want - 1) / want;
-        piece = piece < 32 ? 32 : (piece + 31) / 32 * 32;
+    /* split or whole, by wavefronts w and rows r (2048 channels of 16 states, bf16, graph replays): whole takes
+     * 10 + r (0.55 + 0.00025 w) us (a row of one wavefront is a chain of 0.55 us, few wavefronts hide none of it), split
+     * 19 + 0.00075 w r (every exponential twice, three launches).  Whole / split: 32 w 16 r 17.6 / 20.7, 32 r 26.7 /
+     * 20.8, 8192 r 7622 / 168; 512 w 16 r 18.9 / 28.5, 128 r 107 / 67; 1024 w 64 r 61.6 / 71, 256 r 252 / 166 */
+    if (waves < 1100 && (uint64_t)p->max_rows * (1100 - waves) > 18000) {
+        /* about 4096 wavefronts (four per SIMD: 8192 rows of one stream 335 us with 1024, 210 with 2048, 168), and
+         * pieces of some sqrt(r / 2) rows, between the pieces' time and that of joining them (512 rows: pieces of
+         * 4, 8, 16 and 32 rows 45, 34, 31 and 42 us; 32 rows: 17.8, 20.8, 27.4, 30.1) */
+        uint32_t piece = 8;
+        while (piece * (4096ull / waves) < p->max_rows || 2ull * piece * piece < p->max_rows) piece += 8;
         const uint32_t pieces = (p->max_rows + piece - 1) / piece;
         a.ws = gpu_scratch_ws(g, (size_t)p->nseq * pieces * (p->N + 1) * p->D);
         if (!a.ws) return bad(g, "ssm_scan: scratch unavailable (size it before capture)");
