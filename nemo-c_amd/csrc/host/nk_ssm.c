@@ -66,7 +66,11 @@ int nk_ssm_scan(gpu_t *g, const nk_scan_t *p) {
     char name[32];
     gpu_next_bytes(g, (double)size * p->M * (4.0 * p->D + 2.0 * p->groups * p->N) + 8.0 * p->nseq * p->D * p->N);
     gpu_next_flops(g, (double)p->M * p->D * (7.0 * p->N + 12));
-    if (p->max_rows <= 4) {
+    /* states over lanes for few rows r, by wavefronts w of 64 channels (2048 channels of 16 states, f32, graph replays):
+     * 4 + r max(0.42, 0.0012 w) us against 8 + 0.0067 w + r (0.5 + 0.0001 w) with the states in one lane: 32 w 8 r 7.0
+     * / 12.0, 24 r 13.6 / 19.9; 1024 w 8 r 14.6 / 16.9, 16 r 24.1 / 21.3; 8192 w 4 r 55 / 68, 8 r 95 / 73.  Beyond
+     * 32 rows a few wavefronts are split (64 r 21.0). */
+    if (p->max_rows <= 32 && (int64_t)p->max_rows * ((int64_t)waves * 12 - 5000) < 40000 + 67 * (int64_t)waves) {
         uint32_t q = 1;
         while (4 * q < p->N) q *= 2;
         snprintf(name, sizeof name, "scan_few_%s_%u", type, q);
