@@ -8,6 +8,7 @@
 
 static int bad(gpu_t *g, const char *what) { return gpu_fail(g, what); }
 static int aligned(const void *p, uintptr_t n) { return ((uintptr_t)p & (n - 1)) == 0; }
+#define FP4_STRIDE (1u << 24) /* the products' strides in bytes are below it: 24-bit multiplications, tiles below 4 GB */
 /* codes and scales of rows of K values */
 static int rows_ok(const uint8_t *Q, uint32_t ldq, const uint8_t *S, uint32_t lds, uint32_t K) {
     return Q && S && aligned(Q, 16) && ldq % 16 == 0 && ldq >= NK_FP4_ROW(K) && aligned(S, 4) && lds % 4 == 0 &&
@@ -41,22 +42,54 @@ int nk_fp4_dequant(gpu_t *g, const uint8_t *Q, uint32_t ldq, const uint8_t *S, u
     return convert(g, "fp4_dequant", X, type, ldx, (uint8_t *)Q, ldq, (uint8_t *)S, lds, M, K);
 }
 
+/* The tiles of the many-row 4-bit product.  A launch runs in rounds of `slots` workgroups; a round takes about fix +
+ * step x K steps (256 values) microseconds, step1 when no CU has more than one workgroup (graph replays of
+ * 3584 x 4096 x 8192 and x 4096, 2048 x 4096 x 4096, 1024 x 4096 x 2048, 448 x 4096 x 1024, 448 x 1024 x 4096 and
+ * 128 x 4096 x 4096: 128x256 80, 50, 28, 16.4, 11.1, 17.6 and 17.9 us, 64x128 102, 60, 36, 14.0, 7.9, 11.0 and
+ * 11.3, 64x64 133, 70, 42, 15.3, 7.1, 8.7 and 9.4: the least is picked each time). */
+typedef struct { const char *name; uint16_t bm, bn, threads, slots; float fix, step, step1; } tile_t;
+static const tile_t fp4_tiles[] = {
+    { "128x256", 128, 256, 768, 256, 10.0f, 1.0f, 1.0f },
+    { "64x128", 64, 128, 512, 512, 4.0f, 0.9f, 0.52f },
+    { "64x64", 64, 64, 512, 768, 3.0f, 0.72f, 0.38f }, /* not with GLU: 64 rows of scales are of one half */
+};
+static uint32_t tiles_of(const tile_t *t, uint32_t M, uint32_t nout, int glu) {
+    const uint32_t co = glu ? t->bn / 2u : t->bn;
+    return (M + t->bm - 1) / t->bm * ((nout + co - 1) / co);
+}
+static const tile_t *tile_pick(const tile_t *list, int n, uint32_t M, uint32_t nout, uint32_t K, int glu) {
+    const tile_t *best = NULL;
+    float least = 0;
+    for (const tile_t *t = list; t < list + n; ++t) {
+        if (glu && t->bn < 128) continue;
+        const uint32_t w = tiles_of(t, M, nout, glu), rounds = (w + t->slots - 1) / t->slots;
+        const float us = (float)rounds * (t->fix + (w <= 256 ? t->step1 : t->step) * (float)((K + 255) / 256));
+        if (!best || us < least) { best = t; least = us; }
+    }
+    return best;
+}
+
 /* the checks that both products share, and their launch */
 static int product(gpu_t *g, NkGemm4Args *a) {
     const int glu = a->act == NK_ACT_GLU;
     if (a->act > NK_ACT_GLU) return bad(g, "gemm 4-bit: unknown activation");
-    if (!a->N || a->N > 1u << 28 || !a->K || a->K > 1u << 30 || (glu && (a->N & 1))) return bad(g, "gemm 4-bit: bad shape");
+    if (!a->N || a->N > 1u << 28 || !a->K || (glu && (a->N & 1))) return bad(g, "gemm 4-bit: bad shape");
     if (a->M > 65535 * 64) return bad(g, "gemm 4-bit: too many rows");
-    if (!rows_ok(a->Wq, a->ldw, a->Ws, a->ldws, a->K))
-        return bad(g, "gemm 4-bit: weight codes 16-byte and scales 4-byte aligned, rows padded to 128 values");
+    if (!rows_ok(a->Wq, a->ldw, a->Ws, a->ldws, a->K) || a->ldw >= FP4_STRIDE || a->ldws >= FP4_STRIDE)
+        return bad(g, "gemm 4-bit: weight codes 16-byte and scales 4-byte aligned, rows padded to 128 values, strides below 2^24");
     const uint32_t nout = glu ? a->N / 2 : a->N;
     if (!a->C || !aligned(a->C, 4) || !aligned(a->bias, 4) || a->ldc < nout) return bad(g, "gemm 4-bit: ldc < output width");
     a->vec = aligned(a->C, 16) && a->ldc % 4 == 0;
     gpu_next_bytes(g, 17.0 / 32 * a->N * a->K + (a->A ? 4.0 : 17.0 / 32) * a->M * a->K +
                           4.0 * a->M * nout * (a->accumulate ? 2 : 1) + (a->bias ? 4.0 * a->N : 0.0));
     gpu_next_flops(g, 2.0 * a->M * a->N * a->K);
+    char name[32];
+    if (!a->A && a->M > 64 && a->K > 384) {
+        const tile_t *t = tile_pick(fp4_tiles, 3, a->M, nout, a->K, glu);
+        snprintf(name, sizeof name, "gemm_fp4_%s%s", t->name, glu ? "_glu" : "");
+        return gpu_launch(g, name, a, sizeof *a, (tiles_of(t, a->M, nout, glu) + 7) / 8 * 8, 1, 1, t->threads, 1, 1);
+    }
     const uint32_t cols = glu ? 32 : 64;
-    char name[24];
     snprintf(name, sizeof name, "gemm_%s%s", a->A ? "w4" : "fp4", glu ? "_glu" : "");
     return gpu_launch(g, name, a, sizeof *a, (nout + cols - 1) / cols, (a->M + 63) / 64, 1, 256, 1, 1);
 }
@@ -65,7 +98,8 @@ int nk_gemm_fp4(gpu_t *g, const uint8_t *Aq, uint32_t lda, const uint8_t *As, ui
                 uint32_t ldw, const uint8_t *Ws, uint32_t ldws, const float *bias, float *C, uint32_t ldc, uint32_t M,
                 uint32_t N, uint32_t K, int act, int accumulate, float alpha) {
     if (!M) return 0;
-    if (!rows_ok(Aq, lda, As, ldas, K)) return bad(g, "gemm_fp4: row codes 16-byte and scales 4-byte aligned, rows padded to 128 values");
+    if (!rows_ok(Aq, lda, As, ldas, K) || lda >= FP4_STRIDE || ldas >= FP4_STRIDE)
+        return bad(g, "gemm_fp4: row codes 16-byte and scales 4-byte aligned, rows padded to 128 values, strides below 2^24");
     NkGemm4Args a = { NULL, Aq, As, Wq, Ws, bias, C, lda, ldas, ldw, ldws, ldc, M, N, K, (u32)act, accumulate != 0, 0, alpha };
     return product(g, &a);
 }

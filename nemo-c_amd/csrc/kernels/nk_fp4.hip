@@ -7,6 +7,7 @@
 #include "nk_common.h"
 
 typedef int intx8 __attribute__((ext_vector_type(8)));
+typedef float floatx16 __attribute__((ext_vector_type(16)));
 
 /* the factor of a scale byte as f32: 2^-127 is subnormal, 255 (a block of NaN) a quiet NaN */
 __device__ __forceinline__ float fp4_scale(u32 s) {
@@ -101,37 +102,52 @@ template <bool BF> __device__ __forceinline__ void fp4_dequant_impl(const NkFp4A
 extern "C" __global__ __launch_bounds__(256) void fp4_dequant_f32(const NkFp4Args a) { fp4_dequant_impl<false>(a); }
 extern "C" __global__ __launch_bounds__(256) void fp4_dequant_bf16(const NkFp4Args a) { fp4_dequant_impl<true>(a); }
 
-/* bias, activation, alpha and accumulation of four consecutive columns n.. of row m (GLU: gate sums in t) */
-template <bool GLU> __device__ __forceinline__ void fp4_store4(const NkGemm4Args &a, u32 m, u32 n, floatx4 s, floatx4 t) {
-    const u32 nout = GLU ? a.N / 2 : a.N;
+/* the bias of columns n .. n + 3 (zeros without one; a column past the end counts as the last) */
+__device__ __forceinline__ floatx4 fp4_bias4(const NkGemm4Args &a, u32 n, u32 nout, u32 gate) {
+    floatx4 b = { 0.f, 0.f, 0.f, 0.f };
+    if (a.bias)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) b[e] = a.bias[min(n + e, nout - 1) + gate];
+    return b;
+}
+/* activation of the sums s (bias added; GLU: t the gates'), alpha, accumulation and store of columns n .. n + 3 of
+ * row m */
+template <bool GLU> __device__ __forceinline__ void fp4_store4(const NkGemm4Args &a, u32 m, u32 n, u32 nout, floatx4 s, floatx4 t) {
+    if (GLU)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[e] *= sigmoid_f(t[e]);
+    else if (a.act == NK_ACT_SILU)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[e] = silu_f(s[e]);
+    else if (a.act == NK_ACT_RELU)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[e] = fmaxf(s[e], 0.0f);
     if (m >= a.M || n >= nout) return;
     float *c = a.C + (u64)m * a.ldc + n;
-    const bool vec = a.vec && n + 4 <= nout;
-    floatx4 old = { 0.f, 0.f, 0.f, 0.f }, b = old, d = old;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-        const u32 col = min(n + e, nout - 1);
-        if (a.bias) {
-            b[e] = a.bias[col];
-            if (GLU) d[e] = a.bias[col + nout];
-        }
-        if (a.accumulate && !vec) old[e] = a.C[(u64)m * a.ldc + col];
-    }
-    if (a.accumulate && vec) old = *(const floatx4 *)c;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-        float v = s[e] + b[e];
-        if (GLU) v *= sigmoid_f(t[e] + d[e]);
-        else if (a.act == NK_ACT_SILU) v = silu_f(v);
-        else if (a.act == NK_ACT_RELU) v = fmaxf(v, 0.0f);
-        v *= a.alpha;
-        s[e] = a.accumulate ? old[e] + v : v;
-    }
-    if (vec) *(floatx4 *)c = s;
-    else
+    if (a.vec && n + 4 <= nout) {
+        floatx4 v = s * a.alpha;
+        if (a.accumulate) v = *(const floatx4 *)c + v;
+        *(floatx4 *)c = v;
+    } else {
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-            if (n + e < nout) c[e] = s[e];
+            if (n + e < nout) c[e] = a.accumulate ? c[e] + s[e] * a.alpha : s[e] * a.alpha;
+    }
+}
+/* A wavefront's TI x TJ tiles from row m0 and the columns col[j] on (GLU: the second half of the tiles are gates):
+ * the lane holds row m0 + 16 i + lane % 16, columns col[j] + 4 (lane / 16) .. + 3 */
+template <bool GLU, int TI, int TJ>
+__device__ __forceinline__ void fp4_epilogue(const NkGemm4Args &a, u32 m0, const u32 (&col)[TJ], const floatx4 (&acc)[TI][TJ]) {
+    const u32 lane = threadIdx.x & 63, m = m0 + (lane & 15), nout = GLU ? a.N / 2 : a.N;
+    constexpr int TO = GLU ? TJ / 2 : TJ;
+    floatx4 b[TJ];
+#pragma unroll
+    for (int j = 0; j < TJ; ++j) b[j] = fp4_bias4(a, col[j % TO] + 4 * (lane >> 4), nout, j < TO ? 0 : nout);
+#pragma unroll
+    for (int i = 0; i < TI; ++i)
+#pragma unroll
+        for (int j = 0; j < TO; ++j)
+            fp4_store4<GLU>(a, m + 16 * i, col[j] + 4 * (lane >> 4), nout, acc[i][j] + b[j], acc[i][j + (GLU ? TO : 0)] + b[j + (GLU ? TO : 0)]);
 }
 
 __device__ __forceinline__ intx8 fp4_op(uint4 q) {
@@ -174,16 +190,229 @@ template <bool GLU> __device__ __forceinline__ void gemm_fp4_impl(const NkGemm4A
 #pragma unroll
             for (int j = 0; j < 2; ++j) acc[i][j] = fp4_mfma(wq[j], we[j], xq[i], xe[i], acc[i][j]);
     }
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        if constexpr (GLU) fp4_store4<true>(a, m0 + 16 * i + r, n0 + 4 * f, acc[i][0], acc[i][1]);
-        else
-#pragma unroll
-            for (int j = 0; j < 2; ++j) fp4_store4<false>(a, m0 + 16 * i + r, n0 + 16 * j + 4 * f, acc[i][j], acc[i][j]);
-    }
+    const u32 col[2] = { n0, n0 + (GLU ? 0 : 16) };
+    fp4_epilogue<GLU, 2, 2>(a, m0, col, acc);
 }
 extern "C" __global__ __launch_bounds__(256) void gemm_fp4(const NkGemm4Args a) { gemm_fp4_impl<false>(a); }
 extern "C" __global__ __launch_bounds__(256) void gemm_fp4_glu(const NkGemm4Args a) { gemm_fp4_impl<true>(a); }
+
+/* 16 bytes per lane from global memory at base + off into LDS bytes [lds + 16 i, +16), as dma16 */
+__device__ __forceinline__ void dma16_at(const unsigned char *base, u32 off, lds_char_t *lds) {
+    const u32 m = __builtin_amdgcn_readfirstlane((u32)(size_t)lds);
+    asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(m) : "memory");
+}
+__device__ __forceinline__ const unsigned char *uniform_ptr(const unsigned char *p) {
+    const u32 lo = __builtin_amdgcn_readfirstlane((u32)(u64)p), hi = __builtin_amdgcn_readfirstlane((u32)((u64)p >> 32));
+    return (const unsigned char *)((u64)hi << 32 | lo);
+}
+
+/* the same of 32 weight rows and 32 rows over 64 values: lane l holds the 32 codes of block l / 32 of row l % 32; the
+ * scales are in bytes B */
+template <int B> __device__ __forceinline__ floatx16 fp4_mfma32(uint4 w, u32 ws, uint4 x, u32 xs, floatx16 acc) {
+    return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(fp4_op(w), fp4_op(x), acc, 4, 4, B, (int)ws, B, (int)xs);
+}
+template <int V> struct const_t { static constexpr int v = V; };
+
+/* The product by tiles of BM x BN outputs (K > 384), WGM x WGN wavefronts with (BM / WGM) x (BN / WGN) each and PW that
+ * only load (a wavefront that issues a direct load is held for 70 to 120 cycles), on the 32 x 32 MFMA: from registers
+ * it reaches 9.2 PFLOP/s (7.1 on random codes), the 16 x 16 one 4.8.
+ *
+ * A K step is 256 values, four MFMA groups: whole 128-byte lines of every row.  A ring of NS stages in LDS is filled
+ * by direct loads.  A load takes 8 rows, 8 lanes a row (with the rows side by side over the lanes each lane is a line of
+ * its own: 139 us for 3584 x 4096 x 8192 on 128 x 128 tiles where this took 88); granule g of row r lies in slot
+ * g ^ (r / 2 % 8), so a fragment read (one granule of 32 rows per half of the wavefront) is free of bank conflicts.
+ * Scales come by 16 bytes of a row for two steps, and are read by 8 for one (a byte per fragment: 88 us, 74 with
+ * no scales at all).
+ *
+ * Bound by the loads from L2 at many rows: 2048 x 4096 x 8192 38.4 us (3.6 PFLOP/s; its products alone 15, with the
+ * fragment reads 29), 3584 x 4096 x 8192 74 to 80; tiles of 128 x 128, 256 x 128 and 256 x 256 in other splits over
+ * wavefronts took 80 to 110. */
+template <int BM, int BN, int WGM, int WGN, int PW, int NS, bool GLU>
+__device__ __forceinline__ void gemm_fp4_tile(const NkGemm4Args &a, lds_char_t *const smem) {
+    constexpr int NW = PW, WTM = BM / WGM, WTN = BN / WGN, TI = WTM / 32, TJ = WTN / 32;
+    constexpr u32 ROWS = BM + BN, STAGE = ROWS * 128, SCALES = NS * STAGE, CHUNK = ROWS * 16;
+    constexpr int NC = NS / 2 + 1;                     /* chunks of scales: a stage's and those ahead of it */
+    constexpr int LI = ROWS / 8 / NW;                  /* loads of codes per wavefront and stage */
+    constexpr int LS = (ROWS / 64 + NW - 1) / NW;      /* loads of scales, of 64 rows of one operand (the last may repeat one) */
+    static_assert(LI * NW * 8 == ROWS && BM % 64 == 0 && (GLU ? BN / 2 : BN) % 64 == 0 && NS >= 2 && (NS - 1) * (LI + LS) < 64, "tile shape");
+    const u32 tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const bool loader = wave >= WGM * WGN;
+    const u32 wv = loader ? wave - WGM * WGN : wave, wm = wv / WGN, wn = wv % WGN, r = lane & 31, f = lane >> 5;
+    const u32 nout = GLU ? a.N / 2 : a.N, G = (a.K + 127) / 128, S = (G + 1) / 2;
+    constexpr u32 CO = GLU ? BN / 2 : BN; /* output columns of a tile */
+    const u32 tm = (a.M + BM - 1) / BM, tn = (nout + CO - 1) / CO;
+    /* workgroup b runs on XCD b % 8: each XCD takes a run of tiles, by groups of 8 row tiles */
+    const u32 per = gridDim.x / 8, t = (blockIdx.x % 8) * per + blockIdx.x / 8;
+    if (t >= tm * tn) return;
+    const u32 grp = t / (8 * tn), in = t - grp * 8 * tn, gh = min(tm - grp * 8, 8u);
+    const u32 m0 = (grp * 8 + in % gh) * BM, c0 = in / gh * CO;
+
+    /* At the barrier of step q the loaders have stage q behind them and the others their reads of stage q - 1: the
+     * latter's place takes stage q + NS - 1. */
+    if (loader) {
+        /* Sources as a uniform base and a lane's offset in the load (strides are below 2^24 bytes).  The rows of a load
+         * are of one operand; GLU: the second half of the tile's weight rows are the gates'.  Rows past the end repeat
+         * the last. */
+        const unsigned char *base[LI], *sbase[LS];
+        u32 last[LI], ld[LI], slast[LS], sld[LS]; /* uniform: the last row behind the base, the stride */
+        auto place = [&](u32 q, bool scales, const unsigned char *&b, u32 &end, u32 &stride) {
+            /* q: first row of the load in the stage */
+            const u32 lda = scales ? a.ldas : a.lda, ldw = scales ? a.ldws : a.ldw;
+            if (q < BM) {
+                const u32 m = min(m0 + q, a.M - 1);
+                b = uniform_ptr((scales ? a.As : a.Aq) + (u64)m * lda);
+                end = a.M - 1 - m;
+                stride = lda;
+            } else {
+                const u32 n = q - BM, gate = GLU && n >= CO, c = min(c0 + n - (gate ? CO : 0), nout - 1);
+                b = uniform_ptr((scales ? a.Ws : a.Wq) + (u64)(c + (gate ? nout : 0)) * ldw);
+                end = nout - 1 - c;
+                stride = ldw;
+            }
+        };
+#pragma unroll
+        for (int j = 0; j < LI; ++j) place((NW * j + wv) * 8, false, base[j], last[j], ld[j]);
+#pragma unroll
+        for (int j = 0; j < LS; ++j) place((NW * j + wv) % (ROWS / 64) * 64, true, sbase[j], slast[j], sld[j]);
+        static_assert(NW % 2 == 0, "the swizzle of a wavefront's loads is the same");
+        const u32 row = lane >> 3, gran = (lane & 7) ^ swz_h(wv * 8 + row);
+        u32 slot = 0, chunk = 0; /* places of the stage and of the scales that are loaded next */
+        auto issue = [&](u32 q) {
+            const u32 g = ((G & 1) && q + 1 == S ? gran & 3 : gran) * 16; /* the last lines may have no second half */
+#pragma unroll
+            for (int j = 0; j < LI; ++j) {
+                dma16_at(base[j], __umul24(min(row, last[j]), ld[j]) + g, smem + slot + (NW * j + wv) * 1024);
+                base[j] += 128;
+            }
+            slot = slot + STAGE == NS * STAGE ? 0 : slot + STAGE;
+            if (q & 1) return;
+#pragma unroll
+            for (int j = 0; j < LS; ++j) /* groups 2 q .. 2 q + 3 of 128, or the row's last four */
+                dma16_at(sbase[j] + 4 * min(2 * q, G - 4), __umul24(min(lane, slast[j]), sld[j]),
+                         smem + SCALES + chunk * CHUNK + (NW * j + wv) % (ROWS / 64) * 1024);
+            chunk = chunk + 1 == NC ? 0 : chunk + 1;
+        };
+        for (u32 u = 0; u < min(S, (u32)NS - 1); ++u) issue(u);
+        for (u32 q = 0; q < S; ++q) {
+            wait_steps<NS - 2, LI>(min(S, q + NS - 1) - q - 1);
+            barrier_mem();
+            if (q + NS - 1 < S) issue(q + NS - 1);
+        }
+        return;
+    }
+    typedef const __attribute__((address_space(3))) uint4 *lds4;
+    typedef const __attribute__((address_space(3))) uint2 *lds2;
+    uint4 x[TI], w[TJ];
+    uint2 xs[TI], ws[TJ]; /* a step's eight scales of the lane's row, its own in bytes 0 and 2 of each half */
+    /* the lane's places in a stage, the tiles' at constant distances: codes and scales of A, and of W */
+    const u32 n0 = GLU ? wn * WTN / 2 : wn * WTN, sw = swz_h(r);
+    u32 lo[4]; /* granule 2 h + f of row r */
+#pragma unroll
+    for (u32 h = 0; h < 4; ++h) lo[h] = r * 128 + ((2 * h + f) ^ sw) * 16;
+    const u32 ox = wm * WTM * 128, oxs = (wm * WTM + r) * 16, ow = (BM + n0) * 128, ows = (BM + n0 + r) * 16;
+    auto scales = [&](const lds_char_t *p) {
+        const uint2 v = *(lds2)p;
+        return make_uint2(v.x >> (8 * f), v.y >> (8 * f));
+    };
+    auto read_w = [&](const lds_char_t *p, const lds_char_t *ps, bool fresh) {
+#pragma unroll
+        for (int j = 0; j < TJ; ++j) {
+            /* GLU: the first half of a wavefront's tiles are value columns, the second their gates */
+            const u32 n = GLU && j >= TJ / 2 ? BN / 2 + 32 * (j - TJ / 2) : 32 * j;
+            w[j] = *(lds4)(p + n * 128);
+            if (fresh) ws[j] = scales(ps + n * 16);
+        }
+    };
+    auto read_x = [&](int i, const lds_char_t *p, const lds_char_t *ps, bool fresh) {
+        x[i] = *(lds4)(p + i * 4096);
+        if (fresh) xs[i] = scales(ps + i * 512);
+    };
+    floatx16 acc[TI][TJ] = {};
+    auto mma = [&](int i, auto group) {
+        constexpr int H = decltype(group)::v;
+#pragma unroll
+        for (int j = 0; j < TJ; ++j)
+            acc[i][j] = fp4_mfma32<2 * (H & 1)>(w[j], H < 2 ? ws[j].x : ws[j].y, x[i], H < 2 ? xs[i].x : xs[i].y, acc[i][j]);
+    };
+    const lds_char_t *st, *ss; /* codes and scales of the stage entered last */
+    /* the products of the group before the stage's group H, each row tile's fragment replaced by that group's as soon
+     * as it is used, the weights' behind them */
+    auto group = [&](auto next, bool whole = true) {
+        constexpr int H = decltype(next)::v;
+        const lds_char_t *p = st + ox + lo[H], *ps = ss + oxs;
+#pragma unroll
+        for (int i = 0; i < TI; ++i) {
+            mma(i, const_t<(H + 3) % 4>());
+            __builtin_amdgcn_sched_barrier(0); /* else the reads move up, into registers that are not there */
+            read_x(i, p, ps, H == 0);
+            if (!whole) x[i] = make_uint4(0, 0, 0, 0);
+        }
+        read_w(st + ow + lo[H], ss + ows, H == 0);
+    };
+    auto rest = [&] {
+        group(const_t<1>());
+        group(const_t<2>());
+        group(const_t<3>());
+    };
+    u32 cur = 0, chunk = 0;
+    auto enter = [&](u32 q) {
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        barrier_mem();
+        st = smem + cur;
+        ss = smem + SCALES + chunk * CHUNK + 4 * (2 * q - min(2 * (q & ~1u), G - 4));
+        cur = cur + STAGE == NS * STAGE ? 0 : cur + STAGE;
+        chunk = !(q & 1) ? chunk : chunk + 1 == NC ? 0 : chunk + 1;
+    };
+    enter(0);
+    read_w(st + ow + lo[0], ss + ows, true);
+#pragma unroll
+    for (int i = 0; i < TI; ++i) read_x(i, st + ox + lo[0], ss + oxs, true);
+    for (u32 q = 1; q < S; ++q) {
+        rest();
+        enter(q);
+        group(const_t<0>());
+    }
+    /* the last step, whose second half may not exist: zeros then, under scales of one */
+    const bool whole = !(G & 1);
+    group(const_t<1>());
+#pragma unroll
+    for (int i = 0; i < TI; ++i) xs[i].y = whole ? xs[i].y : 0x007f007f;
+#pragma unroll
+    for (int j = 0; j < TJ; ++j) ws[j].y = whole ? ws[j].y : 0x007f007f;
+    group(const_t<2>(), whole);
+    group(const_t<3>(), whole);
+#pragma unroll
+    for (int i = 0; i < TI; ++i) mma(i, const_t<3>());
+    /* lane l holds row 32 i + l % 32, columns 32 j + 8 q + 4 (l / 32) .. + 3 in its elements 4 q .. */
+    constexpr int TO = GLU ? TJ / 2 : TJ;
+#pragma unroll
+    for (int j = 0; j < TO; ++j)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const u32 n = c0 + n0 + 32 * j + 8 * q + 4 * f;
+            const floatx4 b = fp4_bias4(a, n, nout, 0), d = GLU ? fp4_bias4(a, n, nout, nout) : b;
+#pragma unroll
+            for (int i = 0; i < TI; ++i) {
+                floatx4 v, t;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    v[e] = acc[i][j][4 * q + e] + b[e];
+                    t[e] = acc[i][j + (GLU ? TO : 0)][4 * q + e] + d[e];
+                }
+                fp4_store4<GLU>(a, m0 + wm * WTM + 32 * i + r, n, nout, v, t);
+            }
+        }
+}
+#define FP4_TILE(BM, BN, WGM, WGN, PW, NS, GLU, NAME)                                                          \
+    extern "C" __global__ __launch_bounds__(64 * (WGM * WGN + PW)) void gemm_fp4_##NAME(const NkGemm4Args a) { \
+        __shared__ __attribute__((aligned(1024))) char smem[(BM + BN) * (NS * 128 + (NS / 2 + 1) * 16)];        \
+        gemm_fp4_tile<BM, BN, WGM, WGN, PW, NS, GLU>(a, (lds_char_t *)smem);                                    \
+    }
+FP4_TILE(128, 256, 2, 4, 4, 3, false, 128x256)
+FP4_TILE(128, 256, 2, 4, 4, 3, true, 128x256_glu)
+FP4_TILE(64, 128, 2, 2, 4, 3, false, 64x128)
+FP4_TILE(64, 128, 2, 2, 4, 3, true, 64x128_glu)
+FP4_TILE(64, 64, 2, 2, 4, 3, false, 64x64)
 
 /* f32 rows: A = hi + lo in bf16 (16 significant bits), the weights' values exact in bf16.  Lane group f holds
  * values 32 f .. 32 f + 31 of a group of 128 as in the 4-bit product; MFMA j takes their eighth j, the K order
@@ -229,13 +458,8 @@ template <bool GLU> __device__ __forceinline__ void gemm_w4_impl(const NkGemm4Ar
             }
         }
     }
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        if constexpr (GLU) fp4_store4<true>(a, m0 + 16 * i + r, n0 + 4 * f, acc[i][0], acc[i][1]);
-        else
-#pragma unroll
-            for (int j = 0; j < 2; ++j) fp4_store4<false>(a, m0 + 16 * i + r, n0 + 16 * j + 4 * f, acc[i][j], acc[i][j]);
-    }
+    const u32 col[2] = { n0, n0 + (GLU ? 0 : 16) };
+    fp4_epilogue<GLU, 2, 2>(a, m0, col, acc);
 }
 extern "C" __global__ __launch_bounds__(256) void gemm_w4(const NkGemm4Args a) { gemm_w4_impl<false>(a); }
 extern "C" __global__ __launch_bounds__(256) void gemm_w4_glu(const NkGemm4Args a) { gemm_w4_impl<true>(a); }

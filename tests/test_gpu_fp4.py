@@ -230,6 +230,13 @@ def test_product_epilogues(gpu, kind, m, n, k, act, bias, resid, alpha):
 
 
 @KINDS
+@pytest.mark.parametrize("m,n,k,act", [(2040, 4090, 2180, NONE), (1000, 8190, 2180, GLU)])
+def test_product_widest_tiles(gpu, kind, m, n, k, act):
+    """Enough outputs for the widest tiles, cut off at every side; an odd number of 128 values."""
+    _check(gpu, kind, m, n, k, act, True, act == NONE)
+
+
+@KINDS
 @pytest.mark.parametrize("m,n,k", [(3, 70, 200), (40, 70, 200), (200, 262, 384)])
 @pytest.mark.parametrize("act", [NONE, GLU])
 def test_product_strides_and_room(gpu, kind, m, n, k, act):

@@ -58,9 +58,9 @@ def test_product_refusals(ctx):
         for bad in (dict(a=None), dict(a=P + 4), dict(lda=240 if kind == "fp4" else 508), dict(lda=264 if kind == "fp4" else 514),
                     dict(wq=None), dict(wq=P + 4), dict(ldw=240), dict(ldw=260), dict(ws=None), dict(ws=P + 2), dict(ldws=12),
                     dict(ldws=18), dict(c=None), dict(c=P + 2), dict(bias=P + 1), dict(ldc=63), dict(n=0), dict(n=(1 << 28) + 2, ldc=1 << 29),
-                    dict(act=3, n=63), dict(act=4), dict(act=-1), dict(k=0), dict(m=1 << 23)):
+                    dict(ldw=1 << 24), dict(ldws=1 << 24), dict(act=3, n=63), dict(act=4), dict(act=-1), dict(k=0), dict(m=1 << 23)):
             ctx.refused(call(kind, **bad), "gemm")
-    for bad in (dict(s=None), dict(s=P + 2), dict(lds=12), dict(lds=18)):
+    for bad in (dict(s=None), dict(s=P + 2), dict(lds=12), dict(lds=18), dict(lda=1 << 24), dict(lds=1 << 24)):
         ctx.refused(call("fp4", **bad), "gemm_fp4")
 
 
