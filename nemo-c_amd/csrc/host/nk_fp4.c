@@ -90,7 +90,7 @@ static int product(gpu_t *g, NkGemm4Args *a) {
         return gpu_launch(g, name, a, sizeof *a, (tiles_of(t, a->M, nout, glu) + 7) / 8 * 8, 1, 1, t->threads, 1, 1);
     }
     if (a->M <= (a->A ? 16u : 64u)) {
-        const uint32_t ti = a->M <= 16 ? 16 : a->M <= 32 ? 32 : 64, wide = a->A && !glu && nout > 4096, co = wide ? 32 : 16;
+        const uint32_t ti = a->A && a->M <= 5 ? 5 : a->M <= 16 ? 16 : a->M <= 32 ? 32 : 64, wide = a->A && !glu && nout > 4096, co = wide ? 32 : 16;
         snprintf(name, sizeof name, "gemm_%s_few%u%s", a->A ? "w4" : "fp4", ti, glu ? "_glu" : wide ? "x2" : "");
         return gpu_launch(g, name, a, sizeof *a, (nout + co - 1) / co, 1, 1, 512, 1, 1);
     }

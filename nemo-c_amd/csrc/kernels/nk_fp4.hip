@@ -414,27 +414,19 @@ FP4_TILE(64, 128, 2, 2, 4, 3, false, 64x128)
 FP4_TILE(64, 128, 2, 2, 4, 3, true, 64x128_glu)
 FP4_TILE(64, 64, 2, 2, 4, 3, false, 64x64)
 
-/* 8 f32 values as three bf16 terms each: the upper 16 bits of what is left, so that the terms add up to all 24
- * significant bits (of an infinity the first term is infinite and the others are finite).  Packed in pairs. */
-struct terms { uint4 t[3]; };
-__device__ __forceinline__ terms split3(const float (&v)[8]) {
-    terms o;
-    u32 *p[3] = { (u32 *)&o.t[0], (u32 *)&o.t[1], (u32 *)&o.t[2] };
+/* Two f32 values as three bf16 terms each, packed: the upper 16 bits of what is left, so that the terms add up to all 24
+ * significant bits (of an infinity the first term is infinite and the others are finite) */
+__device__ __forceinline__ void split3(float a, float b, u32 (&t)[3]) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-        float a = v[2 * e], b = v[2 * e + 1];
-#pragma unroll
-        for (int k = 0; k < 3; ++k) {
-            p[k][e] = __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302);
-            a -= __uint_as_float(__float_as_uint(a) & 0xffff0000u);
-            b -= __uint_as_float(__float_as_uint(b) & 0xffff0000u);
-            if (k == 0) {
-                a = __builtin_amdgcn_fmed3f(a, -1.32922800e36f, 1.32922800e36f);
-                b = __builtin_amdgcn_fmed3f(b, -1.32922800e36f, 1.32922800e36f);
-            }
+    for (int k = 0; k < 3; ++k) {
+        t[k] = __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302);
+        a -= __uint_as_float(__float_as_uint(a) & 0xffff0000u);
+        b -= __uint_as_float(__float_as_uint(b) & 0xffff0000u);
+        if (k == 0) {
+            a = __builtin_amdgcn_fmed3f(a, -1.32922800e36f, 1.32922800e36f);
+            b = __builtin_amdgcn_fmed3f(b, -1.32922800e36f, 1.32922800e36f);
         }
     }
-    return o;
 }
 /* 8 codes as bf16 values, exact */
 __device__ __forceinline__ uint4 fp4_bf16x8(u32 q, float f) {
@@ -442,18 +434,41 @@ __device__ __forceinline__ uint4 fp4_bf16x8(u32 q, float f) {
 }
 
 #define FEW_WAVES 8
+/* The sums of a workgroup's wavefronts, added in their order, and the epilogue.  TERMS 3: the rows 5 k + m of a tile are
+ * the k-th terms of row m. */
+template <int TI, int TJ, bool GLU, int TERMS>
+__device__ __forceinline__ void few_out(const NkGemm4Args &a, floatx4 (*part)[TI * TJ][64], u32 n0, const floatx4 (&acc)[TI][TJ]) {
+    constexpr int TO = GLU ? TJ / 2 : TJ;
+    const u32 lane = threadIdx.x & 63, wv = threadIdx.x >> 6, r = lane & 15, f = lane >> 4, nout = GLU ? a.N / 2 : a.N;
+#pragma unroll
+    for (int i = 0; i < TI; ++i)
+#pragma unroll
+        for (int j = 0; j < TJ; ++j) part[wv][i * TJ + j][lane] = acc[i][j];
+    __syncthreads();
+    for (u32 t = wv; t < TI * TO; t += FEW_WAVES) {
+        const u32 i = t / TO, j = t % TO, n = n0 + 16 * j + 4 * f;
+        auto sum = [&](u32 tile) {
+            floatx4 s = { 0.f, 0.f, 0.f, 0.f };
+#pragma unroll
+            for (int k = 0; k < TERMS; ++k)
+#pragma unroll
+                for (int v = 0; v < FEW_WAVES; ++v) s += part[v][tile][TERMS == 1 ? lane : 16 * f + min(r, 5u) + 5 * k];
+            return s;
+        };
+        const floatx4 s = sum(i * TJ + j), d = GLU ? sum(i * TJ + j + TO) : s;
+        fp4_store4<GLU>(a, 16 * i + r, n, nout, s + fp4_bias4(a, n, nout, 0), GLU ? d + fp4_bias4(a, n, nout, nout) : s);
+    }
+}
+
 /* Few rows: the weights are streamed once and everything else is small.  A workgroup takes 16 TO output columns; its
  * wavefronts take every eighth group of 128 values each, fragments straight from global memory into registers,
- * and their sums meet in LDS, in wavefront order.  Lane l of a fragment holds the 32 codes of block l / 16 of row
- * l % 16.  F32: f32 rows as three bf16 terms against the weights' values in bf16, MFMA s of a group taking every
- * block's eighth s; the K order is the same on both sides. */
-template <bool F32, int TI, int TJ, bool GLU> __device__ __forceinline__ void gemm4_few(const NkGemm4Args &a) {
+ * and their sums meet in LDS.  Lane l of a fragment holds the 32 codes of block l / 16 of row l % 16. */
+template <int TI, int TJ, bool GLU> __device__ __forceinline__ void fp4_few(const NkGemm4Args &a) {
     constexpr int TO = GLU ? TJ / 2 : TJ;
     __shared__ floatx4 part[FEW_WAVES][TI * TJ][64];
     const u32 lane = threadIdx.x & 63, wv = threadIdx.x >> 6, r = lane & 15, f = lane >> 4;
     const u32 nout = GLU ? a.N / 2 : a.N, G = (a.K + 127) / 128, n0 = blockIdx.x * 16 * TO;
     const unsigned char *w[TJ], *ws[TJ], *x[TI], *xs[TI];
-    const float *xf[TI];
 #pragma unroll
     for (int j = 0; j < TJ; ++j) {
         const u32 n = min(n0 + 16 * (j % TO) + r, nout - 1) + (j < TO ? 0 : nout);
@@ -463,14 +478,11 @@ template <bool F32, int TI, int TJ, bool GLU> __device__ __forceinline__ void ge
 #pragma unroll
     for (int i = 0; i < TI; ++i) {
         const u32 m = min(16 * i + r, a.M - 1);
-        if (F32) xf[i] = a.A + (u64)m * a.lda;
-        else {
-            x[i] = a.Aq + (u64)m * a.lda + 16 * f;
-            xs[i] = a.As + (u64)m * a.ldas + f;
-        }
+        x[i] = a.Aq + (u64)m * a.lda + 16 * f;
+        xs[i] = a.As + (u64)m * a.ldas + f;
     }
     floatx4 acc[TI][TJ] = {};
-    constexpr int U = F32 ? 1 : 2; /* groups in flight (the last again past the end, not used) */
+    constexpr int U = 2; /* groups in flight (the last again past the end, not used) */
     for (u32 g0 = wv; g0 < G; g0 += U * FEW_WAVES) {
         uint4 wq[U][TJ], xq[U][TI];
         u32 we[U][TJ], xe[U][TI];
@@ -482,69 +494,117 @@ template <bool F32, int TI, int TJ, bool GLU> __device__ __forceinline__ void ge
                 wq[u][j] = *(const uint4 *)(w[j] + 64 * (u64)g);
                 we[u][j] = ws[j][4 * (u64)g];
             }
-            if (!F32)
 #pragma unroll
-                for (int i = 0; i < TI; ++i) {
-                    xq[u][i] = *(const uint4 *)(x[i] + 64 * (u64)g);
-                    xe[u][i] = xs[i][4 * (u64)g];
-                }
+            for (int i = 0; i < TI; ++i) {
+                xq[u][i] = *(const uint4 *)(x[i] + 64 * (u64)g);
+                xe[u][i] = xs[i][4 * (u64)g];
+            }
         }
-        if constexpr (F32) {
-            float v[TI][4][8];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            if (u && g0 + u * FEW_WAVES >= G) break;
 #pragma unroll
             for (int i = 0; i < TI; ++i)
 #pragma unroll
-                for (int s = 0; s < 4; ++s) fp4_load8(v[i][s], xf[i], 128 * g0 + 32 * f + 8 * s, a.K, true);
-#pragma unroll
-            for (int s = 0; s < 4; ++s) {
-                uint4 b[TJ];
-#pragma unroll
-                for (int j = 0; j < TJ; ++j) {
-                    const u32 q[4] = { wq[0][j].x, wq[0][j].y, wq[0][j].z, wq[0][j].w };
-                    b[j] = fp4_bf16x8(q[s], fp4_scale(we[0][j]));
-                }
-#pragma unroll
-                for (int i = 0; i < TI; ++i) {
-                    const terms t = split3(v[i][s]);
-#pragma unroll
-                    for (int k = 0; k < 3; ++k)
-#pragma unroll
-                        for (int j = 0; j < TJ; ++j) acc[i][j] = mfma_bf16(b[j], t.t[k], acc[i][j]);
-                }
-            }
-        } else {
-#pragma unroll
-            for (int u = 0; u < U; ++u) {
-                if (u && g0 + u * FEW_WAVES >= G) break;
-#pragma unroll
-                for (int i = 0; i < TI; ++i)
-#pragma unroll
-                    for (int j = 0; j < TJ; ++j) acc[i][j] = fp4_mfma(wq[u][j], we[u][j], xq[u][i], xe[u][i], acc[i][j]);
-            }
+                for (int j = 0; j < TJ; ++j) acc[i][j] = fp4_mfma(wq[u][j], we[u][j], xq[u][i], xe[u][i], acc[i][j]);
         }
     }
-#pragma unroll
-    for (int i = 0; i < TI; ++i)
-#pragma unroll
-        for (int j = 0; j < TJ; ++j) part[wv][i * TJ + j][lane] = acc[i][j];
-    __syncthreads();
-    for (u32 t = wv; t < TI * TO; t += FEW_WAVES) {
-        const u32 i = t / TO, j = t % TO, n = n0 + 16 * j + 4 * f;
-        floatx4 s = part[0][i * TJ + j][lane], d = GLU ? part[0][i * TJ + j + TO][lane] : s;
-#pragma unroll
-        for (int k = 1; k < FEW_WAVES; ++k) {
-            s += part[k][i * TJ + j][lane];
-            if (GLU) d += part[k][i * TJ + j + TO][lane];
-        }
-        fp4_store4<GLU>(a, 16 * i + r, n, nout, s + fp4_bias4(a, n, nout, 0), GLU ? d + fp4_bias4(a, n, nout, nout) : s);
-    }
+    few_out<TI, TJ, GLU, 1>(a, part, n0, acc);
 }
-#define FEW4(NAME, F32, TI, TJ, GLU) \
-    extern "C" __global__ __launch_bounds__(64 * FEW_WAVES) void gemm_##NAME(const NkGemm4Args a) { gemm4_few<F32, TI, TJ, GLU>(a); }
-FEW4(fp4_few16, false, 1, 1, false) FEW4(fp4_few16_glu, false, 1, 2, true)
-FEW4(fp4_few32, false, 2, 1, false) FEW4(fp4_few32_glu, false, 2, 2, true)
-FEW4(fp4_few64, false, 4, 1, false) FEW4(fp4_few64_glu, false, 4, 2, true)
-FEW4(w4_few16, true, 1, 1, false) FEW4(w4_few16x2, true, 1, 2, false) FEW4(w4_few16_glu, true, 1, 2, true)
+
+/* The same with f32 rows, as three bf16 terms against the weights' values in bf16: MFMA s of a group of 128 takes every
+ * block's eighth s, the K order being the same on both sides.  The rows of a group are read whole (32 lanes a
+ * row), split, and put into the wavefront's part of LDS as fragments (read as fragments from global memory each lane is a
+ * line of its own, and all 16 rows of a fragment are split: 8192 x 2048 of one row 6.2 us against XX).
+ * PACK: at most five rows, whose terms lie in rows m, 5 + m and 10 + m of one fragment. */
+template <int TJ, bool GLU, bool PACK> __device__ __forceinline__ void w4_few(const NkGemm4Args &a) {
+    constexpr int TO = GLU ? TJ / 2 : TJ, T = PACK ? 1 : 3, RL = PACK ? 3 : 8; /* fragments; loads of two rows */
+    constexpr u32 ROWS = FEW_WAVES * T * 4096, PART = FEW_WAVES * TJ * 1024;
+    __shared__ __attribute__((aligned(16))) char mem[ROWS > PART ? ROWS : PART];
+    const u32 lane = threadIdx.x & 63, wv = threadIdx.x >> 6, r = lane & 15, f = lane >> 4;
+    const u32 nout = GLU ? a.N / 2 : a.N, G = (a.K + 127) / 128, n0 = blockIdx.x * 16 * TO;
+    char *frag = mem + wv * T * 4096; /* granule g (8 values) of row r in slot g ^ r */
+    const unsigned char *w[TJ], *ws[TJ];
+#pragma unroll
+    for (int j = 0; j < TJ; ++j) {
+        const u32 n = min(n0 + 16 * (j % TO) + r, nout - 1) + (j < TO ? 0 : nout);
+        w[j] = a.Wq + (u64)n * a.ldw + 16 * f;
+        ws[j] = a.Ws + (u64)n * a.ldws + f;
+    }
+    uint4 wq[TJ];
+    u32 we[TJ];
+    floatx4 x[RL];
+    const u32 i4 = lane & 31, half = lane >> 5;
+    auto load = [&](u32 g) { /* a group; rows past the end repeat the last, their products are not stored */
+#pragma unroll
+        for (int j = 0; j < TJ; ++j) {
+            wq[j] = *(const uint4 *)(w[j] + 64 * (u64)g);
+            we[j] = ws[j][4 * (u64)g];
+        }
+        const u32 k = 128 * g + 4 * i4;
+#pragma unroll
+        for (int l = 0; l < RL; ++l) {
+            if (2 * (u32)l >= a.M) break;
+            const float *row = a.A + (u64)min(2 * l + half, a.M - 1) * a.lda;
+            if (k + 4 <= a.K) x[l] = *(const floatx4 *)(row + k);
+            else
+#pragma unroll
+                for (int e = 0; e < 4; ++e) x[l][e] = k + e < a.K ? row[k + e] : 0.0f;
+        }
+    };
+    if (wv < G) load(wv);
+    /* rows that no load writes: zeros (their products are not stored, or belong to no row) */
+    for (u32 o = lane * 16; o < T * 4096; o += 1024) *(uint4 *)(frag + o) = make_uint4(0, 0, 0, 0);
+    floatx4 acc[1][TJ] = {};
+    for (u32 g = wv; g < G; g += FEW_WAVES) {
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int l = 0; l < RL; ++l) {
+            if (2 * (u32)l >= a.M) break;
+            u32 p[3], q[3];
+            split3(x[l][0], x[l][1], p);
+            split3(x[l][2], x[l][3], q);
+            const u32 m = 2 * l + half;
+#pragma unroll
+            for (int k = 0; k < 3; ++k) {
+                const u32 row = PACK ? min(m, 5u) + 5 * k : m; /* PACK: row 5 of a load overwrites nothing it should not */
+                if (!PACK || m < 5) *(uint2 *)(frag + (PACK ? 0 : k * 4096) + row * 256 + ((i4 / 2) ^ row) * 16 + (i4 & 1) * 8) = make_uint2(p[k], q[k]);
+            }
+        }
+        uint4 b[TJ];
+        u32 q[TJ][4];
+        float s[TJ];
+#pragma unroll
+        for (int j = 0; j < TJ; ++j) {
+            q[j][0] = wq[j].x; q[j][1] = wq[j].y; q[j][2] = wq[j].z; q[j][3] = wq[j].w;
+            s[j] = fp4_scale(we[j]);
+        }
+        if (g + FEW_WAVES < G) load(g + FEW_WAVES);
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+#pragma unroll
+            for (int j = 0; j < TJ; ++j) b[j] = fp4_bf16x8(q[j][e], s[j]);
+#pragma unroll
+            for (int k = 0; k < T; ++k) {
+                const uint4 v = *(const uint4 *)(frag + k * 4096 + r * 256 + ((4 * f + e) ^ r) * 16);
+#pragma unroll
+                for (int j = 0; j < TJ; ++j) acc[0][j] = mfma_bf16(b[j], v, acc[0][j]);
+            }
+        }
+    }
+    __syncthreads(); /* the sums take the fragments' place */
+    few_out<1, TJ, GLU, PACK ? 3 : 1>(a, (floatx4(*)[TJ][64])mem, n0, acc);
+}
+#define FP4_FEW(NAME, TI, TJ, GLU) \
+    extern "C" __global__ __launch_bounds__(64 * FEW_WAVES) void gemm_fp4_##NAME(const NkGemm4Args a) { fp4_few<TI, TJ, GLU>(a); }
+#define W4_FEW(NAME, TJ, GLU, PACK) \
+    extern "C" __global__ __launch_bounds__(64 * FEW_WAVES) void gemm_w4_##NAME(const NkGemm4Args a) { w4_few<TJ, GLU, PACK>(a); }
+FP4_FEW(few16, 1, 1, false) FP4_FEW(few16_glu, 1, 2, true)
+FP4_FEW(few32, 2, 1, false) FP4_FEW(few32_glu, 2, 2, true)
+FP4_FEW(few64, 4, 1, false) FP4_FEW(few64_glu, 4, 2, true)
+W4_FEW(few5, 1, false, true) W4_FEW(few5x2, 2, false, true) W4_FEW(few5_glu, 2, true, true)
+W4_FEW(few16, 1, false, false) W4_FEW(few16x2, 2, false, false) W4_FEW(few16_glu, 2, true, false)
 
 /* f32 rows: A = hi + lo in bf16 (16 significant bits), the weights' values exact in bf16.  Lane group f holds
  * values 32 f .. 32 f + 31 of a group of 128 as in the 4-bit product; MFMA j takes their eighth j, the K order
