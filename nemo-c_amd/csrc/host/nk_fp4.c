@@ -42,29 +42,40 @@ int nk_fp4_dequant(gpu_t *g, const uint8_t *Q, uint32_t ldq, const uint8_t *S, u
     return convert(g, "fp4_dequant", X, type, ldx, (uint8_t *)Q, ldq, (uint8_t *)S, lds, M, K);
 }
 
-/* The tiles of the many-row 4-bit product.  A launch runs in rounds of `slots` workgroups; a round takes about fix +
- * step x K steps (256 values) microseconds, step1 when no CU has more than one workgroup (graph replays of
- * 3584 x 4096 x 8192 and x 4096, 2048 x 4096 x 4096, 1024 x 4096 x 2048, 448 x 4096 x 1024, 448 x 1024 x 4096 and
- * 128 x 4096 x 4096: 128x256 80, 50, 28, 16.4, 11.1, 17.6 and 17.9 us, 64x128 102, 60, 36, 14.0, 7.9, 11.0 and
- * 11.3, 64x64 133, 70, 42, 15.3, 7.1, 8.7 and 9.4: the least is picked each time). */
-typedef struct { const char *name; uint16_t bm, bn, threads, slots; float fix, step, step1; } tile_t;
+/* The products' kernels.  With t workgroups on the fullest CU a launch takes about fix microseconds per `percu` of them
+ * and per K step max(lat, thr x t), fitted to graph replays:
+ *   fp4 (steps of 256) 3584 x 4096 x 8192 and x 4096, 2048 x 4096 x 4096, 1024 x 4096 x 2048, 448 x 4096 x 1024,
+ *   448 x 1024 x 4096, 128 x 4096 x 4096: 128x256 80, 50, 28, 16.4, 11.1, 17.6, 17.9 us, 64x128 102, 60, 36, 14.0, 7.9,
+ *   11.0, 11.3, 64x64 133, 70, 42, 15.3, 7.1, 8.7, 9.4: the least is picked each time;
+ *   w4 (steps of 64) 2048 x 4096 x 8192 and x 2048, 1024 x 4096 x 2048, 448 x 4096 x 1024, 448 x 1024 x 4096: 128x256
+ *   316, 87, 73, 38, 118, 64x256 342, 92, 50, 23, 67, 64x128 390, 103, 55, 19, 48, 32x64 565, 143, 76, 23, 31; few rows
+ *   (16 to a workgroup, one launch of them for 17 and more) against 32x64: 32 x 4096 x 1024 9.4 / 10.2, 48 rows 12.9 /
+ *   10.4, 32 x 4096 x 4096 19.5 / 29.8, 64 rows 35.6 / 30.0, 128 x 1024 x 4096 19.5 / 30.2. */
+typedef struct { const char *name; uint16_t bm, bn, threads, percu; float fix, lat, thr; } tile_t;
 static const tile_t fp4_tiles[] = {
-    { "128x256", 128, 256, 768, 256, 10.0f, 1.0f, 1.0f },
-    { "64x128", 64, 128, 512, 512, 4.0f, 0.9f, 0.52f },
-    { "64x64", 64, 64, 512, 768, 3.0f, 0.72f, 0.38f }, /* not with GLU: 64 rows of scales are of one half */
+    { "128x256", 128, 256, 768, 1, 10.0f, 1.0f, 1.0f },
+    { "64x128", 64, 128, 512, 2, 4.0f, 0.52f, 0.45f },
+    { "64x64", 64, 64, 512, 3, 3.0f, 0.38f, 0.24f },
+};
+static const tile_t w4_tiles[] = {
+    { "128x256", 128, 256, 768, 1, 8.0f, 2.3f, 2.3f },
+    { "64x256", 64, 256, 768, 1, 5.0f, 1.35f, 1.34f },
+    { "64x128", 64, 128, 512, 2, 4.5f, 0.65f, 0.76f },
+    { "32x64", 32, 64, 256, 4, 3.0f, 0.43f, 0.29f },
 };
 static uint32_t tiles_of(const tile_t *t, uint32_t M, uint32_t nout, int glu) {
     const uint32_t co = glu ? t->bn / 2u : t->bn;
     return (M + t->bm - 1) / t->bm * ((nout + co - 1) / co);
 }
-static const tile_t *tile_pick(const tile_t *list, int n, uint32_t M, uint32_t nout, uint32_t K, int glu) {
+/* the tile of the least estimate, and that in *us */
+static const tile_t *tile_pick(const tile_t *list, int n, uint32_t M, uint32_t nout, uint32_t steps, int glu, float *us) {
     const tile_t *best = NULL;
-    float least = 0;
     for (const tile_t *t = list; t < list + n; ++t) {
-        if (glu && t->bn < 128) continue;
-        const uint32_t w = tiles_of(t, M, nout, glu), rounds = (w + t->slots - 1) / t->slots;
-        const float us = (float)rounds * (t->fix + (w <= 256 ? t->step1 : t->step) * (float)((K + 255) / 256));
-        if (!best || us < least) { best = t; least = us; }
+        if (glu && t->bn < 128) continue; /* a wavefront holds 32 value and 32 gate columns, a load of scales one half's */
+        const uint32_t w = (tiles_of(t, M, nout, glu) + 255) / 256;
+        const float step = t->thr * (float)w > t->lat ? t->thr * (float)w : t->lat;
+        const float e = (float)((w + t->percu - 1) / t->percu) * t->fix + step * (float)steps;
+        if (!best || e < *us) { best = t; *us = e; }
     }
     return best;
 }
@@ -74,7 +85,7 @@ static int product(gpu_t *g, NkGemm4Args *a) {
     const int glu = a->act == NK_ACT_GLU;
     if (a->act > NK_ACT_GLU) return bad(g, "gemm 4-bit: unknown activation");
     if (!a->N || a->N > 1u << 28 || !a->K || (glu && (a->N & 1))) return bad(g, "gemm 4-bit: bad shape");
-    if (a->M > 65535 * 64) return bad(g, "gemm 4-bit: too many rows");
+    if (a->M > 65535 * 16) return bad(g, "gemm 4-bit: too many rows");
     if (!rows_ok(a->Wq, a->ldw, a->Ws, a->ldws, a->K) || a->ldw >= FP4_STRIDE || a->ldws >= FP4_STRIDE)
         return bad(g, "gemm 4-bit: weight codes 16-byte and scales 4-byte aligned, rows padded to 128 values, strides below 2^24");
     const uint32_t nout = glu ? a->N / 2 : a->N;
@@ -84,18 +95,26 @@ static int product(gpu_t *g, NkGemm4Args *a) {
                           4.0 * a->M * nout * (a->accumulate ? 2 : 1) + (a->bias ? 4.0 * a->N : 0.0));
     gpu_next_flops(g, 2.0 * a->M * a->N * a->K);
     char name[32];
-    if (!a->A && a->M > 64 && a->K > 384) {
-        const tile_t *t = tile_pick(fp4_tiles, 3, a->M, nout, a->K, glu);
-        snprintf(name, sizeof name, "gemm_fp4_%s%s", t->name, glu ? "_glu" : "");
+    const char *kind = a->A ? "w4" : "fp4", *gl = glu ? "_glu" : "";
+    float us = 0;
+    const tile_t *t = NULL;
+    if (a->A) t = tile_pick(w4_tiles, 4, a->M, nout, (a->K + 63) / 64, glu, &us);
+    else if (a->K > 384) t = tile_pick(fp4_tiles, 3, a->M, nout, (a->K + 255) / 256, glu, &us); /* four scales a load */
+    /* few rows: 16 of them and 16 output columns to a workgroup, wide matrices 32 (f32 rows) */
+    const uint32_t wide = a->A && !glu && nout > 4096, co = wide ? 32 : 16, rows = a->A ? (a->M + 15) / 16 : 1;
+    const uint64_t wgs = (uint64_t)rows * ((nout + co - 1) / co);
+    const float few = 1.5f + (float)((wgs + 255) / 256) * (2.0f + (glu || wide ? 0.28f : 0.21f) * (float)((a->K + 127) / 128));
+    if (a->A ? a->M <= 16 || few < us : a->M <= 64) {
+        const uint32_t ti = a->A && a->M <= 5 ? 5 : a->A || a->M <= 16 ? 16 : a->M <= 32 ? 32 : 64;
+        snprintf(name, sizeof name, "gemm_%s_few%u%s", kind, ti, glu ? gl : wide ? "x2" : "");
+        return gpu_launch(g, name, a, sizeof *a, (nout + co - 1) / co, rows, 1, 512, 1, 1);
+    }
+    if (t) {
+        snprintf(name, sizeof name, "gemm_%s_%s%s", kind, t->name, gl);
         return gpu_launch(g, name, a, sizeof *a, (tiles_of(t, a->M, nout, glu) + 7) / 8 * 8, 1, 1, t->threads, 1, 1);
     }
-    if (a->M <= (a->A ? 16u : 64u)) {
-        const uint32_t ti = a->A && a->M <= 5 ? 5 : a->M <= 16 ? 16 : a->M <= 32 ? 32 : 64, wide = a->A && !glu && nout > 4096, co = wide ? 32 : 16;
-        snprintf(name, sizeof name, "gemm_%s_few%u%s", a->A ? "w4" : "fp4", ti, glu ? "_glu" : wide ? "x2" : "");
-        return gpu_launch(g, name, a, sizeof *a, (nout + co - 1) / co, 1, 1, 512, 1, 1);
-    }
     const uint32_t cols = glu ? 32 : 64;
-    snprintf(name, sizeof name, "gemm_%s%s", a->A ? "w4" : "fp4", glu ? "_glu" : "");
+    snprintf(name, sizeof name, "gemm_fp4%s", gl);
     return gpu_launch(g, name, a, sizeof *a, (nout + cols - 1) / cols, (a->M + 63) / 64, 1, 256, 1, 1);
 }
 

@@ -213,6 +213,31 @@ template <int B> __device__ __forceinline__ floatx16 fp4_mfma32(uint4 w, u32 ws,
 }
 template <int V> struct const_t { static constexpr int v = V; };
 
+/* A wavefront's 32 x 32 tiles from row m0 and column c0 on (GLU: the second half of the tiles are gates): lane l holds row
+ * 32 i + l % 32, columns 32 j + 8 q + 4 (l / 32) .. + 3 in its elements 4 q .. */
+template <bool GLU, int TI, int TJ>
+__device__ __forceinline__ void tile_out(const NkGemm4Args &a, u32 m0, u32 c0, const floatx16 (&acc)[TI][TJ]) {
+    constexpr int TO = GLU ? TJ / 2 : TJ;
+    const u32 r = threadIdx.x & 31, f = threadIdx.x >> 5 & 1, nout = GLU ? a.N / 2 : a.N;
+#pragma unroll
+    for (int j = 0; j < TO; ++j)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const u32 n = c0 + 32 * j + 8 * q + 4 * f;
+            const floatx4 b = fp4_bias4(a, n, nout, 0), d = GLU ? fp4_bias4(a, n, nout, nout) : b;
+#pragma unroll
+            for (int i = 0; i < TI; ++i) {
+                floatx4 v, t;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    v[e] = acc[i][j][4 * q + e] + b[e];
+                    t[e] = acc[i][j + (GLU ? TO : 0)][4 * q + e] + d[e];
+                }
+                fp4_store4<GLU>(a, m0 + 32 * i + r, n, nout, v, t);
+            }
+        }
+}
+
 /* The product by tiles of BM x BN outputs (K > 384), WGM x WGN wavefronts with (BM / WGM) x (BN / WGN) each and PW that
  * only load (a wavefront that issues a direct load is held for 70 to 120 cycles), on the 32 x 32 MFMA: from registers
  * it reaches 9.2 PFLOP/s (7.1 on random codes), the 16 x 16 one 4.8.
@@ -383,25 +408,7 @@ __device__ __forceinline__ void gemm_fp4_tile(const NkGemm4Args &a, lds_char_t *
     group(const_t<3>(), whole);
 #pragma unroll
     for (int i = 0; i < TI; ++i) mma(i, const_t<3>());
-    /* lane l holds row 32 i + l % 32, columns 32 j + 8 q + 4 (l / 32) .. + 3 in its elements 4 q .. */
-    constexpr int TO = GLU ? TJ / 2 : TJ;
-#pragma unroll
-    for (int j = 0; j < TO; ++j)
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-            const u32 n = c0 + n0 + 32 * j + 8 * q + 4 * f;
-            const floatx4 b = fp4_bias4(a, n, nout, 0), d = GLU ? fp4_bias4(a, n, nout, nout) : b;
-#pragma unroll
-            for (int i = 0; i < TI; ++i) {
-                floatx4 v, t;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    v[e] = acc[i][j][4 * q + e] + b[e];
-                    t[e] = acc[i][j + (GLU ? TO : 0)][4 * q + e] + d[e];
-                }
-                fp4_store4<GLU>(a, m0 + wm * WTM + 32 * i + r, n, nout, v, t);
-            }
-        }
+    tile_out<GLU, TI, TJ>(a, m0 + wm * WTM, c0 + n0, acc);
 }
 #define FP4_TILE(BM, BN, WGM, WGN, PW, NS, GLU, NAME)                                                          \
     extern "C" __global__ __launch_bounds__(64 * (WGM * WGN + PW)) void gemm_fp4_##NAME(const NkGemm4Args a) { \
@@ -517,7 +524,12 @@ template <int TI, int TJ, bool GLU> __device__ __forceinline__ void fp4_few(cons
  * row), split, and put into the wavefront's part of LDS as fragments (read as fragments from global memory each lane is a
  * line of its own, and all 16 rows of a fragment are split: 8192 x 2048 of one row 6.2 us against XX).
  * PACK: at most five rows, whose terms lie in rows m, 5 + m and 10 + m of one fragment. */
-template <int TJ, bool GLU, bool PACK> __device__ __forceinline__ void w4_few(const NkGemm4Args &a) {
+template <int TJ, bool GLU, bool PACK> __device__ __forceinline__ void w4_few(NkGemm4Args a) {
+    if (!PACK) { /* 16 rows a workgroup */
+        a.A += (u64)blockIdx.y * 16 * a.lda;
+        a.C += (u64)blockIdx.y * 16 * a.ldc;
+        a.M -= blockIdx.y * 16;
+    }
     constexpr int TO = GLU ? TJ / 2 : TJ, T = PACK ? 1 : 3, RL = PACK ? 3 : 8; /* fragments; loads of two rows */
     constexpr u32 ROWS = FEW_WAVES * T * 4096, PART = FEW_WAVES * TJ * 1024;
     __shared__ __attribute__((aligned(16))) char mem[ROWS > PART ? ROWS : PART];
@@ -606,52 +618,157 @@ FP4_FEW(few64, 4, 1, false) FP4_FEW(few64_glu, 4, 2, true)
 W4_FEW(few5, 1, false, true) W4_FEW(few5x2, 2, false, true) W4_FEW(few5_glu, 2, true, true)
 W4_FEW(few16, 1, false, false) W4_FEW(few16x2, 2, false, false) W4_FEW(few16_glu, 2, true, false)
 
-/* f32 rows: A = hi + lo in bf16 (16 significant bits), the weights' values exact in bf16.  Lane group f holds
- * values 32 f .. 32 f + 31 of a group of 128 as in the 4-bit product; MFMA j takes their eighth j, the K order
- * being the same on both sides. */
-template <bool GLU> __device__ __forceinline__ void gemm_w4_impl(const NkGemm4Args &a) {
-    const u32 lane = threadIdx.x & 63, wv = threadIdx.x >> 6, r = lane & 15, f = lane >> 4;
-    const u32 nout = GLU ? a.N / 2 : a.N, G = (a.K + 127) / 128;
-    const u32 m0 = blockIdx.y * 64 + (wv & 1) * 32, n0 = (blockIdx.x * 2 + (wv >> 1)) * (GLU ? 16 : 32);
-    const unsigned char *w[2], *ws[2];
-    const float *x[2];
+/* f32 rows and 4-bit weights by tiles, K steps of 64 values, on the 32 x 32 x 16 bf16 MFMA (2.2 PFLOP/s from
+ * registers, the 16 x 16 one 1.3).  PW wavefronts load: f32 rows come into registers two steps ahead, are split once into
+ * three bf16 planes (24 bits, every product of a term and a weight exact) and put into one of two LDS stages with
+ * the weights' codes and scales, while the others multiply the stage before.  Lane l of a weight fragment holds the 32
+ * codes of block l / 32 of row l % 32, converted in registers; MFMA s of a step takes every block's eighth s, of A
+ * too. */
+template <int BM, int BN, int WGM, int WGN, int PW, int AHEAD, bool GLU>
+__device__ __forceinline__ void gemm_w4_tile(const NkGemm4Args &a, char *const smem) {
+    constexpr int WTM = BM / WGM, WTN = BN / WGN, TI = WTM / 32, TJ = WTN / 32;
+    constexpr u32 PLANE = BM * 128, CODES = 3 * PLANE, SCALES = CODES + BN * 32, STAGE = SCALES + BN * 4;
+    constexpr int LA = BM * 16 / (PW * 64), LW = BN * 2 / (PW * 64), LS = (BN + PW * 64 - 1) / (PW * 64);
+    static_assert(LA * PW * 64 == BM * 16 && LW * PW * 64 == BN * 2 && TI >= 1 && TJ >= (GLU ? 2 : 1), "tile shape");
+    const u32 tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const u32 nout = GLU ? a.N / 2 : a.N, S = (a.K + 63) / 64;
+    constexpr u32 CO = GLU ? BN / 2 : BN; /* output columns of a tile */
+    const u32 tm = (a.M + BM - 1) / BM, tn = (nout + CO - 1) / CO;
+    /* workgroup b runs on XCD b % 8: each XCD takes a run of tiles, by groups of 8 row tiles */
+    const u32 per = gridDim.x / 8, t = (blockIdx.x % 8) * per + blockIdx.x / 8;
+    if (t >= tm * tn) return;
+    const u32 grp = t / (8 * tn), in = t - grp * 8 * tn, gh = min(tm - grp * 8, 8u);
+    const u32 m0 = (grp * 8 + in % gh) * BM, c0 = in / gh * CO;
+
+    if (wave >= WGM * WGN) {
+        const u32 p = (wave - WGM * WGN) * 64 + lane;
+        /* float4 p % 16 of row p / 16, half p % 2 of the codes of weight row p / 2, and PW * 4 or PW * 32 rows on */
+        const float *ar[LA];
+        const unsigned char *wr[LW], *sr[LS];
+        auto wrow = [&](u32 n) { return min(c0 + (GLU && n >= CO ? n - CO : n), nout - 1) + (GLU && n >= CO ? nout : 0); };
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-        const u32 n = GLU ? min(n0 + r, nout - 1) + j * nout : min(n0 + 16 * j + r, nout - 1);
-        w[j] = a.Wq + (u64)n * a.ldw + 16 * f;
-        ws[j] = a.Ws + (u64)n * a.ldws + f;
-        x[j] = a.A + (u64)min(m0 + 16 * j + r, a.M - 1) * a.lda;
+        for (int j = 0; j < LA; ++j) ar[j] = a.A + (u64)min(m0 + p / 16 + j * PW * 4, a.M - 1) * a.lda + p % 16 * 4;
+#pragma unroll
+        for (int j = 0; j < LW; ++j) wr[j] = a.Wq + (u64)wrow(p / 2 + j * PW * 32) * a.ldw + p % 2 * 16;
+#pragma unroll
+        for (int j = 0; j < LS; ++j) sr[j] = a.Ws + (u64)wrow(min(p + j * PW * 64, (u32)BN - 1)) * a.ldws;
+        struct regs { floatx4 x[LA]; uint4 w[LW]; u32 e[LS]; } R[AHEAD];
+        auto load_w = [&](regs &g, u32 q) {
+#pragma unroll
+            for (int j = 0; j < LW; ++j) g.w[j] = *(const uint4 *)(wr[j] + 32 * (u64)q);
+#pragma unroll
+            for (int j = 0; j < LS; ++j) g.e[j] = *(const u32 *)(sr[j] + 4 * (u64)(q / 2));
+        };
+        auto load_whole = [&](regs &g, u32 q) {
+#pragma unroll
+            for (int j = 0; j < LA; ++j) g.x[j] = *(const floatx4 *)(ar[j] + 64 * (u64)q);
+            load_w(g, q);
+        };
+        auto load = [&](regs &g, u32 q) { /* any step, zeros past the rows' ends; none behind the last */
+            if (q >= S) return;
+            if (64 * q + 64 <= a.K) return load_whole(g, q);
+            const u32 k = 64 * q + p % 16 * 4;
+#pragma unroll
+            for (int j = 0; j < LA; ++j)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) g.x[j][i] = k + i < a.K ? ar[j][64 * (u64)q + i] : 0.0f;
+            load_w(g, q);
+        };
+        auto put = [&](const regs &g, u32 q) {
+            char *st = smem + (q & 1) * STAGE;
+#pragma unroll
+            for (int j = 0; j < LA; ++j) {
+                u32 lo[3], hi[3];
+                split3(g.x[j][0], g.x[j][1], lo);
+                split3(g.x[j][2], g.x[j][3], hi);
+                const u32 row = p / 16 + j * PW * 4, i4 = p % 16, at = row * 128 + ((i4 / 2) ^ swz_h(row)) * 16 + (i4 & 1) * 8;
+#pragma unroll
+                for (int k = 0; k < 3; ++k) *(uint2 *)(st + k * PLANE + at) = make_uint2(lo[k], hi[k]);
+            }
+#pragma unroll
+            for (int j = 0; j < LW; ++j) *(uint4 *)(st + CODES + (p + j * PW * 64) * 16) = g.w[j];
+#pragma unroll
+            for (int j = 0; j < LS; ++j) *(u32 *)(st + SCALES + min(p + j * PW * 64, (u32)BN - 1) * 4) = g.e[j];
+        };
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u) load(R[u], u);
+        /* At a barrier stage q is there and stage q - 1 read.  Whole steps without a branch: the compiler waits for all
+         * loads where paths join, not for the oldest step's. */
+        u32 q = 0;
+        for (; 64 * q + 128 * AHEAD <= a.K; q += AHEAD)
+#pragma unroll
+            for (int u = 0; u < AHEAD; ++u) {
+                put(R[u], q + u);
+                load_whole(R[u], q + u + AHEAD);
+                lds_barrier();
+            }
+        for (; q < S; q += AHEAD)
+#pragma unroll
+            for (int u = 0; u < AHEAD; ++u) {
+                if (q + u >= S) break;
+                put(R[u], q + u);
+                load(R[u], q + u + AHEAD);
+                lds_barrier();
+            }
+        return;
     }
-    floatx4 acc[2][2] = {};
-    for (u32 g = 0; g < G; ++g) {
-        u32 wq[2][4];
-        float we[2];
+    const u32 wm = wave / WGN, wn = wave % WGN, r = lane & 31, f = lane >> 5, sw = swz_h(r);
+    const u32 n0 = GLU ? wn * WTN / 2 : wn * WTN;
+    floatx16 acc[TI][TJ] = {};
+    u32 wq[TJ][4];
+    float ws[TJ];
+    uint4 v[2][3][TI];
+    auto read_w = [&](const char *st, u32 q) {
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-            const uint4 q = *(const uint4 *)(w[j] + 64 * (u64)g);
-            wq[j][0] = q.x; wq[j][1] = q.y; wq[j][2] = q.z; wq[j][3] = q.w;
-            we[j] = fp4_scale(ws[j][4 * (u64)g]);
+        for (int j = 0; j < TJ; ++j) {
+            /* GLU: the first half of a wavefront's tiles are value columns, the second their gates */
+            const u32 n = n0 + r + (GLU && j >= TJ / 2 ? BN / 2 + 32 * (j - TJ / 2) : 32 * j);
+            const uint4 c = *(const uint4 *)(st + CODES + n * 32 + f * 16);
+            wq[j][0] = c.x; wq[j][1] = c.y; wq[j][2] = c.z; wq[j][3] = c.w;
+            ws[j] = fp4_scale(*(const u32 *)(st + SCALES + n * 4) >> (16 * (q & 1) + 8 * f) & 255);
         }
+    };
+    auto read_x = [&](const char *st, int s) {
+#pragma unroll
+        for (int k = 0; k < 3; ++k)
+#pragma unroll
+            for (int i = 0; i < TI; ++i)
+                v[s & 1][k][i] = *(const uint4 *)(st + k * PLANE + (wm * WTM + 32 * i + r) * 128 + ((4 * f + s) ^ sw) * 16);
+    };
+    /* the fragments of MFMA s + 1 are read while those of s multiply */
+    for (u32 q = 0; q < S; ++q) {
+        const char *st = smem + (q & 1) * STAGE;
+        lds_barrier();
+        read_w(st, q);
+        read_x(st, 0);
 #pragma unroll
         for (int s = 0; s < 4; ++s) {
-            uint4 b[2];
+            uint4 b[TJ];
 #pragma unroll
-            for (int j = 0; j < 2; ++j)
-                b[j] = make_uint4(fp4_bf16<0>(wq[j][s], we[j]), fp4_bf16<1>(wq[j][s], we[j]), fp4_bf16<2>(wq[j][s], we[j]),
-                                  fp4_bf16<3>(wq[j][s], we[j]));
+            for (int j = 0; j < TJ; ++j) b[j] = fp4_bf16x8(wq[j][s], ws[j]);
+            if (s < 3) read_x(st, s + 1);
+            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                float v[8];
-                uint4 hi, lo;
-                fp4_load8(v, x[i], 128 * g + 32 * f + 8 * s, a.K, true);
-                split8(v, hi, lo);
+            for (int k = 0; k < 3; ++k)
 #pragma unroll
-                for (int j = 0; j < 2; ++j) acc[i][j] = mfma_bf16(b[j], lo, mfma_bf16(b[j], hi, acc[i][j]));
-            }
+                for (int i = 0; i < TI; ++i)
+#pragma unroll
+                    for (int j = 0; j < TJ; ++j)
+                        acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_bf16x8(b[j]), as_bf16x8(v[s & 1][k][i]), acc[i][j], 0, 0, 0);
+            __builtin_amdgcn_sched_barrier(0);
         }
     }
-    const u32 col[2] = { n0, n0 + (GLU ? 0 : 16) };
-    fp4_epilogue<GLU, 2, 2>(a, m0, col, acc);
+    tile_out<GLU, TI, TJ>(a, m0 + wm * WTM, c0 + n0, acc);
 }
-extern "C" __global__ __launch_bounds__(256) void gemm_w4(const NkGemm4Args a) { gemm_w4_impl<false>(a); }
-extern "C" __global__ __launch_bounds__(256) void gemm_w4_glu(const NkGemm4Args a) { gemm_w4_impl<true>(a); }
+#define W4_TILE(BM, BN, WGM, WGN, PW, AHEAD, GLU, NAME)                                                       \
+    extern "C" __global__ __launch_bounds__(64 * (WGM * WGN + PW)) void gemm_w4_##NAME(const NkGemm4Args a) { \
+        __shared__ __attribute__((aligned(1024))) char smem[2 * (BM * 384 + BN * 36)];                        \
+        gemm_w4_tile<BM, BN, WGM, WGN, PW, AHEAD, GLU>(a, smem);                                               \
+    }
+W4_TILE(128, 256, 2, 4, 4, 2, false, 128x256)
+W4_TILE(128, 256, 2, 4, 4, 2, true, 128x256_glu)
+W4_TILE(64, 128, 2, 2, 4, 4, false, 64x128)
+W4_TILE(64, 128, 2, 2, 4, 4, true, 64x128_glu)
+W4_TILE(32, 64, 1, 2, 2, 4, false, 32x64)
+W4_TILE(64, 256, 2, 4, 4, 3, false, 64x256)
+W4_TILE(64, 256, 2, 4, 4, 3, true, 64x256_glu)
