@@ -524,7 +524,7 @@ typedef struct {
     float *state;     /* [slots][taps - 1][D] */
     const int *seqs;
     void *Y;
-    u32 ldx, ldy, slots, nseq, max_rows, M, D, taps, act, vec;
+    u32 ldx, ldy, slots, nseq, max_rows, M, D, taps, act, tile; /* tile: rows of a workgroup */
 } NkCconvArgs;
 
 typedef struct {

@@ -19,57 +19,112 @@ __device__ __forceinline__ void st_row(float *p, float v) { *p = v; }
 /* to bf16, to nearest even; the conversion keeps infinities and NaN */
 __device__ __forceinline__ void st_row(u16 *p, float v) { *p = __builtin_bit_cast(u16, (__bf16)v); }
 
-#define CCONV_ROWS 32 /* rows of a workgroup's tile */
+/* v / (1 + e^-v) to about three steps in 12 instructions (the IEEE exponential and division take 25, a third of what the
+ * convolution does): 2^(-v log2 e) with the product's rounding put back, the hardware's reciprocal.  The exponent is
+ * kept where neither flushes: below -87 the result is off by less than 2e-36. */
+__device__ __forceinline__ float silu_q(float v) {
+    const float n = __builtin_amdgcn_fmed3f(-v, -104.0f, 87.0f), t = n * 1.44269504f;
+    const float r = fmaf(n, 1.92596299e-8f, fmaf(n, 1.44269504f, -t)), e = __builtin_amdgcn_exp2f(t);
+    return v * __builtin_amdgcn_rcpf(1.0f + fmaf(e, r * 0.693147181f, e));
+}
 
-/* One thread per channel and tile of rows, the last inputs in registers: every row is read once (and the
- * taps - 1 before the tile).  The tile with the sequence's first row reads the slot's rows and then
- * writes the new ones: nothing else touches the slots. */
-template <typename T, int TAPS> __device__ __forceinline__ void cconv_impl(const NkCconvArgs &a) {
+/* V values of a row as they lie in memory */
+template <typename T, int V> struct row_t;
+template <> struct row_t<float, 1> { float v; };
+template <> struct row_t<u16, 1> { u16 v; };
+template <> struct row_t<u16, 2> { u32 v; };
+__device__ __forceinline__ void widen(float (&o)[1], row_t<float, 1> r) { o[0] = r.v; }
+__device__ __forceinline__ void widen(float (&o)[1], row_t<u16, 1> r) { o[0] = bf2f(r.v); }
+__device__ __forceinline__ void widen(float (&o)[2], row_t<u16, 2> r) {
+    o[0] = bf_lo(r.v);
+    o[1] = bf_hi(r.v);
+}
+template <typename T> __device__ __forceinline__ void store_row(T *p, const float (&v)[1]) { st_row(p, v[0]); }
+__device__ __forceinline__ void store_row(u16 *p, const float (&v)[2]) {
+    *(u32 *)p = __builtin_bit_cast(u32, __builtin_convertvector((floatx2){ v[0], v[1] }, bf16x2));
+}
+
+/* One thread per channel (bf16: two where rows allow it) and tile of a.tile rows, the last inputs in registers and eight
+ * rows' loads in flight: every row is read once (and the taps - 1 before the tile).  Bound by memory: 8192 rows of
+ * 2048 channels f32 30 us, bf16 16.  More channels per thread are slower (16 bytes each: 37 and 29 us), their taps being far
+ * apart and their threads few.  The tile with the sequence's first row reads the slot's rows and then writes the new
+ * ones: nothing else touches the slots. */
+template <typename T, int TAPS, int V> __device__ __forceinline__ void cconv_impl(const NkCconvArgs &a) {
     const seq_t s = seq_load(a.seqs, blockIdx.z, a.M, a.max_rows, a.slots);
-    const u32 d = blockIdx.x * 256 + threadIdx.x, t0 = blockIdx.y * CCONV_ROWS;
+    const u32 d = (blockIdx.x * 256 + threadIdx.x) * V, t0 = blockIdx.y * a.tile;
     if (!s.ok || d >= a.D || (t0 && t0 >= s.rows)) return;
-    const T *x = (const T *)a.X + (u64)s.first * a.ldx + d;
-    T *y = (T *)a.Y + (u64)s.first * a.ldy + d;
-    float w[TAPS], v[TAPS];
+    typedef row_t<T, V> row;
+    const T *x = (const T *)a.X + (u64)s.first * a.ldx;
+    T *y = (T *)a.Y + (u64)s.first * a.ldy;
+    const u32 end = min(t0 + a.tile, s.rows);
+    auto load = [&](u32 t) { return *(const row *)(x + (u64)t * a.ldx + d); };
+    constexpr int B = 8; /* rows in flight (the tile's last again past its end, not used) */
+    row q[B];
+    if (t0 < end)
 #pragma unroll
-    for (int j = 0; j < TAPS; ++j) w[j] = a.W[(u64)d * TAPS + j];
-    const float b = a.bias ? a.bias[d] : 0.0f;
+        for (u32 k = 0; k < B; ++k) q[k] = load(min(t0 + k, end - 1));
+    float w[TAPS][V], b[V], v[TAPS - 1 + B][V]; /* v: the inputs before a batch of B rows, then its own */
 #pragma unroll
-    for (int j = 0; j < TAPS - 1; ++j) {
-        if (t0) v[j] = ld_row(x + (u64)(t0 + j - (TAPS - 1)) * a.ldx);
-        else v[j] = s.from < 0 ? 0.0f : a.state[((u64)s.from * (TAPS - 1) + j) * a.D + d];
-    }
+    for (int j = 0; j < TAPS; ++j)
+#pragma unroll
+        for (int e = 0; e < V; ++e) w[j][e] = a.W[(u64)(d + e) * TAPS + j];
+#pragma unroll
+    for (int e = 0; e < V; ++e) b[e] = a.bias ? a.bias[d + e] : 0.0f;
+    if (t0)
+#pragma unroll
+        for (int j = 0; j < TAPS - 1; ++j) widen(v[j], load(t0 + j - (TAPS - 1)));
+    else
+#pragma unroll
+        for (int j = 0; j < TAPS - 1; ++j)
+#pragma unroll
+            for (int e = 0; e < V; ++e) v[j][e] = s.from < 0 ? 0.0f : a.state[((u64)s.from * (TAPS - 1) + j) * a.D + d + e];
     if (!t0 && s.to >= 0) {
-        float n[TAPS - 1];
+        float n[TAPS - 1][V];
 #pragma unroll
         for (int j = 0; j < TAPS - 1; ++j) { /* input rows - (TAPS - 1) + j, from the slot where that is before the first */
             const int t = (int)s.rows - (TAPS - 1) + j;
-            n[j] = 0.0f;
-            if (t >= 0) n[j] = ld_row(x + (u64)t * a.ldx);
+            if (t >= 0) widen(n[j], load((u32)t));
             else
 #pragma unroll
-                for (int q = 0; q < TAPS - 1; ++q)
-                    if (q == t + TAPS - 1) n[j] = v[q];
+                for (int k = 0; k < TAPS - 1; ++k)
+#pragma unroll
+                    for (int e = 0; e < V; ++e) n[j][e] = k == t + TAPS - 1 ? v[k][e] : k ? n[j][e] : 0.0f;
         }
 #pragma unroll
-        for (int j = 0; j < TAPS - 1; ++j) a.state[((u64)s.to * (TAPS - 1) + j) * a.D + d] = n[j];
+        for (int j = 0; j < TAPS - 1; ++j)
+#pragma unroll
+            for (int e = 0; e < V; ++e) a.state[((u64)s.to * (TAPS - 1) + j) * a.D + d + e] = n[j][e];
     }
-    for (u32 t = t0; t < min(t0 + CCONV_ROWS, s.rows); ++t) {
-        v[TAPS - 1] = ld_row(x + (u64)t * a.ldx);
-        float o = b;
+    for (u32 t = t0; t < end; t += B) {
 #pragma unroll
-        for (int j = 0; j < TAPS; ++j) o = fmaf(w[j], v[j], o);
-        if (a.act == NK_ACT_SILU) o = silu_f(o);
-        else if (a.act == NK_ACT_RELU) o = fmaxf(o, 0.0f);
-        st_row(y + (u64)t * a.ldy, o);
+        for (int k = 0; k < B; ++k) widen(v[TAPS - 1 + k], q[k]);
+        if (t + B < end)
 #pragma unroll
-        for (int j = 0; j < TAPS - 1; ++j) v[j] = v[j + 1];
+            for (u32 k = 0; k < B; ++k) q[k] = load(min(t + B + k, end - 1));
+#pragma unroll
+        for (u32 k = 0; k < B; ++k) {
+            float o[V];
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+                o[e] = b[e];
+#pragma unroll
+                for (int j = 0; j < TAPS; ++j) o[e] = fmaf(w[j][e], v[k + j][e], o[e]);
+                if (a.act == NK_ACT_SILU) o[e] = silu_q(o[e]);
+                else if (a.act == NK_ACT_RELU) o[e] = fmaxf(o[e], 0.0f);
+            }
+            if (t + k < end) store_row(y + (u64)(t + k) * a.ldy + d, o);
+        }
+#pragma unroll
+        for (int j = 0; j < TAPS - 1; ++j)
+#pragma unroll
+            for (int e = 0; e < V; ++e) v[j][e] = v[B + j][e];
     }
 }
-#define CCONV(T, NAME, TAPS) \
-    extern "C" __global__ __launch_bounds__(256) void cconv_##NAME##_##TAPS(const NkCconvArgs a) { cconv_impl<T, TAPS>(a); }
-CCONV(float, f32, 2) CCONV(float, f32, 3) CCONV(float, f32, 4)
-CCONV(u16, bf16, 2) CCONV(u16, bf16, 3) CCONV(u16, bf16, 4)
+#define CCONV(T, NAME, TAPS, V) \
+    extern "C" __global__ __launch_bounds__(256) void cconv_##NAME##_##TAPS(const NkCconvArgs a) { cconv_impl<T, TAPS, V>(a); }
+CCONV(float, f32, 2, 1) CCONV(float, f32, 3, 1) CCONV(float, f32, 4, 1)
+CCONV(u16, bf16, 2, 1) CCONV(u16, bf16, 3, 1) CCONV(u16, bf16, 4, 1)
+CCONV(u16, bf16x2, 2, 2) CCONV(u16, bf16x2, 3, 2) CCONV(u16, bf16x2, 4, 2)
 
 /* e^v for v <= 0 to about two steps: 2^(v log2 e) with the product's rounding put back (the hardware's
  * exponential gives 0 below 2^-126) */
@@ -161,7 +216,7 @@ __device__ __forceinline__ void scan_rows(const NkScanArgs &a, const seq_t &s, u
                 }
                 if constexpr (!ENDS) {
                     o = fmaf(skip, xv[k], o);
-                    if (z) o *= silu_f(zv[k]);
+                    if (z) o *= silu_q(zv[k]);
                     if (live && in) st_row(y + (u64)(u + r0 + k) * a.ldy + d, o);
                 }
             }
@@ -304,7 +359,7 @@ template <typename T, int Q> __device__ __forceinline__ void scan_few_impl(const
 #pragma unroll
         for (int w = Q / 2; w > 0; w >>= 1) o += __shfl_xor(o, w, 64);
         o = fmaf(skip, v, o);
-        if (a.z) o *= silu_f(z);
+        if (a.z) o *= silu_q(z);
         if (live && n0 == 0) st_row((T *)a.y + (u64)t * a.ldy + d, o);
     }
     if (s.to < 0 || !live) return;

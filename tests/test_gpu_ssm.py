@@ -135,6 +135,23 @@ def test_conv(gpu, case, D, typ, taps):
     np.testing.assert_array_equal(st, new.astype(np.float32))
 
 
+@pytest.mark.parametrize("typ,D,more", [(BF16, 2050, dict()), (BF16, 2050, dict(ldx=2051)), (F32, 2050, dict(ldy=2052))])
+def test_conv_long(gpu, typ, D, more):
+    """Enough values for longer tiles and two channels a thread (bf16 rows of an even stride)."""
+    rng = np.random.default_rng(D)
+    seqs, M = _seqs([8100, 37, 200], [(0, 0), (-1, 1), (2, 2)], 1)
+    x, w, b = rng.standard_normal((M, D)), rng.standard_normal((D, 4)).astype(np.float32), rng.standard_normal(D).astype(np.float32)
+    state = rng.standard_normal((3, 3, D)).astype(np.float32)
+    y, st = run_conv(gpu, typ, x, w, b, state, seqs, M, 8100, 1, **more)
+    ref, tol, new = conv_ref(_kept(x, typ), w.astype(np.float64), b.astype(np.float64), state.astype(np.float64), seqs, 1)
+    if typ == BF16:
+        tol = tol + 2.0 ** -8 * (np.abs(ref) + tol)
+    for first, n, _, _ in seqs:
+        assert (np.abs(_back(y[first:first + n, :D], typ) - ref[first:first + n]) <= tol[first:first + n] + 1e-37).all()
+    np.testing.assert_array_equal(st, new.astype(np.float32))
+    assert (y[M:] == 9).all() and (y[8100] == 9).all() and (y[:, D:] == 9).all()
+
+
 def test_conv_in_pieces(gpu):
     """A sequence fed in pieces of any length, in one slot, gives the bits of the whole."""
     rng = np.random.default_rng(5)
