@@ -110,9 +110,16 @@ __device__ __forceinline__ floatx4 fp4_bias4(const NkGemm4Args &a, u32 n, u32 no
         for (int e = 0; e < 4; ++e) b[e] = a.bias[min(n + e, nout - 1) + gate];
     return b;
 }
+/* what C holds in columns n .. n + 3 of row m where the product is added to it (four at once; fp4_store4 reads the rest
+ * itself): loaded for several stores ahead, which wait a memory round trip each otherwise */
+__device__ __forceinline__ floatx4 fp4_old4(const NkGemm4Args &a, u32 m, u32 n, u32 nout) {
+    if (a.accumulate && a.vec && m < a.M && n + 4 <= nout) return *(const floatx4 *)(a.C + (u64)m * a.ldc + n);
+    return (floatx4){ 0.f, 0.f, 0.f, 0.f };
+}
 /* activation of the sums s (bias added; GLU: t the gates'), alpha, accumulation and store of columns n .. n + 3 of
- * row m */
-template <bool GLU> __device__ __forceinline__ void fp4_store4(const NkGemm4Args &a, u32 m, u32 n, u32 nout, floatx4 s, floatx4 t) {
+ * row m; old from fp4_old4 */
+template <bool GLU>
+__device__ __forceinline__ void fp4_store4(const NkGemm4Args &a, u32 m, u32 n, u32 nout, floatx4 s, floatx4 t, floatx4 old) {
     if (GLU)
 #pragma unroll
         for (int e = 0; e < 4; ++e) s[e] *= sigmoid_f(t[e]);
@@ -125,9 +132,8 @@ template <bool GLU> __device__ __forceinline__ void fp4_store4(const NkGemm4Args
     if (m >= a.M || n >= nout) return;
     float *c = a.C + (u64)m * a.ldc + n;
     if (a.vec && n + 4 <= nout) {
-        floatx4 v = s * a.alpha;
-        if (a.accumulate) v = *(const floatx4 *)c + v;
-        *(floatx4 *)c = v;
+        const floatx4 v = s * a.alpha;
+        *(floatx4 *)c = a.accumulate ? old + v : v;
     } else {
 #pragma unroll
         for (int e = 0; e < 4; ++e)
@@ -147,7 +153,8 @@ __device__ __forceinline__ void fp4_epilogue(const NkGemm4Args &a, u32 m0, const
     for (int i = 0; i < TI; ++i)
 #pragma unroll
         for (int j = 0; j < TO; ++j)
-            fp4_store4<GLU>(a, m + 16 * i, col[j] + 4 * (lane >> 4), nout, acc[i][j] + b[j], acc[i][j + (GLU ? TO : 0)] + b[j + (GLU ? TO : 0)]);
+            fp4_store4<GLU>(a, m + 16 * i, col[j] + 4 * (lane >> 4), nout, acc[i][j] + b[j], acc[i][j + (GLU ? TO : 0)] + b[j + (GLU ? TO : 0)],
+                            fp4_old4(a, m + 16 * i, col[j] + 4 * (lane >> 4), nout));
 }
 
 __device__ __forceinline__ intx8 fp4_op(uint4 q) {
@@ -220,22 +227,31 @@ __device__ __forceinline__ void tile_out(const NkGemm4Args &a, u32 m0, u32 c0, c
     constexpr int TO = GLU ? TJ / 2 : TJ;
     const u32 r = threadIdx.x & 31, f = threadIdx.x >> 5 & 1, nout = GLU ? a.N / 2 : a.N;
 #pragma unroll
-    for (int j = 0; j < TO; ++j)
+    for (int h = 0; h < 2 * TO; ++h) { /* half a tile at a time: more is spilled */
+        const u32 n = c0 + 16 * h + 4 * f;
+        floatx4 old[2][TI], b[2], d[2];
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-            const u32 n = c0 + 32 * j + 8 * q + 4 * f;
-            const floatx4 b = fp4_bias4(a, n, nout, 0), d = GLU ? fp4_bias4(a, n, nout, nout) : b;
+        for (int q = 0; q < 2; ++q) {
+#pragma unroll
+            for (int i = 0; i < TI; ++i) old[q][i] = fp4_old4(a, m0 + 32 * i + r, n + 8 * q, nout);
+            b[q] = fp4_bias4(a, n + 8 * q, nout, 0);
+            d[q] = GLU ? fp4_bias4(a, n + 8 * q, nout, nout) : b[q];
+        }
+#pragma unroll
+        for (int q = 0; q < 2; ++q)
 #pragma unroll
             for (int i = 0; i < TI; ++i) {
+                const int at = 8 * (h & 1) + 4 * q;
                 floatx4 v, t;
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    v[e] = acc[i][j][4 * q + e] + b[e];
-                    t[e] = acc[i][j + (GLU ? TO : 0)][4 * q + e] + d[e];
+                    v[e] = acc[i][h / 2][at + e] + b[q][e];
+                    t[e] = acc[i][h / 2 + (GLU ? TO : 0)][at + e] + d[q][e];
                 }
-                fp4_store4<GLU>(a, m0 + 32 * i + r, n, nout, v, t);
+                fp4_store4<GLU>(a, m0 + 32 * i + r, n + 8 * q, nout, v, t, old[q][i]);
             }
-        }
+        __builtin_amdgcn_sched_barrier(0);
+    }
 }
 
 /* The product by tiles of BM x BN outputs (K > 384), WGM x WGN wavefronts with (BM / WGM) x (BN / WGN) each and PW that
@@ -454,6 +470,7 @@ __device__ __forceinline__ void few_out(const NkGemm4Args &a, floatx4 (*part)[TI
     __syncthreads();
     for (u32 t = wv; t < TI * TO; t += FEW_WAVES) {
         const u32 i = t / TO, j = t % TO, n = n0 + 16 * j + 4 * f;
+        const floatx4 old = fp4_old4(a, 16 * i + r, n, nout);
         auto sum = [&](u32 tile) {
             floatx4 s = { 0.f, 0.f, 0.f, 0.f };
 #pragma unroll
@@ -463,7 +480,7 @@ __device__ __forceinline__ void few_out(const NkGemm4Args &a, floatx4 (*part)[TI
             return s;
         };
         const floatx4 s = sum(i * TJ + j), d = GLU ? sum(i * TJ + j + TO) : s;
-        fp4_store4<GLU>(a, 16 * i + r, n, nout, s + fp4_bias4(a, n, nout, 0), GLU ? d + fp4_bias4(a, n, nout, nout) : s);
+        fp4_store4<GLU>(a, 16 * i + r, n, nout, s + fp4_bias4(a, n, nout, 0), GLU ? d + fp4_bias4(a, n, nout, nout) : s, old);
     }
 }
 
