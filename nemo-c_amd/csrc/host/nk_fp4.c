@@ -46,7 +46,8 @@ int nk_fp4_dequant(gpu_t *g, const uint8_t *Q, uint32_t ldq, const uint8_t *S, u
  * and per K step max(lat, thr x t), fitted to graph replays:
  *   fp4 (steps of 256) 3584 x 4096 x 8192 and x 4096, 2048 x 4096 x 4096, 1024 x 4096 x 2048, 448 x 4096 x 1024,
  *   448 x 1024 x 4096, 128 x 4096 x 4096: 128x256 80, 50, 28, 16.4, 11.1, 17.6, 17.9 us, 64x128 102, 60, 36, 14.0, 7.9,
- *   11.0, 11.3, 64x64 133, 70, 42, 15.3, 7.1, 8.7, 9.4: the least is picked each time;
+ *   11.0, 11.3, 64x64 133, 70, 42, 15.3, 7.1, 8.7, 9.4: the least is picked each time; few rows against the tiles:
+ *   16 x 8192 x 2048 6.1 us, 32 rows 8.1, 64 rows 11.9, 64 x 8192 x 4096 21.0 / 9.7;
  *   w4 (steps of 64) 2048 x 4096 x 8192 and x 2048, 1024 x 4096 x 2048, 448 x 4096 x 1024, 448 x 1024 x 4096: 128x256
  *   316, 87, 73, 38, 118, 64x256 342, 92, 50, 23, 67, 64x128 390, 103, 55, 19, 48, 32x64 565, 143, 76, 23, 31; few rows
  *   (16 to a workgroup, one launch of them for 17 and more) against 32x64: 32 x 4096 x 1024 9.4 / 10.2, 48 rows 12.9 /
@@ -54,8 +55,8 @@ int nk_fp4_dequant(gpu_t *g, const uint8_t *Q, uint32_t ldq, const uint8_t *S, u
 typedef struct { const char *name; uint16_t bm, bn, threads, percu; float fix, lat, thr; } tile_t;
 static const tile_t fp4_tiles[] = {
     { "128x256", 128, 256, 768, 1, 10.0f, 1.0f, 1.0f },
-    { "64x128", 64, 128, 512, 2, 4.0f, 0.52f, 0.45f },
-    { "64x64", 64, 64, 512, 3, 3.0f, 0.38f, 0.24f },
+    { "64x128", 64, 128, 512, 2, 5.5f, 0.38f, 0.45f },
+    { "64x64", 64, 64, 512, 3, 4.5f, 0.30f, 0.24f },
 };
 static const tile_t w4_tiles[] = {
     { "128x256", 128, 256, 768, 1, 8.0f, 2.3f, 2.3f },
@@ -100,13 +101,14 @@ static int product(gpu_t *g, NkGemm4Args *a) {
     const tile_t *t = NULL;
     if (a->A) t = tile_pick(w4_tiles, 4, a->M, nout, (a->K + 63) / 64, glu, &us);
     else if (a->K > 384) t = tile_pick(fp4_tiles, 3, a->M, nout, (a->K + 255) / 256, glu, &us); /* four scales a load */
-    /* few rows: 16 of them and 16 output columns to a workgroup, wide matrices 32 (f32 rows) */
+    /* few rows, 16 output columns to a workgroup: 4-bit rows up to 64 at a time, f32 rows 16 (wide matrices 32 columns) */
+    const uint32_t G = (a->K + 127) / 128, ti = a->M <= 16 ? 1 : a->M <= 32 ? 2 : 4;
     const uint32_t wide = a->A && !glu && nout > 4096, co = wide ? 32 : 16, rows = a->A ? (a->M + 15) / 16 : 1;
     const uint64_t wgs = (uint64_t)rows * ((nout + co - 1) / co);
-    const float few = 1.5f + (float)((wgs + 255) / 256) * (2.0f + (glu || wide ? 0.28f : 0.21f) * (float)((a->K + 127) / 128));
-    if (a->A ? a->M <= 16 || few < us : a->M <= 64) {
-        const uint32_t ti = a->A && a->M <= 5 ? 5 : a->A || a->M <= 16 ? 16 : a->M <= 32 ? 32 : 64;
-        snprintf(name, sizeof name, "gemm_%s_few%u%s", kind, ti, glu ? gl : wide ? "x2" : "");
+    const float each = a->A ? 2.0f + (glu || wide ? 0.28f : 0.21f) * (float)G : 0.75f + (0.08f + 0.05f * (float)ti) * (float)G;
+    const float few = 1.5f + (float)((wgs + 255) / 256) * each;
+    if ((a->A ? a->M <= 16 : a->M <= 64 && !t) || ((a->A || a->M <= 64) && few < us)) {
+        snprintf(name, sizeof name, "gemm_%s_few%u%s", kind, a->A ? (a->M <= 5 ? 5u : 16u) : 16 * ti, glu ? gl : wide ? "x2" : "");
         return gpu_launch(g, name, a, sizeof *a, (nout + co - 1) / co, rows, 1, 512, 1, 1);
     }
     if (t) {
