@@ -64,16 +64,16 @@ static const tile_t w4_tiles[] = {
     { "64x128", 64, 128, 512, 2, 4.5f, 0.65f, 0.76f },
     { "32x64", 32, 64, 256, 4, 3.0f, 0.43f, 0.29f },
 };
-static uint32_t tiles_of(const tile_t *t, uint32_t M, uint32_t nout, int glu) {
+static uint64_t tiles_of(const tile_t *t, uint32_t M, uint32_t nout, int glu) {
     const uint32_t co = glu ? t->bn / 2u : t->bn;
-    return (M + t->bm - 1) / t->bm * ((nout + co - 1) / co);
+    return (uint64_t)((M + t->bm - 1) / t->bm) * ((nout + co - 1) / co);
 }
 /* the tile of the least estimate, and that in *us */
 static const tile_t *tile_pick(const tile_t *list, int n, uint32_t M, uint32_t nout, uint32_t steps, int glu, float *us) {
     const tile_t *best = NULL;
     for (const tile_t *t = list; t < list + n; ++t) {
         if (glu && t->bn < 128) continue; /* a wavefront holds 32 value and 32 gate columns, a load of scales one half's */
-        const uint32_t w = (tiles_of(t, M, nout, glu) + 255) / 256;
+        const uint64_t w = (tiles_of(t, M, nout, glu) + 255) / 256;
         const float step = t->thr * (float)w > t->lat ? t->thr * (float)w : t->lat;
         const float e = (float)((w + t->percu - 1) / t->percu) * t->fix + step * (float)steps;
         if (!best || e < *us) { best = t; *us = e; }
@@ -85,7 +85,7 @@ static const tile_t *tile_pick(const tile_t *list, int n, uint32_t M, uint32_t n
 static int product(gpu_t *g, NkGemm4Args *a) {
     const int glu = a->act == NK_ACT_GLU;
     if (a->act > NK_ACT_GLU) return bad(g, "gemm 4-bit: unknown activation");
-    if (!a->N || a->N > 1u << 28 || !a->K || (glu && (a->N & 1))) return bad(g, "gemm 4-bit: bad shape");
+    if (!a->N || a->N > 1u << 26 || !a->K || (glu && (a->N & 1))) return bad(g, "gemm 4-bit: bad shape");
     if (a->M > 65535 * 16) return bad(g, "gemm 4-bit: too many rows");
     if (!rows_ok(a->Wq, a->ldw, a->Ws, a->ldws, a->K) || a->ldw >= FP4_STRIDE || a->ldws >= FP4_STRIDE)
         return bad(g, "gemm 4-bit: weight codes 16-byte and scales 4-byte aligned, rows padded to 128 values, strides below 2^24");
@@ -112,8 +112,10 @@ static int product(gpu_t *g, NkGemm4Args *a) {
         return gpu_launch(g, name, a, sizeof *a, (nout + co - 1) / co, rows, 1, 512, 1, 1);
     }
     if (t) {
+        const uint64_t tiles = (tiles_of(t, a->M, nout, glu) + 7) / 8 * 8;
+        if (tiles * t->threads > 0xffffffffu) return bad(g, "gemm 4-bit: more outputs than a launch covers");
         snprintf(name, sizeof name, "gemm_%s_%s%s", kind, t->name, gl);
-        return gpu_launch(g, name, a, sizeof *a, (tiles_of(t, a->M, nout, glu) + 7) / 8 * 8, 1, 1, t->threads, 1, 1);
+        return gpu_launch(g, name, a, sizeof *a, (uint32_t)tiles, 1, 1, t->threads, 1, 1);
     }
     const uint32_t cols = glu ? 32 : 64;
     snprintf(name, sizeof name, "gemm_fp4%s", gl);

@@ -64,12 +64,14 @@ int nk_ssm_scan(gpu_t *g, const nk_scan_t *p) {
     if (p->ldx < p->D || p->lddt < p->D || p->ldy < p->D || (p->z && p->ldz < p->D) || p->ldbc < (uint64_t)p->groups * p->N)
         return bad(g, "ssm_scan: rows of at least D values, B and C of groups * N");
     const uint32_t per = p->D / p->groups, block = per >= 256 ? 256 : (per + 63) / 64 * 64;
-    const uint32_t tiles = p->groups * ((per + block - 1) / block), waves = p->nseq * tiles * (block / 64);
+    const uint32_t tiles = p->groups * ((per + block - 1) / block);
+    const uint64_t waves = (uint64_t)p->nseq * tiles * (block / 64);
     NkScanArgs a = { p->x, p->dt, p->B, p->C, p->z, p->y, p->A, p->skip, p->dt_bias, p->state, p->seqs, NULL,
                      p->ldx, p->lddt, p->ldbc, p->ldz, p->ldy, p->slots, p->nseq, p->max_rows, p->M, p->D, p->N,
                      p->groups, p->softplus != 0, 0, 0,
                      p->N % 4 == 0 && aligned(p->A, 16) && aligned(p->state, 16) };
     const uint32_t ns = p->N <= 8 ? 8 : p->N <= 16 ? 16 : p->N <= 32 ? 32 : 64;
+    if ((uint64_t)tiles * block > 1u << 31) return bad(g, "ssm_scan: more channels than a launch covers");
     const char *type = p->type == NK_F32 ? "f32" : "bf16";
     char name[32];
     gpu_next_bytes(g, (double)size * p->M * (4.0 * p->D + 2.0 * p->groups * p->N) + 8.0 * p->nseq * p->D * p->N);
@@ -78,7 +80,7 @@ int nk_ssm_scan(gpu_t *g, const nk_scan_t *p) {
      * 4 + r max(0.42, 0.0012 w) us against 8 + 0.0067 w + r (0.5 + 0.0001 w) with the states in one lane: 32 w 8 r 7.0
      * / 12.0, 24 r 13.6 / 19.9; 1024 w 8 r 14.6 / 16.9, 16 r 24.1 / 21.3; 8192 w 4 r 55 / 68, 8 r 95 / 73.  Beyond
      * 32 rows a few wavefronts are split (64 r 21.0). */
-    if (p->max_rows <= 32 && (int64_t)p->max_rows * ((int64_t)waves * 12 - 5000) < 40000 + 67 * (int64_t)waves) {
+    if (p->max_rows <= 32 && (double)p->max_rows * (12.0 * (double)waves - 5000.0) < 40000.0 + 67.0 * (double)waves) {
         uint32_t q = 1;
         while (4 * q < p->N) q *= 2;
         snprintf(name, sizeof name, "scan_few_%s_%u", type, q);
@@ -91,9 +93,11 @@ int nk_ssm_scan(gpu_t *g, const nk_scan_t *p) {
     if (waves < 1100 && (uint64_t)p->max_rows * (1100 - waves) > 18000) {
         /* about 4096 wavefronts (four per SIMD: 8192 rows of one stream 335 us with 1024, 210 with 2048, 168), and
          * pieces of some sqrt(r / 2) rows, between the pieces' time and that of joining them (512 rows: pieces of
-         * 4, 8, 16 and 32 rows 45, 34, 31 and 42 us; 32 rows: 17.8, 20.8, 27.4, 30.1) */
+         * 4, 8, 16 and 32 rows 45, 34, 31 and 42 us; 32 rows: 17.8, 20.8, 27.4, 30.1).  By the rows there are: sequences
+         * shorter than the longest fill no pieces (12 of 1 to 1000 rows, 1536 channels: 136 us by max_rows, 111 so) */
+        const uint64_t all = (uint64_t)p->nseq * p->max_rows, rows = all < p->M ? all : p->M;
         uint32_t piece = 8;
-        while (piece * (4096ull / waves) < p->max_rows || 2ull * piece * piece < p->max_rows) piece += 8;
+        while (4096ull * piece < rows * (waves / p->nseq) || 2ull * piece * piece < p->max_rows) piece += 8;
         const uint32_t pieces = (p->max_rows + piece - 1) / piece;
         a.ws = gpu_scratch_ws(g, (size_t)p->nseq * pieces * (p->N + 1) * p->D);
         if (!a.ws) return bad(g, "ssm_scan: scratch unavailable (size it before capture)");
