@@ -319,8 +319,8 @@ int nk_fp4_dequant(gpu_t *g, const uint8_t *Q, uint32_t ldq, const uint8_t *S, u
                    uint32_t ldx, uint32_t M, uint32_t K);
 /* nk_gemm with 4-bit weights: C[m][n] (= or +=) alpha * act(sum_k A[m][k] W[n][k] + bias[n]), the same
  * activations, any M, N and K; sums in f32.  nk_gemm_fp4: A in 4 bits too (the products are exact).
- * nk_gemm_w4: A f32 rows, 16-byte aligned with lda % 4 == 0, with all their 24 bits.  lda, ldas, ldw and ldws are strides in bytes (lda of nk_gemm_w4 in floats).
- * lda, ldas, ldw and ldws are below 2^24 bytes.  C must not overlap the operands. */
+ * nk_gemm_w4: A f32 rows, 16-byte aligned with lda % 4 == 0, with all their 24 bits.  lda (of nk_gemm_w4 in
+ * floats), ldas, ldw and ldws are below 2^24 bytes.  C must not overlap the operands. */
 int nk_gemm_fp4(gpu_t *g, const uint8_t *Aq, uint32_t lda, const uint8_t *As, uint32_t ldas, const uint8_t *Wq,
                 uint32_t ldw, const uint8_t *Ws, uint32_t ldws, const float *bias, float *C, uint32_t ldc, uint32_t M,
                 uint32_t N, uint32_t K, int act, int accumulate, float alpha);

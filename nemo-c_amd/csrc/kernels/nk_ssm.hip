@@ -147,7 +147,12 @@ __device__ __forceinline__ float softplus_f(float v) {
  * e^(s A) is 2^(s A log2 e) by the hardware's exponential (results below 2^-126 come out as 0).  B and C are the
  * same for every channel of the workgroup's group: a tile of their rows lies in LDS as f32, padded
  * with zeros to NS, and is read by all lanes at one address.  ENDS: only the states (from zero) and the
- * sum of the steps are wanted, no rows are written. */
+ * sum of the steps are wanted, no rows are written.
+ *
+ * Bound by the vector units: per state and row an exponential, which takes the time of 1.85 products, and four more
+ * operations, three of them where only the ends are wanted.  8192 rows of 2048 channels of 16 states, bf16: ends 64
+ * us, rows 95, the joining between them 13, where those operations alone are 43 and 52 us at the 30 T products/s that
+ * this card reaches; the softplus, the gate and the conversions of every row are the rest. */
 template <typename T, int NS, bool ENDS>
 __device__ __forceinline__ void scan_rows(const NkScanArgs &a, const seq_t &s, u32 t0, u32 t1, u32 g, u32 d, bool live,
                                           float (&h)[NS], float &sum, float *lds) {
@@ -305,7 +310,8 @@ extern "C" __global__ __launch_bounds__(256) void scan_join(const NkScanArgs a) 
 
 /* Few rows (tokens): every state row is read and written once and the rows are nothing beside them, so the
  * states are spread over lanes: Q lanes per channel with four consecutive states each, a row's output
- * summed over the Q lanes. */
+ * summed over the Q lanes.  One token of 2048 channels of 16 states: 1 stream 3.9 us, 64 streams 8.3, 256 streams 20.3
+ * (its states read and written at 3.3 TB/s). */
 template <typename T, int Q> __device__ __forceinline__ void scan_few_impl(const NkScanArgs &a) {
     const seq_t s = seq_load(a.seqs, blockIdx.y, a.M, a.max_rows, a.slots);
     const u32 i = blockIdx.x * 256 + threadIdx.x, n0 = 4 * (i % Q);
