@@ -19,13 +19,14 @@ __device__ __forceinline__ void st_row(float *p, float v) { *p = v; }
 /* to bf16, to nearest even; the conversion keeps infinities and NaN */
 __device__ __forceinline__ void st_row(u16 *p, float v) { *p = __builtin_bit_cast(u16, (__bf16)v); }
 
-/* v / (1 + e^-v) to about three steps in 12 instructions (the IEEE exponential and division take 25, a third of what the
+/* v / (1 + e^-v) to about four steps in 12 instructions (the IEEE exponential and division take 25, a third of what the
  * convolution does): 2^(-v log2 e) with the product's rounding put back, the hardware's reciprocal.  The exponent is
- * kept where neither flushes: below -87 the result is off by less than 2e-36. */
+ * kept where its own arithmetic is finite; from 2^128 on the exponential is infinite and its reciprocal zero (what is
+ * flushed below v = -87 is under 2e-36). */
 __device__ __forceinline__ float silu_q(float v) {
-    const float n = __builtin_amdgcn_fmed3f(-v, -104.0f, 87.0f), t = n * 1.44269504f;
+    const float n = __builtin_amdgcn_fmed3f(-v, -104.0f, 104.0f), t = n * 1.44269504f;
     const float r = fmaf(n, 1.92596299e-8f, fmaf(n, 1.44269504f, -t)), e = __builtin_amdgcn_exp2f(t);
-    return v * __builtin_amdgcn_rcpf(1.0f + fmaf(e, r * 0.693147181f, e));
+    return v * __builtin_amdgcn_rcpf(fmaf(e, fmaf(r, 0.693147181f, 1.0f), 1.0f));
 }
 
 /* V values of a row as they lie in memory */

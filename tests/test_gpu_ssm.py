@@ -152,6 +152,35 @@ def test_conv_long(gpu, typ, D, more):
     assert (y[M:] == 9).all() and (y[8100] == 9).all() and (y[:, D:] == 9).all()
 
 
+@pytest.mark.parametrize("typ", [F32, BF16])
+def test_silu_of_far_values(gpu, typ):
+    """SiLU of values down to the lowest: zero there, NaN at -infinity as the quotient gives, in the convolution and
+    the gate (8 roundings, and 2e-36 where the hardware's reciprocal flushes)."""
+    far = np.array([-3e38, -1e30, -1e10, -1000, -104.5, -103, -89, -88, -87, -80, 80, 87, 88.5, 104.5, 1e10, 3e38, np.inf, -np.inf, np.nan])
+    D, v = len(far), _kept(far, typ)
+    with np.errstate(invalid="ignore"):
+        want = v * _sig(v)
+    ok = np.isfinite(want)
+
+    def check(row):
+        got = _back(row, typ)
+        tol = (8 * U + (2.0 ** -8 if typ == BF16 else 0)) * np.abs(want) + 2e-36
+        assert (np.isnan(got) == np.isnan(want)).all() and (got[np.isinf(want)] == np.inf).all()
+        assert (np.abs(got - want)[ok] <= tol[ok]).all()
+
+    y, _ = run_conv(gpu, typ, far[None], np.repeat([[0.0, 1.0]], D, 0), None, np.zeros((1, 1, D)), np.array([[0, 1, -1, -1]], np.int32), 1, 1)
+    check(y[0])
+    for rows in (1, 40, 700):
+        o = operands(np.random.default_rng(0), typ, rows, D, 4, 1, 1)
+        o["z"] = np.repeat(v[None], rows, 0)
+        o["x"], o["B"], o["C"], o["skip"] = np.ones((rows, D)), 0 * o["B"], 0 * o["C"], np.ones(D)
+        c = ScanCall(gpu, typ, o, np.array([[0, rows, -1, -1]], np.int32), rows, 1)
+        y, _ = c.run()
+        c.free()
+        for r in y[:rows]:
+            check(r)
+
+
 def test_conv_in_pieces(gpu):
     """A sequence fed in pieces of any length, in one slot, gives the bits of the whole."""
     rng = np.random.default_rng(5)
