@@ -142,6 +142,13 @@ __device__ __forceinline__ float softplus_f(float v) {
     return fmaxf(v, 0.0f) + 2.0f * fmaf(f * w, q, q); /* NaN comes through q */
 }
 
+/* A log2 e, the factor of a step in the exponent.  An infinite one counts as the largest number: the steps of zero that
+ * fill a tile up would make it NaN. */
+__device__ __forceinline__ float scan_rate(float A) {
+    const float v = A * 1.44269504f;
+    return __builtin_isinf(v) ? copysignf(3.4028235e38f, v) : v;
+}
+
 #define SCAN_TILE 64 /* rows whose B and C are in LDS at a time */
 
 /* Rows t0 .. t1 - 1 of a sequence, one thread per channel with its NS >= N states in registers.
@@ -167,7 +174,7 @@ __device__ __forceinline__ void scan_rows(const NkScanArgs &a, const seq_t &s, u
 #pragma unroll
     for (int n = 0; n < NS; ++n) {
         const float v = a.A[(u64)d * a.N + min((u32)n, a.N - 1)];
-        A[n] = (u32)n < a.N ? v * 1.44269504f : 0.0f;
+        A[n] = (u32)n < a.N ? scan_rate(v) : 0.0f;
     }
     for (u32 u = t0; u < t1; u += SCAN_TILE) {
         const u32 rows = min(t1 - u, (u32)SCAN_TILE);
@@ -280,14 +287,15 @@ SCAN(float, f32, 8) SCAN(float, f32, 16) SCAN(float, f32, 32) SCAN(float, f32, 6
 SCAN(u16, bf16, 8) SCAN(u16, bf16, 16) SCAN(u16, bf16, 32) SCAN(u16, bf16, 64)
 
 /* The pieces of a sequence one after another: H <- e^(A sum) H + end, the state that the next piece starts from,
- * takes the place of the piece's own end.  One thread per state; the loads of JOIN pieces are in flight at a time
+ * takes the place of the piece's own end.  The factor by halves: a piece of growing steps may pass 2^128 by itself where
+ * no state does, and one that is zero stays so whatever the factor.  One thread per state; the loads of JOIN pieces are in flight at a time
  * (one at a time 36 us for 128 pieces of 2048 channels, a memory round trip each). */
 #define JOIN 16
 extern "C" __global__ __launch_bounds__(256) void scan_join(const NkScanArgs a) {
     const seq_t s = seq_load(a.seqs, blockIdx.z, a.M, a.max_rows, a.slots);
     const u32 d = blockIdx.x * 256 + threadIdx.x, n = blockIdx.y;
     if (!s.ok || d >= a.D || s.rows <= a.piece) return;
-    const float A = a.A[(u64)d * a.N + n] * 1.44269504f;
+    const float A = 0.5f * scan_rate(a.A[(u64)d * a.N + n]);
     float h = s.from >= 0 ? a.state[((u64)s.from * a.D + d) * a.N + n] : 0.0f;
     const u32 ends = (s.rows - 1) / a.piece; /* pieces that another follows */
     const u64 step = (u64)(a.N + 1) * a.D;
@@ -303,7 +311,8 @@ extern "C" __global__ __launch_bounds__(256) void scan_join(const NkScanArgs a) 
 #pragma unroll
         for (u32 k = 0; k < JOIN; ++k) {
             if (i + k >= ends) break;
-            h = fmaf(__builtin_amdgcn_exp2f(sum[k] * A), h, end[k]);
+            const float e = __builtin_amdgcn_exp2f(sum[k] * A);
+            h = h == 0.0f ? end[k] : fmaf(e, e * h, end[k]);
             w[(i + k) * step + (u64)n * a.D] = h;
         }
     }
@@ -341,7 +350,7 @@ template <typename T, int Q> __device__ __forceinline__ void scan_few_impl(const
     }
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-        A[e] = n0 + e < a.N ? A[e] * 1.44269504f : 0.0f;
+        A[e] = n0 + e < a.N ? scan_rate(A[e]) : 0.0f;
         h[e] = n0 + e < a.N ? h[e] : 0.0f;
     }
     const float skip = a.skip ? a.skip[d] : 0.0f, db = a.dt_bias ? a.dt_bias[d] : 0.0f;

@@ -374,6 +374,39 @@ def test_scan_no_softplus_and_far_steps(gpu, rows):
     check_scan(gpu, F32, o, seqs, rows)
 
 
+@pytest.mark.parametrize("rows", [3, 37, 90, 601])
+def test_scan_forgets_at_once(gpu, rows):
+    """A of -infinity: every row's state is its own input's, also where rows do not fill a tile."""
+    rng = np.random.default_rng(rows)
+    seqs, M = _seqs([rows], [(0, 1)])
+    o = operands(rng, F32, M, 64, 16, 1, 2)
+    o["dt"] = np.maximum(o["dt"], -8.0)
+    o["A"][:, ::3] = -np.inf
+    c = ScanCall(gpu, F32, o, seqs, rows, 1)
+    y, st = c.run()
+    c.free()
+    o["A"][:, ::3] = -1e30  # the same: e^(sA) is zero for every step here
+    ref, tol, new, enew = scan_ref(o, seqs, 1)
+    assert (np.abs(y[:M] - ref) <= tol + 1e-37).all() and (np.abs(st - new) <= enew + 1e-37).all()
+
+
+def test_scan_of_growing_steps(gpu):
+    """Steps below zero, which let states grow: a factor over many rows that passes the type's range takes a state
+    of zero, or a tiny one, to where the recurrence does."""
+    rng = np.random.default_rng(4)
+    rows = 600
+    seqs, M = _seqs([rows], [(0, 1)])
+    o = operands(rng, F32, M, 64, 16, 1, 2, db=False)
+    o["A"] = np.full((64, 16), -1.0)
+    o["x"] *= 0
+    o["state"][0, ::2] = 0
+    o["state"][0, 1::2] = _kept(1e-37 * (1 + np.abs(o["state"][0, 1::2])), F32)
+    o["dt"] = np.full((M, 64), -0.25)  # e^150 = 2^216 over the rows, e^8 over a piece of 32
+    check_scan(gpu, F32, o, seqs, rows, softplus=0)
+    o["dt"] = np.where(np.arange(M)[:, None] < 16, -9.0, 0.0) * np.ones((M, 64))  # 2^104 over 8 rows, 2^207 over 16
+    check_scan(gpu, F32, o, seqs, rows, softplus=0)
+
+
 @pytest.mark.parametrize("rows", [4, 600])
 def test_scan_not_finite(gpu, rows):
     """An infinity or NaN in one channel's row reaches that channel's later rows of that sequence, and nothing else."""
