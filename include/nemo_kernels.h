@@ -332,7 +332,8 @@ int nk_gemm_w4(gpu_t *g, const float *A, uint32_t lda, const uint8_t *Wq, uint32
  * The two operators of a selective-scan block over the sequences of a batch (no counterpart in the
  * reference).  seqs (device, 16-byte aligned) has four ints per sequence: { first row, rows, the slot whose
  * state it goes on from or -1 for zeros, the slot that takes the state behind its last row or -1 for
- * none }.  The slots may be the same; no slot is written by two sequences, or by one and read by another.
+ * none }.  The slots may be the same; no slot is written by two sequences, or by one and read by another,
+ * and no row is in two sequences.
  * A sequence of no rows hands its state on.  Rows that no sequence has are not written.  The rows of a
  * sequence are below M and its slots below `slots`; max_rows is at least the longest sequence: a
  * sequence that breaks these is left out (nothing of it is written).

@@ -68,7 +68,7 @@ int nk_ssm_scan(gpu_t *g, const nk_scan_t *p) {
     const uint64_t waves = (uint64_t)p->nseq * tiles * (block / 64);
     NkScanArgs a = { p->x, p->dt, p->B, p->C, p->z, p->y, p->A, p->skip, p->dt_bias, p->state, p->seqs, NULL,
                      p->ldx, p->lddt, p->ldbc, p->ldz, p->ldy, p->slots, p->nseq, p->max_rows, p->M, p->D, p->N,
-                     p->groups, p->softplus != 0, 0, 0,
+                     p->groups, p->softplus != 0, 0, 0, 0,
                      p->N % 4 == 0 && aligned(p->A, 16) && aligned(p->state, 16) };
     const uint32_t ns = p->N <= 8 ? 8 : p->N <= 16 ? 16 : p->N <= 32 ? 32 : 64;
     if ((uint64_t)tiles * block > 1u << 31) return bad(g, "ssm_scan: more channels than a launch covers");
@@ -99,7 +99,11 @@ int nk_ssm_scan(gpu_t *g, const nk_scan_t *p) {
         uint32_t piece = 8;
         while (4096ull * piece < rows * (waves / p->nseq) || 2ull * piece * piece < p->max_rows) piece += 8;
         const uint32_t pieces = (p->max_rows + piece - 1) / piece;
-        a.ws = gpu_scratch_ws(g, (size_t)p->nseq * pieces * (p->N + 1) * p->D);
+        /* places for all sequences' pieces, or, where that is fewer (one long sequence among many short ones, max_rows far
+         * above the longest), for one of each `piece` rows */
+        const uint64_t table = (uint64_t)p->nseq * pieces, byrow = ((uint64_t)p->M + piece - 1) / piece + 1;
+        a.byrow = byrow < table;
+        a.ws = gpu_scratch_ws(g, (size_t)(a.byrow ? byrow : table) * (p->N + 1) * p->D);
         if (!a.ws) return bad(g, "ssm_scan: scratch unavailable (size it before capture)");
         a.piece = piece;
         a.pieces = pieces;

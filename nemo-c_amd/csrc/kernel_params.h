@@ -533,9 +533,9 @@ typedef struct {
     const float *A, *skip, *dt_bias;
     float *state;     /* [slots][D][N] */
     const int *seqs;
-    float *ws;        /* split sequences: per sequence and piece N states, then the sum of the steps, of D channels */
+    float *ws;        /* split sequences: per piece N states, then the sum of the steps, of D channels */
     u32 ldx, lddt, ldbc, ldz, ldy, slots, nseq, max_rows, M, D, N, groups, softplus;
-    u32 piece, pieces, vec; /* vec: four states are read and written at once */
+    u32 piece, pieces, byrow, vec; /* byrow: places in ws by the rows; vec: four states are read and written at once */
 } NkScanArgs;
 
 #endif

@@ -248,6 +248,14 @@ __device__ __forceinline__ chan_t scan_channel(const NkScanArgs &a) {
     return (chan_t){ g, g * per + min(c, per - 1), c < per };
 }
 
+/* A piece's place in the scratch: N states of D channels, then the sums.  Places are needed only by pieces that another
+ * follows, which are whole.  Either all sequences have a.pieces of them, or a piece's place is that of the one
+ * multiple of a.piece among its rows' numbers: no row is in two sequences, so no place is in two pieces. */
+__device__ __forceinline__ float *scan_place(const NkScanArgs &a, u32 i, const seq_t &s, u32 piece) {
+    const u64 at = a.byrow ? (s.first + a.piece - 1) / a.piece + piece : (u64)i * a.pieces + piece;
+    return a.ws + at * (a.N + 1) * a.D;
+}
+
 /* PART 0: whole sequences.  PART 1: the states that the pieces of a.piece rows end in from zero, and their
  * sums of steps (of all but a sequence's last, which nothing follows).  PART 2: the pieces again from the
  * states that scan_join has put in their predecessors' places. */
@@ -258,8 +266,7 @@ template <typename T, int NS, int PART> __device__ __forceinline__ void scan_imp
     const u32 t0 = PART ? blockIdx.z * a.piece : 0, t1 = PART ? min(t0 + a.piece, s.rows) : s.rows;
     if (!s.ok || (PART == 1 ? t0 + a.piece >= s.rows : PART == 2 && t0 && t0 >= s.rows)) return;
     float h[NS], sum = 0.0f;
-    /* scratch: per piece N states of D channels, then the sums */
-    float *ws = PART ? a.ws + ((u64)blockIdx.y * a.pieces + blockIdx.z) * (a.N + 1) * a.D + c.d : nullptr;
+    float *ws = PART ? scan_place(a, blockIdx.y, s, blockIdx.z) + c.d : nullptr;
 #pragma unroll
     for (int n = 0; n < NS; ++n) h[n] = 0.0f;
     const bool joined = PART == 2 && t0;
@@ -299,7 +306,7 @@ extern "C" __global__ __launch_bounds__(256) void scan_join(const NkScanArgs a) 
     float h = s.from >= 0 ? a.state[((u64)s.from * a.D + d) * a.N + n] : 0.0f;
     const u32 ends = (s.rows - 1) / a.piece; /* pieces that another follows */
     const u64 step = (u64)(a.N + 1) * a.D;
-    float *w = a.ws + (u64)blockIdx.z * a.pieces * step + d;
+    float *w = scan_place(a, blockIdx.z, s, 0) + d;
     for (u32 i = 0; i < ends; i += JOIN) {
         float end[JOIN], sum[JOIN];
 #pragma unroll

@@ -374,6 +374,23 @@ def test_scan_no_softplus_and_far_steps(gpu, rows):
     check_scan(gpu, F32, o, seqs, rows)
 
 
+@pytest.mark.parametrize("typ,D,N", [(F32, 64, 16), (BF16, 100, 5)])
+@pytest.mark.parametrize("max_rows", [650, 1 << 18])
+def test_scan_skewed_batch(gpu, typ, D, N, max_rows):
+    """Long sequences among many short ones, in any order and with rows between them, and a max_rows far above the
+    longest: the scratch goes by the rows that there are."""
+    import torch
+
+    rng = np.random.default_rng(D)
+    lens = np.concatenate([rng.integers(0, 4, 120), [650, 65, 64, 333, 1, 24, 25]])
+    seqs, M = _seqs(lens.tolist(), [((-1, i)[i % 2], i if i % 3 else -1) for i in range(len(lens))], 1)
+    seqs = np.ascontiguousarray(seqs[rng.permutation(len(seqs))])
+    o = operands(rng, typ, M, D, N, 1, len(lens))
+    before = torch.cuda.mem_get_info()[0]
+    check_scan(gpu, typ, o, seqs, max_rows)
+    assert before - torch.cuda.mem_get_info()[0] < 64 << 20
+
+
 @pytest.mark.parametrize("rows", [3, 37, 90, 601])
 def test_scan_forgets_at_once(gpu, rows):
     """A of -infinity: every row's state is its own input's, also where rows do not fill a tile."""
