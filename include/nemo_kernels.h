@@ -319,8 +319,8 @@ int nk_fp4_dequant(gpu_t *g, const uint8_t *Q, uint32_t ldq, const uint8_t *S, u
                    uint32_t ldx, uint32_t M, uint32_t K);
 /* nk_gemm with 4-bit weights: C[m][n] (= or +=) alpha * act(sum_k A[m][k] W[n][k] + bias[n]), the same
  * activations, any M, N and K; sums in f32.  nk_gemm_fp4: A in 4 bits too (the products are exact).
- * nk_gemm_w4: A f32 rows, 16-byte aligned with lda % 4 == 0, with all their 24 bits.  lda (of nk_gemm_w4 in
- * floats), ldas, ldw and ldws are below 2^24 bytes.  C must not overlap the operands. */
+ * nk_gemm_w4: A f32 rows, 16-byte aligned with lda (in floats) % 4 == 0, with all their 24 bits.  Strides of codes and
+ * scales are below 2^24 bytes.  C must not overlap the operands. */
 int nk_gemm_fp4(gpu_t *g, const uint8_t *Aq, uint32_t lda, const uint8_t *As, uint32_t ldas, const uint8_t *Wq,
                 uint32_t ldw, const uint8_t *Ws, uint32_t ldws, const float *bias, float *C, uint32_t ldc, uint32_t M,
                 uint32_t N, uint32_t K, int act, int accumulate, float alpha);
@@ -340,7 +340,8 @@ int nk_gemm_w4(gpu_t *g, const float *A, uint32_t lda, const uint8_t *Wq, uint32
  *
  * nk_causal_conv: Y[t][d] = act(bias[d] + sum_j W[d][j] X[t - (taps - 1) + j][d]) for D channels, with X before
  * the sequence's first row from the slot: state is [slots][taps - 1][D] f32, the last inputs, oldest
- * first.  W [D][taps], bias may be NULL, taps 2, 3 or 4, act none, SiLU or ReLU; X and Y of one type. */
+ * first.  W [D][taps], bias may be NULL, taps 2, 3 or 4, act none, SiLU or ReLU; X and Y of one type, Y not
+ * overlapping X. */
 int nk_causal_conv(gpu_t *g, const void *X, int type, uint32_t ldx, const float *W, const float *bias, float *state,
                    uint32_t slots, const int *seqs, uint32_t nseq, uint32_t max_rows, void *Y, uint32_t ldy, uint32_t M,
                    uint32_t D, uint32_t taps, int act);

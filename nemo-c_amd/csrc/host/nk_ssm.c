@@ -30,6 +30,7 @@ int nk_causal_conv(gpu_t *g, const void *X, int type, uint32_t ldx, const float 
         return bad(g, "causal_conv: 2 to 4 taps, no activation, SiLU or ReLU");
     if (!X || !Y || !W || !aligned(X, size) || !aligned(Y, size) || !aligned(W, 4) || !aligned(bias, 4) || ldx < D || ldy < D)
         return bad(g, "causal_conv: aligned rows of at least D values");
+    if (X == Y) return bad(g, "causal_conv: Y must not overlap X");
     const uint64_t rows = (uint64_t)nseq * max_rows < M ? (uint64_t)nseq * max_rows : M;
     /* bf16: two channels a thread from 16 Mi values on (17760 rows of 2048 channels 39.5 -> 33.8 us; 8192 rows 15.9 / 16.1,
      * 4096 rows of 512 5.8 / 6.3) */
@@ -63,6 +64,8 @@ int nk_ssm_scan(gpu_t *g, const nk_scan_t *p) {
         return bad(g, "ssm_scan: x, dt, B, C, y and A aligned to their values");
     if (p->ldx < p->D || p->lddt < p->D || p->ldy < p->D || (p->z && p->ldz < p->D) || p->ldbc < (uint64_t)p->groups * p->N)
         return bad(g, "ssm_scan: rows of at least D values, B and C of groups * N");
+    if (p->y == p->x || p->y == p->dt || p->y == p->B || p->y == p->C || p->y == p->z)
+        return bad(g, "ssm_scan: y must not overlap the inputs");
     const uint32_t per = p->D / p->groups, block = per >= 256 ? 256 : (per + 63) / 64 * 64;
     const uint32_t tiles = p->groups * ((per + block - 1) / block);
     const uint64_t waves = (uint64_t)p->nseq * tiles * (block / 64);

@@ -441,8 +441,11 @@ FP4_TILE(64, 128, 2, 2, 4, 3, true, 64x128_glu)
 FP4_TILE(64, 64, 2, 2, 4, 3, false, 64x64)
 
 /* Two f32 values as three bf16 terms each, packed: the upper 16 bits of what is left, so that the terms add up to all 24
- * significant bits (of an infinity the first term is infinite and the others are finite) */
+ * significant bits (of an infinity the first term is infinite and the others are finite; a NaN is made quiet, whose
+ * mark is in the upper half) */
 __device__ __forceinline__ void split3(float a, float b, u32 (&t)[3]) {
+    a = __builtin_canonicalizef(a);
+    b = __builtin_canonicalizef(b);
 #pragma unroll
     for (int k = 0; k < 3; ++k) {
         t[k] = __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302);

@@ -279,6 +279,16 @@ def test_w4_infinite_row(gpu, m):
     np.testing.assert_array_equal(got[1], [np.nan] + [np.inf] * 7 + [np.nan] + [-np.inf] * 7)
 
 
+@pytest.mark.parametrize("m", [3, 9, 40, 200])
+def test_w4_signalling_nan(gpu, m):
+    """A NaN whose payload lies in its lower half alone is a NaN in its row, no infinity."""
+    w = random_rows(np.random.default_rng(m), 64, 200)
+    x = np.ones((m, 200), np.float32)
+    x.view(np.uint32)[1, 77] = 0x7F800001
+    got = _product(gpu, "w4", x, w)
+    assert np.isnan(got[1]).all() and np.isfinite(np.delete(got, 1, 0)).all()
+
+
 @KINDS
 def test_product_is_repeatable_and_captures(gpu, kind):
     """The same bits from every replay of a captured product, with other work between the replays."""

@@ -72,6 +72,7 @@ def test_conv_refusals(ctx):
         return L.nk_causal_conv(ctx.h, x, typ, ldx, w, bias, state, slots, seqs, nseq, max_rows, y, ldy, m, d, taps, act)
 
     assert call(nseq=0) == 0 and call(d=0) == 0
+    ctx.refused(call(x=P, y=P), "Y must not overlap X")
     for bad in (dict(seqs=None), dict(seqs=P + 4), dict(nseq=65536), dict(state=None), dict(state=P + 2), dict(slots=1 << 31),
                 dict(max_rows=(1 << 30) + 1), dict(d=(1 << 28) + 1, ldx=1 << 29, ldy=1 << 29)):
         ctx.refused(call(**bad), "sequences")
@@ -96,6 +97,9 @@ def test_scan_refusals(ctx):
                 [{k: 99} for k in ("ldx", "lddt", "ldz", "ldy")] +
                 [dict(type=1, x=P + 1), dict(type=2), dict(ldbc=31), dict(N=0), dict(N=65, ldbc=200), dict(groups=0), dict(groups=3)]):
         ctx.refused(call(**bad), "ssm_scan")
+    for k in ("x", "dt", "B", "C", "z"):
+        far = dict(x=P + 4096, dt=P + 8192, B=P + 12288, C=P + 16384, z=P + 20480)
+        ctx.refused(call(**dict(far, **{k: P})), "y must not overlap the inputs")
     assert L.nk_ssm_scan(ctx.h, None) == -1
 
 
