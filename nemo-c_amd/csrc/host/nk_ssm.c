@@ -96,11 +96,13 @@ int nk_ssm_scan(gpu_t *g, const nk_scan_t *p) {
     if (waves < 1100 && (uint64_t)p->max_rows * (1100 - waves) > 18000) {
         /* about 4096 wavefronts (four per SIMD: 8192 rows of one stream 335 us with 1024, 210 with 2048, 168), and
          * pieces of some sqrt(r / 2) rows, between the pieces' time and that of joining them (512 rows: pieces of
-         * 4, 8, 16 and 32 rows 45, 34, 31 and 42 us; 32 rows: 17.8, 20.8, 27.4, 30.1).  By the rows there are: sequences
-         * shorter than the longest fill no pieces (12 of 1 to 1000 rows, 1536 channels: 136 us by max_rows, 111 so) */
+         * 4, 8, 16 and 32 rows 45, 34, 31 and 42 us; 32 rows: 17.8, 20.8, 27.4, 30.1).  By the rows there are, a
+         * sequence's last piece being half one: beyond 4096 the rest takes a round of its own (8 sequences of 0 to 2000
+         * rows 241 us without the halves, 186 with them; 5 of up to 4000 192 / 155, 12 of up to 1000 114 / 102). */
         const uint64_t all = (uint64_t)p->nseq * p->max_rows, rows = all < p->M ? all : p->M;
-        uint32_t piece = 8;
-        while (4096ull * piece < rows * (waves / p->nseq) || 2ull * piece * piece < p->max_rows) piece += 8;
+        const uint64_t fill = rows * (waves / p->nseq) / (4096 - waves / 2);
+        uint32_t piece = (uint32_t)fill / 4 * 4 + 4;
+        while (piece < 8 || 2ull * piece * piece < p->max_rows) piece += 4;
         const uint32_t pieces = (p->max_rows + piece - 1) / piece;
         /* places for all sequences' pieces, or, where that is fewer (one long sequence among many short ones, max_rows far
          * above the longest), for one of each `piece` rows */
@@ -108,13 +110,16 @@ int nk_ssm_scan(gpu_t *g, const nk_scan_t *p) {
         a.byrow = byrow < table;
         a.ws = gpu_scratch_ws(g, (size_t)(a.byrow ? byrow : table) * (p->N + 1) * p->D);
         if (!a.ws) return bad(g, "ssm_scan: scratch unavailable (size it before capture)");
+        /* workgroups for the pieces that there can be, numbered over all sequences (a sequence of no rows has one) */
+        const uint64_t most = rows / piece + p->nseq;
+        const uint32_t all_pieces = (uint32_t)(most < table ? most : table);
         a.piece = piece;
         a.pieces = pieces;
         snprintf(name, sizeof name, "scan_ends_%s_%u", type, ns);
-        if (gpu_launch(g, name, &a, sizeof a, tiles, p->nseq, pieces, block, 1, 1)) return -1;
+        if (gpu_launch(g, name, &a, sizeof a, tiles, all_pieces, 1, block, 1, 1)) return -1;
         if (gpu_launch(g, "scan_join", &a, sizeof a, (p->D + 255) / 256, p->N, p->nseq, 256, 1, 1)) return -1;
         snprintf(name, sizeof name, "scan_from_%s_%u", type, ns);
-        return gpu_launch(g, name, &a, sizeof a, tiles, p->nseq, pieces, block, 1, 1);
+        return gpu_launch(g, name, &a, sizeof a, tiles, all_pieces, 1, block, 1, 1);
     }
     snprintf(name, sizeof name, "scan_%s_%u", type, ns);
     return gpu_launch(g, name, &a, sizeof a, tiles, p->nseq, 1, block, 1, 1);
