@@ -179,9 +179,20 @@ __device__ __forceinline__ void scan_rows(const NkScanArgs &a, const seq_t &s, u
     for (u32 u = t0; u < t1; u += SCAN_TILE) {
         const u32 rows = min(t1 - u, (u32)SCAN_TILE);
         __syncthreads();
-        for (u32 i = threadIdx.x; i < (rows + 3) / 4 * 4 * W; i += blockDim.x) {
-            const u32 r = i / W, n = i % W, m = n % NS;
-            lds[i] = r < rows && m < a.N ? ld_row((n < NS ? B : C) + (u64)(u + r) * a.ldbc + m) : 0.0f;
+        constexpr int L = 8; /* loads in flight (from places past the end: of the last) */
+        const u32 all = (rows + 3) / 4 * 4 * W;
+        for (u32 i0 = threadIdx.x; i0 < all; i0 += L * blockDim.x) {
+            float v[L];
+#pragma unroll
+            for (u32 k = 0; k < L; ++k) {
+                const u32 i = i0 + k * blockDim.x, r = min(i / W, rows - 1), n = i % W;
+                v[k] = ld_row((n < NS ? B : C) + (u64)(u + r) * a.ldbc + min(n % NS, a.N - 1));
+            }
+#pragma unroll
+            for (u32 k = 0; k < L; ++k) {
+                const u32 i = i0 + k * blockDim.x;
+                if (i < all) lds[i] = i / W < rows && i % NS < a.N ? v[k] : 0.0f;
+            }
         }
         __syncthreads();
         /* four rows at a time, the next four's loads in flight; past the end a step of zero, which leaves the states
