@@ -166,7 +166,8 @@ __device__ __forceinline__ void scan_rows(const NkScanArgs &a, const seq_t &s, u
                                           float (&h)[NS], float &sum, float *lds) {
     const T *x = (const T *)a.x + (u64)s.first * a.ldx, *dt = (const T *)a.dt + (u64)s.first * a.lddt;
     const T *B = (const T *)a.B + (u64)s.first * a.ldbc + (u64)g * a.N, *C = (const T *)a.C + (u64)s.first * a.ldbc + (u64)g * a.N;
-    const T *z = a.z ? (const T *)a.z + (u64)s.first * a.ldz : nullptr;
+    const u32 ldz = a.z ? a.ldz : a.ldx; /* no gate: x is read in its place, and not used */
+    const T *z = a.z ? (const T *)a.z + (u64)s.first * a.ldz : x;
     T *y = (T *)a.y + (u64)s.first * a.ldy;
     const float skip = a.skip ? a.skip[d] : 0.0f, db = a.dt_bias ? a.dt_bias[d] : 0.0f;
     constexpr u32 W = ENDS ? NS : 2 * NS;
@@ -196,7 +197,8 @@ __device__ __forceinline__ void scan_rows(const NkScanArgs &a, const seq_t &s, u
         }
         __syncthreads();
         /* four rows at a time, the next four's loads in flight; past the end a step of zero, which leaves the states
-         * as they are */
+         * as they are.  What is the same for all rows (softplus, the gate) is asked once for the four: a branch a row
+         * keeps the rows' chains of instructions apart. */
         float xn[4], pn[4], zn[4];
         auto load = [&](u32 r0) {
 #pragma unroll
@@ -204,28 +206,31 @@ __device__ __forceinline__ void scan_rows(const NkScanArgs &a, const seq_t &s, u
                 const u64 t = u + min(r0 + k, rows - 1);
                 xn[k] = ld_row(x + t * a.ldx + d);
                 pn[k] = ld_row(dt + t * a.lddt + d);
-                if constexpr (!ENDS) zn[k] = z ? ld_row(z + t * a.ldz + d) : 0.0f;
+                if constexpr (!ENDS) zn[k] = ld_row(z + t * ldz + d);
             }
         };
         load(0);
 #pragma unroll 1
         for (u32 r0 = 0; r0 < rows; r0 += 4) {
-            float xv[4], pv[4], zv[4];
+            float xv[4], p[4], zv[4], o[4];
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
                 xv[k] = xn[k];
-                pv[k] = pn[k];
+                p[k] = pn[k] + db;
                 if constexpr (!ENDS) zv[k] = zn[k];
             }
             load(r0 + 4);
+            if (a.softplus)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) p[k] = softplus_f(p[k]);
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
                 const bool in = r0 + k < rows;
-                float p = a.softplus ? softplus_f(pv[k] + db) : pv[k] + db, v = p * xv[k];
-                p = in ? p : 0.0f;
+                float v = p[k] * xv[k];
+                p[k] = in ? p[k] : 0.0f;
                 v = in ? v : 0.0f;
-                if constexpr (ENDS) sum += p;
-                float o = 0.0f;
+                if constexpr (ENDS) sum += p[k];
+                o[k] = 0.0f;
                 const floatx4 *bc = (const floatx4 *)(lds + (r0 + k) * W);
 #pragma unroll
                 for (int n = 0; n < NS; n += 4) {
@@ -234,15 +239,20 @@ __device__ __forceinline__ void scan_rows(const NkScanArgs &a, const seq_t &s, u
                     if constexpr (!ENDS) c = bc[(NS + n) / 4];
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        h[n + e] = fmaf(__builtin_amdgcn_exp2f(p * A[n + e]), h[n + e], v * b[e]);
-                        if constexpr (!ENDS) o = fmaf(c[e], h[n + e], o);
+                        h[n + e] = fmaf(__builtin_amdgcn_exp2f(p[k] * A[n + e]), h[n + e], v * b[e]);
+                        if constexpr (!ENDS) o[k] = fmaf(c[e], h[n + e], o[k]);
                     }
                 }
-                if constexpr (!ENDS) {
-                    o = fmaf(skip, xv[k], o);
-                    if (z) o *= silu_q(zv[k]);
-                    if (live && in) st_row(y + (u64)(u + r0 + k) * a.ldy + d, o);
-                }
+                if constexpr (!ENDS) o[k] = fmaf(skip, xv[k], o[k]);
+            }
+            if constexpr (!ENDS) {
+                if (a.z)
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) o[k] *= silu_q(zv[k]);
+                if (live)
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                        if (r0 + k < rows) st_row(y + (u64)(u + r0 + k) * a.ldy + d, o[k]);
             }
         }
     }
