@@ -161,7 +161,7 @@ __device__ __forceinline__ float scan_rate(float A) {
  * operations, three of them where only the ends are wanted.  8192 rows of 2048 channels of 16 states, bf16: ends 64
  * us, rows 95, the joining between them 13, where those operations alone are 43 and 52 us at the 30 T products/s that
  * this card reaches; the softplus, the gate and the conversions of every row are the rest. */
-template <typename T, int NS, bool ENDS>
+template <typename T, int NS, bool ENDS, bool WHOLE>
 __device__ __forceinline__ void scan_rows(const NkScanArgs &a, const seq_t &s, u32 t0, u32 t1, u32 g, u32 d, bool live,
                                           float (&h)[NS], float &sum, float *lds) {
     const T *x = (const T *)a.x + (u64)s.first * a.ldx, *dt = (const T *)a.dt + (u64)s.first * a.lddt;
@@ -186,6 +186,7 @@ __device__ __forceinline__ void scan_rows(const NkScanArgs &a, const seq_t &s, u
             float v[L];
 #pragma unroll
             for (u32 k = 0; k < L; ++k) {
+                if (!WHOLE && k && i0 - threadIdx.x + k * blockDim.x >= all) break; /* pieces of a few rows */
                 const u32 i = i0 + k * blockDim.x, r = min(i / W, rows - 1), n = i % W;
                 v[k] = ld_row((n < NS ? B : C) + (u64)(u + r) * a.ldbc + min(n % NS, a.N - 1));
             }
@@ -342,7 +343,7 @@ template <typename T, int NS, int PART> __device__ __forceinline__ void scan_imp
             h[n] = (u32)n < a.N ? v : 0.0f;
         }
     }
-    scan_rows<T, NS, PART == 1>(a, s, t0, t1, c.g, c.d, c.live, h, sum, lds);
+    scan_rows<T, NS, PART == 1, PART == 0>(a, s, t0, t1, c.g, c.d, c.live, h, sum, lds);
     if (!c.live || (PART != 1 && (s.to < 0 || t1 < s.rows))) return;
     float *to = PART == 1 ? ws : a.state + ((u64)s.to * a.D + c.d) * a.N;
 #pragma unroll
