@@ -79,28 +79,31 @@ int nk_ssm_scan(gpu_t *g, const nk_scan_t *p) {
     char name[32];
     gpu_next_bytes(g, (double)size * p->M * (4.0 * p->D + 2.0 * p->groups * p->N) + 8.0 * p->nseq * p->D * p->N);
     gpu_next_flops(g, (double)p->M * p->D * (7.0 * p->N + 12));
-    /* states over lanes for few rows r, by wavefronts w of 64 channels (2048 channels of 16 states, f32, graph replays):
-     * 4 + r max(0.42, 0.0012 w) us against 8 + 0.0067 w + r (0.5 + 0.0001 w) with the states in one lane: 32 w 8 r 7.0
-     * / 12.0, 24 r 13.6 / 19.9; 1024 w 8 r 14.6 / 16.9, 16 r 24.1 / 21.3; 8192 w 4 r 55 / 68, 8 r 95 / 73.  Beyond
-     * 32 rows a few wavefronts are split (64 r 21.0). */
-    if (p->max_rows <= 32 && (double)p->max_rows * (12.0 * (double)waves - 5000.0) < 40000.0 + 67.0 * (double)waves) {
+    /* Estimates in us by wavefronts w of 64 channels, rows r of the longest sequence and R there can be, fitted to graph
+     * replays with 16 states: states over lanes (few rows), sequences whole with the states in one lane, split along
+     * their rows (every exponential twice, three launches).  Few / whole: 32 w 16 r 14.1 / 17.0, 32 r 22.7 / 23.7; 1024 w
+     * 8 r 14.6 / 16.6, 16 r 21.2 / 21.0; 8192 w 4 r 44.5 / 73, 8 r 79 / 78.  Whole / split: 32 w 48 r 31 / 20, 1024 r
+     * 466 / 50; 512 w 64 r 39.8 / 51, 600 r 283 / 185; 768 w 256 r 127 / 143, 600 r 284 / 249; 1024 w 600 r 287 / 337, of
+     * ragged sequences with half the rows 281 / 188; 2048 w 2000 r, ragged, 1158 / 923. */
+    const uint64_t all = (uint64_t)p->nseq * p->max_rows, R = all < p->M ? all : p->M;
+    const double w = (double)waves, r = p->max_rows, x = (double)R * (double)(waves / p->nseq);
+    const double few = 4.0 + r * (w < 350.0 ? 0.42 : 0.0012 * w), whole = 10.0 + 0.0045 * w + r * (0.39 + 0.0001 * w);
+    const double split = 24.0 + 0.0005 * x + 0.0003 * (x < 65536.0 ? x : 65536.0) + 0.03 * p->nseq;
+    if (p->max_rows <= 32 && few < whole) {
         uint32_t q = 1;
         while (4 * q < p->N) q *= 2;
         snprintf(name, sizeof name, "scan_few_%s_%u", type, q);
         return gpu_launch(g, name, &a, sizeof a, (uint32_t)(((uint64_t)p->D * q + 255) / 256), p->nseq, 1, 256, 1, 1);
     }
-    /* split or whole, by wavefronts w and rows r (2048 channels of 16 states, bf16, graph replays): whole takes
-     * 10 + r (0.55 + 0.00025 w) us (a row of one wavefront is a chain of 0.55 us, few wavefronts hide none of it), split
-     * 19 + 0.00075 w r (every exponential twice, three launches).  Whole / split: 32 w 16 r 17.6 / 20.7, 32 r 26.7 /
-     * 20.8, 8192 r 7622 / 168; 512 w 16 r 18.9 / 28.5, 128 r 107 / 67; 1024 w 64 r 61.6 / 71, 256 r 252 / 166 */
-    if (waves < 1100 && (uint64_t)p->max_rows * (1100 - waves) > 18000) {
-        /* about 4096 wavefronts (four per SIMD: 8192 rows of one stream 335 us with 1024, 210 with 2048, 168), and
-         * pieces of some sqrt(r / 2) rows, between the pieces' time and that of joining them (512 rows: pieces of
-         * 4, 8, 16 and 32 rows 45, 34, 31 and 42 us; 32 rows: 17.8, 20.8, 27.4, 30.1).  By the rows there are, a
-         * sequence's last piece being half one: beyond 4096 the rest takes a round of its own (8 sequences of 0 to 2000
-         * rows 241 us without the halves, 186 with them; 5 of up to 4000 192 / 155, 12 of up to 1000 114 / 102). */
-        const uint64_t all = (uint64_t)p->nseq * p->max_rows, rows = all < p->M ? all : p->M;
-        const uint64_t fill = rows * (waves / p->nseq) / (4096 - waves / 2);
+    if (split < whole && p->nseq <= 4096) {
+        /* about 4096 wavefronts (four per SIMD: 8192 rows of one stream 335 us with 1024, 210 with 2048, 168), twice that
+         * where each has enough to do (32 ragged sequences of up to 600 rows 202 / 188, 2000 rows 1297 / 923; 24 of 64 rows
+         * 64 / 79), and pieces of some sqrt(r / 2) rows, between the pieces' time and that of joining them (512 rows:
+         * pieces of 4, 8, 16 and 32 rows 45, 34, 31 and 42 us; 32 rows: 17.8, 20.8, 27.4, 30.1).  By the rows there are, a
+         * sequence's last piece being half one: beyond the aim the rest takes a round of its own (8 sequences of 0 to
+         * 2000 rows 241 us without the halves, 186 with them; 5 of up to 4000 192 / 155, 12 of up to 1000 114 / 102). */
+        const uint64_t aim = x < 250000.0 ? 4096 : 8192;
+        const uint64_t fill = R * (waves / p->nseq) / ((aim < waves ? waves : aim) - waves / 2);
         uint32_t piece = (uint32_t)fill / 4 * 4 + 4;
         while (piece < 8 || 2ull * piece * piece < p->max_rows) piece += 4;
         const uint32_t pieces = (p->max_rows + piece - 1) / piece;
@@ -111,7 +114,7 @@ int nk_ssm_scan(gpu_t *g, const nk_scan_t *p) {
         a.ws = gpu_scratch_ws(g, (size_t)(a.byrow ? byrow : table) * (p->N + 1) * p->D);
         if (!a.ws) return bad(g, "ssm_scan: scratch unavailable (size it before capture)");
         /* workgroups for the pieces that there can be, numbered over all sequences (a sequence of no rows has one) */
-        const uint64_t most = rows / piece + p->nseq;
+        const uint64_t most = R / piece + p->nseq;
         const uint32_t all_pieces = (uint32_t)(most < table ? most : table);
         a.piece = piece;
         a.pieces = pieces;
