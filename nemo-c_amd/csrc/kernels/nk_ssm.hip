@@ -158,8 +158,8 @@ __device__ __forceinline__ float scan_rate(float A) {
  * sum of the steps are wanted, no rows are written.
  *
  * Bound by the vector units: per state and row an exponential, which takes the time of 1.85 products, and four more
- * operations, three of them where only the ends are wanted.  8192 rows of 2048 channels of 16 states, bf16: ends 64
- * us, rows 95, the joining between them 13, where those operations alone are 43 and 52 us at the 30 T products/s that
+ * operations, three of them where only the ends are wanted.  8192 rows of 2048 channels of 16 states, bf16: ends 66
+ * us, rows 85, the joining between them 15, where those operations alone are 43 and 52 us at the 30 T products/s that
  * this card reaches; the softplus, the gate and the conversions of every row are the rest. */
 template <typename T, int NS, bool ENDS, bool WHOLE>
 __device__ __forceinline__ void scan_rows(const NkScanArgs &a, const seq_t &s, u32 t0, u32 t1, u32 g, u32 d, bool live,
