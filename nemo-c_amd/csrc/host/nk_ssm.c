@@ -69,7 +69,7 @@ int nk_ssm_scan(gpu_t *g, const nk_scan_t *p) {
     const uint32_t per = p->D / p->groups, block = per >= 256 ? 256 : (per + 63) / 64 * 64;
     const uint32_t tiles = p->groups * ((per + block - 1) / block);
     const uint64_t waves = (uint64_t)p->nseq * tiles * (block / 64);
-    NkScanArgs a = { p->x, p->dt, p->B, p->C, p->z, p->y, p->A, p->skip, p->dt_bias, p->state, p->seqs, NULL,
+    NkScanArgs a = { p->x, p->dt, p->B, p->C, p->z, p->y, p->A, p->skip, p->dt_bias, p->state, p->seqs, NULL, NULL,
                      p->ldx, p->lddt, p->ldbc, p->ldz, p->ldy, p->slots, p->nseq, p->max_rows, p->M, p->D, p->N,
                      p->groups, p->softplus != 0, 0, 0, 0,
                      p->N % 4 == 0 && aligned(p->A, 16) && aligned(p->state, 16) };
@@ -111,8 +111,10 @@ int nk_ssm_scan(gpu_t *g, const nk_scan_t *p) {
          * above the longest), for one of each `piece` rows */
         const uint64_t table = (uint64_t)p->nseq * pieces, byrow = ((uint64_t)p->M + piece - 1) / piece + 1;
         a.byrow = byrow < table;
-        a.ws = gpu_scratch_ws(g, (size_t)(a.byrow ? byrow : table) * (p->N + 1) * p->D);
+        const uint64_t places = (a.byrow ? byrow : table) * (p->N + 1) * p->D;
+        a.ws = gpu_scratch_ws(g, (size_t)(places + (uint64_t)p->nseq * p->N * p->D));
         if (!a.ws) return bad(g, "ssm_scan: scratch unavailable (size it before capture)");
+        a.first = a.ws + places;
         /* workgroups for the pieces that there can be, numbered over all sequences (a sequence of no rows has one) */
         const uint64_t most = R / piece + p->nseq;
         const uint32_t all_pieces = (uint32_t)(most < table ? most : table);

@@ -534,6 +534,7 @@ typedef struct {
     float *state;     /* [slots][D][N] */
     const int *seqs;
     float *ws;        /* split sequences: per piece N states, then the sum of the steps, of D channels */
+    float *first;     /* and per sequence the N states it goes on from */
     u32 ldx, lddt, ldbc, ldz, ldy, slots, nseq, max_rows, M, D, N, groups, softplus;
     u32 piece, pieces, byrow, vec; /* byrow: places in ws by the rows; vec: four states are read and written at once */
 } NkScanArgs;

@@ -316,7 +316,7 @@ __device__ __forceinline__ bool scan_find(const NkScanArgs &a, u32 p, seq_t &s, 
 
 /* PART 0: whole sequences.  PART 1: the states that the pieces of a.piece rows end in from zero, and their
  * sums of steps (of all but a sequence's last, which nothing follows).  PART 2: the pieces again from the
- * states that scan_join has put in their predecessors' places. */
+ * states that scan_join has put in their predecessors' places, a sequence's first from the copy of its slot. */
 template <typename T, int NS, int PART> __device__ __forceinline__ void scan_impl(const NkScanArgs &a) {
     __shared__ float lds[SCAN_TILE * NS * (PART == 1 ? 1 : 2)];
     seq_t s;
@@ -334,12 +334,14 @@ template <typename T, int NS, int PART> __device__ __forceinline__ void scan_imp
     float *ws = PART ? scan_place(a, i, s, piece) + c.d : nullptr;
 #pragma unroll
     for (int n = 0; n < NS; ++n) h[n] = 0.0f;
-    const bool joined = PART == 2 && t0;
+    /* the slot of a sequence of several pieces may be written by its last before its first reads it */
+    const bool joined = PART == 2 && t0, kept = PART == 2 && !t0 && s.rows > a.piece;
     if (joined || (PART != 1 && !t0 && s.from >= 0)) {
-        const float *from = joined ? ws - (u64)(a.N + 1) * a.D : a.state + ((u64)s.from * a.D + c.d) * a.N;
+        const float *from = joined ? ws - (u64)(a.N + 1) * a.D : kept ? a.first + (u64)i * a.N * a.D + c.d
+                                                                       : a.state + ((u64)s.from * a.D + c.d) * a.N;
 #pragma unroll
         for (int n = 0; n < NS; ++n) {
-            const float v = from[min((u32)n, a.N - 1) * (joined ? (u64)a.D : 1)];
+            const float v = from[min((u32)n, a.N - 1) * (joined || kept ? (u64)a.D : 1)];
             h[n] = (u32)n < a.N ? v : 0.0f;
         }
     }
@@ -369,6 +371,7 @@ extern "C" __global__ __launch_bounds__(256) void scan_join(const NkScanArgs a) 
     if (!s.ok || d >= a.D || s.rows <= a.piece) return;
     const float A = 0.5f * scan_rate(a.A[(u64)d * a.N + n]);
     float h = s.from >= 0 ? a.state[((u64)s.from * a.D + d) * a.N + n] : 0.0f;
+    if (s.from >= 0) a.first[((u64)blockIdx.z * a.N + n) * a.D + d] = h;
     const u32 ends = (s.rows - 1) / a.piece; /* pieces that another follows */
     const u64 step = (u64)(a.N + 1) * a.D;
     float *w = scan_place(a, blockIdx.z, s, 0) + d;

@@ -402,6 +402,27 @@ def test_scan_skewed_batch(gpu, typ, D, N, max_rows):
     c.free()
 
 
+@pytest.mark.parametrize("D,N,G", [(24, 16, 1), (40, 5, 2), (70, 8, 1), (12, 33, 3), (9, 64, 1)])
+@pytest.mark.parametrize("typ", [F32, BF16])
+def test_scan_many_sequences(gpu, typ, D, N, G):
+    """Thousands of sequences, most of them tokens or empty, a few of several tiles, in any order: each whole."""
+    rng = np.random.default_rng([D, N])
+    lens = np.concatenate([rng.integers(0, 3, 4196), [130, 64, 65, 41]])
+    seqs, M = _seqs(lens.tolist(), [((-1, i)[i % 2], i if i % 3 else -1) for i in range(len(lens))], 1)
+    seqs = np.ascontiguousarray(seqs[rng.permutation(len(seqs))])
+    k = (D + typ) % 3
+    o = operands(rng, typ, M, D, N, G, len(lens), z=k != 0, skip=k != 1, db=k != 2)
+    check_scan(gpu, typ, o, seqs, 130, pad=3 * (k == 1))
+
+
+@pytest.mark.parametrize("rows", [36, 129])
+def test_scan_whole_of_wide_rows(gpu, rows):
+    """Enough channels and sequences that a split does not pay."""
+    rng = np.random.default_rng(rows)
+    seqs, M = _seqs([rows] * 60, [(i, i) for i in range(60)])
+    check_scan(gpu, BF16, operands(rng, BF16, M, 512, 16, 1, 60), seqs, rows)
+
+
 @pytest.mark.parametrize("rows", [3, 37, 90, 601])
 def test_scan_forgets_at_once(gpu, rows):
     """A of -infinity: every row's state is its own input's, also where rows do not fill a tile."""
