@@ -50,8 +50,9 @@ int nk_fp4_dequant(gpu_t *g, const uint8_t *Q, uint32_t ldq, const uint8_t *S, u
  *   16 x 8192 x 2048 6.1 us, 32 rows 8.1, 64 rows 11.9, 64 x 8192 x 4096 21.0 / 9.7;
  *   w4 (steps of 64) 2048 x 4096 x 8192 and x 2048, 1024 x 4096 x 2048, 448 x 4096 x 1024, 448 x 1024 x 4096: 128x256
  *   316, 87, 73, 38, 118, 64x256 342, 92, 50, 23, 67, 64x128 390, 103, 55, 19, 48, 32x64 565, 143, 76, 23, 31; few rows
- *   (16 to a workgroup, one launch of them for 17 and more) against 32x64: 32 x 4096 x 1024 9.4 / 10.2, 48 rows 12.9 /
- *   10.4, 32 x 4096 x 4096 19.5 / 29.8, 64 rows 35.6 / 30.0, 128 x 1024 x 4096 19.5 / 30.2. */
+ *   (16 to a workgroup, one launch of them for 17 and more) with 16 and 32 columns against 32x64: 32 x 4096 x 1024 9.7,
+ *   6.7 / 10.2, 48 rows 13.0, 10.6 / 10.2, 32 x 4096 x 4096 19.6, 12.7 / 30.3, 32 x 16384 x 1024 33, 20 / 11.7, 128 x 1024
+ *   x 4096 19.9, 12.9 / 30.8, 64 x 1024 x 4096 10.9, 11.9 / 29.1. */
 typedef struct { const char *name; uint16_t bm, bn, threads, percu; float fix, lat, thr; } tile_t;
 static const tile_t fp4_tiles[] = {
     { "128x256", 128, 256, 768, 1, 10.0f, 1.0f, 1.0f },
@@ -101,12 +102,16 @@ static int product(gpu_t *g, NkGemm4Args *a) {
     const tile_t *t = NULL;
     if (a->A) t = tile_pick(w4_tiles, 4, a->M, nout, (a->K + 63) / 64, glu, &us);
     else if (a->K > 384) t = tile_pick(fp4_tiles, 3, a->M, nout, (a->K + 255) / 256, glu, &us); /* four scales a load */
-    /* few rows, 16 output columns to a workgroup: 4-bit rows up to 64 at a time, f32 rows 16 (wide matrices 32 columns) */
-    const uint32_t G = (a->K + 127) / 128, ti = a->M <= 16 ? 1 : a->M <= 32 ? 2 : 4;
-    const uint32_t wide = a->A && !glu && nout > 4096, co = wide ? 32 : 16, rows = a->A ? (a->M + 15) / 16 : 1;
-    const uint64_t wgs = (uint64_t)rows * ((nout + co - 1) / co);
-    const float each = a->A ? 2.0f + (glu || wide ? 0.28f : 0.21f) * (float)G : 0.75f + (0.08f + 0.05f * (float)ti) * (float)G;
-    const float few = 1.5f + (float)((wgs + 255) / 256) * each;
+    /* few rows, 16 output columns to a workgroup: 4-bit rows up to 64 at a time, f32 rows 16 (or 32 columns, where that
+     * takes fewer rounds of workgroups; up to five rows share a CU, there from 4096 columns on).  GLU: 16 and their gates */
+    const uint32_t G = (a->K + 127) / 128, ti = a->M <= 16 ? 1 : a->M <= 32 ? 2 : 4, rows = a->A ? (a->M + 15) / 16 : 1;
+    const uint64_t wg16 = (uint64_t)rows * ((nout + 15) / 16), wg32 = (uint64_t)rows * ((nout + 31) / 32);
+    const float one = a->A ? 2.3f + 0.215f * (float)G : 0.75f + (0.08f + 0.05f * (float)ti) * (float)G;
+    const float two = 2.6f + 0.26f * (float)G;
+    const float few16 = 1.5f + (float)((wg16 + 255) / 256) * (a->A && glu ? two : one);
+    const float few32 = 1.8f + (float)((wg32 + 255) / 256) * two;
+    const uint32_t wide = a->A && !glu && (a->M <= 5 ? nout > 4096 : few32 < few16), co = wide ? 32 : 16;
+    const float few = wide ? few32 : few16;
     if ((a->A ? a->M <= 16 : a->M <= 64 && !t) || ((a->A || a->M <= 64) && few < us)) {
         snprintf(name, sizeof name, "gemm_%s_few%u%s", kind, a->A ? (a->M <= 5 ? 5u : 16u) : 16 * ti, glu ? gl : wide ? "x2" : "");
         return gpu_launch(g, name, a, sizeof *a, (nout + co - 1) / co, rows, 1, 512, 1, 1);

@@ -548,7 +548,9 @@ template <int TI, int TJ, bool GLU> __device__ __forceinline__ void fp4_few(cons
  * row), split, and put into the wavefront's part of LDS as fragments (read as fragments from global memory each lane is a
  * line of its own, and all 16 rows of a fragment are split: 8192 x 2048 of one row 6.2 us against 5.6; 5 rows now
  * take 6.2 us and 16 rows 8.6).
- * PACK: at most five rows, whose terms lie in rows m, 5 + m and 10 + m of one fragment. */
+ * PACK: at most five rows, whose terms lie in rows m, 5 + m and 10 + m of one fragment.  Otherwise 16 rows a workgroup, two
+ * column tiles where that saves a round of workgroups (32 x 4096 x 4096 13 us, 19.6 with one; 32 rows a workgroup on four
+ * wavefronts 25). */
 template <int TJ, bool GLU, bool PACK> __device__ __forceinline__ void w4_few(NkGemm4Args a) {
     if (!PACK) { /* 16 rows a workgroup */
         a.A += (u64)blockIdx.y * 16 * a.lda;

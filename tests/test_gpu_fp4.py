@@ -236,6 +236,15 @@ def test_product_widest_tiles(gpu, kind, m, n, k, act):
     _check(gpu, kind, m, n, k, act, True, act == NONE)
 
 
+@pytest.mark.parametrize("m,n,k", [(24, 4090, 2300), (6, 8190, 1100), (50, 2047, 4100)])
+@pytest.mark.parametrize("act", [NONE, SILU, GLU])
+def test_w4_few_rows_of_wide_weights(gpu, m, n, k, act):
+    """Rows by 16 and columns by 32, both cut off."""
+    n -= act == GLU and n % 2
+    _check(gpu, "w4", m, n, k, act, True, True, 0.5, ldc=n + 3, pad=2, off=1)
+    _check(gpu, "w4", m, n, k, act, False, True, 1.0, ldc=-(-n // 4) * 4 + 4, pad=1)
+
+
 @KINDS
 @pytest.mark.parametrize("m,n,k", [(3, 70, 200), (40, 70, 200), (200, 262, 384)])
 @pytest.mark.parametrize("act", [NONE, GLU])
