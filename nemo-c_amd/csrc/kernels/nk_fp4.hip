@@ -441,21 +441,39 @@ FP4_TILE(64, 128, 2, 2, 4, 3, true, 64x128_glu)
 FP4_TILE(64, 64, 2, 2, 4, 3, false, 64x64)
 
 /* Two f32 values as three bf16 terms each, packed: the upper 16 bits of what is left, so that the terms add up to all 24
- * significant bits (of an infinity the first term is infinite and the others are finite; a NaN is made quiet, whose
- * mark is in the upper half) */
-__device__ __forceinline__ void split3(float a, float b, u32 (&t)[3]) {
-    a = __builtin_canonicalizef(a);
-    b = __builtin_canonicalizef(b);
+ * significant bits (what is below 2^-133, the least bf16, is dropped).  FINITE: neither is an infinity or NaN.  Else of an
+ * infinity the first term is infinite and the others are zero: anything else times large weights could pass the type's
+ * range with the other sign.  What is left of a NaN is a quiet NaN, also where its mark is in the lower half alone. */
+template <bool FINITE> __device__ __forceinline__ void split3(float a, float b, u32 (&t)[3]) {
+    if (!FINITE) asm("" : "+v"(a), "+v"(b)); /* else what both have in common moves ahead of the question, into registers */
+    const bool ia = !FINITE && __builtin_isinf(a), ib = !FINITE && __builtin_isinf(b);
 #pragma unroll
     for (int k = 0; k < 3; ++k) {
         t[k] = __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302);
         a -= __uint_as_float(__float_as_uint(a) & 0xffff0000u);
         b -= __uint_as_float(__float_as_uint(b) & 0xffff0000u);
         if (k == 0) {
-            a = __builtin_amdgcn_fmed3f(a, -1.32922800e36f, 1.32922800e36f);
-            b = __builtin_amdgcn_fmed3f(b, -1.32922800e36f, 1.32922800e36f);
+            a = ia ? 0.0f : a;
+            b = ib ? 0.0f : b;
         }
     }
+}
+/* Calls split(finite) for the values x[0 .. n - 1] of the wavefront's lanes, finite saying whether all are: half an
+ * instruction a value to ask, where the care for the others takes two (448 x 1024 x 4096 on tiles of 32 x 64: 33.7 us, 35.5
+ * with care in every split).  ASK: without the question, for the few values of up to five rows (8192 x 2048 of one
+ * row 5.6 us, 5.7 with it). */
+template <bool ASK, int N, typename F> __device__ __forceinline__ void split_rows(const floatx4 (&x)[N], u32 n, F split) {
+    if constexpr (ASK) {
+        float top = 0.0f; /* the maximum that NaN wins */
+#pragma unroll
+        for (int l = 0; l < N; ++l) {
+            if ((u32)l >= n) break;
+            top = __builtin_elementwise_maximum(__builtin_elementwise_maximum(top, fabsf(x[l][0])), fabsf(x[l][1]));
+            top = __builtin_elementwise_maximum(__builtin_elementwise_maximum(top, fabsf(x[l][2])), fabsf(x[l][3]));
+        }
+        if (!__builtin_amdgcn_ballot_w64(!(top < __builtin_inff()))) return split(const_t<1>());
+    }
+    split(const_t<0>());
 }
 /* 8 codes as bf16 values, exact */
 __device__ __forceinline__ uint4 fp4_bf16x8(u32 q, float f) {
@@ -597,19 +615,21 @@ template <int TJ, bool GLU, bool PACK> __device__ __forceinline__ void w4_few(Nk
     floatx4 acc[1][TJ] = {};
     for (u32 g = wv; g < G; g += FEW_WAVES) {
         __builtin_amdgcn_wave_barrier();
+        split_rows<!PACK>(x, (a.M + 1) / 2, [&](auto finite) {
 #pragma unroll
-        for (int l = 0; l < RL; ++l) {
-            if (2 * (u32)l >= a.M) break;
-            u32 p[3], q[3];
-            split3(x[l][0], x[l][1], p);
-            split3(x[l][2], x[l][3], q);
-            const u32 m = 2 * l + half;
+            for (int l = 0; l < RL; ++l) {
+                if (2 * (u32)l >= a.M) break;
+                u32 p[3], q[3];
+                split3<decltype(finite)::v>(x[l][0], x[l][1], p);
+                split3<decltype(finite)::v>(x[l][2], x[l][3], q);
+                const u32 m = 2 * l + half;
 #pragma unroll
-            for (int k = 0; k < 3; ++k) {
-                const u32 row = PACK ? min(m, 5u) + 5 * k : m; /* PACK: row 5 of a load overwrites nothing it should not */
-                if (!PACK || m < 5) *(uint2 *)(frag + (PACK ? 0 : k * 4096) + row * 256 + ((i4 / 2) ^ row) * 16 + (i4 & 1) * 8) = make_uint2(p[k], q[k]);
+                for (int k = 0; k < 3; ++k) {
+                    const u32 row = PACK ? min(m, 5u) + 5 * k : m; /* PACK: row 5 of a load overwrites nothing it should not */
+                    if (!PACK || m < 5) *(uint2 *)(frag + (PACK ? 0 : k * 4096) + row * 256 + ((i4 / 2) ^ row) * 16 + (i4 & 1) * 8) = make_uint2(p[k], q[k]);
+                }
             }
-        }
+        });
         uint4 b[TJ];
         u32 q[TJ][4];
         float s[TJ];
@@ -704,15 +724,17 @@ __device__ __forceinline__ void gemm_w4_tile(const NkGemm4Args &a, char *const s
         };
         auto put = [&](const regs &g, u32 q) {
             char *st = smem + (q & 1) * STAGE;
+            split_rows<true>(g.x, LA, [&](auto finite) {
 #pragma unroll
-            for (int j = 0; j < LA; ++j) {
-                u32 lo[3], hi[3];
-                split3(g.x[j][0], g.x[j][1], lo);
-                split3(g.x[j][2], g.x[j][3], hi);
-                const u32 row = p / 16 + j * PW * 4, i4 = p % 16, at = row * 128 + ((i4 / 2) ^ swz_h(row)) * 16 + (i4 & 1) * 8;
+                for (int j = 0; j < LA; ++j) {
+                    u32 lo[3], hi[3];
+                    split3<decltype(finite)::v>(g.x[j][0], g.x[j][1], lo);
+                    split3<decltype(finite)::v>(g.x[j][2], g.x[j][3], hi);
+                    const u32 row = p / 16 + j * PW * 4, i4 = p % 16, at = row * 128 + ((i4 / 2) ^ swz_h(row)) * 16 + (i4 & 1) * 8;
 #pragma unroll
-                for (int k = 0; k < 3; ++k) *(uint2 *)(st + k * PLANE + at) = make_uint2(lo[k], hi[k]);
-            }
+                    for (int k = 0; k < 3; ++k) *(uint2 *)(st + k * PLANE + at) = make_uint2(lo[k], hi[k]);
+                }
+            });
 #pragma unroll
             for (int j = 0; j < LW; ++j) *(uint4 *)(st + CODES + (p + j * PW * 64) * 16) = g.w[j];
 #pragma unroll
@@ -788,15 +810,17 @@ __device__ __forceinline__ void gemm_w4_tile(const NkGemm4Args &a, char *const s
     }
     tile_out<GLU, TI, TJ>(a, m0 + wm * WTM, c0 + n0, acc);
 }
-#define W4_TILE(BM, BN, WGM, WGN, PW, AHEAD, GLU, NAME)                                                       \
-    extern "C" __global__ __launch_bounds__(64 * (WGM * WGN + PW)) void gemm_w4_##NAME(const NkGemm4Args a) { \
-        __shared__ __attribute__((aligned(1024))) char smem[2 * (BM * 384 + BN * 36)];                        \
-        gemm_w4_tile<BM, BN, WGM, WGN, PW, AHEAD, GLU>(a, smem);                                               \
+/* SIMD: wavefronts on a SIMD with the workgroups that the LDS of a CU holds (the widest tiles: one; 32 x 64 keeps three
+ * registers in memory for it, outside its loops) */
+#define W4_TILE(BM, BN, WGM, WGN, PW, AHEAD, SIMD, GLU, NAME)                                                       \
+    extern "C" __global__ __launch_bounds__(64 * (WGM * WGN + PW), SIMD) void gemm_w4_##NAME(const NkGemm4Args a) { \
+        __shared__ __attribute__((aligned(1024))) char smem[2 * (BM * 384 + BN * 36)];                              \
+        gemm_w4_tile<BM, BN, WGM, WGN, PW, AHEAD, GLU>(a, smem);                                                    \
     }
-W4_TILE(128, 256, 2, 4, 4, 2, false, 128x256)
-W4_TILE(128, 256, 2, 4, 4, 2, true, 128x256_glu)
-W4_TILE(64, 128, 2, 2, 4, 4, false, 64x128)
-W4_TILE(64, 128, 2, 2, 4, 4, true, 64x128_glu)
-W4_TILE(32, 64, 1, 2, 2, 4, false, 32x64)
-W4_TILE(64, 256, 2, 4, 4, 3, false, 64x256)
-W4_TILE(64, 256, 2, 4, 4, 3, true, 64x256_glu)
+W4_TILE(128, 256, 2, 4, 4, 2, 3, false, 128x256)
+W4_TILE(128, 256, 2, 4, 4, 2, 3, true, 128x256_glu)
+W4_TILE(64, 128, 2, 2, 4, 4, 4, false, 64x128)
+W4_TILE(64, 128, 2, 2, 4, 4, 4, true, 64x128_glu)
+W4_TILE(32, 64, 1, 2, 2, 4, 4, false, 32x64)
+W4_TILE(64, 256, 2, 4, 4, 3, 3, false, 64x256)
+W4_TILE(64, 256, 2, 4, 4, 3, 3, true, 64x256_glu)

@@ -288,6 +288,24 @@ def test_w4_infinite_row(gpu, m):
     np.testing.assert_array_equal(got[1], [np.nan] + [np.inf] * 7 + [np.nan] + [-np.inf] * 7)
 
 
+@pytest.mark.parametrize("m,n", [(3, 16), (4, 4112), (9, 16), (24, 4096), (40, 16), (200, 16)])
+@pytest.mark.parametrize("scale,count", [(140, 1), (127, 48), (252, 1)])
+def test_w4_infinite_row_of_large_weights(gpu, m, n, scale, count):
+    """An infinite value stays one however large its weights are, and however many it has."""
+    k = 64
+    code = np.zeros((n, 128), np.uint8)
+    code[:, 3:3 + count] = (np.arange(n) % 16)[:, None]
+    w = (code[:, 0::2] | code[:, 1::2] << 4, np.full((n, 4), scale, np.uint8))
+    x = np.zeros((m, k), np.float32)
+    x[1, 3:3 + count] = np.inf
+    x[2, 3] = -np.inf
+    got = _product(gpu, "w4", x, w)
+    want = np.tile(np.array([np.nan] + [np.inf] * 7 + [np.nan] + [-np.inf] * 7, np.float32), n // 16)
+    assert not np.delete(got, (1, 2), 0).any()
+    np.testing.assert_array_equal(got[1], want)
+    np.testing.assert_array_equal(got[2], -want)
+
+
 @pytest.mark.parametrize("m", [3, 9, 40, 200])
 def test_w4_signalling_nan(gpu, m):
     """A NaN whose payload lies in its lower half alone is a NaN in its row, no infinity."""
