@@ -155,13 +155,14 @@ __device__ __forceinline__ float scan_rate(float A) {
  * e^(s A) is 2^(s A log2 e) by the hardware's exponential (results below 2^-126 come out as 0).  B and C are the
  * same for every channel of the workgroup's group: a tile of their rows lies in LDS as f32, padded
  * with zeros to NS, and is read by all lanes at one address.  ENDS: only the states (from zero) and the
- * sum of the steps are wanted, no rows are written.
+ * sum of the steps are wanted, no rows are written.  CARE: the states that fill N up to NS, zero as long as the inputs are
+ * finite and NaN after an infinite one, are left out of the outputs.
  *
  * Bound by the vector units: per state and row an exponential, which takes the time of 1.85 products, and four more
  * operations, three of them where only the ends are wanted.  8192 rows of 2048 channels of 16 states, bf16: ends 66
  * us, rows 85, the joining between them 15, where those operations alone are 43 and 52 us at the 30 T products/s that
  * this card reaches; the softplus, the gate and the conversions of every row are the rest. */
-template <typename T, int NS, bool ENDS, bool WHOLE>
+template <typename T, int NS, bool ENDS, bool WHOLE, bool CARE>
 __device__ __forceinline__ void scan_rows(const NkScanArgs &a, const seq_t &s, u32 t0, u32 t1, u32 g, u32 d, bool live,
                                           float (&h)[NS], float &sum, float *lds) {
     const T *x = (const T *)a.x + (u64)s.first * a.ldx, *dt = (const T *)a.dt + (u64)s.first * a.lddt;
@@ -241,7 +242,7 @@ __device__ __forceinline__ void scan_rows(const NkScanArgs &a, const seq_t &s, u
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
                         h[n + e] = fmaf(__builtin_amdgcn_exp2f(p[k] * A[n + e]), h[n + e], v * b[e]);
-                        if constexpr (!ENDS) o[k] = fmaf(c[e], h[n + e], o[k]);
+                        if constexpr (!ENDS) o[k] = !CARE || (u32)(n + e) < a.N ? fmaf(c[e], h[n + e], o[k]) : o[k];
                     }
                 }
                 if constexpr (!ENDS) o[k] = fmaf(skip, xv[k], o[k]);
@@ -332,20 +333,30 @@ template <typename T, int NS, int PART> __device__ __forceinline__ void scan_imp
     if (PART == 1 && t0 + a.piece >= s.rows) return;
     float h[NS], sum = 0.0f;
     float *ws = PART ? scan_place(a, i, s, piece) + c.d : nullptr;
-#pragma unroll
-    for (int n = 0; n < NS; ++n) h[n] = 0.0f;
     /* the slot of a sequence of several pieces may be written by its last before its first reads it */
     const bool joined = PART == 2 && t0, kept = PART == 2 && !t0 && s.rows > a.piece;
-    if (joined || (PART != 1 && !t0 && s.from >= 0)) {
-        const float *from = joined ? ws - (u64)(a.N + 1) * a.D : kept ? a.first + (u64)i * a.N * a.D + c.d
-                                                                       : a.state + ((u64)s.from * a.D + c.d) * a.N;
+    auto start = [&] {
 #pragma unroll
-        for (int n = 0; n < NS; ++n) {
-            const float v = from[min((u32)n, a.N - 1) * (joined || kept ? (u64)a.D : 1)];
-            h[n] = (u32)n < a.N ? v : 0.0f;
+        for (int n = 0; n < NS; ++n) h[n] = 0.0f;
+        if (joined || (PART != 1 && !t0 && s.from >= 0)) {
+            const float *from = joined ? ws - (u64)(a.N + 1) * a.D : kept ? a.first + (u64)i * a.N * a.D + c.d
+                                                                           : a.state + ((u64)s.from * a.D + c.d) * a.N;
+#pragma unroll
+            for (int n = 0; n < NS; ++n) {
+                const float v = from[min((u32)n, a.N - 1) * (joined || kept ? (u64)a.D : 1)];
+                h[n] = (u32)n < a.N ? v : 0.0f;
+            }
         }
+    };
+    start();
+    scan_rows<T, NS, PART == 1, PART == 0, false>(a, s, t0, t1, c.g, c.d, c.live, h, sum, lds);
+    /* An input that is not finite makes the filling states NaN, and they stay so: the rows again without them.  Asked once
+     * behind the rows, which costs 0 to 2%; asked for every four rows it took up to 70 registers, and a wavefront less on
+     * every SIMD. */
+    if (PART != 1 && __builtin_expect(a.N < NS, 0) && __builtin_expect(__syncthreads_or(h[NS - 1] != h[NS - 1]), 0)) {
+        start();
+        scan_rows<T, NS, false, PART == 0, true>(a, s, t0, t1, c.g, c.d, c.live, h, sum, lds);
     }
-    scan_rows<T, NS, PART == 1, PART == 0>(a, s, t0, t1, c.g, c.d, c.live, h, sum, lds);
     if (!c.live || (PART != 1 && (s.to < 0 || t1 < s.rows))) return;
     float *to = PART == 1 ? ws : a.state + ((u64)s.to * a.D + c.d) * a.N;
 #pragma unroll

@@ -479,6 +479,61 @@ def test_scan_not_finite(gpu, rows):
     assert np.isnan(s[0, 7]).all()
 
 
+def plain_scan(o, seqs, softplus):
+    """Rows and states of the recurrence in 64 bits, infinities and NaN as they come."""
+    M, D = o["x"].shape
+    G, N = o["B"].shape[1:]
+    y, new = np.zeros((M, D)), o["state"].copy()
+    with np.errstate(all="ignore"):
+        for first, n, a0, b0 in seqs:
+            h = o["state"][a0].copy() if a0 >= 0 else np.zeros((D, N))
+            for t in range(first, first + n):
+                v = o["dt"][t] + (o["dt_bias"] if o["dt_bias"] is not None else 0)
+                s = (np.maximum(v, 0) + np.log1p(np.exp(-np.abs(v))) if softplus else v)[:, None]
+                h = np.exp(s * o["A"]) * h + s * np.repeat(o["B"][t], D // G, 0) * o["x"][t][:, None]
+                y[t] = (np.repeat(o["C"][t], D // G, 0) * h).sum(1)
+                if o["skip"] is not None:
+                    y[t] += o["skip"] * o["x"][t]
+                if o["z"] is not None:
+                    y[t] *= o["z"][t] * _sig(o["z"][t])
+            if b0 >= 0:
+                new[b0] = h
+    return y, new
+
+
+def same_kind(got, want):
+    """NaN where the recurrence has it, infinities with its sign, finite elsewhere."""
+    np.testing.assert_array_equal(np.isnan(got), np.isnan(want))
+    np.testing.assert_array_equal(np.where(np.isinf(got), got, 0), np.where(np.isinf(want), want, 0))
+
+
+@pytest.mark.parametrize("N", [1, 3, 5, 8, 11, 16, 24, 33])
+@pytest.mark.parametrize("rows,nseq", [(4, 2), (40, 2), (90, 60), (600, 2)])
+@pytest.mark.parametrize("typ", [F32, BF16])
+def test_scan_infinite_inputs(gpu, N, rows, nseq, typ):
+    """Infinite inputs and steps give what the recurrence gives, whatever the number of states and whichever kernel
+    runs: rows with the states over lanes, whole sequences, split ones.  Channels beside them keep their bits."""
+    rng = np.random.default_rng([N, rows])
+    D = 512 if nseq > 2 else 96
+    seqs, M = _seqs([rows] * nseq, [(i, i) for i in range(nseq)])
+    o = operands(rng, typ, M, D, N, 1, nseq)
+    o["dt_bias"] = _kept(-4 + 0.3 * rng.standard_normal(D), F32)
+    clean = ScanCall(gpu, typ, o, seqs, rows, 1)
+    y0, s0 = clean.run()
+    clean.free()
+    o["x"][1, 7], o["x"][rows // 2, 9], o["x"][2, 30], o["dt"][rows + 1, 40] = np.inf, -np.inf, np.nan, np.inf
+    o["B"][rows + 2, 0, N - 1] = np.inf
+    o["B"][rows + 2, 0, :N - 1] = 0
+    c = ScanCall(gpu, typ, o, seqs, rows, 1)
+    y, s = c.run()
+    c.free()
+    want, new = plain_scan(o, seqs, 1)
+    same_kind(_back(y[:M, :D], typ), want)
+    same_kind(s, new)
+    np.testing.assert_array_equal(y[:rows, 50:D], y0[:rows, 50:D])
+    np.testing.assert_array_equal(s[0, 50:], s0[0, 50:])
+
+
 def test_scan_in_pieces(gpu):
     """A sequence fed in pieces of any length, tokens among them, in one slot: the whole's result within the bounds."""
     rng = np.random.default_rng(8)
