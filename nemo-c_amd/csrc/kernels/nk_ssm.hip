@@ -373,14 +373,18 @@ SCAN(u16, bf16, 8) SCAN(u16, bf16, 16) SCAN(u16, bf16, 32) SCAN(u16, bf16, 64)
 
 /* The pieces of a sequence one after another: H <- e^(A sum) H + end, the state that the next piece starts from,
  * takes the place of the piece's own end.  The factor by halves: a piece of growing steps may pass 2^128 by itself where
- * no state does, and one that is zero stays so whatever the factor.  One thread per state; the loads of JOIN pieces are in flight at a time
- * (one at a time 36 us for 128 pieces of 2048 channels, a memory round trip each). */
+ * no state does, and one that is zero stays so whatever the factor.  An infinite state stays infinite: the factor may be
+ * below the type's range where no row's is (but not where a step or the rate is infinite: zero times infinity there too).
+ * One thread per state; the loads of JOIN pieces are in flight at a time (one at a time 36 us for 128 pieces of 2048
+ * channels, a memory round trip each). */
 #define JOIN 16
 extern "C" __global__ __launch_bounds__(256) void scan_join(const NkScanArgs a) {
     const seq_t s = seq_load(a.seqs, blockIdx.z, a.M, a.max_rows, a.slots);
     const u32 d = blockIdx.x * 256 + threadIdx.x, n = blockIdx.y;
     if (!s.ok || d >= a.D || s.rows <= a.piece) return;
-    const float A = 0.5f * scan_rate(a.A[(u64)d * a.N + n]);
+    const float rate = a.A[(u64)d * a.N + n], A = 0.5f * scan_rate(rate);
+    enum { ZEROS = 0x60, INFS = 0x204 }; /* classes of the values whatever the factor */
+    const u32 kept = __builtin_isinf(rate) ? ZEROS : ZEROS | INFS;
     float h = s.from >= 0 ? a.state[((u64)s.from * a.D + d) * a.N + n] : 0.0f;
     if (s.from >= 0) a.first[((u64)blockIdx.z * a.N + n) * a.D + d] = h;
     const u32 ends = (s.rows - 1) / a.piece; /* pieces that another follows */
@@ -398,7 +402,8 @@ extern "C" __global__ __launch_bounds__(256) void scan_join(const NkScanArgs a) 
         for (u32 k = 0; k < JOIN; ++k) {
             if (i + k >= ends) break;
             const float e = __builtin_amdgcn_exp2f(sum[k] * A);
-            h = h == 0.0f ? end[k] : fmaf(e, e * h, end[k]);
+            const u32 keep = fabsf(sum[k]) < __builtin_inff() ? kept : ZEROS;
+            h = __builtin_amdgcn_classf(h, (int)keep) ? h + end[k] : fmaf(e, e * h, end[k]);
             w[(i + k) * step + (u64)n * a.D] = h;
         }
     }

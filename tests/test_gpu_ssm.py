@@ -534,6 +534,28 @@ def test_scan_infinite_inputs(gpu, N, rows, nseq, typ):
     np.testing.assert_array_equal(s[0, 50:], s0[0, 50:])
 
 
+@pytest.mark.parametrize("rows", [20, 200, 600])
+def test_scan_infinite_state_is_kept(gpu, rows):
+    """A state that is infinite stays so over any number of rows, of long steps too, as it does row by row; a rate of
+    -infinity makes it NaN."""
+    rng = np.random.default_rng(rows)
+    seqs, M = _seqs([rows, rows], [(0, 0), (1, 1)])
+    o = operands(rng, F32, M, 64, 16, 1, 2, db=False)
+    o["A"] = _kept(np.full((64, 16), -16.0), F32)
+    o["B"], o["C"], o["skip"] = np.abs(o["B"]), np.abs(o["C"]) + 0.1, np.abs(o["skip"])
+    o["z"] = np.abs(o["z"]) + 0.1
+    o["dt"] = np.full((M, 64), 1.0)  # e^-16 a row
+    o["x"][3, 7], o["state"][1, 20, 4], o["x"][rows + 1, 33] = np.inf, -np.inf, np.inf
+    o["A"][33, 2] = -np.inf
+    c = ScanCall(gpu, F32, o, seqs, rows, 0)
+    y, s = c.run()
+    c.free()
+    want, new = plain_scan(o, seqs, 0)
+    same_kind(y[:M], want)
+    same_kind(s, new)
+    assert np.isposinf(y[rows - 1, 7]) and np.isneginf(s[1, 20, 4]) and np.isnan(s[1, 33, 2]) and np.isposinf(s[1, 33, 1])
+
+
 def test_scan_in_pieces(gpu):
     """A sequence fed in pieces of any length, tokens among them, in one slot: the whole's result within the bounds."""
     rng = np.random.default_rng(8)
