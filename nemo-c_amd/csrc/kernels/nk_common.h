@@ -56,6 +56,8 @@ __device__ __forceinline__ float div_ge1(float n, float d) { return div_by_rcp(n
  * 3.8e-8 in 2-norm over |v| <= 1. */
 __device__ __forceinline__ float div_1pexp(float n, float d) { return div_by_rcp(n, d, 0.25f * __builtin_amdgcn_rcpf(0.25f * d)); }
 __device__ __forceinline__ float sigmoid_f(float v) { return div_1pexp(1.0f, 1.0f + expf(-v)); }
+/* max(v, 0), NaN where v is */
+__device__ __forceinline__ float relu_nan(float v) { return __builtin_elementwise_maximum(v, 0.0f); }
 __device__ __forceinline__ float silu_f(float v) { return div_1pexp(v, 1.0f + expf(-v)); }
 
 /* Butterfly sum over the 64 lanes of a wavefront; every lane ends with the same total. */

@@ -129,7 +129,7 @@ __device__ __forceinline__ void fp4_store4(const NkGemm4Args &a, u32 m, u32 n, u
         for (int e = 0; e < 4; ++e) s[e] = silu_f(s[e]);
     else if (a.act == NK_ACT_RELU)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) s[e] = fmaxf(s[e], 0.0f);
+        for (int e = 0; e < 4; ++e) s[e] = relu_nan(s[e]);
     if (m >= a.M || n >= nout) return;
     float *c = a.C + (u64)m * a.ldc + n;
     if (a.vec && n + 4 <= nout) {

@@ -111,7 +111,7 @@ template <typename T, int TAPS, int V> __device__ __forceinline__ void cconv_imp
 #pragma unroll
                 for (int j = 0; j < TAPS; ++j) o[e] = fmaf(w[j][e], v[k + j][e], o[e]);
                 if (a.act == NK_ACT_SILU) o[e] = silu_q(o[e]);
-                else if (a.act == NK_ACT_RELU) o[e] = fmaxf(o[e], 0.0f);
+                else if (a.act == NK_ACT_RELU) o[e] = relu_nan(o[e]);
             }
             if (t + k < end) store_row(y + (u64)(t + k) * a.ldy + d, o);
         }

@@ -274,6 +274,23 @@ def test_product_not_finite(gpu, kind, m):
     assert np.isfinite(got[~bad]).all()
 
 
+@KINDS
+@pytest.mark.parametrize("m", [2, 20, 300])
+@pytest.mark.parametrize("act", [SILU, RELU, GLU])
+def test_activations_keep_nan(gpu, kind, m, act):
+    """A NaN goes through every activation: what the quantisation marks in a block is not lost."""
+    rng = np.random.default_rng([m, act])
+    n, k = 160, 420
+    w = random_rows(rng, n, k)
+    w[1][17, 3] = 255
+    x = rng.standard_normal((m, k)).astype(np.float32)
+    x[1, 5] = np.inf if kind == "fp4" else np.nan
+    got = _product(gpu, kind, (*quant(x), k) if kind == "fp4" else x, w, act=act)
+    bad = np.zeros(got.shape, bool)
+    bad[1], bad[:, 17] = True, True
+    np.testing.assert_array_equal(np.isnan(got), bad)
+
+
 @pytest.mark.parametrize("m", [3, 9, 40, 200])
 def test_w4_infinite_row(gpu, m):
     """An infinite value of a row meets weights of either sign: infinite with the product's sign, NaN against zeros."""

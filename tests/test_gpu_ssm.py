@@ -181,6 +181,20 @@ def test_silu_of_far_values(gpu, typ):
             check(r)
 
 
+@pytest.mark.parametrize("typ", [F32, BF16])
+@pytest.mark.parametrize("act", [0, 1, 2])
+def test_conv_keeps_nan(gpu, typ, act):
+    """A NaN reaches the rows of its channel that its taps reach, through every activation."""
+    rng = np.random.default_rng(act)
+    D, n = 70, 40
+    x, w = rng.standard_normal((n, D)), 1 + rng.standard_normal((D, 3)).astype(np.float32) ** 2
+    x[11, 5] = np.nan
+    y, _ = run_conv(gpu, typ, x, w, None, np.zeros((1, 2, D)), np.array([[0, n, -1, -1]], np.int32), n, n, act)
+    bad = np.zeros((n, D), bool)
+    bad[11:14, 5] = True
+    np.testing.assert_array_equal(np.isnan(_back(y[:n], typ)), bad)
+
+
 def test_conv_in_pieces(gpu):
     """A sequence fed in pieces of any length, in one slot, gives the bits of the whole."""
     rng = np.random.default_rng(5)
