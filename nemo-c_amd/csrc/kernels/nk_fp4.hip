@@ -211,6 +211,11 @@ __device__ __forceinline__ void dma16_at(const unsigned char *base, u32 off, lds
     const u32 m = __builtin_amdgcn_readfirstlane((u32)(size_t)lds);
     asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(m) : "memory");
 }
+/* and 4 bytes per lane into [lds + 4 i, +4) */
+__device__ __forceinline__ void dma4_at(const unsigned char *base, u32 off, lds_char_t *lds) {
+    const u32 m = __builtin_amdgcn_readfirstlane((u32)(size_t)lds);
+    asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dword %0, %1" ::"v"(off), "s"(base), "s"(m) : "memory");
+}
 __device__ __forceinline__ const unsigned char *uniform_ptr(const unsigned char *p) {
     const u32 lo = __builtin_amdgcn_readfirstlane((u32)(u64)p), hi = __builtin_amdgcn_readfirstlane((u32)((u64)p >> 32));
     return (const unsigned char *)((u64)hi << 32 | lo);
@@ -266,7 +271,8 @@ __device__ __forceinline__ void tile_out(const NkGemm4Args &a, u32 m0, u32 c0, c
  * its own: 139 us for 3584 x 4096 x 8192 on 128 x 128 tiles where this took 88); granule g of row r lies in slot
  * g ^ (r / 2 % 8), so a fragment read (one granule of 32 rows per half of the wavefront) is free of bank conflicts.
  * Scales come by 16 bytes of a row for two steps, and are read by 8 for one (a byte per fragment: 88 us, 74 with
- * no scales at all).
+ * no scales at all; by two times 4, as groups at odd places would need: 5% more).  Those of an odd last group come by
+ * themselves, 4 bytes of a row.
  *
  * Bound by the loads from L2 at many rows: 2048 x 4096 x 8192 38.4 us (3.6 PFLOP/s; its products alone 15, with the
  * fragment reads 29), 3584 x 4096 x 8192 74 to 80; tiles of 128 x 128, 256 x 128 and 256 x 256 in other splits over
@@ -274,15 +280,16 @@ __device__ __forceinline__ void tile_out(const NkGemm4Args &a, u32 m0, u32 c0, c
 template <int BM, int BN, int WGM, int WGN, int PW, int NS, bool GLU>
 __device__ __forceinline__ void gemm_fp4_tile(const NkGemm4Args &a, lds_char_t *const smem) {
     constexpr int NW = PW, WTM = BM / WGM, WTN = BN / WGN, TI = WTM / 32, TJ = WTN / 32;
-    constexpr u32 ROWS = BM + BN, STAGE = ROWS * 128, SCALES = NS * STAGE, CHUNK = ROWS * 16;
     constexpr int NC = NS / 2 + 1;                     /* chunks of scales: a stage's and those ahead of it */
+    constexpr u32 ROWS = BM + BN, STAGE = ROWS * 128, SCALES = NS * STAGE, CHUNK = ROWS * 16, LAST = SCALES + NC * CHUNK;
     constexpr int LI = ROWS / 8 / NW;                  /* loads of codes per wavefront and stage */
     constexpr int LS = (ROWS / 64 + NW - 1) / NW;      /* loads of scales, of 64 rows of one operand (the last may repeat one) */
-    static_assert(LI * NW * 8 == ROWS && BM % 64 == 0 && (GLU ? BN / 2 : BN) % 64 == 0 && NS >= 2 && (NS - 1) * (LI + LS) < 64, "tile shape");
+    static_assert(LI * NW * 8 == ROWS && BM % 64 == 0 && (GLU ? BN / 2 : BN) % 64 == 0 && NS >= 2 && (NS - 1) * (LI + LS) + LS < 64, "tile shape");
     const u32 tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const bool loader = wave >= WGM * WGN;
     const u32 wv = loader ? wave - WGM * WGN : wave, wm = wv / WGN, wn = wv % WGN, r = lane & 31, f = lane >> 5;
     const u32 nout = GLU ? a.N / 2 : a.N, G = (a.K + 127) / 128, S = (G + 1) / 2;
+    const u32 even = (G - 4) & ~1u; /* the last group that a load of four groups' scales begins at: reads of 8 are aligned */
     constexpr u32 CO = GLU ? BN / 2 : BN; /* output columns of a tile */
     const u32 tm = (a.M + BM - 1) / BM, tn = (nout + CO - 1) / CO;
     /* workgroup b runs on XCD b % 8: each XCD takes a run of tiles, by groups of 8 row tiles */
@@ -329,10 +336,14 @@ __device__ __forceinline__ void gemm_fp4_tile(const NkGemm4Args &a, lds_char_t *
                 base[j] += 128;
             }
             slot = slot + STAGE == NS * STAGE ? 0 : slot + STAGE;
+            if ((G & 1) && q + 1 == S)
+#pragma unroll
+                for (int j = 0; j < LS; ++j)
+                    dma4_at(sbase[j] + 4 * (G - 1), __umul24(min(lane, slast[j]), sld[j]), smem + LAST + (NW * j + wv) % (ROWS / 64) * 256);
             if (q & 1) return;
 #pragma unroll
             for (int j = 0; j < LS; ++j) /* groups 2 q .. 2 q + 3 of 128, or the row's last four */
-                dma16_at(sbase[j] + 4 * min(2 * q, G - 4), __umul24(min(lane, slast[j]), sld[j]),
+                dma16_at(sbase[j] + 4 * min(2 * q, even), __umul24(min(lane, slast[j]), sld[j]),
                          smem + SCALES + chunk * CHUNK + (NW * j + wv) % (ROWS / 64) * 1024);
             chunk = chunk + 1 == NC ? 0 : chunk + 1;
         };
@@ -346,6 +357,7 @@ __device__ __forceinline__ void gemm_fp4_tile(const NkGemm4Args &a, lds_char_t *
     }
     typedef const __attribute__((address_space(3))) uint4 *lds4;
     typedef const __attribute__((address_space(3))) uint2 *lds2;
+    typedef const __attribute__((address_space(3))) u32 *lds1;
     uint4 x[TI], w[TJ];
     uint2 xs[TI], ws[TJ]; /* a step's eight scales of the lane's row, its own in bytes 0 and 2 of each half */
     /* the lane's places in a stage, the tiles' at constant distances: codes and scales of A, and of W */
@@ -358,13 +370,13 @@ __device__ __forceinline__ void gemm_fp4_tile(const NkGemm4Args &a, lds_char_t *
         const uint2 v = *(lds2)p;
         return make_uint2(v.x >> (8 * f), v.y >> (8 * f));
     };
+    /* GLU: the first half of a wavefront's tiles are value columns, the second their gates */
+    auto wcol = [](int j) { return (u32)(GLU && j >= TJ / 2 ? BN / 2 + 32 * (j - TJ / 2) : 32 * j); };
     auto read_w = [&](const lds_char_t *p, const lds_char_t *ps, bool fresh) {
 #pragma unroll
         for (int j = 0; j < TJ; ++j) {
-            /* GLU: the first half of a wavefront's tiles are value columns, the second their gates */
-            const u32 n = GLU && j >= TJ / 2 ? BN / 2 + 32 * (j - TJ / 2) : 32 * j;
-            w[j] = *(lds4)(p + n * 128);
-            if (fresh) ws[j] = scales(ps + n * 16);
+            w[j] = *(lds4)(p + wcol(j) * 128);
+            if (fresh) ws[j] = scales(ps + wcol(j) * 16);
         }
     };
     auto read_x = [&](int i, const lds_char_t *p, const lds_char_t *ps, bool fresh) {
@@ -403,7 +415,7 @@ __device__ __forceinline__ void gemm_fp4_tile(const NkGemm4Args &a, lds_char_t *
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
         barrier_mem();
         st = smem + cur;
-        ss = smem + SCALES + chunk * CHUNK + 4 * (2 * q - min(2 * (q & ~1u), G - 4));
+        ss = smem + SCALES + chunk * CHUNK + min(4 * (2 * q - min(2 * (q & ~1u), even)), 8u); /* an odd last group's: not used */
         cur = cur + STAGE == NS * STAGE ? 0 : cur + STAGE;
         chunk = !(q & 1) ? chunk : chunk + 1 == NC ? 0 : chunk + 1;
     };
@@ -418,11 +430,14 @@ __device__ __forceinline__ void gemm_fp4_tile(const NkGemm4Args &a, lds_char_t *
     }
     /* the last step, whose second half may not exist: zeros then, under scales of one */
     const bool whole = !(G & 1);
+    if (!whole) {
+        auto one = [&](u32 row) { return make_uint2(*(lds1)(smem + LAST + row * 4) >> (8 * f), 0x007f007f); };
+#pragma unroll
+        for (int j = 0; j < TJ; ++j) ws[j] = one(BM + n0 + r + wcol(j));
+#pragma unroll
+        for (int i = 0; i < TI; ++i) xs[i] = one(wm * WTM + r + 32 * i);
+    }
     group(const_t<1>());
-#pragma unroll
-    for (int i = 0; i < TI; ++i) xs[i].y = whole ? xs[i].y : 0x007f007f;
-#pragma unroll
-    for (int j = 0; j < TJ; ++j) ws[j].y = whole ? ws[j].y : 0x007f007f;
     group(const_t<2>(), whole);
     group(const_t<3>(), whole);
 #pragma unroll
@@ -431,7 +446,7 @@ __device__ __forceinline__ void gemm_fp4_tile(const NkGemm4Args &a, lds_char_t *
 }
 #define FP4_TILE(BM, BN, WGM, WGN, PW, NS, GLU, NAME)                                                          \
     extern "C" __global__ __launch_bounds__(64 * (WGM * WGN + PW)) void gemm_fp4_##NAME(const NkGemm4Args a) { \
-        __shared__ __attribute__((aligned(1024))) char smem[(BM + BN) * (NS * 128 + (NS / 2 + 1) * 16)];        \
+        __shared__ __attribute__((aligned(1024))) char smem[(BM + BN) * (NS * 128 + (NS / 2 + 1) * 16 + 4)];    \
         gemm_fp4_tile<BM, BN, WGM, WGN, PW, NS, GLU>(a, (lds_char_t *)smem);                                    \
     }
 FP4_TILE(128, 256, 2, 4, 4, 3, false, 128x256)

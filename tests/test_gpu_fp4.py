@@ -236,6 +236,17 @@ def test_product_widest_tiles(gpu, kind, m, n, k, act):
     _check(gpu, kind, m, n, k, act, True, act == NONE)
 
 
+@KINDS
+@pytest.mark.parametrize("m,n,k,act", [(200, 1000, 513, NONE), (200, 1000, 640, NONE), (200, 1000, 770, NONE), (200, 1000, 640, GLU),
+                                       (1024, 4096, 1152, NONE), (1000, 4090, 1130, NONE), (1000, 8180, 1400, GLU),
+                                       (2040, 4090, 2170, NONE), (1000, 8190, 2170, GLU), (70, 333, 4870, NONE)])
+def test_product_odd_groups(gpu, kind, m, n, k, act):
+    """Rows of an odd number of groups of 128 values (5, 7, 9, 11, 17, 39): the last step of 256 is half one, its
+    scales alone behind the others'."""
+    assert -(-k // 128) % 2 == 1
+    _check(gpu, kind, m, n, k, act, True, act == NONE)
+
+
 @pytest.mark.parametrize("m,n,k", [(24, 4090, 2300), (6, 8190, 1100), (50, 2047, 4100)])
 @pytest.mark.parametrize("act", [NONE, SILU, GLU])
 def test_w4_few_rows_of_wide_weights(gpu, m, n, k, act):
