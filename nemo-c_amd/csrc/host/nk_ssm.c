@@ -41,13 +41,20 @@ int nk_causal_conv(gpu_t *g, const void *X, int type, uint32_t ldx, const float 
      * 33.8 us) */
     uint64_t tile = rows * blocks / 4096 / 8 * 8;
     tile = tile < 8 ? 8 : tile > 64 ? 64 : tile;
-    while ((max_rows + tile - 1) / tile > 65535) tile *= 2;
-    const uint32_t tiles = max_rows ? (uint32_t)((max_rows + tile - 1) / tile) : 1;
+    /* Workgroups for the longest sequence that may be, all sequences alike, but no more than four times what the rows need or
+     * 16384 in all: those with no rows cost 0.45 us a thousand, and a longer sequence goes round (64 tokens with max_rows
+     * 2^12 or 2^18 7.6 us, by the longest alone 112 us and 16 million workgroups; a prompt of 8192 rows beside 63 tokens 55 /
+     * 131, beside 255 132 / 462, with 65536 in all 41 and 62 but the tokens 31). */
+    const uint64_t last = max_rows < M ? max_rows : M, longest = (last + tile - 1) / tile;
+    const uint64_t share = 4 * (rows / tile / nseq + 1), room = 16384 / ((uint64_t)blocks * nseq);
+    uint64_t tiles = share > room ? share : room;
+    if (tiles > longest) tiles = longest;
+    tiles = tiles < 1 ? 1 : tiles > 65535 ? 65535 : tiles;
     NkCconvArgs a = { X, W, bias, state, seqs, Y, ldx, ldy, slots, nseq, max_rows, M, D, taps, (u32)act, (u32)tile };
     char name[24];
     snprintf(name, sizeof name, "cconv_%s_%u", type == NK_F32 ? "f32" : two ? "bf16x2" : "bf16", taps);
     gpu_next_bytes(g, 2.0 * size * M * D + 8.0 * nseq * (taps - 1) * D + 4.0 * D * (taps + 1));
-    return gpu_launch(g, name, &a, sizeof a, blocks, tiles, nseq, 256, 1, 1);
+    return gpu_launch(g, name, &a, sizeof a, blocks, (uint32_t)tiles, nseq, 256, 1, 1);
 }
 
 int nk_ssm_scan(gpu_t *g, const nk_scan_t *p) {

@@ -45,25 +45,29 @@ __device__ __forceinline__ void store_row(u16 *p, const float (&v)[2]) {
     *(u32 *)p = __builtin_bit_cast(u32, __builtin_convertvector((floatx2){ v[0], v[1] }, bf16x2));
 }
 
-/* One thread per channel (bf16: two where rows allow it) and tile of a.tile rows, the last inputs in registers and eight
- * rows' loads in flight: every row is read once (and the taps - 1 before the tile).  Bound by memory: 8192 rows of
- * 2048 channels f32 30 us, bf16 16.  More channels per thread are slower (16 bytes each: 37 and 29 us), their taps being far
- * apart and their threads few.  The tile with the sequence's first row reads the slot's rows and then writes the new
+/* One thread per channel (bf16: two where rows allow it) and tile of a.tile rows (where a sequence has more of them than the
+ * grid, every gridDim.y-th), the last inputs in registers and eight rows' loads in flight: every row is read once (and the
+ * taps - 1 before the tile).  Bound by memory: 8192 rows of 2048 channels f32 30 us, bf16 16.  More channels per thread are
+ * slower (16 bytes each: 37 and 29 us), their taps being far apart and their threads few.  The tile with the sequence's first row reads the slot's rows and then writes the new
  * ones: nothing else touches the slots. */
 template <typename T, int TAPS, int V> __device__ __forceinline__ void cconv_impl(const NkCconvArgs &a) {
     const seq_t s = seq_load(a.seqs, blockIdx.z, a.M, a.max_rows, a.slots);
-    const u32 d = (blockIdx.x * 256 + threadIdx.x) * V, t0 = blockIdx.y * a.tile;
+    const u32 d = (blockIdx.x * 256 + threadIdx.x) * V, step = gridDim.y * a.tile;
+    u32 t0 = blockIdx.y * a.tile, end;
     if (!s.ok || d >= a.D || (t0 && t0 >= s.rows)) return;
     typedef row_t<T, V> row;
     const T *x = (const T *)a.X + (u64)s.first * a.ldx;
     T *y = (T *)a.Y + (u64)s.first * a.ldy;
-    const u32 end = min(t0 + a.tile, s.rows);
     auto load = [&](u32 t) { return *(const row *)(x + (u64)t * a.ldx + d); };
     constexpr int B = 8; /* rows in flight (the tile's last again past its end, not used) */
     row q[B];
-    if (t0 < end)
+    auto first = [&] {
+        end = min(t0 + a.tile, s.rows);
+        if (t0 < end)
 #pragma unroll
-        for (u32 k = 0; k < B; ++k) q[k] = load(min(t0 + k, end - 1));
+            for (u32 k = 0; k < B; ++k) q[k] = load(min(t0 + k, end - 1));
+    };
+    first();
     float w[TAPS][V], b[V], v[TAPS - 1 + B][V]; /* v: the inputs before a batch of B rows, then its own */
 #pragma unroll
     for (int j = 0; j < TAPS; ++j)
@@ -71,9 +75,11 @@ template <typename T, int TAPS, int V> __device__ __forceinline__ void cconv_imp
         for (int e = 0; e < V; ++e) w[j][e] = a.W[(u64)(d + e) * TAPS + j];
 #pragma unroll
     for (int e = 0; e < V; ++e) b[e] = a.bias ? a.bias[d + e] : 0.0f;
-    if (t0)
+    auto before = [&] {
 #pragma unroll
         for (int j = 0; j < TAPS - 1; ++j) widen(v[j], load(t0 + j - (TAPS - 1)));
+    };
+    if (t0) before();
     else
 #pragma unroll
         for (int j = 0; j < TAPS - 1; ++j)
@@ -96,29 +102,35 @@ template <typename T, int TAPS, int V> __device__ __forceinline__ void cconv_imp
 #pragma unroll
             for (int e = 0; e < V; ++e) a.state[((u64)s.to * (TAPS - 1) + j) * a.D + d + e] = n[j][e];
     }
-    for (u32 t = t0; t < end; t += B) {
+    for (;;) {
+        for (u32 t = t0; t < end; t += B) {
 #pragma unroll
-        for (int k = 0; k < B; ++k) widen(v[TAPS - 1 + k], q[k]);
-        if (t + B < end)
+            for (int k = 0; k < B; ++k) widen(v[TAPS - 1 + k], q[k]);
+            if (t + B < end)
 #pragma unroll
-            for (u32 k = 0; k < B; ++k) q[k] = load(min(t + B + k, end - 1));
+                for (u32 k = 0; k < B; ++k) q[k] = load(min(t + B + k, end - 1));
 #pragma unroll
-        for (u32 k = 0; k < B; ++k) {
-            float o[V];
+            for (u32 k = 0; k < B; ++k) {
+                float o[V];
 #pragma unroll
-            for (int e = 0; e < V; ++e) {
-                o[e] = b[e];
+                for (int e = 0; e < V; ++e) {
+                    o[e] = b[e];
 #pragma unroll
-                for (int j = 0; j < TAPS; ++j) o[e] = fmaf(w[j][e], v[k + j][e], o[e]);
-                if (a.act == NK_ACT_SILU) o[e] = silu_q(o[e]);
-                else if (a.act == NK_ACT_RELU) o[e] = relu_nan(o[e]);
+                    for (int j = 0; j < TAPS; ++j) o[e] = fmaf(w[j][e], v[k + j][e], o[e]);
+                    if (a.act == NK_ACT_SILU) o[e] = silu_q(o[e]);
+                    else if (a.act == NK_ACT_RELU) o[e] = relu_nan(o[e]);
+                }
+                if (t + k < end) store_row(y + (u64)(t + k) * a.ldy + d, o);
             }
-            if (t + k < end) store_row(y + (u64)(t + k) * a.ldy + d, o);
+#pragma unroll
+            for (int j = 0; j < TAPS - 1; ++j)
+#pragma unroll
+                for (int e = 0; e < V; ++e) v[j][e] = v[B + j][e];
         }
-#pragma unroll
-        for (int j = 0; j < TAPS - 1; ++j)
-#pragma unroll
-            for (int e = 0; e < V; ++e) v[j][e] = v[B + j][e];
+        t0 += step;
+        if (t0 >= s.rows) return;
+        first();
+        before();
     }
 }
 #define CCONV(T, NAME, TAPS, V) \

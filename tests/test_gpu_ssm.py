@@ -152,6 +152,31 @@ def test_conv_long(gpu, typ, D, more):
     assert (y[M:] == 9).all() and (y[8100] == 9).all() and (y[:, D:] == 9).all()
 
 
+@pytest.mark.parametrize("typ,D,taps", [(F32, 2048, 4), (BF16, 2048, 3), (F32, 70, 2), (BF16, 512, 4)])
+def test_conv_skewed_batch(gpu, typ, D, taps):
+    """One long sequence among hundreds of tokens, in any order, and a max_rows far above it: the long one goes round
+    a grid of fewer tiles, and max_rows changes no bit."""
+    rng = np.random.default_rng(D)
+    lens = np.concatenate([rng.integers(0, 4, 300), [3001, 64, 9]])
+    seqs, M = _seqs(lens.tolist(), [((-1, i)[i % 2], i if i % 3 else -1) for i in range(len(lens))], 1)
+    seqs = np.ascontiguousarray(seqs[rng.permutation(len(seqs))])
+    x, w, b = rng.standard_normal((M, D)), rng.standard_normal((D, taps)).astype(np.float32), rng.standard_normal(D).astype(np.float32)
+    state = rng.standard_normal((len(lens), taps - 1, D)).astype(np.float32)
+    y, st = run_conv(gpu, typ, x, w, b, state, seqs, M, 3001)
+    ref, tol, new = conv_ref(_kept(x, typ), w.astype(np.float64), b.astype(np.float64), state.astype(np.float64), seqs, 1)
+    if typ == BF16:
+        tol = tol + 2.0 ** -8 * (np.abs(ref) + tol)
+    mine = np.zeros(M + 2, bool)
+    for first, n, _, _ in seqs:
+        mine[first:first + n] = True
+    assert (np.abs(_back(y[:M], typ) - ref)[mine[:M]] <= tol[mine[:M]] + 1e-37).all() and (y[~mine] == 9).all()
+    np.testing.assert_array_equal(st, new.astype(np.float32))
+    for max_rows in (1 << 18, 1 << 30):
+        y2, st2 = run_conv(gpu, typ, x, w, b, state, seqs, M, max_rows)
+        np.testing.assert_array_equal(y2, y)
+        np.testing.assert_array_equal(st2, st)
+
+
 @pytest.mark.parametrize("typ", [F32, BF16])
 def test_silu_of_far_values(gpu, typ):
     """SiLU of values down to the lowest: zero there, NaN at -infinity as the quotient gives, in the convolution and
