@@ -153,6 +153,24 @@ def test_dequant_every_code_and_scale(gpu):
         b.free()
 
 
+@pytest.mark.parametrize("m,k,more", [(5, 64, 0), (9, 1000, 0), (9, 1000, 8), (33, 4096, 16), (3, 40, 8), (7, 1003, 5)])
+@pytest.mark.parametrize("typ", [0, 1])
+def test_dequant_rows_of_whole_16_bytes(gpu, m, k, more, typ):
+    """Rows whose values are stored 16 bytes at a time, their last run cut off or not."""
+    ld, dt = k + more, (np.float32, np.uint16)[typ]
+    assert ld % 8 == 0
+    q, s = random_rows(np.random.default_rng([m, k]), m, k)
+    dq, ds, dy = gpu.put(q), gpu.put(s), gpu.put(np.full((m, ld), 7, dt))
+    gpu.begin()
+    gpu.check(_lib().nk_fp4_dequant(gpu.h, dq.ptr, q.shape[1], ds.ptr, s.shape[1], dy.ptr, typ, ld, m, k))
+    gpu.end()
+    y = dy.read((m, ld), dt)
+    assert (y[:, k:] == 7).all()
+    np.testing.assert_array_equal(oracle.bf16_to_f32(y[:, :k]) if typ else y[:, :k], values(q, s, k))
+    for b in (dq, ds, dy):
+        b.free()
+
+
 # ---- products ----------------------------------------------------------------------------------------
 
 
@@ -234,6 +252,21 @@ def test_product_epilogues(gpu, kind, m, n, k, act, bias, resid, alpha):
 def test_product_widest_tiles(gpu, kind, m, n, k, act):
     """Enough outputs for the widest tiles, cut off at every side; an odd number of 128 values."""
     _check(gpu, kind, m, n, k, act, True, act == NONE)
+
+
+@pytest.mark.parametrize("m", [1, 3, 5])
+@pytest.mark.parametrize("n,k", [(4100, 650), (8192, 2048), (5001, 97)])
+@pytest.mark.parametrize("act,bias,resid", [(NONE, True, False), (SILU, False, True)])
+def test_w4_up_to_five_rows_of_wide_weights(gpu, m, n, k, act, bias, resid):
+    """32 columns a workgroup, cut off too."""
+    _check(gpu, "w4", m, n, k, act, bias, resid, 0.5)
+
+
+@pytest.mark.parametrize("m,n,k", [(448, 4096, 1024), (440, 4090, 1000), (500, 4001, 1500)])
+@pytest.mark.parametrize("act,bias,resid", [(NONE, True, True), (SILU, False, False)])
+def test_w4_of_hundreds_of_rows(gpu, m, n, k, act, bias, resid):
+    """Tiles of 64 x 128, cut off too."""
+    _check(gpu, "w4", m, n, k, act, bias, resid, 0.5)
 
 
 @KINDS

@@ -152,6 +152,25 @@ def test_conv_long(gpu, typ, D, more):
     assert (y[M:] == 9).all() and (y[8100] == 9).all() and (y[:, D:] == 9).all()
 
 
+@pytest.mark.parametrize("taps,act", [(2, 2), (3, 1), (3, 0)])
+def test_conv_long_of_fewer_taps(gpu, taps, act):
+    """Two bf16 channels a thread with two and three taps."""
+    rng = np.random.default_rng(taps)
+    D = 2050
+    seqs, M = _seqs([8100, 1, 37, 200], [(0, 0), (3, 3), (-1, 1), (2, 2)], 1)
+    x, w = rng.standard_normal((M, D)), rng.standard_normal((D, taps)).astype(np.float32)
+    b = rng.standard_normal(D).astype(np.float32) if act else None
+    state = rng.standard_normal((4, taps - 1, D)).astype(np.float32)
+    y, st = run_conv(gpu, BF16, x, w, b, state, seqs, M, 8100, act, ldx=2052, ldy=2054)
+    ref, tol, new = conv_ref(_kept(x, BF16), w.astype(np.float64), None if b is None else b.astype(np.float64), state.astype(np.float64),
+                             seqs, act)
+    tol = tol + 2.0 ** -8 * (np.abs(ref) + tol)
+    for first, n, _, _ in seqs:
+        assert (np.abs(_back(y[first:first + n, :D], BF16) - ref[first:first + n]) <= tol[first:first + n] + 1e-37).all()
+    np.testing.assert_array_equal(st, new.astype(np.float32))
+    assert (y[M:] == 9).all() and (y[8100] == 9).all() and (y[:, D:] == 9).all()
+
+
 @pytest.mark.parametrize("typ,D,taps", [(F32, 2048, 4), (BF16, 2048, 3), (F32, 70, 2), (BF16, 512, 4)])
 def test_conv_skewed_batch(gpu, typ, D, taps):
     """One long sequence among hundreds of tokens, in any order, and a max_rows far above it: the long one goes round
@@ -387,6 +406,20 @@ def test_scan(gpu, case, D, N, G, typ):
     k = (case + D) % 4
     o = operands(rng, typ, M, D, N, G, 7, z=k != 0, skip=k != 1, db=k != 2)
     check_scan(gpu, typ, o, seqs, max(lens) + (case % 2) * 40, 1, [0, 8, 3][(case + N) % 3])
+
+
+@pytest.mark.parametrize("case", range(len(SCAN_CASES)))
+@pytest.mark.parametrize("D,N,G", [(64, 17, 1), (100, 20, 2), (96, 32, 3), (70, 31, 1), (260, 32, 1), (66, 48, 1)])
+@pytest.mark.parametrize("typ", [F32, BF16])
+def test_scan_more_states(gpu, case, D, N, G, typ):
+    """17 to 32 states, and 48, in every form."""
+    test_scan(gpu, case, D, N, G, typ)
+
+
+@pytest.mark.parametrize("D,N,G", [(40, 20, 2), (24, 32, 1)])
+@pytest.mark.parametrize("typ", [F32, BF16])
+def test_scan_many_sequences_of_more_states(gpu, typ, D, N, G):
+    test_scan_many_sequences(gpu, typ, D, N, G)
 
 
 @pytest.mark.parametrize("rows", [1, 2, 500])
