@@ -318,9 +318,10 @@ int nk_fp4_quant(gpu_t *g, const void *X, int type, uint32_t ldx, uint8_t *Q, ui
 int nk_fp4_dequant(gpu_t *g, const uint8_t *Q, uint32_t ldq, const uint8_t *S, uint32_t lds, void *X, int type,
                    uint32_t ldx, uint32_t M, uint32_t K);
 /* nk_gemm with 4-bit weights: C[m][n] (= or +=) alpha * act(sum_k A[m][k] W[n][k] + bias[n]), the same
- * activations, any M, N and K; sums in f32.  nk_gemm_fp4: A in 4 bits too (the products are exact).
- * nk_gemm_w4: A f32 rows, 16-byte aligned with lda (in floats) % 4 == 0, with all their 24 bits.  Strides of codes and
- * scales are below 2^24 bytes.  C must not overlap the operands. */
+ * activations (a NaN goes through all of them, ReLU too), up to 1048560 rows, 2^26 weight rows and any K that the strides
+ * hold; sums in f32.  nk_gemm_fp4: A in 4 bits too (the products are exact).  nk_gemm_w4: A f32 rows, 16-byte aligned with
+ * lda (in floats) % 4 == 0, with all their 24 bits down to 2^-133; weights below 2^128 (scales up to 252: what nk_fp4_quant
+ * makes).  Strides of codes and scales are below 2^24 bytes.  C must not overlap the operands. */
 int nk_gemm_fp4(gpu_t *g, const uint8_t *Aq, uint32_t lda, const uint8_t *As, uint32_t ldas, const uint8_t *Wq,
                 uint32_t ldw, const uint8_t *Ws, uint32_t ldws, const float *bias, float *C, uint32_t ldc, uint32_t M,
                 uint32_t N, uint32_t K, int act, int accumulate, float alpha);
@@ -336,7 +337,9 @@ int nk_gemm_w4(gpu_t *g, const float *A, uint32_t lda, const uint8_t *Wq, uint32
  * and no row is in two sequences.
  * A sequence of no rows hands its state on.  Rows that no sequence has are not written.  The rows of a
  * sequence are below M and its slots below `slots`; max_rows is at least the longest sequence: a
- * sequence that breaks these is left out (nothing of it is written).
+ * sequence that breaks these is left out (nothing of it is written).  At most 65535 sequences, 2^27 channels and
+ * max_rows of 2^30; work and scratch go by M, so max_rows may be far above the longest sequence, as in a captured graph
+ * that is replayed with other tables.  Infinities and NaN give what the formulas give, in their sequence and channels alone.
  *
  * nk_causal_conv: Y[t][d] = act(bias[d] + sum_j W[d][j] X[t - (taps - 1) + j][d]) for D channels, with X before
  * the sequence's first row from the slot: state is [slots][taps - 1][D] f32, the last inputs, oldest
@@ -351,7 +354,7 @@ int nk_causal_conv(gpu_t *g, const void *X, int type, uint32_t ldx, const float 
  *   y[t][d] = (sum_n C[t][g][n] h[n] + skip[d] x[t][d]) * SiLU(z[t][d])
  * x, dt, B, C, z, y are rows of one type; B and C rows have the stride ldbc and [groups][N] values (two
  * parts of one projection's rows, say); A [D][N], skip, dt_bias and the state [slots][D][N] are f32.  skip,
- * dt_bias and z (no gate) may be NULL.  y must not overlap the inputs.  Long sequences of few channels are
+ * dt_bias and z (no gate) may be NULL.  Exponentials below 2^-126 are zero.  y must not overlap the inputs.  Long sequences of few channels are
  * split along their rows: the pieces' states lie in the context's scratch (no residual update may be
  * pending; a capture needs the scratch sized by a call before it). */
 typedef struct {

@@ -299,6 +299,33 @@ def test_product_strides_and_room(gpu, kind, m, n, k, act):
 
 
 @KINDS
+@pytest.mark.parametrize("m", [5, 9, 40, 200])
+@pytest.mark.parametrize("k", [128, 640])
+def test_product_of_far_scales(gpu, kind, m, k):
+    """Rows and weights under scales from the least to the largest (of f32 rows' weights those below 2^128), every pair of
+    them whose sums of magnitudes are between 1e-30 and 1e38.  f32 rows lose what is below 2^-133 of a value."""
+    rng = np.random.default_rng([m, k])
+    ss = np.array([0, 1, 2, 7, 60, 126, 200, 250, 252] + [253, 254] * (kind == "fp4"))
+    n = 5 * len(ss)
+    w = random_rows(rng, n, k)
+    w[1][:] = ss[np.arange(n) % len(ss)][:, None]
+    wv, xs = values(*w, k), ss[np.arange(m) % len(ss)]
+    if kind == "fp4":
+        x = random_rows(rng, m, k)
+        x[1][:] = xs[:, None]
+        got, xv = _product(gpu, kind, (*x, k), w), values(*x, k)
+    else:
+        x = (rng.standard_normal((m, k)) * np.exp2(xs - 127.0)[:, None]).astype(np.float32)
+        got, xv = _product(gpu, kind, x, w), x.astype(np.float64)
+    ref, mag = xv @ wv.T, np.abs(xv) @ np.abs(wv).T
+    tol = mag * STEP * (k + 2)
+    if kind == "w4":
+        tol = tol + mag * STEP * 2 * k + 2.0 ** -133 * np.abs(wv).sum(1)
+    ok = (mag < 1e38) & (mag > 1e-30)
+    assert ok.sum() > m * n / 3 and (np.abs(got - ref)[ok] <= tol[ok]).all()
+
+
+@KINDS
 @pytest.mark.parametrize("m", [2, 20, 300])
 def test_product_not_finite(gpu, kind, m):
     """A NaN in a row, or in a block of weights, reaches that row, or that column, and no other."""
