@@ -825,7 +825,7 @@ __device__ __forceinline__ void gemm_w4_tile(const NkGemm4Args &a, char *const s
     }
     tile_out<GLU, TI, TJ>(a, m0 + wm * WTM, c0 + n0, acc);
 }
-/* SIMD: wavefronts on a SIMD with the workgroups that the LDS of a CU holds (the widest tiles: one; 32 x 64 keeps three
+/* SIMD: wavefronts on a SIMD with the workgroups that the LDS of a CU holds (the widest tiles: one; 32 x 64 keeps a few
  * registers in memory for it, outside its loops) */
 #define W4_TILE(BM, BN, WGM, WGN, PW, AHEAD, SIMD, GLU, NAME)                                                       \
     extern "C" __global__ __launch_bounds__(64 * (WGM * WGN + PW), SIMD) void gemm_w4_##NAME(const NkGemm4Args a) { \

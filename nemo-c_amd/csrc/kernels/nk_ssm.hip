@@ -161,6 +161,8 @@ __device__ __forceinline__ float scan_rate(float A) {
     return __builtin_isinf(v) ? copysignf(3.4028235e38f, v) : v;
 }
 
+template <bool V> struct flag_t { static constexpr bool v = V; };
+
 #define SCAN_TILE 64 /* rows whose B and C are in LDS at a time */
 
 /* Rows t0 .. t1 - 1 of a sequence, one thread per channel with its NS >= N states in registers.
@@ -347,9 +349,9 @@ template <typename T, int NS, int PART> __device__ __forceinline__ void scan_imp
     float *ws = PART ? scan_place(a, i, s, piece) + c.d : nullptr;
     /* the slot of a sequence of several pieces may be written by its last before its first reads it */
     const bool joined = PART == 2 && t0, kept = PART == 2 && !t0 && s.rows > a.piece;
-    auto start = [&] {
 #pragma unroll
-        for (int n = 0; n < NS; ++n) h[n] = 0.0f;
+    for (int n = 0; n < NS; ++n) h[n] = 0.0f;
+    auto start = [&] {
         if (joined || (PART != 1 && !t0 && s.from >= 0)) {
             const float *from = joined ? ws - (u64)(a.N + 1) * a.D : kept ? a.first + (u64)i * a.N * a.D + c.d
                                                                            : a.state + ((u64)s.from * a.D + c.d) * a.N;
@@ -360,12 +362,14 @@ template <typename T, int NS, int PART> __device__ __forceinline__ void scan_imp
             }
         }
     };
-    start();
+    if (PART != 1) start();
     scan_rows<T, NS, PART == 1, PART == 0, false>(a, s, t0, t1, c.g, c.d, c.live, h, sum, lds);
     /* An input that is not finite makes the filling states NaN, and they stay so: the rows again without them.  Asked once
      * behind the rows, which costs 0 to 2%; asked for every four rows it took up to 70 registers, and a wavefront less on
      * every SIMD. */
     if (PART != 1 && __builtin_expect(a.N < NS, 0) && __builtin_expect(__syncthreads_or(h[NS - 1] != h[NS - 1]), 0)) {
+#pragma unroll
+        for (int n = 0; n < NS; ++n) h[n] = 0.0f;
         start();
         scan_rows<T, NS, false, PART == 0, true>(a, s, t0, t1, c.g, c.d, c.live, h, sum, lds);
     }
@@ -386,7 +390,8 @@ SCAN(u16, bf16, 8) SCAN(u16, bf16, 16) SCAN(u16, bf16, 32) SCAN(u16, bf16, 64)
 /* The pieces of a sequence one after another: H <- e^(A sum) H + end, the state that the next piece starts from,
  * takes the place of the piece's own end.  The factor by halves: a piece of growing steps may pass 2^128 by itself where
  * no state does, and one that is zero stays so whatever the factor.  An infinite state stays infinite: the factor may be
- * below the type's range where no row's is (but not where a step or the rate is infinite: zero times infinity there too).
+ * below the type's range where no row's is (but not where a step or the rate is infinite: zero times infinity there too);
+ * only batches that end in one ask for that.
  * One thread per state; the loads of JOIN pieces are in flight at a time (one at a time 36 us for 128 pieces of 2048
  * channels, a memory round trip each). */
 #define JOIN 16
@@ -394,9 +399,7 @@ extern "C" __global__ __launch_bounds__(256) void scan_join(const NkScanArgs a) 
     const seq_t s = seq_load(a.seqs, blockIdx.z, a.M, a.max_rows, a.slots);
     const u32 d = blockIdx.x * 256 + threadIdx.x, n = blockIdx.y;
     if (!s.ok || d >= a.D || s.rows <= a.piece) return;
-    const float rate = a.A[(u64)d * a.N + n], A = 0.5f * scan_rate(rate);
-    enum { ZEROS = 0x60, INFS = 0x204 }; /* classes of the values whatever the factor */
-    const u32 kept = __builtin_isinf(rate) ? ZEROS : ZEROS | INFS;
+    const float A = 0.5f * scan_rate(a.A[(u64)d * a.N + n]), RATE_MAX = 0.5f * 3.4028235e38f;
     float h = s.from >= 0 ? a.state[((u64)s.from * a.D + d) * a.N + n] : 0.0f;
     if (s.from >= 0) a.first[((u64)blockIdx.z * a.N + n) * a.D + d] = h;
     const u32 ends = (s.rows - 1) / a.piece; /* pieces that another follows */
@@ -410,13 +413,21 @@ extern "C" __global__ __launch_bounds__(256) void scan_join(const NkScanArgs a) 
             end[k] = p[(u64)n * a.D];
             sum[k] = p[(u64)a.N * a.D];
         }
+        auto join = [&](auto finite) {
 #pragma unroll
-        for (u32 k = 0; k < JOIN; ++k) {
-            if (i + k >= ends) break;
-            const float e = __builtin_amdgcn_exp2f(sum[k] * A);
-            const u32 keep = fabsf(sum[k]) < __builtin_inff() ? kept : ZEROS;
-            h = __builtin_amdgcn_classf(h, (int)keep) ? h + end[k] : fmaf(e, e * h, end[k]);
-            w[(i + k) * step + (u64)n * a.D] = h;
+            for (u32 k = 0; k < JOIN; ++k) {
+                if (i + k >= ends) break;
+                const float e = __builtin_amdgcn_exp2f(sum[k] * A);
+                const bool keep = !decltype(finite)::v && __builtin_isinf(h) && fabsf(sum[k]) < __builtin_inff() && fabsf(A) < RATE_MAX;
+                h = h == 0.0f ? end[k] : keep ? h + end[k] : fmaf(e, e * h, end[k]);
+                w[(i + k) * step + (u64)n * a.D] = h;
+            }
+        };
+        const float before = h;
+        join(flag_t<true>());
+        if (!(fabsf(h) < __builtin_inff())) { /* no state comes back from there: the batch again */
+            h = before;
+            join(flag_t<false>());
         }
     }
 }
