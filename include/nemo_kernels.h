@@ -354,9 +354,9 @@ int nk_causal_conv(gpu_t *g, const void *X, int type, uint32_t ldx, const float 
  *   y[t][d] = (sum_n C[t][g][n] h[n] + skip[d] x[t][d]) * SiLU(z[t][d])
  * x, dt, B, C, z, y are rows of one type; B and C rows have the stride ldbc and [groups][N] values (two
  * parts of one projection's rows, say); A [D][N], skip, dt_bias and the state [slots][D][N] are f32.  skip,
- * dt_bias and z (no gate) may be NULL.  Exponentials below 2^-126 are zero.  y must not overlap the inputs.  Long sequences of few channels are
- * split along their rows: the pieces' states lie in the context's scratch (no residual update may be
- * pending; a capture needs the scratch sized by a call before it). */
+ * dt_bias and z (no gate) may be NULL.  Exponentials below 2^-126 are zero.  y must not overlap the inputs.  Long
+ * sequences of few channels are split along their rows: the pieces' states lie in the context's scratch (no residual update
+ * may be pending; a capture needs the scratch sized by a call before it). */
 typedef struct {
     int type;
     uint32_t ldx, lddt, ldbc, ldz, ldy;

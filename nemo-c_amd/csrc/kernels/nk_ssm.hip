@@ -48,8 +48,8 @@ __device__ __forceinline__ void store_row(u16 *p, const float (&v)[2]) {
 /* One thread per channel (bf16: two where rows allow it) and tile of a.tile rows (where a sequence has more of them than the
  * grid, every gridDim.y-th), the last inputs in registers and eight rows' loads in flight: every row is read once (and the
  * taps - 1 before the tile).  Bound by memory: 8192 rows of 2048 channels f32 30 us, bf16 16.  More channels per thread are
- * slower (16 bytes each: 37 and 29 us), their taps being far apart and their threads few.  The tile with the sequence's first row reads the slot's rows and then writes the new
- * ones: nothing else touches the slots. */
+ * slower (16 bytes each: 37 and 29 us), their taps being far apart and their threads few.  The tile with the sequence's
+ * first row reads the slot's rows and then writes the new ones: nothing else touches the slots. */
 template <typename T, int TAPS, int V> __device__ __forceinline__ void cconv_impl(const NkCconvArgs &a) {
     const seq_t s = seq_load(a.seqs, blockIdx.z, a.M, a.max_rows, a.slots);
     const u32 d = (blockIdx.x * 256 + threadIdx.x) * V, step = gridDim.y * a.tile;
@@ -174,7 +174,7 @@ template <bool V> struct flag_t { static constexpr bool v = V; };
  *
  * Bound by the vector units: per state and row an exponential, which takes the time of 1.85 products, and four more
  * operations, three of them where only the ends are wanted.  8192 rows of 2048 channels of 16 states, bf16: ends 66
- * us, rows 85, the joining between them 15, where those operations alone are 43 and 52 us at the 30 T products/s that
+ * us, rows 85, the joining between them 13, where those operations alone are 43 and 52 us at the 30 T products/s that
  * this card reaches; the softplus, the gate and the conversions of every row are the rest. */
 template <typename T, int NS, bool ENDS, bool WHOLE, bool CARE>
 __device__ __forceinline__ void scan_rows(const NkScanArgs &a, const seq_t &s, u32 t0, u32 t1, u32 g, u32 d, bool live,
