@@ -719,6 +719,100 @@ def test_scan_captures(gpu, rows):
         c.free()
 
 
+@pytest.mark.parametrize("typ,D,N,max_rows", [(F32, 128, 16, 700), (BF16, 70, 5, 700), (F32, 64, 16, 1 << 18), (F32, 100, 24, 32)])
+def test_captured_block_takes_other_tables(gpu, typ, D, N, max_rows):
+    """A captured convolution and scan, replayed with other sequences in the table: each replay gives the bits of the
+    same calls made one by one, and of empty or unfitting entries nothing."""
+    L = nemoasr.lib()
+    rng = np.random.default_rng(D)
+    M, ns, taps = 900, 6, 4
+    o = operands(rng, typ, M, D, N, 1, ns)
+    w, bias, cs = (rng.standard_normal(s).astype(np.float32) for s in ((D, taps), (D,), (ns, taps - 1, D)))
+    long = min(max_rows, 650)
+    tables = [[(0, long, 0, 0), (long, 30, -1, 1), (700, 1, 2, 3)] + [(0, 0, -1, -1)] * 3,
+              [(i * 20, 1 + 3 * i, i, i) for i in range(ns)],
+              [(800, 31, 5, 5), (0, 0, 4, 4), (M, 1, 3, 3), (100, 32, -1, 2), (40, 7, ns, 1), (60, 2, 0, 0)]]
+    c = ScanCall(gpu, typ, o, np.array(tables[0], np.int32), max_rows, 1)
+    f = [gpu.put(a) for a in (w, bias, cs, np.full((M, D), 9, c.dt))]
+
+    def launch():
+        gpu.check(L.nk_causal_conv(gpu.h, c.args.x, typ, c.args.ldx, f[0].ptr, f[1].ptr, f[2].ptr, ns, c.args.seqs, ns, max_rows, f[3].ptr, D,
+                                   M, D, taps, 1))
+        c.launch()
+
+    def clear(table):
+        f[2].write(cs)
+        f[3].write(np.full((M, D), 9, c.dt))
+        c.bufs["seqs"].write(np.array(table, np.int32))
+        c.bufs["state"].write(o["state"].astype(np.float32))
+        c.bufs["y"].write(np.full(c.shape, 9, c.dt))
+
+    def result():
+        return [f[2].read(cs.shape), f[3].read((M, D), c.dt), *c.read()]
+
+    want = []
+    for t in tables:
+        clear(t)
+        gpu.begin()
+        launch()
+        gpu.end()
+        want.append(result())
+    gpu.begin()
+    gpu.check(L.gpu_capture_begin(gpu.h))
+    launch()
+    gr = L.gpu_capture_end(gpu.h)
+    gpu.end()
+    assert gr
+    for i in (1, 0, 2, 1):
+        clear(tables[i])
+        gpu.begin()
+        gpu.check(L.gpu_graph_launch(gpu.h, gr))
+        gpu.end()
+        for a, b in zip(want[i], result()):
+            np.testing.assert_array_equal(a, b)
+    L.gpu_graph_free(gr)
+    c.free()
+    for b in f:
+        b.free()
+
+
+@pytest.mark.parametrize("typ", [F32, BF16])
+def test_most_sequences(gpu, typ):
+    """65535 tokens in a call, their slots in another order."""
+    rng = np.random.default_rng(7)
+    n, D, N = 65535, 8, 4
+    slot = rng.permutation(n)
+    seqs = np.stack([np.arange(n), np.ones(n), slot, slot], 1).astype(np.int32)
+    o = operands(rng, typ, n, D, N, 1, n)
+    c = ScanCall(gpu, typ, o, seqs, 1, 1)
+    y, st = c.run()
+    c.free()
+    v = o["dt"] + o["dt_bias"]
+    s = (np.maximum(v, 0) + np.log1p(np.exp(-np.abs(v))))[:, :, None]
+    h0, add = o["state"][slot], s * o["B"][:, 0, None] * o["x"][:, :, None]
+    h = np.exp(s * o["A"]) * h0 + add
+    # s is off by 4u and what its sum's rounding makes of it, as in scan_ref; |s A| is below 40 here
+    r = _sig(v)[:, :, None] * U * np.abs(v)[:, :, None] / s + 4 * U
+    e = np.abs(np.exp(s * o["A"]) * h0) * (np.abs(s * o["A"]) * (r + 3 * U) + 3 * U) + np.abs(add) * (r + 3 * U) + U * np.abs(h) + 1e-38
+    assert (np.abs(st[slot] - h) <= 2 * e).all()
+    gate = o["z"] * _sig(o["z"])
+    m = (np.abs(o["C"][:, 0, None] * h)).sum(2) + np.abs(o["skip"] * o["x"])
+    ref = ((o["C"][:, 0, None] * h).sum(2) + o["skip"] * o["x"]) * gate
+    tol = ((np.abs(o["C"][:, 0, None]) * 2 * e).sum(2) + (N + 4) * U * m) * np.abs(gate) + 8 * U * np.abs(ref)
+    if typ == BF16:
+        tol = tol + 2.0 ** -8 * (np.abs(ref) + tol)
+    assert (np.abs(_back(y[:n, :D], typ) - ref) <= tol + 1e-37).all()
+    w, cs = rng.standard_normal((D, 4)).astype(np.float32), rng.standard_normal((n, 3, D)).astype(np.float32)
+    y, st = run_conv(gpu, typ, o["x"], w, None, cs, seqs, n, 1, act=0)
+    line = np.concatenate([cs[slot].astype(np.float64), o["x"][:, None]], 1)
+    terms = line * w.T.astype(np.float64)
+    tol = 6 * U * np.abs(terms).sum(1)
+    if typ == BF16:
+        tol = tol + 2.0 ** -8 * (np.abs(terms.sum(1)) + tol)
+    assert (np.abs(_back(y[:n], typ) - terms.sum(1)) <= tol + 1e-37).all()
+    np.testing.assert_array_equal(st[slot], line[:, 1:].astype(np.float32))
+
+
 # ---- a block -----------------------------------------------------------------------------------------
 
 
