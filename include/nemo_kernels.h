@@ -370,6 +370,82 @@ typedef struct {
 } nk_scan_t;
 int nk_ssm_scan(gpu_t *g, const nk_scan_t *a);
 
+/* ---- paged key and value cache, attention over it -------------------------------------------------
+ * For blocks that attend over long contexts (no counterpart in the reference, whose cache is a few frames).  A
+ * sequence's tokens lie in pages; kv->table (device) has the pages of its tokens 0, 1, ... in order, an entry outside
+ * 0 .. pages - 1 for a page that it has not (dropped behind a window, say).  A page has `page` tokens (a power of two
+ * from 16) of every head of the cache: k and v are [pages][heads][page][dh], dh a multiple of 16 up to 256, 16-byte aligned.
+ * NK_BF16: bf16.  NK_E4M3: 8-bit floating-point codes (a sign, 4 bits of exponent, 3 of fraction; up to 448, no infinity),
+ * with a scale byte s (2^(s - 127), s 10 to 247) for every block of 16 tokens and head: ks, vs [pages][heads][page / 16].
+ *
+ * seqs (device, 16-byte aligned) has four ints per sequence: { first row, rows, tokens before them, row of the table }.  Row i
+ * of it stands at position "tokens before them" + i.  No row is in two sequences; a sequence of no rows has nothing
+ * done; its rows are below M and at most max_rows, its tokens within its table row, which is one of `tables` rows of ldt
+ * entries: a sequence that breaks these is left out.  Rows that no sequence has are not written.  At most 65535 sequences.
+ * max_rows may be far above the longest, as in a captured graph that is replayed with other tables.
+ *
+ * The same table serves an append and the attention of the rows that were appended.  Sequences may share pages that
+ * they only read; a block is appended to by one. */
+enum { NK_E4M3 = 2 };
+typedef struct {
+    int type;
+    uint32_t heads, dh, page, pages;
+    void *k, *v;
+    uint8_t *ks, *vs;
+    const int *table;
+    uint32_t ldt, tables;
+} nk_kv_t;
+/* Host: radians per position of the rot / 2 pairs, base^(-2 i / rot), for contexts longer than trained with:
+ * NK_ROPE_LINEAR all divided by factor; NK_ROPE_BASE a larger base that divides the slowest by factor;
+ * NK_ROPE_TURNS divided by factor where a pair turns at most `lo` times in old_len positions, kept where at least `hi` times,
+ * blended by its turns between.  -1 for arguments that make no sense. */
+enum { NK_ROPE_PLAIN = 0, NK_ROPE_LINEAR = 1, NK_ROPE_BASE = 2, NK_ROPE_TURNS = 3 };
+int nk_rope_freqs(float *freq, uint32_t rot, double base, int scaling, double factor, double old_len, double lo, double hi);
+/* nk_kv_append: the rows' queries and keys rotated by their positions, keys and values put into their pages.  q [M][heads][dh],
+ * k and v [M][kv->heads][dh] are rows of one type (parts of one projection's rows, say); qo may be q.  q may be NULL (nothing
+ * rotated but the keys), or k and v (nothing appended).  The first rot values of a head turn in pairs (i, i + rot / 2), or
+ * (2 i, 2 i + 1) where inter is set, by the angle position * freq[i] (device, rot / 2 floats; counted in 64 bits), both times
+ * amp; the rest is as it was.  Sums in f32, rounded once.
+ * NK_E4M3: a block's scale is the least power of two of which 448 times reach its largest new value, and at least what the
+ * block's older tokens have; where that grows their codes are rounded again.  Values are rounded to the nearest, ties to
+ * the even code; an infinity becomes NaN. */
+typedef struct {
+    int type;
+    uint32_t ldq, ldk, ldv, ldqo;
+    const void *q, *k, *v;
+    void *qo;
+    uint32_t heads, rot;
+    int inter;
+    const float *freq;
+    float amp;
+    const int *seqs;
+    uint32_t nseq, max_rows, M;
+} nk_append_t;
+int nk_kv_append(gpu_t *g, const nk_kv_t *kv, const nk_append_t *a);
+/* Cached tokens back to rows [M][kv->heads][dh] (exact in either type): row i of a sequence is its token "tokens before" + i, zeros
+ * where its page is not there.  K or V may be NULL. */
+int nk_kv_read(gpu_t *g, const nk_kv_t *kv, void *K, uint32_t ldk, void *V, uint32_t ldv, int type, const int *seqs, uint32_t nseq,
+               uint32_t max_rows, uint32_t M);
+/* Attention of rows q [M][heads][dh] over the cache (heads a multiple of kv->heads, whose heads they share in order), to o
+ * (not overlapping q): softmax of scale q.k over the tokens that a row sees, in f32.  A row at position p sees token j
+ * where j <= p, its page is there and, with a window (0: none), j > p - window or j < sinks; a row that sees none
+ * gets zeros.  scale > 0.  max_len is at least the longest sequence's tokens, its rows among them (one that has more is left
+ * out), and may be far above.  bf16 rows: probabilities are rounded to bf16; f32 rows keep 24 bits.  Infinities and NaN
+ * count in the rows that see them alone, where they give what the formula gives.  Few rows behind many tokens are split along
+ * the tokens: the parts lie in the context's scratch (no residual update may be pending; a capture needs the scratch sized by
+ * a call with its arguments before it). */
+typedef struct {
+    int type;
+    uint32_t ldq, ldo;
+    const void *q;
+    void *o;
+    uint32_t heads, window, sinks;
+    float scale;
+    const int *seqs;
+    uint32_t nseq, max_rows, max_len, M;
+} nk_attend_t;
+int nk_attention_kv(gpu_t *g, const nk_kv_t *kv, const nk_attend_t *a);
+
 #ifdef __cplusplus
 }
 #endif

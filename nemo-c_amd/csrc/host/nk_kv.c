@@ -1,0 +1,166 @@
+/* Launchers of the paged key and value cache and the attention over it (include/nemo_kernels.h): arguments are checked
+ * before any launch; the tables lie on the device and are checked by the kernels. */
+#include "nemo_kernels.h"
+#include "gpu.h"
+#include "../kernel_params.h"
+#include <math.h>
+#include <stdio.h>
+
+static int bad(gpu_t *g, const char *what) { return gpu_fail(g, what); }
+static int aligned(const void *p, uintptr_t n) { return ((uintptr_t)p & (n - 1)) == 0; }
+
+int nk_rope_freqs(float *freq, uint32_t rot, double base, int scaling, double factor, double old_len, double lo, double hi) {
+    if (!freq || !rot || rot % 2 || !(base > 0.0) || !isfinite(base) || scaling < NK_ROPE_PLAIN || scaling > NK_ROPE_TURNS) return -1;
+    if (scaling != NK_ROPE_PLAIN && (!(factor > 0.0) || !isfinite(factor))) return -1;
+    if (scaling == NK_ROPE_BASE && rot < 4) return -1;
+    if (scaling == NK_ROPE_TURNS && (!(old_len > 0.0) || !(lo < hi) || !isfinite(old_len) || !isfinite(lo) || !isfinite(hi))) return -1;
+    if (scaling == NK_ROPE_BASE) base *= pow(factor, rot / (rot - 2.0)); /* the last pair's exponent is (rot - 2) / rot */
+    for (uint32_t i = 0; i < rot / 2; ++i) {
+        double f = pow(base, -2.0 * i / rot);
+        if (scaling == NK_ROPE_LINEAR) f /= factor;
+        if (scaling == NK_ROPE_TURNS) {
+            double keep = (old_len * f / 6.283185307179586476925 - lo) / (hi - lo);
+            keep = keep < 0.0 ? 0.0 : keep > 1.0 ? 1.0 : keep;
+            f *= keep + (1.0 - keep) / factor;
+        }
+        freq[i] = (float)f;
+    }
+    return 0;
+}
+
+/* what all ask of the cache and the batch */
+static const char *cache_bad(const nk_kv_t *c, NkKv *kv, const int *seqs, uint32_t nseq, uint32_t max_rows) {
+    if (c->type != NK_BF16 && c->type != NK_E4M3) return "kv: a cache of bf16 or e4m3";
+    if (!c->heads || c->heads > 65535 || !c->dh || c->dh % 16 || c->dh > 256) return "kv: heads of 16 to 256 values, a multiple of 16";
+    if (c->page < NK_KV_BLOCK || c->page & (c->page - 1) || c->page > 1u << 20) return "kv: pages of 16 to 2^20 tokens, a power of two";
+    if (!c->pages || c->pages > 0x7fffffffu || !c->k || !c->v || !aligned(c->k, 16) || !aligned(c->v, 16)) return "kv: pages, 16-byte aligned";
+    if (c->type == NK_E4M3 && (!c->ks || !c->vs)) return "kv: scales of an 8-bit cache";
+    if (!c->table || !aligned(c->table, 4) || !c->ldt || !c->tables || c->tables > 0x7fffffffu) return "kv: a table of pages";
+    if (!seqs || !aligned(seqs, 16)) return "kv: a 16-byte aligned table of sequences";
+    if (nseq > 65535) return "kv: at most 65535 sequences in a call";
+    if (max_rows > 1u << 30) return "kv: at most 2^30 rows a sequence";
+    uint32_t shift = 0;
+    while (1u << shift < c->page) ++shift;
+    *kv = (NkKv){ c->k, c->v, c->type == NK_E4M3 ? c->ks : NULL, c->type == NK_E4M3 ? c->vs : NULL, c->table, c->heads, c->dh, shift,
+                  c->pages, c->ldt, c->tables };
+    return NULL;
+}
+/* the most blocks of 16 tokens that the rows of the sequences touch */
+static uint64_t blocks_of(uint32_t nseq, uint32_t max_rows, uint32_t M) {
+    const uint64_t by_rows = M / NK_KV_BLOCK + 2ull * nseq, by_seqs = (uint64_t)nseq * ((max_rows + NK_KV_BLOCK - 1) / NK_KV_BLOCK + 1);
+    return by_rows < by_seqs ? by_rows : by_seqs;
+}
+static const char *cache_name(const NkKv *kv) { return kv->ks ? "e4m3" : "bf16"; }
+
+int nk_kv_append(gpu_t *g, const nk_kv_t *c, const nk_append_t *p) {
+    if (!c || !p) return bad(g, "kv_append: no arguments");
+    if (!p->nseq || !p->max_rows || !p->M) return 0;
+    NkKv kv;
+    const char *why = cache_bad(c, &kv, p->seqs, p->nseq, p->max_rows);
+    if (why) return bad(g, why);
+    if (p->type != NK_F32 && p->type != NK_BF16) return bad(g, "kv_append: rows are f32 or bf16");
+    const uintptr_t size = p->type == NK_F32 ? 4 : 2;
+    if ((!p->q && !p->k) || !p->k != !p->v || !p->q != !p->qo) return bad(g, "kv_append: queries with a place for them, or keys and values");
+    if (!aligned(p->q, size) || !aligned(p->k, size) || !aligned(p->v, size) || !aligned(p->qo, size))
+        return bad(g, "kv_append: rows aligned to their values");
+    const uint64_t nk = (uint64_t)kv.heads * kv.dh, nq = (uint64_t)p->heads * kv.dh;
+    if ((p->q && (!p->heads || p->heads > 65535 || p->ldq < nq || p->ldqo < nq)) || (p->k && (p->ldk < nk || p->ldv < nk)))
+        return bad(g, "kv_append: rows of at least all heads' values");
+    if (p->q == p->qo && p->q && p->ldq != p->ldqo) return bad(g, "kv_append: queries in place keep their stride");
+    if (p->rot % 2 || p->rot > kv.dh || (p->rot && (!p->freq || !aligned(p->freq, 4))))
+        return bad(g, "kv_append: an even number of rotated values, at most a head's, and their frequencies");
+    /* pairs at a time: as many as lie in 16 bytes, where the parts of a head and the rows allow it */
+    uint32_t P = 16 / size;
+    for (; P > 1; P = P == 8 ? 4 : 1) {
+        const uintptr_t b = P * size;
+        const uint32_t half = p->rot / 2, tail = kv.dh - p->rot;
+        const int rows = (!p->q || (aligned(p->q, b) && aligned(p->qo, b) && p->ldq % P == 0 && p->ldqo % P == 0)) &&
+                         (!p->k || (aligned(p->k, b) && aligned(p->v, b) && p->ldk % P == 0 && p->ldv % P == 0));
+        if (half % P == 0 && tail % (2 * P) == 0 && rows) break;
+    }
+    const uint64_t blocks = blocks_of(p->nseq, p->max_rows, p->M);
+    const uint32_t units = (p->q ? p->heads : 0) + (p->k ? 2 * kv.heads : 0);
+    if (blocks > 1u << 23) return bad(g, "kv_append: more rows than a launch covers");
+    uint32_t gy = (units + 3) / 4;
+    while (gy > 1 && blocks * gy > 4096) gy = (gy + 1) / 2;
+    NkAppendArgs a = { kv, p->q, p->k, p->v, p->qo, p->freq, p->seqs, p->ldq, p->ldk, p->ldv, p->ldqo, p->heads, p->rot, p->inter != 0,
+                       p->nseq, p->max_rows, p->M, p->amp };
+    char name[32];
+    snprintf(name, sizeof name, "kv_append_%sx%u_%s", p->type == NK_F32 ? "f32" : "bf16", P, cache_name(&kv));
+    gpu_next_bytes(g, (double)p->M * ((p->q ? 2.0 * size * nq : 0.0) + (p->k ? 2.0 * nk * (size + (kv.ks ? 1 : 2)) : 0.0)));
+    return gpu_launch(g, name, &a, sizeof a, (uint32_t)blocks, gy, 1, 256, 1, 1);
+}
+
+int nk_kv_read(gpu_t *g, const nk_kv_t *c, void *K, uint32_t ldk, void *V, uint32_t ldv, int type, const int *seqs, uint32_t nseq,
+               uint32_t max_rows, uint32_t M) {
+    if (!c) return bad(g, "kv_read: no cache");
+    if (!nseq || !max_rows || !M || (!K && !V)) return 0;
+    NkKv kv;
+    const char *why = cache_bad(c, &kv, seqs, nseq, max_rows);
+    if (why) return bad(g, why);
+    if (type != NK_F32 && type != NK_BF16) return bad(g, "kv_read: rows are f32 or bf16");
+    const uint32_t size = type == NK_F32 ? 4 : 2;
+    const uint64_t nk = (uint64_t)kv.heads * kv.dh;
+    if (!aligned(K, size) || !aligned(V, size) || (K && ldk < nk) || (V && ldv < nk))
+        return bad(g, "kv_read: aligned rows of at least all heads' values");
+    const uint32_t P = 16 / size;
+    const int vec = aligned(K, 16) && aligned(V, 16) && (!K || ldk % P == 0) && (!V || ldv % P == 0);
+    const uint64_t blocks = blocks_of(nseq, max_rows, M);
+    if (blocks > 1u << 23) return bad(g, "kv_read: more rows than a launch covers");
+    uint32_t gy = (2 * kv.heads + 3) / 4;
+    while (gy > 1 && blocks * gy > 4096) gy = (gy + 1) / 2;
+    NkKvReadArgs a = { kv, K, V, seqs, ldk, ldv, nseq, max_rows, M };
+    char name[32];
+    snprintf(name, sizeof name, "kv_read_%sx%u_%s", type == NK_F32 ? "f32" : "bf16", vec ? P : 1, cache_name(&kv));
+    gpu_next_bytes(g, 2.0 * M * nk * (size + (kv.ks ? 1 : 2)));
+    return gpu_launch(g, name, &a, sizeof a, (uint32_t)blocks, gy, 1, 256, 1, 1);
+}
+
+int nk_attention_kv(gpu_t *g, const nk_kv_t *c, const nk_attend_t *p) {
+    if (!c || !p) return bad(g, "attention_kv: no arguments");
+    if (!p->nseq || !p->max_rows || !p->M) return 0;
+    NkKv kv;
+    const char *why = cache_bad(c, &kv, p->seqs, p->nseq, p->max_rows);
+    if (why) return bad(g, why);
+    if (p->type != NK_F32 && p->type != NK_BF16) return bad(g, "attention_kv: rows are f32 or bf16");
+    const uintptr_t size = p->type == NK_F32 ? 4 : 2;
+    if (!p->heads || p->heads % kv.heads || p->heads / kv.heads > 1024) return bad(g, "attention_kv: heads a multiple of the cache's");
+    const uint64_t nq = (uint64_t)p->heads * kv.dh;
+    if (!p->q || !p->o || !aligned(p->q, size) || !aligned(p->o, size) || p->ldq < nq || p->ldo < nq)
+        return bad(g, "attention_kv: aligned rows of at least all heads' values");
+    if (p->q == p->o) return bad(g, "attention_kv: o must not overlap q");
+    if (!(p->scale > 0.0f) || !isfinite(p->scale)) return bad(g, "attention_kv: a scale above zero");
+    if (p->max_len > 1u << 30) return bad(g, "attention_kv: at most 2^30 tokens a sequence");
+    const uint32_t group = p->heads / kv.heads;
+    const uint32_t window = p->window >= p->max_len ? 0 : p->window, sinks = p->sinks < p->max_len ? p->sinks : p->max_len;
+    NkAttnKvArgs a = { kv, p->q, p->o, p->seqs, NULL, p->ldq, p->ldo, p->heads, group, window, sinks, p->nseq, p->max_rows, p->max_len, p->M,
+                       0, p->max_rows, 0, 0, 0, 0, 0, p->scale };
+    a.vec = aligned(p->q, 16) && aligned(p->o, 4 * size) && p->ldq % (16 / size) == 0 && p->ldo % 4 == 0;
+    const uint32_t rows = p->max_rows < p->M ? p->max_rows : p->M, DH = kv.dh <= 64 ? 64 : kv.dh <= 128 ? 128 : 256;
+    const uint32_t QT = (uint64_t)rows * group > 16 && (DH < 256 || p->type == NK_BF16) ? 2 : 1;
+    a.tile = 16 * QT;
+    a.step = 32;
+    a.least = 8;
+    /* tiles that there can be, and the pieces that a tile can have */
+    const uint64_t each = ((uint64_t)rows * group + a.tile - 1) / a.tile, by_rows = (uint64_t)p->M * group / a.tile + p->nseq;
+    const uint64_t tiles = p->nseq * each < by_rows ? p->nseq * each : by_rows;
+    const uint64_t pieces = ((p->max_len + a.step - 1) / a.step + a.least - 1) / a.least;
+    if (tiles > 1u << 23) return bad(g, "attention_kv: more rows than a launch covers");
+    uint64_t items = tiles;
+    if (pieces > 1) {
+        a.slots = (1024 + kv.heads - 1) / kv.heads;
+        const uint64_t split = tiles * pieces < 2ull * a.slots ? tiles * pieces : 2ull * a.slots;
+        if (items < split) items = split;
+        a.ws = gpu_scratch_ws(g, (size_t)(split * kv.heads * a.tile * (kv.dh + 2)));
+        if (!a.ws) return bad(g, "attention_kv: scratch unavailable (size it before capture)");
+    }
+    const char *type = p->type == NK_F32 ? "f32" : "bf16";
+    char name[40];
+    snprintf(name, sizeof name, "attn_few_%s_%s_%u_%u", type, cache_name(&kv), DH, QT);
+    gpu_next_bytes(g, 2.0 * size * p->M * nq);
+    if (gpu_launch(g, name, &a, sizeof a, (uint32_t)items, kv.heads, 1, 256, 1, 1)) return -1;
+    if (!a.slots) return 0;
+    snprintf(name, sizeof name, "attn_join_%s", type);
+    const uint64_t most = (uint64_t)rows * group < a.tile ? (uint64_t)rows * group : a.tile;
+    return gpu_launch(g, name, &a, sizeof a, (uint32_t)(tiles < a.slots ? tiles : a.slots), kv.heads, (uint32_t)(most + 3) / 4, 256, 1, 1);
+}

@@ -539,4 +539,56 @@ typedef struct {
     u32 piece, pieces, byrow, vec; /* byrow: places in ws by the rows; vec: four states are read and written at once */
 } NkScanArgs;
 
+/* ---- paged key and value cache --------------------------------------------------------------------
+ * k, v [pages][heads][1 << shift][dh] (bf16, or e4m3 codes with scale bytes ks, vs [pages][heads][(1 << shift) / 16]);
+ * table [tables][ldt]: the pages of a sequence's tokens, in order. */
+typedef struct {
+    void *k, *v;
+    unsigned char *ks, *vs;
+    const int *table;
+    u32 heads, dh, shift, pages, ldt, tables;
+} NkKv;
+#define NK_KV_BLOCK 16 /* tokens that share a scale byte */
+
+/* Whether an entry { first row, rows, tokens before them, row of the table } of seqs fits: rows below M and at most
+ * max_rows of them, tokens within the table's row and at most max_len. */
+#ifdef __HIPCC__
+__host__ __device__
+#endif
+static inline int nk_kv_seq_ok(int first, int rows, int len, int row, u32 M, u32 max_rows, u32 tables, unsigned long long room) {
+    return first >= 0 && rows >= 0 && (u32)first <= M && (u32)rows <= M - (u32)first && (u32)rows <= max_rows && len >= 0 &&
+           row >= 0 && (u32)row < tables && (unsigned long long)len + (u32)rows <= room;
+}
+
+typedef struct {
+    NkKv kv;
+    const void *q, *k, *v; /* rows; q or k and v may be NULL */
+    void *qo;
+    const float *freq;     /* radians per position of the rot / 2 pairs */
+    const int *seqs;
+    u32 ldq, ldk, ldv, ldqo, heads, rot, inter, nseq, max_rows, M;
+    float amp;
+} NkAppendArgs;
+
+typedef struct {
+    NkKv kv;
+    void *k, *v; /* rows that the tokens are read to */
+    const int *seqs;
+    u32 ldk, ldv, nseq, max_rows, M;
+} NkKvReadArgs;
+
+typedef struct {
+    NkKv kv;
+    const void *q;
+    void *o;
+    const int *seqs;
+    float *ws;        /* split sequences: per piece, head of the cache and row m, l and dh sums */
+    u32 ldq, ldo, heads, group, window, sinks, nseq, max_rows, max_len, M;
+    u32 over, upto;   /* sequences of more than `over` and at most `upto` rows are this launch's */
+    u32 tile, step;   /* rows (of all heads of a group) of a workgroup; tokens of a step */
+    u32 slots, least; /* workgroups per head of the cache that are wanted; the fewest steps of a piece */
+    u32 vec;          /* rows are read and written 16 (bf16: 8) bytes at a time */
+    float scale;
+} NkAttnKvArgs;
+
 #endif

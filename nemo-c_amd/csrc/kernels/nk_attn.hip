@@ -1,0 +1,489 @@
+/* Attention over the paged key and value cache.  Row i of a sequence stands behind `len` tokens at position
+ * p = len + i and sees token j where j <= p and (no window, or j > p - window, or j < sinks); tokens of a page that there
+ * is none of are not seen.  The rows of the heads that share a head of the cache lie one behind another ("packed":
+ * row * group + head of the group), so its keys and values are read once for all of them.
+ *
+ *   o = sum_j 2^(x_j - m) v_j / sum_j 2^(x_j - m),   x_j = scale log2(e) q.k_j,   m = max_j x_j
+ *
+ * in one pass over the tokens, with the running maximum, sum and sums of v in 32 bits.  The products are on the matrix
+ * units: keys and values are exact in bf16 (8-bit codes with their power of two too); bf16 rows are, and their
+ * probabilities are rounded to bf16 (a relative 2^-9 of each, as much as the output's own rounding); f32 rows and
+ * their probabilities are three bf16 terms, 24 bits.
+ *
+ * Rows whose result is not finite (an infinity or NaN was near, also in a token that only some rows see: 0 times it is
+ * NaN in a product), or whose sum is zero, are computed again by the formula, row by row. */
+#include "nk_common.h"
+
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+
+/* a 16-lane group's 4 rows of 16 values from LDS, each lane with its column's four: lane i gives the address of row i / 4,
+ * values 4 (i % 4) on */
+__device__ __forceinline__ uint2 lds_column4(const u16 *p) {
+    return __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4bf16((__attribute__((address_space(3))) bf16x4 *)p));
+}
+__device__ __forceinline__ void swap32(float &a, float &b) { /* b's lower half <-> a's upper half */
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(a), __float_as_uint(b), false, false);
+    a = __uint_as_float(r[0]);
+    b = __uint_as_float(r[1]);
+}
+__device__ __forceinline__ void swap16(float &a, float &b) {
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(a), __float_as_uint(b), false, false);
+    a = __uint_as_float(r[0]);
+    b = __uint_as_float(r[1]);
+}
+/* over the lanes that agree in their low four bits (16: five) */
+__device__ __forceinline__ float max_over32(float a) { float b = a; swap32(a, b); return fmaxf(a, b); }
+__device__ __forceinline__ float sum_over32(float a) { float b = a; swap32(a, b); return a + b; }
+__device__ __forceinline__ float max_over16(float a) { float b = a; swap16(a, b); return max_over32(fmaxf(a, b)); }
+__device__ __forceinline__ float sum_over16(float a) { float b = a; swap16(a, b); return sum_over32(a + b); }
+
+/* 8 codes to bf16 with the power of two of their block */
+__device__ __forceinline__ u32x4 e4m3_bf16(u32 a, u32 b, float s) {
+    return (u32x4){ __builtin_bit_cast(u32, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a, s, false)),
+                    __builtin_bit_cast(u32, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a, s, true)),
+                    __builtin_bit_cast(u32, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, s, false)),
+                    __builtin_bit_cast(u32, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, s, true)) };
+}
+__device__ __forceinline__ floatx4 attn_mfma(u32x4 a, u32x4 b, floatx4 acc) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), acc, 0, 0, 0);
+}
+
+/* 8 f32 values as TERMS bf16 fragments: to nearest each, the first of what the values are, the next of what is left */
+template <int TERMS> __device__ __forceinline__ void attn_terms(const float (&x)[8], u32x4 (&t)[TERMS]) {
+    floatx2 r[4];
+#pragma unroll
+    for (int p = 0; p < 4; ++p) r[p] = (floatx2){ x[2 * p], x[2 * p + 1] };
+#pragma unroll
+    for (int k = 0; k < TERMS; ++k) {
+        u32 w[4];
+#pragma unroll
+        for (int p = 0; p < 4; ++p) {
+            w[p] = __builtin_bit_cast(u32, __builtin_convertvector(r[p], bf16x2));
+            if (k + 1 < TERMS) r[p] -= (floatx2){ bf_lo(w[p]), bf_hi(w[p]) };
+        }
+        t[k] = (u32x4){ w[0], w[1], w[2], w[3] };
+    }
+}
+
+/* ---- who does what ------------------------------------------------------------------------------------
+ * A sequence's packed rows go in tiles of a.tile; a tile's tokens in steps of a.step: the steps of the first tokens that
+ * stay visible (`sinks`), then those from the first row's window to the last row.  Where all tiles are fewer than the
+ * workgroups wanted, their steps are split into pieces of equal length, by all the work that there is (the lengths are
+ * known here alone); a piece's sums go to the scratch, and attn_join adds them up.  Items are numbered over all
+ * sequences. */
+typedef struct {
+    u32 first, rows, len, row;  /* the sequence */
+    u32 r0, nr;                 /* the tile's packed rows */
+    u32 lo_step, sink_steps, steps; /* its steps: sink_steps from 0 on, the others from lo_step on */
+    u32 from, to;               /* the piece's */
+    u32 pieces, item;           /* pieces of every tile of the sequence; this one's number over all */
+    u32 piece;
+} attn_work_t;
+
+__device__ __forceinline__ u32 attn_tiles(const NkAttnKvArgs &a, const kvseq_t &s) {
+    return s.ok && s.rows > a.over && s.rows <= a.upto ? (s.rows * a.group - 1) / a.tile + 1 : 0;
+}
+/* the most steps that a tile of the sequence has */
+__device__ __forceinline__ u32 attn_most_steps(const NkAttnKvArgs &a, const kvseq_t &s) {
+    const u32 all = (s.len + s.rows - 1) / a.step + 1;
+    if (!a.window) return all;
+    const u64 some = ((u64)a.window + (a.tile - 1) / a.group + 2 + a.step - 1) / a.step + 1 + ((u64)a.sinks + a.step - 1) / a.step;
+    return some < all ? (u32)some : all;
+}
+__device__ __forceinline__ void attn_steps(const NkAttnKvArgs &a, attn_work_t &w) {
+    const u32 lowest = w.len + w.r0 / a.group, last = w.len + (w.r0 + w.nr - 1) / a.group;
+    const u32 lo = a.window && lowest >= a.window ? lowest + 1 - a.window : 0;
+    w.lo_step = lo / a.step;
+    w.sink_steps = a.window ? min((u32)(((u64)a.sinks + a.step - 1) / a.step), w.lo_step) : 0;
+    w.steps = w.sink_steps + last / a.step - w.lo_step + 1;
+}
+__device__ __forceinline__ kvseq_t attn_seq(const NkAttnKvArgs &a, u32 i) {
+    return kvseq_load(a.seqs, i, a.M, a.max_rows, a.kv.tables, min(kv_room(a.kv), (u64)a.max_len));
+}
+__device__ __forceinline__ u64 wave_sum64(u64 v) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) v += shfl_xor_u64(v, o);
+    return v;
+}
+/* steps of a piece; 0: nothing is split */
+__device__ __forceinline__ u32 attn_piece(const NkAttnKvArgs &a) {
+    u64 tiles = 0, steps = 0;
+    for (u32 i = threadIdx.x & 63; i < a.nseq; i += 64) {
+        const kvseq_t s = attn_seq(a, i);
+        const u32 n = attn_tiles(a, s);
+        tiles += n;
+        steps += n ? (u64)n * attn_most_steps(a, s) : 0;
+    }
+    tiles = wave_sum64(tiles);
+    if (tiles >= a.slots) return 0;
+    steps = wave_sum64(steps);
+    return max((u32)((steps + a.slots - 1) / a.slots), a.least);
+}
+__device__ __forceinline__ u32 attn_pieces(const NkAttnKvArgs &a, const kvseq_t &s, u32 piece) {
+    return piece ? (attn_most_steps(a, s) - 1) / piece + 1 : 1;
+}
+__device__ __forceinline__ bool attn_find(const NkAttnKvArgs &a, u32 id, attn_work_t &w) {
+    const u32 piece = a.slots ? attn_piece(a) : 0;
+    const kvitem_t it = kv_find(a.nseq, id, [&](u32 i) {
+        const kvseq_t s = attn_seq(a, i);
+        const u32 n = attn_tiles(a, s);
+        return n ? n * attn_pieces(a, s, piece) : 0;
+    });
+    if (!it.found) return false;
+    const kvseq_t s = attn_seq(a, it.seq);
+    w.first = s.first, w.rows = s.rows, w.len = s.len, w.row = s.row;
+    w.pieces = attn_pieces(a, s, piece);
+    w.item = id;
+    w.piece = it.local % w.pieces;
+    w.r0 = (attn_tiles(a, s) - 1 - it.local / w.pieces) * a.tile; /* the last rows, which see most, first */
+    w.nr = min(a.tile, s.rows * a.group - w.r0);
+    attn_steps(a, w);
+    w.from = piece ? w.piece * piece : 0;
+    w.to = piece ? min(w.steps, w.from + piece) : w.steps;
+    return true;
+}
+/* a piece's place in the scratch: m and l of its rows, then their sums */
+__device__ __forceinline__ float *attn_part(const NkAttnKvArgs &a, u32 item, u32 h) {
+    return a.ws + ((u64)item * a.kv.heads + h) * a.tile * (a.kv.dh + 2);
+}
+
+__device__ __forceinline__ float kv_value(const NkKv &kv, const void *c, const unsigned char *s, u64 slot, u32 d) {
+    if (!s) return bf2f(((const u16 *)c)[slot * kv.dh + d]);
+    return __builtin_amdgcn_cvt_f32_fp8(((const unsigned char *)c)[slot * kv.dh + d], 0) * scale8(s[slot / NK_KV_BLOCK]);
+}
+__device__ __forceinline__ float ld_q(const float *p) { return *p; }
+__device__ __forceinline__ float ld_q(const u16 *p) { return bf2f(*p); }
+__device__ __forceinline__ void st_o(float *p, float v) { *p = v; }
+__device__ __forceinline__ void st_o(u16 *p, float v) { *p = (u16)pk_bf16(v, 0.0f); }
+
+/* Packed row r of a sequence by the formula: one wavefront, a lane's dims d = lane, lane + 64, ...; first the maximum, then
+ * the sums.  No token seen: zeros. */
+template <typename T> __device__ __forceinline__ void attn_by_formula(const NkAttnKvArgs &a, u32 first, u32 len, u32 row, u32 r, u32 h) {
+    const NkKv &kv = a.kv;
+    const u32 lane = threadIdx.x & 63, i = r / a.group, p = len + i;
+    const u64 at = (u64)(h * a.group + r % a.group) * kv.dh;
+    const T *q = (const T *)a.q + (u64)(first + i) * a.ldq + at;
+    T *o = (T *)a.o + (u64)(first + i) * a.ldo + at;
+    const u32 lo = a.window && p >= a.window ? p + 1 - a.window : 0, sinks = a.window ? min(a.sinks, lo) : 0;
+    float m = -INFINITY, l = 0.0f, acc[4] = { 0.0f, 0.0f, 0.0f, 0.0f };
+    bool any = false;
+    for (int pass = 0; pass < 2; ++pass)
+        for (u32 k = 0; k < sinks + p + 1 - lo; ++k) {
+            const u32 j = k < sinks ? k : lo + k - sinks;
+            const int pe = kv.table[(u64)row * kv.ldt + (j >> kv.shift)];
+            if ((u32)pe >= kv.pages) continue;
+            const u64 slot = (((u64)(u32)pe * kv.heads + h) << kv.shift) + (j & ((1u << kv.shift) - 1));
+            float s = 0.0f;
+            for (u32 d = lane; d < kv.dh; d += 64) s = fmaf(ld_q(q + d), kv_value(kv, kv.k, kv.ks, slot, d), s);
+            s = wave_sum(s) * a.scale;
+            if (!pass) {
+                m = !any || s > m || s != s ? s : m; /* a NaN stays */
+                any = true;
+                continue;
+            }
+            const float e = expf(s - m);
+            l += e;
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const u32 d = lane + 64 * u;
+                if (d < kv.dh) acc[u] = fmaf(e, kv_value(kv, kv.v, kv.vs, slot, d), acc[u]);
+            }
+        }
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+        if (lane + 64 * u < kv.dh) st_o(o + lane + 64 * u, any ? acc[u] / l : 0.0f);
+}
+
+/* ---- few rows: wavefronts over the tokens --------------------------------------------------------------
+ * A workgroup's 16 QT packed rows; its four wavefronts take every fourth step of 32 tokens, each with sums of its own that
+ * are joined at the end.  Keys go from memory into fragments (a fragment's sum may take its values in any order: lane
+ * group g of a chunk pair has the values 16 g on), values through the wavefront's own LDS for their columns;
+ * the next step's loads are in flight. */
+#define ATTN_STEP 32
+template <typename T, typename CT, int DH, int QT> __device__ __forceinline__ void attn_few(const NkAttnKvArgs &a) {
+    constexpr bool E4M3 = sizeof(CT) == 1;
+    constexpr int NC = DH / 32, ND = DH / 16, TERMS = sizeof(T) == 4 ? 3 : 1, ROWS = 16 * QT;
+    constexpr int LDV = DH + 16; /* u16 of a token's row in LDS: 32 bytes more, so that four tokens' are in other banks */
+    constexpr int NK = E4M3 ? DH / 64 : DH / 32, NV = E4M3 ? DH / 32 : DH / 16; /* 16-byte loads of a lane: per 16 tokens; per step */
+    constexpr u32 VBYTES = 4 * ATTN_STEP * LDV * 2, OBYTES = 4 * 16 * DH * 4;
+    __shared__ __align__(16) char lds[VBYTES > OBYTES ? VBYTES : OBYTES];
+    __shared__ float wm[4][ROWS], wl[4][ROWS];
+    __shared__ u32 wrong[ROWS];
+    const NkKv &kv = a.kv;
+    const u32 h = blockIdx.y, lane = threadIdx.x & 63, c16 = lane & 15, g4 = lane >> 4;
+    const u32 wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), dh = kv.dh;
+    attn_work_t w;
+    if (!attn_find(a, blockIdx.x, w) || w.from >= w.to) return;
+    if (threadIdx.x < ROWS) wrong[threadIdx.x] = 0;
+    const u32 pos_lo = w.len + w.r0 / a.group, pos_hi = w.len + (w.r0 + w.nr - 1) / a.group;
+
+    u32x4 qf[QT][NC][TERMS];
+    u32 pos[QT];
+#pragma unroll
+    for (int t = 0; t < QT; ++t) {
+        const u32 r = w.r0 + min(16 * t + c16, w.nr - 1), i = r / a.group;
+        pos[t] = w.len + i;
+        const T *q = (const T *)a.q + (u64)(w.first + i) * a.ldq + (u64)(h * a.group + r % a.group) * dh;
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+            const u32 d = 64 * (c / 2) + 16 * g4 + 8 * (c % 2);
+            const T *p = q + min(d, dh - 8);
+            float v[8];
+            if (a.vec) kv_load<8>(v, p);
+            else
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[e] = ld_q(p + e);
+            if (d >= dh)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[e] = 0.0f;
+            attn_terms<TERMS>(v, qf[t][c]);
+        }
+    }
+
+    u32x4 kr[2][NK], vr[NV];
+    u32 ksb[2], vsb[2];
+    int pe[2];
+    auto token = [&](u32 u) { return (u < w.sink_steps ? u : w.lo_step + u - w.sink_steps) * ATTN_STEP; };
+    auto lookup = [&](u32 u) {
+#pragma unroll
+        for (int b = 0; b < 2; ++b) pe[b] = kv.table[(u64)w.row * kv.ldt + (min(token(u) + 16 * b, pos_hi) >> kv.shift)];
+    };
+    bool there[2];
+    auto load = [&](u32 u) { /* from the pages that pe has */
+        const u32 t0 = token(u);
+        u64 at[2];
+        u32 last[2]; /* tokens behind the last row's are not read: that one again */
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+            const u32 tb = min(t0 + 16 * b, pos_hi & ~15u);
+            there[b] = (u32)pe[b] < kv.pages;
+            const u64 slot = (((u64)(u32)(there[b] ? pe[b] : 0) * kv.heads + h) << kv.shift) + (tb & ((1u << kv.shift) - 1));
+            at[b] = slot * dh;
+            last[b] = min(pos_hi - tb, 15u);
+            if constexpr (E4M3) {
+                ksb[b] = kv.ks[slot / NK_KV_BLOCK];
+                vsb[b] = kv.vs[slot / NK_KV_BLOCK];
+            }
+            const u32 tok = min(c16, last[b]);
+#pragma unroll
+            for (int c = 0; c < NK; ++c) {
+                const u32 d = E4M3 ? min(64 * c + 16 * g4, dh - 16) : min(64 * (c / 2) + 16 * g4 + 8 * (c % 2), dh - 8);
+                kr[b][c] = *(const u32x4 *)((const CT *)kv.k + at[b] + tok * dh + d);
+            }
+        }
+        constexpr int PER = E4M3 ? DH / 16 : DH / 8; /* lanes of a token's row */
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            constexpr int each = 64 / PER;
+            const int b = i * each / 16;
+            const u32 tok = min(i * each % 16 + lane / PER, last[b]), d = min(lane % PER * (16 / (u32)sizeof(CT)), dh - 16 / (u32)sizeof(CT));
+            vr[i] = *(const u32x4 *)((const CT *)kv.v + at[b] + tok * dh + d);
+        }
+    };
+
+    floatx4 o[QT][ND];
+    float m[QT], l[QT];
+#pragma unroll
+    for (int t = 0; t < QT; ++t) {
+        m[t] = -1e30f, l[t] = 0.0f;
+#pragma unroll
+        for (int n = 0; n < ND; ++n) o[t][n] = (floatx4){ 0, 0, 0, 0 };
+    }
+    u16 *vl = (u16 *)lds + wave * ATTN_STEP * LDV;
+    const float scale2 = a.scale * 1.44269504f;
+
+    u32 u = w.from + wave;
+    if (u < w.to) {
+        lookup(u);
+        load(u);
+        lookup(min(u + 4, w.steps - 1));
+    }
+#pragma unroll 1
+    for (; u < w.to; u += 4) {
+        const u32 t0 = token(u);
+        floatx4 s[QT][2];
+        const bool th[2] = { there[0], there[1] };
+#pragma unroll
+        for (int t = 0; t < QT; ++t) s[t][0] = s[t][1] = (floatx4){ 0, 0, 0, 0 };
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+#pragma unroll
+            for (int c = 0; c < NC; ++c) {
+                u32x4 kf;
+                if constexpr (E4M3) kf = c % 2 ? e4m3_bf16(kr[b][c / 2].z, kr[b][c / 2].w, scale8(ksb[b])) : e4m3_bf16(kr[b][c / 2].x, kr[b][c / 2].y, scale8(ksb[b]));
+                else kf = kr[b][c];
+#pragma unroll
+                for (int t = 0; t < QT; ++t)
+#pragma unroll
+                    for (int k = TERMS - 1; k >= 0; --k) s[t][b] = attn_mfma(kf, qf[t][c][k], s[t][b]);
+            }
+        constexpr int PER = E4M3 ? DH / 16 : DH / 8, each = 64 / PER;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            u16 *p = vl + (i * each + lane / PER) * LDV + lane % PER * (16 / (u32)sizeof(CT));
+            if constexpr (E4M3) {
+                const float f = scale8(vsb[i * each / 16]);
+                *(u32x4 *)p = e4m3_bf16(vr[i].x, vr[i].y, f);
+                *(u32x4 *)(p + 8) = e4m3_bf16(vr[i].z, vr[i].w, f);
+            } else *(u32x4 *)p = vr[i];
+        }
+        if (u + 4 < w.to) {
+            load(u + 4);
+            lookup(min(u + 8, w.steps - 1));
+        }
+        const bool whole = t0 + ATTN_STEP - 1 <= pos_lo && th[0] && th[1] &&
+                           (!a.window || t0 + a.window > pos_hi || t0 + ATTN_STEP <= a.sinks);
+        u32x4 pf[QT][TERMS];
+#pragma unroll
+        for (int t = 0; t < QT; ++t) {
+            if (!whole) {
+#pragma unroll
+                for (int b = 0; b < 2; ++b)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const u32 j = t0 + 16 * b + 4 * g4 + i;
+                        const bool see = th[b] && j <= pos[t] && (!a.window || pos[t] - j < a.window || j < a.sinks);
+                        s[t][b][i] = see ? s[t][b][i] : -INFINITY;
+                    }
+            }
+            float top = fmaxf(fmaxf(fmaxf(s[t][0][0], s[t][0][1]), fmaxf(s[t][0][2], s[t][0][3])),
+                              fmaxf(fmaxf(s[t][1][0], s[t][1][1]), fmaxf(s[t][1][2], s[t][1][3])));
+            top = fmaxf(m[t], max_over16(top) * scale2);
+            const float old = __builtin_amdgcn_exp2f(m[t] - top);
+            m[t] = top;
+            float p[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) p[i] = __builtin_amdgcn_exp2f(fmaf(s[t][i / 4][i % 4], scale2, -top));
+            l[t] = fmaf(l[t], old, ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7])));
+            attn_terms<TERMS>(p, pf[t]);
+#pragma unroll
+            for (int n = 0; n < ND; ++n) o[t][n] *= old;
+        }
+        asm volatile("" ::: "memory"); /* the wavefront's own LDS, in order */
+#pragma unroll
+        for (int n = 0; n < ND; ++n) {
+            const u16 *p = vl + (4 * g4 + c16 / 4) * LDV + 16 * n + 4 * (c16 % 4);
+            const uint2 x = lds_column4(p), y = lds_column4(p + 16 * LDV);
+            const u32x4 vf = { x.x, x.y, y.x, y.y };
+#pragma unroll
+            for (int t = 0; t < QT; ++t)
+#pragma unroll
+                for (int k = TERMS - 1; k >= 0; --k) o[t][n] = attn_mfma(vf, pf[t][k], o[t][n]);
+        }
+        asm volatile("" ::: "memory");
+    }
+
+    float *part = w.pieces > 1 ? attn_part(a, w.item, h) : NULL;
+    float *ol = (float *)lds;
+#pragma unroll
+    for (int t = 0; t < QT; ++t) {
+        l[t] = sum_over16(l[t]);
+        __syncthreads();
+        if (lane < 16) wm[wave][16 * t + lane] = m[t], wl[wave][16 * t + lane] = l[t];
+#pragma unroll
+        for (int n = 0; n < ND; ++n) *(floatx4 *)(ol + (wave * 16 + c16) * DH + 16 * n + 4 * g4) = o[t][n];
+        __syncthreads();
+        for (u32 i = threadIdx.x; i < 16 * DH / 4; i += 256) {
+            const u32 r = i / (DH / 4), d = i % (DH / 4) * 4, rt = 16 * t + r;
+            if (rt >= w.nr || d >= dh) continue;
+            float top = wm[0][rt], sum = 0.0f;
+#pragma unroll
+            for (int k = 1; k < 4; ++k) top = fmaxf(top, wm[k][rt]);
+            floatx4 v = { 0, 0, 0, 0 };
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const float f = __builtin_amdgcn_exp2f(wm[k][rt] - top);
+                sum = fmaf(wl[k][rt], f, sum);
+                v += f * *(const floatx4 *)(ol + (k * 16 + r) * DH + d);
+            }
+            if (part) {
+                if (!d) part[2 * rt] = top, part[2 * rt + 1] = sum;
+                *(floatx2 *)(part + 2 * a.tile + (u64)rt * dh + d) = v.xy;
+                *(floatx2 *)(part + 2 * a.tile + (u64)rt * dh + d + 2) = v.zw;
+                continue;
+            }
+            v /= sum;
+            const u32 pr = w.r0 + rt;
+            T *out = (T *)a.o + (u64)(w.first + pr / a.group) * a.ldo + (u64)(h * a.group + pr % a.group) * dh + d;
+            if (!(fabsf(v.x) < INFINITY && fabsf(v.y) < INFINITY && fabsf(v.z) < INFINITY && fabsf(v.w) < INFINITY)) wrong[rt] = 1;
+            const float e[4] = { v.x, v.y, v.z, v.w };
+            if (a.vec) kv_store<4>(out, e);
+            else
+#pragma unroll
+                for (int k = 0; k < 4; ++k) st_o(out + k, e[k]);
+        }
+    }
+    if (part) return;
+    __syncthreads();
+    for (u32 r = wave; r < w.nr; r += 4)
+        if (wrong[r]) attn_by_formula<T>(a, w.first, w.len, w.row, w.r0 + r, h);
+}
+#define ATTN_FEW(T, TN, CT, CN, DH, QT)                                                                                         \
+    extern "C" __global__ __launch_bounds__(256) void attn_few_##TN##_##CN##_##DH##_##QT(const NkAttnKvArgs a) {                \
+        attn_few<T, CT, DH, QT>(a);                                                                                             \
+    }
+#define ATTN_FEW_DH(DH, QT)                                                                                                     \
+    ATTN_FEW(u16, bf16, u16, bf16, DH, QT) ATTN_FEW(u16, bf16, unsigned char, e4m3, DH, QT)                                     \
+    ATTN_FEW(float, f32, u16, bf16, DH, QT) ATTN_FEW(float, f32, unsigned char, e4m3, DH, QT)
+ATTN_FEW_DH(64, 1) ATTN_FEW_DH(128, 1) ATTN_FEW_DH(256, 1) ATTN_FEW_DH(64, 2) ATTN_FEW_DH(128, 2)
+ATTN_FEW(u16, bf16, u16, bf16, 256, 2) ATTN_FEW(u16, bf16, unsigned char, e4m3, 256, 2)
+
+/* The pieces of split sequences added up: a wavefront per packed row. */
+template <typename T> __device__ __forceinline__ void attn_join(const NkAttnKvArgs &a) {
+    const u32 lane = threadIdx.x & 63, h = blockIdx.y, dh = a.kv.dh, piece = attn_piece(a);
+    if (!piece) return;
+    const kvitem_t it = kv_find(a.nseq, blockIdx.x, [&](u32 i) {
+        const kvseq_t s = attn_seq(a, i);
+        const u32 n = attn_tiles(a, s);
+        return n && attn_pieces(a, s, piece) > 1 ? n : 0;
+    });
+    if (!it.found) return;
+    u32 before = 0; /* items of the sequences before this one */
+    for (u32 i = lane; i < it.seq; i += 64) {
+        const kvseq_t s = attn_seq(a, i);
+        const u32 n = attn_tiles(a, s);
+        before += n ? n * attn_pieces(a, s, piece) : 0;
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) before += (u32)__shfl_xor((int)before, o, 64);
+    const kvseq_t s = attn_seq(a, it.seq);
+    attn_work_t w;
+    w.len = s.len;
+    w.r0 = (attn_tiles(a, s) - 1 - it.local) * a.tile;
+    w.nr = min(a.tile, s.rows * a.group - w.r0);
+    attn_steps(a, w);
+    const u32 r = blockIdx.z * 4 + threadIdx.x / 64;
+    if (r >= w.nr) return;
+    const u32 pieces = (w.steps - 1) / piece + 1, item = before + it.local * attn_pieces(a, s, piece);
+    const u64 stride = (u64)a.kv.heads * a.tile * (dh + 2);
+    const float *part = attn_part(a, item, h);
+    float top = -1e30f;
+    for (u32 k = lane; k < pieces; k += 64) top = fmaxf(top, part[k * stride + 2 * r]);
+    top = wmax(top);
+    float sum = 0.0f, v[4] = { 0.0f, 0.0f, 0.0f, 0.0f };
+#pragma unroll 4
+    for (u32 k = 0; k < pieces; ++k) {
+        const float *p = part + k * stride;
+        const float f = __builtin_amdgcn_exp2f(p[2 * r] - top);
+        sum = fmaf(p[2 * r + 1], f, sum);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const u32 d = min(lane + 64 * e, dh - 1);
+            if (64 * e < (int)dh) v[e] = fmaf(f, p[2 * a.tile + (u64)r * dh + d], v[e]);
+        }
+    }
+    const u32 pr = w.r0 + r;
+    T *out = (T *)a.o + (u64)(s.first + pr / a.group) * a.ldo + (u64)(h * a.group + pr % a.group) * dh;
+    bool bad = false;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+        if (lane + 64 * e < dh) {
+            const float x = v[e] / sum;
+            bad |= !(fabsf(x) < INFINITY);
+            st_o(out + lane + 64 * e, x);
+        }
+    if (__ballot(bad)) attn_by_formula<T>(a, s.first, s.len, s.row, pr, h);
+}
+extern "C" __global__ __launch_bounds__(256) void attn_join_f32(const NkAttnKvArgs a) { attn_join<float>(a); }
+extern "C" __global__ __launch_bounds__(256) void attn_join_bf16(const NkAttnKvArgs a) { attn_join<u16>(a); }

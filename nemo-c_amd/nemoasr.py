@@ -179,6 +179,10 @@ API = {
     "nk_causal_conv": (C.c_int, [_vp, _vp, C.c_int, _u32, _vp, _vp, _vp, _u32, _vp, _u32, _u32, _vp, _u32, _u32, _u32,
                                  _u32, C.c_int]),
     "nk_ssm_scan": (C.c_int, [_vp, _vp]),
+    "nk_rope_freqs": (C.c_int, [_vp, _u32, C.c_double, C.c_int] + [C.c_double] * 4),
+    "nk_kv_append": (C.c_int, [_vp, _vp, _vp]),
+    "nk_kv_read": (C.c_int, [_vp, _vp, _vp, _u32, _vp, _u32, C.c_int, _vp, _u32, _u32, _u32]),
+    "nk_attention_kv": (C.c_int, [_vp, _vp, _vp]),
     # include/nemo_gpu.h (the reference's runtime interface; gpu_arg_t arrays are GpuArg below)
     "gpu_buf_ptr": (_vp, [_vp]),
     "gpu_dispatch": (C.c_int, [_vp, C.c_char_p, _vp, C.c_int] + [_u32] * 6),
@@ -247,6 +251,26 @@ class Scan(C.Structure):
     _fields_ = ([("type", C.c_int)] + [(n, _u32) for n in ("ldx", "lddt", "ldbc", "ldz", "ldy")] +
                 [(n, _vp) for n in ("x", "dt", "B", "C", "z", "y", "A", "skip", "dt_bias", "state", "seqs")] +
                 [(n, _u32) for n in ("slots", "nseq", "max_rows", "M", "D", "N", "groups")] + [("softplus", C.c_int)])
+
+
+class Kv(C.Structure):
+    """nk_kv_t: a paged key and value cache (device addresses)."""
+    _fields_ = ([("type", C.c_int)] + [(n, _u32) for n in ("heads", "dh", "page", "pages")] +
+                [(n, _vp) for n in ("k", "v", "ks", "vs", "table")] + [(n, _u32) for n in ("ldt", "tables")])
+
+
+class Append(C.Structure):
+    """nk_append_t: the operands of nk_kv_append (device addresses; lengths in elements)."""
+    _fields_ = ([("type", C.c_int)] + [(n, _u32) for n in ("ldq", "ldk", "ldv", "ldqo")] + [(n, _vp) for n in ("q", "k", "v", "qo")] +
+                [(n, _u32) for n in ("heads", "rot")] + [("inter", C.c_int), ("freq", _vp), ("amp", C.c_float), ("seqs", _vp)] +
+                [(n, _u32) for n in ("nseq", "max_rows", "M")])
+
+
+class Attend(C.Structure):
+    """nk_attend_t: the operands of nk_attention_kv (device addresses; lengths in elements)."""
+    _fields_ = ([("type", C.c_int)] + [(n, _u32) for n in ("ldq", "ldo")] + [(n, _vp) for n in ("q", "o")] +
+                [(n, _u32) for n in ("heads", "window", "sinks")] + [("scale", C.c_float), ("seqs", _vp)] +
+                [(n, _u32) for n in ("nseq", "max_rows", "max_len", "M")])
 
 
 def fp4_row(k: int) -> int:
