@@ -134,21 +134,27 @@ int nk_attention_kv(gpu_t *g, const nk_kv_t *c, const nk_attend_t *p) {
     const uint32_t group = p->heads / kv.heads;
     const uint32_t window = p->window >= p->max_len ? 0 : p->window, sinks = p->sinks < p->max_len ? p->sinks : p->max_len;
     NkAttnKvArgs a = { kv, p->q, p->o, p->seqs, NULL, p->ldq, p->ldo, p->heads, group, window, sinks, p->nseq, p->max_rows, p->max_len, p->M,
-                       0, p->max_rows, 0, 0, 0, 0, 0, p->scale };
+                       0, p->max_rows, 0, 0, 0, 0, 0, 0, p->scale };
     a.vec = aligned(p->q, 16) && aligned(p->o, 4 * size) && p->ldq % (16 / size) == 0 && p->ldo % 4 == 0;
-    const uint32_t rows = p->max_rows < p->M ? p->max_rows : p->M, DH = kv.dh <= 64 ? 64 : kv.dh <= 128 ? 128 : 256;
-    const uint32_t QT = (uint64_t)rows * group > 16 && (DH < 256 || p->type == NK_BF16) ? 2 : 1;
-    a.tile = 16 * QT;
-    a.step = 32;
-    a.least = 8;
+    const uint32_t rows = p->max_rows < p->M ? p->max_rows : p->M;
+    uint32_t DH = kv.dh <= 64 ? 64 : kv.dh <= 128 ? 128 : 256;
+    const uint64_t packed = (uint64_t)rows * group;
+    const int many = packed > 64 && DH < 256;
+    const uint32_t QT = packed > 16 && (DH < 256 || p->type == NK_BF16) ? 2 : 1;
+    const uint32_t NW = 4;
+    if (many && kv.dh > 64 && kv.dh <= 96) DH = 96;
+    a.tile = many ? 32 * NW : 16 * QT;
+    a.step = many ? 64 : 32;
+    a.least = many ? 4 : 8;
     /* tiles that there can be, and the pieces that a tile can have */
     const uint64_t each = ((uint64_t)rows * group + a.tile - 1) / a.tile, by_rows = (uint64_t)p->M * group / a.tile + p->nseq;
     const uint64_t tiles = p->nseq * each < by_rows ? p->nseq * each : by_rows;
     const uint64_t pieces = ((p->max_len + a.step - 1) / a.step + a.least - 1) / a.least;
     if (tiles > 1u << 23) return bad(g, "attention_kv: more rows than a launch covers");
     uint64_t items = tiles;
-    if (pieces > 1) {
-        a.slots = (1024 + kv.heads - 1) / kv.heads;
+    const uint32_t slots = (1024 + kv.heads - 1) / kv.heads;
+    if (pieces > 1 && (uint64_t)p->M * group / a.tile < slots) {
+        a.slots = slots;
         const uint64_t split = tiles * pieces < 2ull * a.slots ? tiles * pieces : 2ull * a.slots;
         if (items < split) items = split;
         a.ws = gpu_scratch_ws(g, (size_t)(split * kv.heads * a.tile * (kv.dh + 2)));
@@ -156,11 +162,18 @@ int nk_attention_kv(gpu_t *g, const nk_kv_t *c, const nk_attend_t *p) {
     }
     const char *type = p->type == NK_F32 ? "f32" : "bf16";
     char name[40];
-    snprintf(name, sizeof name, "attn_few_%s_%s_%u_%u", type, cache_name(&kv), DH, QT);
+    if (many) snprintf(name, sizeof name, "attn_many_%s_%s_%u_%u", type, cache_name(&kv), DH, NW);
+    else snprintf(name, sizeof name, "attn_few_%s_%s_%u_%u_%u", type, cache_name(&kv), DH, QT, NW);
     gpu_next_bytes(g, 2.0 * size * p->M * nq);
-    if (gpu_launch(g, name, &a, sizeof a, (uint32_t)items, kv.heads, 1, 256, 1, 1)) return -1;
+    if (items * kv.heads > 1u << 22) return bad(g, "attention_kv: more rows than a launch covers");
+    if (gpu_launch(g, name, &a, sizeof a, (uint32_t)items * kv.heads, 1, 1, NW * 64, 1, 1)) return -1;
     if (!a.slots) return 0;
     snprintf(name, sizeof name, "attn_join_%s", type);
-    const uint64_t most = (uint64_t)rows * group < a.tile ? (uint64_t)rows * group : a.tile;
-    return gpu_launch(g, name, &a, sizeof a, (uint32_t)(tiles < a.slots ? tiles : a.slots), kv.heads, (uint32_t)(most + 3) / 4, 256, 1, 1);
+    const uint64_t most = (uint64_t)rows * group < a.tile ? (uint64_t)rows * group : a.tile, some = tiles < a.slots ? tiles : a.slots;
+    /* a row to a workgroup, or its wavefronts a row each and going round: some 2048 workgroups */
+    a.share = some * kv.heads * most <= 2048;
+    uint64_t z = 2048 / (some * kv.heads);
+    if (a.share) z = most;
+    else if (z > (most + 3) / 4) z = (most + 3) / 4;
+    return gpu_launch(g, name, &a, sizeof a, (uint32_t)some, kv.heads, z ? (uint32_t)z : 1, 256, 1, 1);
 }

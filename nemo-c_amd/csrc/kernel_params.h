@@ -587,6 +587,7 @@ typedef struct {
     u32 over, upto;   /* sequences of more than `over` and at most `upto` rows are this launch's */
     u32 tile, step;   /* rows (of all heads of a group) of a workgroup; tokens of a step */
     u32 slots, least; /* workgroups per head of the cache that are wanted; the fewest steps of a piece */
+    u32 share;        /* attn_join: four wavefronts to a row */
     u32 vec;          /* rows are read and written 16 (bf16: 8) bytes at a time */
     float scale;
 } NkAttnKvArgs;

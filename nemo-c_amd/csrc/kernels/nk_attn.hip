@@ -101,45 +101,47 @@ __device__ __forceinline__ void attn_steps(const NkAttnKvArgs &a, attn_work_t &w
 __device__ __forceinline__ kvseq_t attn_seq(const NkAttnKvArgs &a, u32 i) {
     return kvseq_load(a.seqs, i, a.M, a.max_rows, a.kv.tables, min(kv_room(a.kv), (u64)a.max_len));
 }
-__device__ __forceinline__ u64 wave_sum64(u64 v) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v += shfl_xor_u64(v, o);
-    return v;
-}
+/* the sequence of this lane, of the first 64 */
+__device__ __forceinline__ kvseq_t attn_mine(const NkAttnKvArgs &a) { return attn_seq(a, min(threadIdx.x & 63, a.nseq - 1)); }
 /* steps of a piece; 0: nothing is split */
-__device__ __forceinline__ u32 attn_piece(const NkAttnKvArgs &a) {
+__device__ __forceinline__ u32 attn_piece(const NkAttnKvArgs &a, kvseq_t s) {
+    const u32 lane = threadIdx.x & 63;
+    if (!a.slots) return 0;
     u64 tiles = 0, steps = 0;
-    for (u32 i = threadIdx.x & 63; i < a.nseq; i += 64) {
-        const kvseq_t s = attn_seq(a, i);
+    for (u32 i = lane; i < a.nseq; i += 64) {
+        if (i != lane) s = attn_seq(a, i);
         const u32 n = attn_tiles(a, s);
         tiles += n;
         steps += n ? (u64)n * attn_most_steps(a, s) : 0;
     }
-    tiles = wave_sum64(tiles);
+    auto total = [](u64 v) { return ((u64)lane_of(wave_scan((u32)(v >> 24)), 63) << 24) + lane_of(wave_scan((u32)v & 0xffffffu), 63); };
+    tiles = total(tiles);
     if (tiles >= a.slots) return 0;
-    steps = wave_sum64(steps);
+    steps = total(steps);
     return max((u32)((steps + a.slots - 1) / a.slots), a.least);
 }
 __device__ __forceinline__ u32 attn_pieces(const NkAttnKvArgs &a, const kvseq_t &s, u32 piece) {
     return piece ? (attn_most_steps(a, s) - 1) / piece + 1 : 1;
 }
+__device__ __forceinline__ void attn_tile(const NkAttnKvArgs &a, const kvseq_t &s, u32 tile, attn_work_t &w) {
+    w.first = s.first, w.rows = s.rows, w.len = s.len, w.row = s.row;
+    w.r0 = (attn_tiles(a, s) - 1 - tile) * a.tile; /* the last rows, which see most, first */
+    w.nr = min(a.tile, s.rows * a.group - w.r0);
+    attn_steps(a, w);
+}
 __device__ __forceinline__ bool attn_find(const NkAttnKvArgs &a, u32 id, attn_work_t &w) {
-    const u32 piece = a.slots ? attn_piece(a) : 0;
-    const kvitem_t it = kv_find(a.nseq, id, [&](u32 i) {
-        const kvseq_t s = attn_seq(a, i);
+    const kvseq_t mine = attn_mine(a);
+    const u32 piece = attn_piece(a, mine);
+    const kvitem_t it = kv_find(a.nseq, id, mine, [&](u32 i) { return attn_seq(a, i); }, [&](const kvseq_t &s) {
         const u32 n = attn_tiles(a, s);
         return n ? n * attn_pieces(a, s, piece) : 0;
     });
     if (!it.found) return false;
-    const kvseq_t s = attn_seq(a, it.seq);
-    w.first = s.first, w.rows = s.rows, w.len = s.len, w.row = s.row;
-    w.pieces = attn_pieces(a, s, piece);
+    w.pieces = attn_pieces(a, it.seq, piece);
     w.item = id;
     w.piece = it.local % w.pieces;
-    w.r0 = (attn_tiles(a, s) - 1 - it.local / w.pieces) * a.tile; /* the last rows, which see most, first */
-    w.nr = min(a.tile, s.rows * a.group - w.r0);
-    attn_steps(a, w);
-    w.from = piece ? w.piece * piece : 0;
+    attn_tile(a, it.seq, it.local / w.pieces, w);
+    w.from = w.piece * piece;
     w.to = piece ? min(w.steps, w.from + piece) : w.steps;
     return true;
 }
@@ -201,20 +203,20 @@ template <typename T> __device__ __forceinline__ void attn_by_formula(const NkAt
  * group g of a chunk pair has the values 16 g on), values through the wavefront's own LDS for their columns;
  * the next step's loads are in flight. */
 #define ATTN_STEP 32
-template <typename T, typename CT, int DH, int QT> __device__ __forceinline__ void attn_few(const NkAttnKvArgs &a) {
+template <typename T, typename CT, int DH, int QT, int NW> __device__ __forceinline__ void attn_few(const NkAttnKvArgs &a) {
     constexpr bool E4M3 = sizeof(CT) == 1;
     constexpr int NC = DH / 32, ND = DH / 16, TERMS = sizeof(T) == 4 ? 3 : 1, ROWS = 16 * QT;
     constexpr int LDV = DH + 16; /* u16 of a token's row in LDS: 32 bytes more, so that four tokens' are in other banks */
     constexpr int NK = E4M3 ? DH / 64 : DH / 32, NV = E4M3 ? DH / 32 : DH / 16; /* 16-byte loads of a lane: per 16 tokens; per step */
-    constexpr u32 VBYTES = 4 * ATTN_STEP * LDV * 2, OBYTES = 4 * 16 * DH * 4;
+    constexpr u32 VBYTES = NW * ATTN_STEP * LDV * 2, OBYTES = NW * 16 * DH * 4;
     __shared__ __align__(16) char lds[VBYTES > OBYTES ? VBYTES : OBYTES];
-    __shared__ float wm[4][ROWS], wl[4][ROWS];
+    __shared__ float wm[NW][ROWS], wl[NW][ROWS];
     __shared__ u32 wrong[ROWS];
     const NkKv &kv = a.kv;
-    const u32 h = blockIdx.y, lane = threadIdx.x & 63, c16 = lane & 15, g4 = lane >> 4;
+    const u32 h = blockIdx.x % kv.heads, lane = threadIdx.x & 63, c16 = lane & 15, g4 = lane >> 4;
     const u32 wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), dh = kv.dh;
     attn_work_t w;
-    if (!attn_find(a, blockIdx.x, w) || w.from >= w.to) return;
+    if (!attn_find(a, blockIdx.x / kv.heads, w) || w.from >= w.to) return;
     if (threadIdx.x < ROWS) wrong[threadIdx.x] = 0;
     const u32 pos_lo = w.len + w.r0 / a.group, pos_hi = w.len + (w.r0 + w.nr - 1) / a.group;
 
@@ -297,10 +299,10 @@ template <typename T, typename CT, int DH, int QT> __device__ __forceinline__ vo
     if (u < w.to) {
         lookup(u);
         load(u);
-        lookup(min(u + 4, w.steps - 1));
+        lookup(min(u + NW, w.steps - 1));
     }
 #pragma unroll 1
-    for (; u < w.to; u += 4) {
+    for (; u < w.to; u += NW) {
         const u32 t0 = token(u);
         floatx4 s[QT][2];
         const bool th[2] = { there[0], there[1] };
@@ -328,9 +330,9 @@ template <typename T, typename CT, int DH, int QT> __device__ __forceinline__ vo
                 *(u32x4 *)(p + 8) = e4m3_bf16(vr[i].z, vr[i].w, f);
             } else *(u32x4 *)p = vr[i];
         }
-        if (u + 4 < w.to) {
-            load(u + 4);
-            lookup(min(u + 8, w.steps - 1));
+        if (u + NW < w.to) {
+            load(u + NW);
+            lookup(min(u + 2 * NW, w.steps - 1));
         }
         const bool whole = t0 + ATTN_STEP - 1 <= pos_lo && th[0] && th[1] &&
                            (!a.window || t0 + a.window > pos_hi || t0 + ATTN_STEP <= a.sinks);
@@ -384,15 +386,15 @@ template <typename T, typename CT, int DH, int QT> __device__ __forceinline__ vo
 #pragma unroll
         for (int n = 0; n < ND; ++n) *(floatx4 *)(ol + (wave * 16 + c16) * DH + 16 * n + 4 * g4) = o[t][n];
         __syncthreads();
-        for (u32 i = threadIdx.x; i < 16 * DH / 4; i += 256) {
+        for (u32 i = threadIdx.x; i < 16 * DH / 4; i += NW * 64) {
             const u32 r = i / (DH / 4), d = i % (DH / 4) * 4, rt = 16 * t + r;
             if (rt >= w.nr || d >= dh) continue;
             float top = wm[0][rt], sum = 0.0f;
 #pragma unroll
-            for (int k = 1; k < 4; ++k) top = fmaxf(top, wm[k][rt]);
+            for (int k = 1; k < NW; ++k) top = fmaxf(top, wm[k][rt]);
             floatx4 v = { 0, 0, 0, 0 };
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
+            for (int k = 0; k < NW; ++k) {
                 const float f = __builtin_amdgcn_exp2f(wm[k][rt] - top);
                 sum = fmaf(wl[k][rt], f, sum);
                 v += f * *(const floatx4 *)(ol + (k * 16 + r) * DH + d);
@@ -416,74 +418,361 @@ template <typename T, typename CT, int DH, int QT> __device__ __forceinline__ vo
     }
     if (part) return;
     __syncthreads();
-    for (u32 r = wave; r < w.nr; r += 4)
+    for (u32 r = wave; r < w.nr; r += NW)
         if (wrong[r]) attn_by_formula<T>(a, w.first, w.len, w.row, w.r0 + r, h);
 }
-#define ATTN_FEW(T, TN, CT, CN, DH, QT)                                                                                         \
-    extern "C" __global__ __launch_bounds__(256) void attn_few_##TN##_##CN##_##DH##_##QT(const NkAttnKvArgs a) {                \
-        attn_few<T, CT, DH, QT>(a);                                                                                             \
+#ifndef OCC_B
+#define OCC_B 2
+#define OCC_E 3
+#endif
+#define ATTN_FEW(T, TN, CT, CN, DH, QT, NW, OCC)                                                                                \
+    extern "C" __global__ __launch_bounds__(NW * 64, OCC) void attn_few_##TN##_##CN##_##DH##_##QT##_##NW(const NkAttnKvArgs a) { \
+        attn_few<T, CT, DH, QT, NW>(a);                                                                                         \
     }
-#define ATTN_FEW_DH(DH, QT)                                                                                                     \
-    ATTN_FEW(u16, bf16, u16, bf16, DH, QT) ATTN_FEW(u16, bf16, unsigned char, e4m3, DH, QT)                                     \
-    ATTN_FEW(float, f32, u16, bf16, DH, QT) ATTN_FEW(float, f32, unsigned char, e4m3, DH, QT)
-ATTN_FEW_DH(64, 1) ATTN_FEW_DH(128, 1) ATTN_FEW_DH(256, 1) ATTN_FEW_DH(64, 2) ATTN_FEW_DH(128, 2)
-ATTN_FEW(u16, bf16, u16, bf16, 256, 2) ATTN_FEW(u16, bf16, unsigned char, e4m3, 256, 2)
+#define ATTN_FEW_DH(DH, QT, NW)                                                                                                 \
+    ATTN_FEW(u16, bf16, u16, bf16, DH, QT, NW, 1) ATTN_FEW(u16, bf16, unsigned char, e4m3, DH, QT, NW, 1)                       \
+    ATTN_FEW(float, f32, u16, bf16, DH, QT, NW, 1) ATTN_FEW(float, f32, unsigned char, e4m3, DH, QT, NW, 1)
+ATTN_FEW_DH(64, 1, 4) ATTN_FEW_DH(256, 1, 4) ATTN_FEW_DH(64, 2, 4) ATTN_FEW_DH(128, 2, 4)
+ATTN_FEW(u16, bf16, u16, bf16, 256, 2, 4, 1) ATTN_FEW(u16, bf16, unsigned char, e4m3, 256, 2, 4, 1)
+ATTN_FEW(u16, bf16, u16, bf16, 128, 1, 4, OCC_B) ATTN_FEW(u16, bf16, unsigned char, e4m3, 128, 1, 4, OCC_E)
+ATTN_FEW(float, f32, u16, bf16, 128, 1, 4, 1) ATTN_FEW(float, f32, unsigned char, e4m3, 128, 1, 4, 1)
+ATTN_FEW_DH(64, 1, 8) ATTN_FEW_DH(256, 1, 8)
+ATTN_FEW(u16, bf16, u16, bf16, 128, 1, 8, 2) ATTN_FEW(u16, bf16, unsigned char, e4m3, 128, 1, 8, 2)
+ATTN_FEW(float, f32, u16, bf16, 128, 1, 8, 2) ATTN_FEW(float, f32, unsigned char, e4m3, 128, 1, 8, 2)
 
-/* The pieces of split sequences added up: a wavefront per packed row. */
+/* ---- many rows: wavefronts over the rows ----------------------------------------------------------------
+ * A workgroup's 32 NW packed rows, 32 to a wavefront, over steps of 64 tokens whose keys and values lie in LDS for all of
+ * them, the next step's on the way meanwhile.  Products on 32x32x16: first S^T = K Q^T, so that a lane has one row's logits
+ * (its maximum and sum are the lane's own and one swap), then O^T = V^T P^T with P straight from those registers: their
+ * tokens 4 hh + (0..3) and 8 on of every 16 (hh: the lane's half) are the order in which the columns of V are read.
+ * A row of LDS is DH values; its 16-byte chunks are mixed by the token so that the lanes of a read spread over all
+ * banks.  The maximum follows only where a logit is 2^8 times above it: 2^(x - m) may exceed 1 as well as not, and the
+ * sums are rescaled once or twice a row instead of every step. */
+typedef float floatx16 __attribute__((ext_vector_type(16)));
+__device__ __forceinline__ floatx16 attn_mfma32(u32x4 a, u32x4 b, floatx16 acc) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), acc, 0, 0, 0);
+}
+#define ATTN_MANY 64
+template <typename T, typename CT, int DC, int NW> __device__ __forceinline__ void attn_many(const NkAttnKvArgs &a) {
+    constexpr bool E4M3 = sizeof(CT) == 1;
+    constexpr int DH = DC <= 64 ? 64 : 128; /* values of a row in LDS, of which DC count */
+    constexpr int NC = DC / 16, ND = DC / 32, TERMS = sizeof(T) == 4 ? 3 : 1, CH = DH / 8; /* 16-byte chunks of a row */
+    constexpr int TOK = ATTN_MANY / NW;                     /* tokens that a wavefront brings */
+    constexpr int PER = E4M3 ? DH / 16 : DH / 8, NL = TOK * PER / 64; /* lanes to a token; loads a wavefront, of keys and of values */
+    static_assert(NL >= 1 && TOK <= 16, "loads");
+    __shared__ __align__(16) u16 lds[2][2][ATTN_MANY * DH];
+    const NkKv &kv = a.kv;
+    const u32 h = blockIdx.x % kv.heads, lane = threadIdx.x & 63, c32 = lane & 31, hh = lane >> 5, dh = kv.dh;
+    const u32 wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+    attn_work_t w;
+    if (!attn_find(a, blockIdx.x / kv.heads, w) || w.from >= w.to) return;
+    const u32 pos_lo = w.len + w.r0 / a.group, pos_hi = w.len + (w.r0 + w.nr - 1) / a.group;
+    const u32 row = 32 * wave + c32, pr = w.r0 + min(row, w.nr - 1), pos = w.len + pr / a.group;
+    const u64 at_head = (u64)(h * a.group + pr % a.group) * dh;
+
+    u32x4 qf[NC][TERMS];
+    {
+        const T *q = (const T *)a.q + (u64)(w.first + pr / a.group) * a.ldq + at_head;
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+            const u32 d = 16 * c + 8 * hh;
+            const T *p = q + min(d, dh - 8);
+            float v[8];
+            if (a.vec) kv_load<8>(v, p);
+            else
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[e] = ld_q(p + e);
+            if (d >= dh)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[e] = 0.0f;
+            attn_terms<TERMS>(v, qf[c]);
+        }
+    }
+
+    auto token = [&](u32 u) { return (u < w.sink_steps ? u : w.lo_step + u - w.sink_steps) * ATTN_MANY; };
+    auto mixk = [](u32 t) { return DH == 64 ? (t >> 1) & 7 : t & 15; };
+    auto mixv = [](u32 t) { return DH == 64 ? (t << 1) & 4 : (t << 2) & 12; };
+    int pe[4];
+    auto lookup = [&](u32 u) {
+        const u32 t0 = token(u);
+#pragma unroll
+        for (int b = 0; b < 4; ++b) pe[b] = kv.table[(u64)w.row * kv.ldt + (min(t0 + 16 * b, pos_hi) >> kv.shift)];
+    };
+    u32x4 kr[E4M3 ? NL : 1], vr[E4M3 ? NL : 1];
+    u32 ksb, vsb;
+    auto load = [&](u32 u, u32 buf) { /* this wavefront's tokens, from the page that pe has */
+        const u32 tt = token(u) + TOK * wave, mine = TOK * wave / 16;
+        const u32 tb = min(tt & ~15u, pos_hi & ~15u);
+        const int p = mine == 0 ? pe[0] : mine == 1 ? pe[1] : mine == 2 ? pe[2] : pe[3];
+        const u64 slot = (((u64)(u32)((u32)p < kv.pages ? p : 0) * kv.heads + h) << kv.shift) + (tb & ((1u << kv.shift) - 1));
+        const u32 last = min(pos_hi - tb, 15u);
+        if constexpr (E4M3) {
+            ksb = kv.ks[slot / NK_KV_BLOCK];
+            vsb = kv.vs[slot / NK_KV_BLOCK];
+        }
+#pragma unroll
+        for (int i = 0; i < NL; ++i) {
+            const u32 t = TOK * wave % 16 + i * (64 / PER) + lane / PER, tok = min(t, last);
+            if constexpr (E4M3) {
+                const u64 o = slot * dh + tok * dh + min(lane % PER * 16, dh - 16);
+                kr[i] = *(const u32x4 *)((const CT *)kv.k + o);
+                vr[i] = *(const u32x4 *)((const CT *)kv.v + o);
+            } else {
+                const u64 r = slot * dh + tok * dh;
+                const u32 to = (TOK * wave + i * (64 / PER)) * DH;
+                dma16((const CT *)kv.k + r + min((lane % CH ^ mixk(t)) * 8, dh - 8), (lds_char_t *)&lds[buf][0][to]);
+                dma16((const CT *)kv.v + r + min((lane % CH ^ mixv(t)) * 8, dh - 8), (lds_char_t *)&lds[buf][1][to]);
+            }
+        }
+    };
+    auto put = [&](u32 buf) { /* what load has in registers: two chunks a lane */
+        if constexpr (E4M3)
+#pragma unroll
+            for (int i = 0; i < NL; ++i) {
+                const u32 t = TOK * wave + i * (64 / PER) + lane / PER, c = 2 * (lane % PER);
+                const float fk = scale8(ksb), fv = scale8(vsb);
+                *(u32x4 *)&lds[buf][0][t * DH + (c ^ mixk(t)) * 8] = e4m3_bf16(kr[i].x, kr[i].y, fk);
+                *(u32x4 *)&lds[buf][0][t * DH + ((c + 1) ^ mixk(t)) * 8] = e4m3_bf16(kr[i].z, kr[i].w, fk);
+                *(u32x4 *)&lds[buf][1][t * DH + (c ^ mixv(t)) * 8] = e4m3_bf16(vr[i].x, vr[i].y, fv);
+                *(u32x4 *)&lds[buf][1][t * DH + ((c + 1) ^ mixv(t)) * 8] = e4m3_bf16(vr[i].z, vr[i].w, fv);
+            }
+    };
+
+    floatx16 o[ND];
+#pragma unroll
+    for (int n = 0; n < ND; ++n)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[n][i] = 0.0f;
+    float m = -1e30f, l = 0.0f;
+    const float scale2 = a.scale * 1.44269504f;
+    /* where this lane's first reads lie; the others by xor and constant distances */
+    const u32 kat = c32 * DH * 2 + ((hh ^ mixk(c32)) << 4);
+    const u32 vt = 4 * hh + (lane & 15) / 4, vat = vt * DH * 2 + (((lane >> 4 & 1) * 2 + (lane & 3) / 2) ^ mixv(vt)) * 16 + (lane & 1) * 8;
+
+    u32 there = 15, next = 15; /* which of the step's four blocks have a page */
+    auto known = [&] {
+        u32 v = 0;
+#pragma unroll
+        for (int b = 0; b < 4; ++b) v |= (u32)pe[b] < kv.pages ? 1u << b : 0;
+        return v;
+    };
+    lookup(w.from);
+    load(w.from, 0);
+    next = known();
+    lookup(min(w.from + 1, w.to - 1));
+    const u32 reach = a.window ? a.window : 1u << 31;
+#pragma unroll 1
+    for (u32 u = w.from; u < w.to; ++u) {
+        const u32 buf = (u - w.from) & 1, t0 = token(u);
+        put(buf);
+        there = next;
+        wait_vm_lgkm<0>(); /* this step's keys and values, of all wavefronts; no one reads the other half any more */
+        barrier_mem();
+        if (u + 1 < w.to) {
+            load(u + 1, buf ^ 1);
+            next = known();
+            lookup(min(u + 2, w.to - 1));
+        }
+        const char *kl = (const char *)lds[buf][0], *vl = (const char *)lds[buf][1];
+        floatx16 s[2];
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) s[b][i] = 0.0f;
+#pragma unroll
+        for (int c = 0; c < NC; ++c)
+#pragma unroll
+            for (int b = 0; b < 2; ++b) {
+                const u32x4 kf = *(const u32x4 *)(kl + (kat ^ (c << 5)) + b * 32 * DH * 2);
+#pragma unroll
+                for (int k = TERMS - 1; k >= 0; --k) s[b] = attn_mfma32(kf, qf[c][k], s[b]);
+            }
+        if (t0 + ATTN_MANY - 1 > pos_lo || there != 15 || (t0 + reach <= pos_hi && t0 + ATTN_MANY > a.sinks)) {
+            const u32 back = pos - t0 - 4 * hh; /* how far back token t0 + 4 hh lies; what lies ahead is far above `reach` */
+            const bool first = a.window && t0 < a.sinks;
+#pragma unroll
+            for (int b = 0; b < 2; ++b)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const u32 j = 32 * b + 8 * (i / 4) + i % 4;
+                    s[b][i] = back - j < reach ? s[b][i] : first && back - j < 1u << 31 && t0 + 4 * hh + j < a.sinks ? s[b][i] : -INFINITY;
+                }
+            if (there != 15)
+#pragma unroll
+                for (int b = 0; b < 2; ++b)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) s[b][i] = there >> (2 * b + i / 8) & 1 ? s[b][i] : -INFINITY;
+        }
+        float top = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) top = fmaxf(top, fmaxf(s[0][i], s[1][i]));
+        top = max_over32(top) * scale2;
+        if (__ballot(top > m + 8.0f)) {
+            top = fmaxf(m, top);
+            const float old = __builtin_amdgcn_exp2f(m - top);
+            m = top;
+            l *= old;
+#pragma unroll
+            for (int n = 0; n < ND; ++n) o[n] *= old;
+        }
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            float p[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) p[i] = __builtin_amdgcn_exp2f(fmaf(s[g / 2][8 * (g % 2) + i], scale2, -m));
+            l += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
+            u32x4 pf[TERMS];
+            attn_terms<TERMS>(p, pf);
+#pragma unroll
+            for (int n = 0; n < ND; ++n) {
+                const u16 *q = (const u16 *)(vl + (vat ^ (n << 6)) + g * 16 * DH * 2);
+                const uint2 x = lds_column4(q), y = lds_column4(q + 8 * DH);
+                const u32x4 vf = { x.x, x.y, y.x, y.y };
+#pragma unroll
+                for (int k = TERMS - 1; k >= 0; --k) o[n] = attn_mfma32(vf, pf[k], o[n]);
+            }
+        }
+    }
+
+    l = sum_over32(l);
+    if (w.pieces > 1) {
+        float *part = attn_part(a, w.item, h);
+        if (row < w.nr) {
+            if (!hh) part[2 * row] = m, part[2 * row + 1] = l;
+#pragma unroll
+            for (int n = 0; n < ND; ++n)
+#pragma unroll
+                for (int i = 0; i < 16; i += 4) {
+                    const u32 d = 32 * n + 2 * i + 4 * hh;
+                    if (d < dh) *(floatx4 *)(part + 2 * a.tile + (u64)row * dh + d) = (floatx4){ o[n][i], o[n][i + 1], o[n][i + 2], o[n][i + 3] };
+                }
+        }
+        return;
+    }
+    bool bad = false;
+    if (row < w.nr) {
+        T *out = (T *)a.o + (u64)(w.first + pr / a.group) * a.ldo + at_head;
+#pragma unroll
+        for (int n = 0; n < ND; ++n)
+#pragma unroll
+            for (int i = 0; i < 16; i += 4) {
+                const u32 d = 32 * n + 2 * i + 4 * hh;
+                if (d >= dh) continue;
+                float e[4];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    e[k] = o[n][i + k] / l;
+                    bad |= !(fabsf(e[k]) < INFINITY);
+                }
+                if (a.vec) kv_store<4>(out + d, e);
+                else
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) st_o(out + d + k, e[k]);
+            }
+    }
+    u64 wrong = __ballot(bad);
+    for (wrong = (wrong | wrong >> 32) & 0xffffffffu; wrong; wrong &= wrong - 1)
+        attn_by_formula<T>(a, w.first, w.len, w.row, w.r0 + 32 * wave + (u32)__ffsll((unsigned long long)wrong) - 1, h);
+}
+#define ATTN_MANY_K(T, TN, CT, CN, DH, NW)                                                                                   \
+    extern "C" __global__ __launch_bounds__(NW * 64, 2) void attn_many_##TN##_##CN##_##DH##_##NW(const NkAttnKvArgs a) {     \
+        attn_many<T, CT, DH, NW>(a);                                                                                         \
+    }
+#define ATTN_MANY_DH(DH, NW)                                                                                                 \
+    ATTN_MANY_K(u16, bf16, u16, bf16, DH, NW) ATTN_MANY_K(u16, bf16, unsigned char, e4m3, DH, NW)                            \
+    ATTN_MANY_K(float, f32, u16, bf16, DH, NW) ATTN_MANY_K(float, f32, unsigned char, e4m3, DH, NW)
+ATTN_MANY_DH(64, 4) ATTN_MANY_DH(96, 4) ATTN_MANY_DH(128, 4)
+#ifdef W8
+ATTN_MANY_DH(96, 8) ATTN_MANY_DH(128, 8)
+#endif
+
+/* The pieces of split sequences added up: a wavefront per packed row, or (share) four; a lane has
+ * two neighbouring sums (and two more 128 on), eight pieces' in flight. */
 template <typename T> __device__ __forceinline__ void attn_join(const NkAttnKvArgs &a) {
-    const u32 lane = threadIdx.x & 63, h = blockIdx.y, dh = a.kv.dh, piece = attn_piece(a);
+    __shared__ float4 sums[3][64];
+    __shared__ float total[3];
+    const u32 lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), h = blockIdx.y, dh = a.kv.dh;
+    const kvseq_t mine = attn_mine(a);
+    const u32 piece = attn_piece(a, mine);
     if (!piece) return;
-    const kvitem_t it = kv_find(a.nseq, blockIdx.x, [&](u32 i) {
-        const kvseq_t s = attn_seq(a, i);
+    auto load = [&](u32 i) { return attn_seq(a, i); };
+    const kvitem_t it = kv_find(a.nseq, blockIdx.x, mine, load, [&](const kvseq_t &s) {
         const u32 n = attn_tiles(a, s);
         return n && attn_pieces(a, s, piece) > 1 ? n : 0;
     });
     if (!it.found) return;
     u32 before = 0; /* items of the sequences before this one */
-    for (u32 i = lane; i < it.seq; i += 64) {
-        const kvseq_t s = attn_seq(a, i);
+    for (u32 i = lane; i < it.i; i += 64) {
+        const kvseq_t s = i == lane ? mine : load(i);
         const u32 n = attn_tiles(a, s);
         before += n ? n * attn_pieces(a, s, piece) : 0;
     }
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) before += (u32)__shfl_xor((int)before, o, 64);
-    const kvseq_t s = attn_seq(a, it.seq);
+    before = lane_of(wave_scan(before), 63);
     attn_work_t w;
-    w.len = s.len;
-    w.r0 = (attn_tiles(a, s) - 1 - it.local) * a.tile;
-    w.nr = min(a.tile, s.rows * a.group - w.r0);
-    attn_steps(a, w);
-    const u32 r = blockIdx.z * 4 + threadIdx.x / 64;
-    if (r >= w.nr) return;
-    const u32 pieces = (w.steps - 1) / piece + 1, item = before + it.local * attn_pieces(a, s, piece);
+    attn_tile(a, it.seq, it.local, w);
+    const u32 pieces = (w.steps - 1) / piece + 1, item = before + it.local * attn_pieces(a, it.seq, piece);
     const u64 stride = (u64)a.kv.heads * a.tile * (dh + 2);
-    const float *part = attn_part(a, item, h);
-    float top = -1e30f;
-    for (u32 k = lane; k < pieces; k += 64) top = fmaxf(top, part[k * stride + 2 * r]);
-    top = wmax(top);
-    float sum = 0.0f, v[4] = { 0.0f, 0.0f, 0.0f, 0.0f };
-#pragma unroll 4
-    for (u32 k = 0; k < pieces; ++k) {
-        const float *p = part + k * stride;
-        const float f = __builtin_amdgcn_exp2f(p[2 * r] - top);
-        sum = fmaf(p[2 * r + 1], f, sum);
+    const bool shared = a.share;
+    const u32 begin = shared ? wave : 0, by = shared ? 4 : 1, d0 = min(2 * lane, dh - 2), d1 = min(128 + 2 * lane, dh - 2);
+    for (u32 r = shared ? blockIdx.z : blockIdx.z * 4 + wave; r < w.nr; r += gridDim.z * (shared ? 1 : 4)) {
+        const float *part = attn_part(a, item, h), *rows = part + 2 * a.tile + (u64)r * dh;
+        float top = -1e30f;
+        for (u32 k = lane; k < pieces; k += 64) top = fmaxf(top, part[k * stride + 2 * r]);
+        top = wmax(top);
+        float sum = 0.0f;
+        floatx2 v = { 0, 0 }, v1 = { 0, 0 };
+        for (u32 k0 = 0; k0 < pieces; k0 += 64) {
+            const float *p = part + min(k0 + lane, pieces - 1) * stride + 2 * r;
+            const float f = k0 + lane < pieces ? __builtin_amdgcn_exp2f(p[0] - top) : 0.0f, l = f * p[1];
+            const u32 n = min(pieces - k0, 64u);
+            for (u32 k = begin; k < n; k += 8 * by) {
+                floatx2 x[8], y[8];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const u32 d = min(lane + 64 * e, dh - 1);
-            if (64 * e < (int)dh) v[e] = fmaf(f, p[2 * a.tile + (u64)r * dh + d], v[e]);
+                for (u32 e = 0; e < 8; ++e) {
+                    const float *q = rows + (u64)(k0 + min(k + e * by, n - 1)) * stride;
+                    x[e] = *(const floatx2 *)(q + d0);
+                    if (dh > 128) y[e] = *(const floatx2 *)(q + d1);
+                }
+#pragma unroll
+                for (u32 e = 0; e < 8; ++e)
+                    if (k + e * by < n) {
+                        const float g = __uint_as_float(lane_of(__float_as_uint(f), (int)(k + e * by)));
+                        v += g * x[e];
+                        if (dh > 128) v1 += g * y[e];
+                        sum += __uint_as_float(lane_of(__float_as_uint(l), (int)(k + e * by)));
+                    }
+            }
         }
+        if (shared) {
+            __syncthreads();
+            if (wave) {
+                sums[wave - 1][lane] = make_float4(v.x, v.y, v1.x, v1.y);
+                total[wave - 1] = sum;
+            }
+            __syncthreads();
+            if (wave) continue;
+#pragma unroll
+            for (int k = 0; k < 3; ++k) {
+                const float4 q = sums[k][lane];
+                v += (floatx2){ q.x, q.y };
+                v1 += (floatx2){ q.z, q.w };
+                sum += total[k];
+            }
+        }
+        const u32 pr = w.r0 + r;
+        T *out = (T *)a.o + (u64)(w.first + pr / a.group) * a.ldo + (u64)(h * a.group + pr % a.group) * dh;
+        const float e[4] = { v.x / sum, v.y / sum, v1.x / sum, v1.y / sum };
+        bool bad = false;
+#pragma unroll
+        for (u32 k = 0; k < 4; ++k) {
+            const u32 d = 128 * (k / 2) + 2 * lane + k % 2;
+            if (d < dh) {
+                bad |= !(fabsf(e[k]) < INFINITY);
+                st_o(out + d, e[k]);
+            }
+        }
+        if (__ballot(bad)) attn_by_formula<T>(a, w.first, w.len, w.row, pr, h);
     }
-    const u32 pr = w.r0 + r;
-    T *out = (T *)a.o + (u64)(s.first + pr / a.group) * a.ldo + (u64)(h * a.group + pr % a.group) * dh;
-    bool bad = false;
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-        if (lane + 64 * e < dh) {
-            const float x = v[e] / sum;
-            bad |= !(fabsf(x) < INFINITY);
-            st_o(out + lane + 64 * e, x);
-        }
-    if (__ballot(bad)) attn_by_formula<T>(a, s.first, s.len, s.row, pr, h);
 }
 extern "C" __global__ __launch_bounds__(256) void attn_join_f32(const NkAttnKvArgs a) { attn_join<float>(a); }
 extern "C" __global__ __launch_bounds__(256) void attn_join_bf16(const NkAttnKvArgs a) { attn_join<u16>(a); }

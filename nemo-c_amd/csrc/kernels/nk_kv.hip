@@ -12,32 +12,48 @@ __device__ __forceinline__ kvseq_t kvseq_load(const int *seqs, u32 i, u32 M, u32
 }
 __device__ __forceinline__ u64 kv_room(const NkKv &kv) { return (u64)kv.ldt << kv.shift; }
 
-/* The sequence that has number `id` when every sequence i has count(i) of them, and its number there.  Every wavefront
- * looks by itself, 64 sequences at a time. */
+/* blocks of 16 tokens that a sequence's rows touch */
+__device__ __forceinline__ u32 kv_blocks(const kvseq_t &s) {
+    return s.ok && s.rows ? (s.len % NK_KV_BLOCK + s.rows - 1) / NK_KV_BLOCK + 1 : 0;
+}
+
+/* sums over the lanes up to this one (rows of 16, then what the rows before have) */
+__device__ __forceinline__ u32 wave_scan(u32 v) {
+#define SCAN_DPP(CTRL, ROWS) v += (u32)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xF, false)
+    SCAN_DPP(0x111, 0xF); /* row_shr 1, 2, 4, 8 */
+    SCAN_DPP(0x112, 0xF);
+    SCAN_DPP(0x114, 0xF);
+    SCAN_DPP(0x118, 0xF);
+    SCAN_DPP(0x142, 0xA); /* the last of a row to the next one, of the second to the upper two */
+    SCAN_DPP(0x143, 0xC);
+#undef SCAN_DPP
+    return v;
+}
+__device__ __forceinline__ u32 lane_of(u32 v, int lane) { return (u32)__builtin_amdgcn_readlane((int)v, lane); }
+
+/* The sequence that has number `id` when every sequence has count(it) of them, and its number there.  Every wavefront
+ * looks by itself, a sequence a lane; `mine` is that of the first 64, load(i) any other. */
 typedef struct {
-    u32 seq, local;
+    kvseq_t seq;
+    u32 i, local;
     bool found;
 } kvitem_t;
-template <typename F> __device__ __forceinline__ kvitem_t kv_find(u32 nseq, u32 id, F count) {
+template <typename L, typename F> __device__ __forceinline__ kvitem_t kv_find(u32 nseq, u32 id, kvseq_t mine, L load, F count) {
     const u32 lane = threadIdx.x & 63;
     u32 before = 0;
-    for (u32 i0 = 0; i0 < nseq; i0 += 64) {
-        const u32 n = i0 + lane < nseq ? count(i0 + lane) : 0;
-        u32 sum = n;
-#pragma unroll
-        for (int o = 1; o < 64; o *= 2) {
-            const u32 v = (u32)__shfl_up((int)sum, o, 64);
-            sum += lane >= (u32)o ? v : 0;
-        }
+    for (u32 i0 = 0;;) {
+        const u32 n = i0 + lane < nseq ? count(mine) : 0, sum = wave_scan(n);
         const u64 past = __ballot(before + sum > id);
         if (past) {
             const int at = __ffsll((unsigned long long)past) - 1;
-            const u32 local = id - before - (u32)__builtin_amdgcn_readlane((int)(sum - n), at);
-            return (kvitem_t){ i0 + (u32)at, local, true };
+            const kvseq_t s = { lane_of(mine.first, at), lane_of(mine.rows, at), lane_of(mine.len, at), lane_of(mine.row, at), true };
+            return (kvitem_t){ s, i0 + (u32)at, id - before - lane_of(sum - n, at), true };
         }
-        before += (u32)__builtin_amdgcn_readlane((int)sum, 63);
+        before += lane_of(sum, 63);
+        if ((i0 += 64) >= nseq) break;
+        mine = load(min(i0 + lane, nseq - 1));
     }
-    return (kvitem_t){ 0, 0, false };
+    return (kvitem_t){ mine, 0, 0, false };
 }
 
 /* P values of a row as f32, and back */
@@ -107,6 +123,24 @@ __device__ __forceinline__ float2 kv_turn(u32 pos, float freq, float amp) {
     return make_float2(amp * (k & 2 ? -x : x), amp * (k & 2 ? -y : y));
 }
 
+/* The same in 64 bits: the codes of 8-bit keys.  Half a step of theirs is 2^-4 of a value, so that a rounding on the way
+ * (2^-24) next to a border between two codes would move the value by a whole step. */
+__device__ __forceinline__ double2 kv_turn64(u32 pos, float freq, float amp) {
+    const double q = (double)pos * ((double)freq * (2.0 / 6.283185307179586476925)), n = rint(q);
+    double s, c;
+    sincospi(q - n, &s, &c);
+    const double f = fma(-2.0, floor(n * 0.5), n) != 0.0 ? -(double)amp : (double)amp;
+    return make_double2(f * c, f * s);
+}
+/* to f32 with the last bit set where it is not exact: rounds on to fewer bits as the value itself does */
+__device__ __forceinline__ float to_odd(double d) {
+    const float f = (float)d;
+    const double b = (double)f;
+    u32 u = __float_as_uint(f);
+    if (b != d) u = (u - (fabs(b) > fabs(d))) | 1u;
+    return __uint_as_float(u);
+}
+
 #define KV_PAIRS 128 /* dh / 2 at most */
 
 /* A workgroup takes the rows of a sequence that fall into one block of 16 tokens; its wavefronts take heads, one at a
@@ -117,20 +151,22 @@ __device__ __forceinline__ float2 kv_turn(u32 pos, float freq, float amp) {
  * those that become subnormal). */
 template <typename T, int P, bool E4M3> __device__ __forceinline__ void kv_append(const NkAppendArgs &a) {
     __shared__ float2 turn[NK_KV_BLOCK][KV_PAIRS];
+    __shared__ double2 turn64[E4M3 ? NK_KV_BLOCK : 1][E4M3 ? KV_PAIRS : 1]; /* of the keys */
     const NkKv &kv = a.kv;
     const u64 room = kv_room(kv);
     auto load = [&](u32 i) { return kvseq_load(a.seqs, i, a.M, a.max_rows, kv.tables, room); };
-    const kvitem_t it = kv_find(a.nseq, blockIdx.x, [&](u32 i) {
-        const kvseq_t s = load(i);
-        return s.ok && s.rows ? (s.len % NK_KV_BLOCK + s.rows - 1) / NK_KV_BLOCK + 1 : 0;
-    });
+    const kvitem_t it = kv_find(a.nseq, blockIdx.x, load(min(threadIdx.x & 63, a.nseq - 1)), load, kv_blocks);
     if (!it.found) return;
-    const kvseq_t s = load(it.seq);
+    const kvseq_t s = it.seq;
     const u32 t0 = (s.len / NK_KV_BLOCK + it.local) * NK_KV_BLOCK;
     const u32 lo = max(s.len, t0) - t0, hi = min(s.len + s.rows - t0, (u32)NK_KV_BLOCK), half = a.rot / 2;
     for (u32 i = threadIdx.x; i < (hi - lo) * half; i += 256) {
         const u32 t = lo + i / half, j = i % half;
-        turn[t][j] = kv_turn(t0 + t, a.freq[j], a.amp);
+        if constexpr (E4M3) {
+            const double2 c = kv_turn64(t0 + t, a.freq[j], a.amp);
+            turn64[t][j] = c;
+            turn[t][j] = make_float2((float)c.x, (float)c.y);
+        } else turn[t][j] = kv_turn(t0 + t, a.freq[j], a.amp);
     }
     __syncthreads();
     const int pe = kv.table[(u64)s.row * kv.ldt + (t0 >> kv.shift)];
@@ -156,31 +192,30 @@ template <typename T, int P, bool E4M3> __device__ __forceinline__ void kv_appen
             const T *r = src + (row0 + t) * ld;
             kv_load<P>(x, r + oa);
             kv_load<P>(y, r + ob);
-            if (j < half) {
-                if (a.inter) {
-                    if constexpr (P == 1) {
-                        const float2 c = turn[t][j];
-                        const float v = fmaf(x[0], c.x, -(y[0] * c.y));
-                        y[0] = fmaf(y[0], c.x, x[0] * c.y);
-                        x[0] = v;
-                    } else
-#pragma unroll
-                        for (int i = 0; i < P; ++i) {
-                            float &p = i < P / 2 ? x[2 * i] : y[2 * i - P], &q = i < P / 2 ? x[2 * i + 1] : y[2 * i + 1 - P];
-                            const float2 c = turn[t][j + i];
-                            const float v = fmaf(p, c.x, -(q * c.y));
-                            q = fmaf(q, c.x, p * c.y);
-                            p = v;
-                        }
-                } else
-#pragma unroll
-                    for (int i = 0; i < P; ++i) {
-                        const float2 c = turn[t][j + i];
-                        const float v = fmaf(x[i], c.x, -(y[i] * c.y));
-                        y[i] = fmaf(y[i], c.x, x[i] * c.y);
-                        x[i] = v;
+            if (j >= half) return;
+            auto pair = [&](int i, float &p, float &q) {
+                if constexpr (E4M3)
+                    if (!isq) {
+                        const double2 c = turn64[t][j + i];
+                        const double v = fma((double)p, c.x, -((double)q * c.y));
+                        q = to_odd(fma((double)q, c.x, (double)p * c.y));
+                        p = to_odd(v);
+                        return;
                     }
-            }
+                const float2 c = turn[t][j + i];
+                const float v = fmaf(p, c.x, -(q * c.y));
+                q = fmaf(q, c.x, p * c.y);
+                p = v;
+            };
+            if (P > 1 && a.inter)
+#pragma unroll
+                for (int i = 0; i < P / 2; ++i) {
+                    pair(i, x[2 * i], x[2 * i + 1]);
+                    pair(i + P / 2, y[2 * i], y[2 * i + 1]);
+                }
+            else
+#pragma unroll
+                for (int i = 0; i < P; ++i) pair(i, x[i], y[i]);
         };
         auto each = [&](auto f) {
             for (u32 t = lo + tk0; t < hi; t += tpp)
@@ -248,12 +283,9 @@ template <typename T, int P, bool E4M3> __device__ __forceinline__ void kv_read(
     const NkKv &kv = a.kv;
     const u64 room = kv_room(kv);
     auto load = [&](u32 i) { return kvseq_load(a.seqs, i, a.M, a.max_rows, kv.tables, room); };
-    const kvitem_t it = kv_find(a.nseq, blockIdx.x, [&](u32 i) {
-        const kvseq_t s = load(i);
-        return s.ok && s.rows ? (s.len % NK_KV_BLOCK + s.rows - 1) / NK_KV_BLOCK + 1 : 0;
-    });
+    const kvitem_t it = kv_find(a.nseq, blockIdx.x, load(min(threadIdx.x & 63, a.nseq - 1)), load, kv_blocks);
     if (!it.found) return;
-    const kvseq_t s = load(it.seq);
+    const kvseq_t s = it.seq;
     const u32 t0 = (s.len / NK_KV_BLOCK + it.local) * NK_KV_BLOCK;
     const u32 lo = max(s.len, t0) - t0, hi = min(s.len + s.rows - t0, (u32)NK_KV_BLOCK), n = kv.dh / P;
     const int pe = kv.table[(u64)s.row * kv.ldt + (t0 >> kv.shift)];
