@@ -139,20 +139,19 @@ int nk_attention_kv(gpu_t *g, const nk_kv_t *c, const nk_attend_t *p) {
     const uint32_t rows = p->max_rows < p->M ? p->max_rows : p->M;
     uint32_t DH = kv.dh <= 64 ? 64 : kv.dh <= 128 ? 128 : 256;
     const uint64_t packed = (uint64_t)rows * group;
-    const int many = packed > 64 && DH < 256;
+    const int many = packed > 64;
     const uint32_t QT = packed > 16 && (DH < 256 || p->type == NK_BF16) ? 2 : 1;
-    const uint32_t NW = 4;
-    if (many && kv.dh > 64 && kv.dh <= 96) DH = 96;
-    a.tile = many ? 32 * NW : 16 * QT;
+    if (many) DH = kv.dh > 64 && kv.dh <= 96 ? 96 : kv.dh > 128 && kv.dh <= 192 ? 192 : DH;
+    a.tile = many ? 128 : 16 * QT;
     a.step = many ? 64 : 32;
-    a.least = many ? 4 : 8;
+    a.least = many && p->type == NK_F32 ? 4 : 8;
     /* tiles that there can be, and the pieces that a tile can have */
     const uint64_t each = ((uint64_t)rows * group + a.tile - 1) / a.tile, by_rows = (uint64_t)p->M * group / a.tile + p->nseq;
     const uint64_t tiles = p->nseq * each < by_rows ? p->nseq * each : by_rows;
     const uint64_t pieces = ((p->max_len + a.step - 1) / a.step + a.least - 1) / a.least;
     if (tiles > 1u << 23) return bad(g, "attention_kv: more rows than a launch covers");
     uint64_t items = tiles;
-    const uint32_t slots = (1024 + kv.heads - 1) / kv.heads;
+    const uint32_t wanted = packed > 16 ? many && p->type == NK_F32 ? 512 : 256 : p->nseq > 1 ? 1024 : 512, slots = (wanted + kv.heads - 1) / kv.heads;
     if (pieces > 1 && (uint64_t)p->M * group / a.tile < slots) {
         a.slots = slots;
         const uint64_t split = tiles * pieces < 2ull * a.slots ? tiles * pieces : 2ull * a.slots;
@@ -162,11 +161,11 @@ int nk_attention_kv(gpu_t *g, const nk_kv_t *c, const nk_attend_t *p) {
     }
     const char *type = p->type == NK_F32 ? "f32" : "bf16";
     char name[40];
-    if (many) snprintf(name, sizeof name, "attn_many_%s_%s_%u_%u", type, cache_name(&kv), DH, NW);
-    else snprintf(name, sizeof name, "attn_few_%s_%s_%u_%u_%u", type, cache_name(&kv), DH, QT, NW);
+    if (many) snprintf(name, sizeof name, "attn_many_%s_%s_%u", type, cache_name(&kv), DH);
+    else snprintf(name, sizeof name, "attn_few_%s_%s_%u_%u_4", type, cache_name(&kv), DH, QT);
     gpu_next_bytes(g, 2.0 * size * p->M * nq);
     if (items * kv.heads > 1u << 22) return bad(g, "attention_kv: more rows than a launch covers");
-    if (gpu_launch(g, name, &a, sizeof a, (uint32_t)items * kv.heads, 1, 1, NW * 64, 1, 1)) return -1;
+    if (gpu_launch(g, name, &a, sizeof a, (uint32_t)items * kv.heads, 1, 1, 256, 1, 1)) return -1;
     if (!a.slots) return 0;
     snprintf(name, sizeof name, "attn_join_%s", type);
     const uint64_t most = (uint64_t)rows * group < a.tile ? (uint64_t)rows * group : a.tile, some = tiles < a.slots ? tiles : a.slots;

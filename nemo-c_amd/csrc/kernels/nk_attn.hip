@@ -32,6 +32,8 @@ __device__ __forceinline__ void swap16(float &a, float &b) {
     a = __uint_as_float(r[0]);
     b = __uint_as_float(r[1]);
 }
+/* one instruction for three, NaN if any is (fmaxf takes another to quiet a product's) */
+__device__ __forceinline__ float max3(float a, float b, float c) { return __builtin_elementwise_maximum(__builtin_elementwise_maximum(a, b), c); }
 /* over the lanes that agree in their low four bits (16: five) */
 __device__ __forceinline__ float max_over32(float a) { float b = a; swap32(a, b); return fmaxf(a, b); }
 __device__ __forceinline__ float sum_over32(float a) { float b = a; swap32(a, b); return a + b; }
@@ -66,6 +68,17 @@ template <int TERMS> __device__ __forceinline__ void attn_terms(const float (&x)
     }
 }
 
+/* the sum of eight probabilities: of bf16 rows as they were rounded, so that their weights add up to one */
+template <int TERMS> __device__ __forceinline__ float attn_sum(float l, const float (&p)[8], u32x4 t) {
+    if constexpr (TERMS > 1) return l + (((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7])));
+    else {
+        const bf16x2 one = { (__bf16)1.0f, (__bf16)1.0f };
+#pragma unroll
+        for (int i = 0; i < 4; ++i) l = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, (u32)t[i]), one, l, false);
+        return l;
+    }
+}
+
 /* ---- who does what ------------------------------------------------------------------------------------
  * A sequence's packed rows go in tiles of a.tile; a tile's tokens in steps of a.step: the steps of the first tokens that
  * stay visible (`sinks`), then those from the first row's window to the last row.  Where all tiles are fewer than the
@@ -77,16 +90,15 @@ typedef struct {
     u32 r0, nr;                 /* the tile's packed rows */
     u32 lo_step, sink_steps, steps; /* its steps: sink_steps from 0 on, the others from lo_step on */
     u32 from, to;               /* the piece's */
-    u32 pieces, item;           /* pieces of every tile of the sequence; this one's number over all */
-    u32 piece;
+    u32 split, item;            /* whether it has other pieces; this one's number over all */
 } attn_work_t;
 
 __device__ __forceinline__ u32 attn_tiles(const NkAttnKvArgs &a, const kvseq_t &s) {
     return s.ok && s.rows > a.over && s.rows <= a.upto ? (s.rows * a.group - 1) / a.tile + 1 : 0;
 }
-/* the most steps that a tile of the sequence has */
-__device__ __forceinline__ u32 attn_most_steps(const NkAttnKvArgs &a, const kvseq_t &s) {
-    const u32 all = (s.len + s.rows - 1) / a.step + 1;
+/* the most steps that a tile has whose last row is the sequence's row `rows` - 1 */
+__device__ __forceinline__ u32 attn_most_steps(const NkAttnKvArgs &a, const kvseq_t &s, u32 rows) {
+    const u32 all = (s.len + rows - 1) / a.step + 1;
     if (!a.window) return all;
     const u64 some = ((u64)a.window + (a.tile - 1) / a.group + 2 + a.step - 1) / a.step + 1 + ((u64)a.sinks + a.step - 1) / a.step;
     return some < all ? (u32)some : all;
@@ -112,7 +124,7 @@ __device__ __forceinline__ u32 attn_piece(const NkAttnKvArgs &a, kvseq_t s) {
         if (i != lane) s = attn_seq(a, i);
         const u32 n = attn_tiles(a, s);
         tiles += n;
-        steps += n ? (u64)n * attn_most_steps(a, s) : 0;
+        if (n) steps += (u64)n * (attn_most_steps(a, s, s.rows) + attn_most_steps(a, s, min(s.rows, a.tile / a.group + 1))) / 2;
     }
     auto total = [](u64 v) { return ((u64)lane_of(wave_scan((u32)(v >> 24)), 63) << 24) + lane_of(wave_scan((u32)v & 0xffffffu), 63); };
     tiles = total(tiles);
@@ -121,13 +133,18 @@ __device__ __forceinline__ u32 attn_piece(const NkAttnKvArgs &a, kvseq_t s) {
     return max((u32)((steps + a.slots - 1) / a.slots), a.least);
 }
 __device__ __forceinline__ u32 attn_pieces(const NkAttnKvArgs &a, const kvseq_t &s, u32 piece) {
-    return piece ? (attn_most_steps(a, s) - 1) / piece + 1 : 1;
+    return piece ? (attn_most_steps(a, s, s.rows) - 1) / piece + 1 : 1;
 }
 __device__ __forceinline__ void attn_tile(const NkAttnKvArgs &a, const kvseq_t &s, u32 tile, attn_work_t &w) {
     w.first = s.first, w.rows = s.rows, w.len = s.len, w.row = s.row;
     w.r0 = (attn_tiles(a, s) - 1 - tile) * a.tile; /* the last rows, which see most, first */
     w.nr = min(a.tile, s.rows * a.group - w.r0);
     attn_steps(a, w);
+}
+__device__ __forceinline__ void attn_uniform(attn_work_t &w) {
+    u32 *p = &w.first;
+#pragma unroll
+    for (u32 i = 0; i < sizeof w / 4; ++i) p[i] = (u32)__builtin_amdgcn_readfirstlane((int)p[i]);
 }
 __device__ __forceinline__ bool attn_find(const NkAttnKvArgs &a, u32 id, attn_work_t &w) {
     const kvseq_t mine = attn_mine(a);
@@ -137,17 +154,23 @@ __device__ __forceinline__ bool attn_find(const NkAttnKvArgs &a, u32 id, attn_wo
         return n ? n * attn_pieces(a, s, piece) : 0;
     });
     if (!it.found) return false;
-    w.pieces = attn_pieces(a, it.seq, piece);
+    const u32 pieces = attn_pieces(a, it.seq, piece);
     w.item = id;
-    w.piece = it.local % w.pieces;
-    attn_tile(a, it.seq, it.local / w.pieces, w);
-    w.from = w.piece * piece;
+    attn_tile(a, it.seq, it.local / pieces, w);
+    w.from = it.local % pieces * piece;
     w.to = piece ? min(w.steps, w.from + piece) : w.steps;
+    w.split = w.steps > w.to - w.from;
+    attn_uniform(w); /* or the compiler keeps all that follows from it per lane */
     return true;
 }
 /* a piece's place in the scratch: m and l of its rows, then their sums */
 __device__ __forceinline__ float *attn_part(const NkAttnKvArgs &a, u32 item, u32 h) {
     return a.ws + ((u64)item * a.kv.heads + h) * a.tile * (a.kv.dh + 2);
+}
+
+/* the page of a token, the same for all lanes (nothing writes the table meanwhile) */
+__device__ __forceinline__ int attn_page(const NkKv &kv, u32 row, u32 token) {
+    return ((const __attribute__((address_space(4))) int *)kv.table)[(u64)row * kv.ldt + (token >> kv.shift)];
 }
 
 __device__ __forceinline__ float kv_value(const NkKv &kv, const void *c, const unsigned char *s, u64 slot, u32 d) {
@@ -249,7 +272,7 @@ template <typename T, typename CT, int DH, int QT, int NW> __device__ __forceinl
     auto token = [&](u32 u) { return (u < w.sink_steps ? u : w.lo_step + u - w.sink_steps) * ATTN_STEP; };
     auto lookup = [&](u32 u) {
 #pragma unroll
-        for (int b = 0; b < 2; ++b) pe[b] = kv.table[(u64)w.row * kv.ldt + (min(token(u) + 16 * b, pos_hi) >> kv.shift)];
+        for (int b = 0; b < 2; ++b) pe[b] = attn_page(kv, w.row, min(token(u) + 16 * b, pos_hi));
     };
     bool there[2];
     auto load = [&](u32 u) { /* from the pages that pe has */
@@ -294,6 +317,7 @@ template <typename T, typename CT, int DH, int QT, int NW> __device__ __forceinl
     }
     u16 *vl = (u16 *)lds + wave * ATTN_STEP * LDV;
     const float scale2 = a.scale * 1.44269504f;
+    const u32 reach = a.window ? a.window : 1u << 31; /* tokens that a row sees back: what lies ahead of it is far above */
 
     u32 u = w.from + wave;
     if (u < w.to) {
@@ -345,20 +369,20 @@ template <typename T, typename CT, int DH, int QT, int NW> __device__ __forceinl
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         const u32 j = t0 + 16 * b + 4 * g4 + i;
-                        const bool see = th[b] && j <= pos[t] && (!a.window || pos[t] - j < a.window || j < a.sinks);
+const bool see = th[b] & ((pos[t] - j < reach) | ((j < a.sinks) & (j <= pos[t]) & (reach < 1u << 31)));
                         s[t][b][i] = see ? s[t][b][i] : -INFINITY;
                     }
             }
-            float top = fmaxf(fmaxf(fmaxf(s[t][0][0], s[t][0][1]), fmaxf(s[t][0][2], s[t][0][3])),
-                              fmaxf(fmaxf(s[t][1][0], s[t][1][1]), fmaxf(s[t][1][2], s[t][1][3])));
+            float top = max3(max3(s[t][0][0], s[t][0][1], s[t][0][2]), max3(s[t][1][0], s[t][1][1], s[t][1][2]),
+                             __builtin_elementwise_maximum(s[t][0][3], s[t][1][3]));
             top = fmaxf(m[t], max_over16(top) * scale2);
             const float old = __builtin_amdgcn_exp2f(m[t] - top);
             m[t] = top;
             float p[8];
 #pragma unroll
             for (int i = 0; i < 8; ++i) p[i] = __builtin_amdgcn_exp2f(fmaf(s[t][i / 4][i % 4], scale2, -top));
-            l[t] = fmaf(l[t], old, ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7])));
             attn_terms<TERMS>(p, pf[t]);
+            l[t] = attn_sum<TERMS>(l[t] * old, p, pf[t][0]);
 #pragma unroll
             for (int n = 0; n < ND; ++n) o[t][n] *= old;
         }
@@ -376,7 +400,7 @@ template <typename T, typename CT, int DH, int QT, int NW> __device__ __forceinl
         asm volatile("" ::: "memory");
     }
 
-    float *part = w.pieces > 1 ? attn_part(a, w.item, h) : NULL;
+    float *part = w.split ? attn_part(a, w.item, h) : NULL;
     float *ol = (float *)lds;
 #pragma unroll
     for (int t = 0; t < QT; ++t) {
@@ -441,7 +465,7 @@ ATTN_FEW(u16, bf16, u16, bf16, 128, 1, 8, 2) ATTN_FEW(u16, bf16, unsigned char, 
 ATTN_FEW(float, f32, u16, bf16, 128, 1, 8, 2) ATTN_FEW(float, f32, unsigned char, e4m3, 128, 1, 8, 2)
 
 /* ---- many rows: wavefronts over the rows ----------------------------------------------------------------
- * A workgroup's 32 NW packed rows, 32 to a wavefront, over steps of 64 tokens whose keys and values lie in LDS for all of
+ * A workgroup's 128 packed rows, 32 to a wavefront, over steps of 64 tokens whose keys and values lie in LDS for all of
  * them, the next step's on the way meanwhile.  Products on 32x32x16: first S^T = K Q^T, so that a lane has one row's logits
  * (its maximum and sum are the lane's own and one swap), then O^T = V^T P^T with P straight from those registers: their
  * tokens 4 hh + (0..3) and 8 on of every 16 (hh: the lane's half) are the order in which the columns of V are read.
@@ -452,15 +476,22 @@ typedef float floatx16 __attribute__((ext_vector_type(16)));
 __device__ __forceinline__ floatx16 attn_mfma32(u32x4 a, u32x4 b, floatx16 acc) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), acc, 0, 0, 0);
 }
+/* dma16 (see there) from a base that all lanes share and 32 bits of a lane's own, to an LDS address; it writes where nothing
+ * is read before the next wait and barrier, so that the reads around it may move */
+__device__ __forceinline__ void dma16_at(const char *base, u32 off, u32 to) {
+    asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(to));
+}
 #define ATTN_MANY 64
-template <typename T, typename CT, int DC, int NW> __device__ __forceinline__ void attn_many(const NkAttnKvArgs &a) {
+template <typename T, typename CT, int DC> __device__ __forceinline__ void attn_many(const NkAttnKvArgs &a) {
     constexpr bool E4M3 = sizeof(CT) == 1;
-    constexpr int DH = DC <= 64 ? 64 : 128; /* values of a row in LDS, of which DC count */
+    constexpr int DH = DC <= 64 ? 64 : DC <= 128 ? 128 : 256; /* values of a row in LDS, of which DC count */
     constexpr int NC = DC / 16, ND = DC / 32, TERMS = sizeof(T) == 4 ? 3 : 1, CH = DH / 8; /* 16-byte chunks of a row */
-    constexpr int TOK = ATTN_MANY / NW;                     /* tokens that a wavefront brings */
+    constexpr int TOK = ATTN_MANY / 4;                                /* tokens that a wavefront brings: a block */
     constexpr int PER = E4M3 ? DH / 16 : DH / 8, NL = TOK * PER / 64; /* lanes to a token; loads a wavefront, of keys and of values */
-    static_assert(NL >= 1 && TOK <= 16, "loads");
-    __shared__ __align__(16) u16 lds[2][2][ATTN_MANY * DH];
+    static_assert(NL >= 1 && TOK == NK_KV_BLOCK, "loads");
+    constexpr u32 HALF = ATTN_MANY * DH * 2;
+    __shared__ __align__(16) char lds[4 * HALF]; /* keys of two steps, values of two */
+    __shared__ __align__(4) unsigned char page_of[2][4];
     const NkKv &kv = a.kv;
     const u32 h = blockIdx.x % kv.heads, lane = threadIdx.x & 63, c32 = lane & 31, hh = lane >> 5, dh = kv.dh;
     const u32 wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
@@ -469,6 +500,65 @@ template <typename T, typename CT, int DC, int NW> __device__ __forceinline__ vo
     const u32 pos_lo = w.len + w.r0 / a.group, pos_hi = w.len + (w.r0 + w.nr - 1) / a.group;
     const u32 row = 32 * wave + c32, pr = w.r0 + min(row, w.nr - 1), pos = w.len + pr / a.group;
     const u64 at_head = (u64)(h * a.group + pr % a.group) * dh;
+
+    auto token = [&](u32 u) { return (u < w.sink_steps ? u : w.lo_step + u - w.sink_steps) * ATTN_MANY; };
+    auto mixk = [](u32 t) { return DH == 64 ? (t >> 1) & 7 : t & 15; };
+    auto mixv = [](u32 t) { return DH == 64 ? (t << 1) & 4 : (t << 2) & 12; };
+    /* A wavefront brings a block of 16 tokens, from one page; whether there is one, all learn through LDS. */
+    int pe;
+    u64 slot;   /* of the block's first token, and the last one that is read: behind the last row, that one again */
+    u32 last;
+    auto lookup = [&](u32 u) { pe = attn_page(kv, w.row, min(token(min(u, w.to - 1)) + TOK * wave, pos_hi)); };
+    u32x4 kr[E4M3 ? NL : 1], vr[E4M3 ? NL : 1];
+    u32 ksb, vsb;
+    const u32 lds0 = __builtin_amdgcn_readfirstlane((u32)(size_t)(lds_char_t *)lds) + TOK * wave * DH * 2;
+    const u32 lt = lane / PER, bytes = dh * sizeof(CT), lc = lane % PER;
+    auto place = [&](u32 u) { /* the block of step u, whose page pe has */
+        const u32 tb = min(token(u) + TOK * wave, pos_hi & ~15u);
+        const bool ok = (u32)pe < kv.pages;
+        last = min(pos_hi - tb, 15u);
+        slot = (((u64)(ok ? (u32)pe : 0) * kv.heads + h) << kv.shift) + (tb & ((1u << kv.shift) - 1));
+        return ok;
+    };
+    auto load = [&](const void *from, u32 to, u32x4 &r, int i, bool v) { /* the i-th of NL loads */
+        const u32 t = i * (64 / PER) + lt, at = __umul24(min(t, last), bytes);
+        const char *base = (const char *)from + slot * bytes;
+        if constexpr (E4M3) r = *(const u32x4 *)(base + (at + min(lc * 16, bytes - 16)));
+        else dma16_at(base, at + min((lc ^ (v ? mixv(t) : mixk(t))) * 16, bytes - 16), to + i * (64 / PER) * DH * 2);
+    };
+    auto load_k = [&](u32 buf, int i) { load(kv.k, lds0 + buf * HALF, kr[E4M3 ? i : 0], i, false); };
+    auto load_v = [&](u32 buf, int i) { load(kv.v, lds0 + (2 + buf) * HALF, vr[E4M3 ? i : 0], i, true); };
+    auto put = [&](u32 to, u32 sb, u32x4 r, int i, bool v) { /* 8-bit codes from registers: two chunks a lane */
+        const u32 t = TOK * wave + i * (64 / PER) + lt, x = v ? mixv(t) : mixk(t);
+        const float f = scale8(sb);
+        *(u32x4 *)(lds + to + t * DH * 2 + ((2 * lc) ^ x) * 16) = e4m3_bf16(r.x, r.y, f);
+        *(u32x4 *)(lds + to + t * DH * 2 + ((2 * lc + 1) ^ x) * 16) = e4m3_bf16(r.z, r.w, f);
+    };
+    auto put_k = [&](u32 buf) {
+        if constexpr (E4M3)
+#pragma unroll
+            for (int i = 0; i < NL; ++i) put(buf * HALF, ksb, kr[i], i, false);
+    };
+    auto put_v = [&](u32 buf) {
+        if constexpr (E4M3)
+#pragma unroll
+            for (int i = 0; i < NL; ++i) put((2 + buf) * HALF, vsb, vr[i], i, true);
+    };
+    auto begin_k = [&](u32 u, u32 buf) {
+        const bool ok = place(u);
+        if (lane == 0) page_of[buf][wave] = ok;
+        if constexpr (E4M3) ksb = kv.ks[slot / NK_KV_BLOCK];
+    };
+    auto begin_v = [&] {
+        if constexpr (E4M3) vsb = kv.vs[slot / NK_KV_BLOCK];
+    };
+
+    lookup(w.from);
+    begin_k(w.from, 0);
+    begin_v();
+#pragma unroll
+    for (int i = 0; i < NL; ++i) load_k(0, i), load_v(0, i);
+    lookup(w.from + 1);
 
     u32x4 qf[NC][TERMS];
     {
@@ -488,56 +578,6 @@ template <typename T, typename CT, int DC, int NW> __device__ __forceinline__ vo
             attn_terms<TERMS>(v, qf[c]);
         }
     }
-
-    auto token = [&](u32 u) { return (u < w.sink_steps ? u : w.lo_step + u - w.sink_steps) * ATTN_MANY; };
-    auto mixk = [](u32 t) { return DH == 64 ? (t >> 1) & 7 : t & 15; };
-    auto mixv = [](u32 t) { return DH == 64 ? (t << 1) & 4 : (t << 2) & 12; };
-    int pe[4];
-    auto lookup = [&](u32 u) {
-        const u32 t0 = token(u);
-#pragma unroll
-        for (int b = 0; b < 4; ++b) pe[b] = kv.table[(u64)w.row * kv.ldt + (min(t0 + 16 * b, pos_hi) >> kv.shift)];
-    };
-    u32x4 kr[E4M3 ? NL : 1], vr[E4M3 ? NL : 1];
-    u32 ksb, vsb;
-    auto load = [&](u32 u, u32 buf) { /* this wavefront's tokens, from the page that pe has */
-        const u32 tt = token(u) + TOK * wave, mine = TOK * wave / 16;
-        const u32 tb = min(tt & ~15u, pos_hi & ~15u);
-        const int p = mine == 0 ? pe[0] : mine == 1 ? pe[1] : mine == 2 ? pe[2] : pe[3];
-        const u64 slot = (((u64)(u32)((u32)p < kv.pages ? p : 0) * kv.heads + h) << kv.shift) + (tb & ((1u << kv.shift) - 1));
-        const u32 last = min(pos_hi - tb, 15u);
-        if constexpr (E4M3) {
-            ksb = kv.ks[slot / NK_KV_BLOCK];
-            vsb = kv.vs[slot / NK_KV_BLOCK];
-        }
-#pragma unroll
-        for (int i = 0; i < NL; ++i) {
-            const u32 t = TOK * wave % 16 + i * (64 / PER) + lane / PER, tok = min(t, last);
-            if constexpr (E4M3) {
-                const u64 o = slot * dh + tok * dh + min(lane % PER * 16, dh - 16);
-                kr[i] = *(const u32x4 *)((const CT *)kv.k + o);
-                vr[i] = *(const u32x4 *)((const CT *)kv.v + o);
-            } else {
-                const u64 r = slot * dh + tok * dh;
-                const u32 to = (TOK * wave + i * (64 / PER)) * DH;
-                dma16((const CT *)kv.k + r + min((lane % CH ^ mixk(t)) * 8, dh - 8), (lds_char_t *)&lds[buf][0][to]);
-                dma16((const CT *)kv.v + r + min((lane % CH ^ mixv(t)) * 8, dh - 8), (lds_char_t *)&lds[buf][1][to]);
-            }
-        }
-    };
-    auto put = [&](u32 buf) { /* what load has in registers: two chunks a lane */
-        if constexpr (E4M3)
-#pragma unroll
-            for (int i = 0; i < NL; ++i) {
-                const u32 t = TOK * wave + i * (64 / PER) + lane / PER, c = 2 * (lane % PER);
-                const float fk = scale8(ksb), fv = scale8(vsb);
-                *(u32x4 *)&lds[buf][0][t * DH + (c ^ mixk(t)) * 8] = e4m3_bf16(kr[i].x, kr[i].y, fk);
-                *(u32x4 *)&lds[buf][0][t * DH + ((c + 1) ^ mixk(t)) * 8] = e4m3_bf16(kr[i].z, kr[i].w, fk);
-                *(u32x4 *)&lds[buf][1][t * DH + (c ^ mixv(t)) * 8] = e4m3_bf16(vr[i].x, vr[i].y, fv);
-                *(u32x4 *)&lds[buf][1][t * DH + ((c + 1) ^ mixv(t)) * 8] = e4m3_bf16(vr[i].z, vr[i].w, fv);
-            }
-    };
-
     floatx16 o[ND];
 #pragma unroll
     for (int n = 0; n < ND; ++n)
@@ -545,67 +585,54 @@ template <typename T, typename CT, int DC, int NW> __device__ __forceinline__ vo
         for (int i = 0; i < 16; ++i) o[n][i] = 0.0f;
     float m = -1e30f, l = 0.0f;
     const float scale2 = a.scale * 1.44269504f;
+    const u32 reach = a.window ? a.window : 1u << 31;
     /* where this lane's first reads lie; the others by xor and constant distances */
     const u32 kat = c32 * DH * 2 + ((hh ^ mixk(c32)) << 4);
     const u32 vt = 4 * hh + (lane & 15) / 4, vat = vt * DH * 2 + (((lane >> 4 & 1) * 2 + (lane & 3) / 2) ^ mixv(vt)) * 16 + (lane & 1) * 8;
 
-    u32 there = 15, next = 15; /* which of the step's four blocks have a page */
-    auto known = [&] {
-        u32 v = 0;
-#pragma unroll
-        for (int b = 0; b < 4; ++b) v |= (u32)pe[b] < kv.pages ? 1u << b : 0;
-        return v;
+    auto key = [&](u32 buf, int c, int b) { return *(const u32x4 *)(lds + buf * HALF + (kat ^ (c << 5)) + b * 32 * DH * 2); };
+    auto value = [&](u32 buf, int g, int n) {
+        const u16 *q = (const u16 *)(lds + (2 + buf) * HALF + (vat ^ (n << 6)) + g * 16 * DH * 2);
+        const uint2 x = lds_column4(q), y = lds_column4(q + 8 * DH);
+        return (u32x4){ x.x, x.y, y.x, y.y };
     };
-    lookup(w.from);
-    load(w.from, 0);
-    next = known();
-    lookup(min(w.from + 1, w.to - 1));
-    const u32 reach = a.window ? a.window : 1u << 31;
-#pragma unroll 1
-    for (u32 u = w.from; u < w.to; ++u) {
-        const u32 buf = (u - w.from) & 1, t0 = token(u);
-        put(buf);
-        there = next;
-        wait_vm_lgkm<0>(); /* this step's keys and values, of all wavefronts; no one reads the other half any more */
-        barrier_mem();
-        if (u + 1 < w.to) {
-            load(u + 1, buf ^ 1);
-            next = known();
-            lookup(min(u + 2, w.to - 1));
-        }
-        const char *kl = (const char *)lds[buf][0], *vl = (const char *)lds[buf][1];
-        floatx16 s[2];
+    /* logits of tokens that a row does not see */
+    auto hide = [&](floatx16 (&s)[2], u32 u, u32 buf) {
+        const u32 t0 = token(u), there = (u32)__builtin_amdgcn_readfirstlane(*(const int *)page_of[buf]); /* a byte for every block */
+        if (t0 + ATTN_MANY - 1 <= pos_lo && there == 0x01010101u && (t0 + reach > pos_hi || t0 + ATTN_MANY <= a.sinks)) return;
+        const u32 back = pos - t0 - 4 * hh; /* how far back token t0 + 4 hh lies; what lies ahead is far above `reach` */
+        if (!a.window || t0 >= a.sinks)
 #pragma unroll
-        for (int b = 0; b < 2; ++b)
+            for (int b = 0; b < 2; ++b)
 #pragma unroll
-            for (int i = 0; i < 16; ++i) s[b][i] = 0.0f;
-#pragma unroll
-        for (int c = 0; c < NC; ++c)
-#pragma unroll
-            for (int b = 0; b < 2; ++b) {
-                const u32x4 kf = *(const u32x4 *)(kl + (kat ^ (c << 5)) + b * 32 * DH * 2);
-#pragma unroll
-                for (int k = TERMS - 1; k >= 0; --k) s[b] = attn_mfma32(kf, qf[c][k], s[b]);
-            }
-        if (t0 + ATTN_MANY - 1 > pos_lo || there != 15 || (t0 + reach <= pos_hi && t0 + ATTN_MANY > a.sinks)) {
-            const u32 back = pos - t0 - 4 * hh; /* how far back token t0 + 4 hh lies; what lies ahead is far above `reach` */
-            const bool first = a.window && t0 < a.sinks;
+                for (int i = 0; i < 16; ++i) s[b][i] = back - (32 * b + 8 * (i / 4) + i % 4) < reach ? s[b][i] : -INFINITY;
+        else {
+            const u32 left = a.sinks - t0; /* > 0; and what is ahead is behind pos */
 #pragma unroll
             for (int b = 0; b < 2; ++b)
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
                     const u32 j = 32 * b + 8 * (i / 4) + i % 4;
-                    s[b][i] = back - j < reach ? s[b][i] : first && back - j < 1u << 31 && t0 + 4 * hh + j < a.sinks ? s[b][i] : -INFINITY;
+                    s[b][i] = (back - j < reach) | ((4 * hh + j < left) & ((int)(back - j) >= 0)) ? s[b][i] : -INFINITY;
                 }
-            if (there != 15)
-#pragma unroll
-                for (int b = 0; b < 2; ++b)
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) s[b][i] = there >> (2 * b + i / 8) & 1 ? s[b][i] : -INFINITY;
         }
-        float top = -INFINITY;
+        if (there != 0x01010101u)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) top = fmaxf(top, fmaxf(s[0][i], s[1][i]));
+            for (int b = 0; b < 2; ++b)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) s[b][i] = there >> (8 * (2 * b + i / 8)) & 1 ? s[b][i] : -INFINITY;
+    };
+    auto largest = [&](const floatx16 (&s)[2]) {
+        float t[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            t[k] = __builtin_elementwise_maximum(s[0][4 * k], s[1][4 * k]);
+#pragma unroll
+            for (int i = 1; i < 4; ++i) t[k] = max3(t[k], s[0][4 * k + i], s[1][4 * k + i]);
+        }
+        return max3(t[0], t[1], __builtin_elementwise_maximum(t[2], t[3]));
+    };
+    auto follow = [&](float top) { /* the maximum, where it has to */
         top = max_over32(top) * scale2;
         if (__ballot(top > m + 8.0f)) {
             top = fmaxf(m, top);
@@ -615,19 +642,50 @@ template <typename T, typename CT, int DC, int NW> __device__ __forceinline__ vo
 #pragma unroll
             for (int n = 0; n < ND; ++n) o[n] *= old;
         }
+    };
+    auto weights = [&](const floatx16 (&s)[2], int g, u32x4 (&pf)[TERMS]) { /* of 16 tokens */
+        float p[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) p[i] = __builtin_amdgcn_exp2f(fmaf(s[g / 2][8 * (g % 2) + i], scale2, -m));
+        attn_terms<TERMS>(p, pf);
+        l = attn_sum<TERMS>(l, p, pf[0]);
+    };
+
+#pragma unroll 1
+    for (u32 u = w.from, buf = 0; u < w.to; ++u, buf ^= 1) {
+        put_k(buf);
+        put_v(buf);
+        wait_vm_lgkm<0>(); /* this step's keys and values, of all wavefronts; no one reads the other halves any more */
+        barrier_mem();
+        if (u + 1 < w.to) {
+            begin_k(u + 1, buf ^ 1);
+            begin_v();
+#pragma unroll
+            for (int i = 0; i < NL; ++i) load_k(buf ^ 1, i), load_v(buf ^ 1, i);
+            lookup(u + 2);
+        }
+        floatx16 s[2];
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) s[b][i] = 0.0f;
+#pragma unroll
+        for (int c = 0; c < NC; ++c)
+#pragma unroll
+            for (int b = 0; b < 2; ++b) {
+                const u32x4 kf = key(buf, c, b);
+#pragma unroll
+                for (int k = TERMS - 1; k >= 0; --k) s[b] = attn_mfma32(kf, qf[c][k], s[b]);
+            }
+        hide(s, u, buf);
+        follow(largest(s));
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
-            float p[8];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) p[i] = __builtin_amdgcn_exp2f(fmaf(s[g / 2][8 * (g % 2) + i], scale2, -m));
-            l += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
             u32x4 pf[TERMS];
-            attn_terms<TERMS>(p, pf);
+            weights(s, g, pf);
 #pragma unroll
             for (int n = 0; n < ND; ++n) {
-                const u16 *q = (const u16 *)(vl + (vat ^ (n << 6)) + g * 16 * DH * 2);
-                const uint2 x = lds_column4(q), y = lds_column4(q + 8 * DH);
-                const u32x4 vf = { x.x, x.y, y.x, y.y };
+                const u32x4 vf = value(buf, g, n);
 #pragma unroll
                 for (int k = TERMS - 1; k >= 0; --k) o[n] = attn_mfma32(vf, pf[k], o[n]);
             }
@@ -635,7 +693,7 @@ template <typename T, typename CT, int DC, int NW> __device__ __forceinline__ vo
     }
 
     l = sum_over32(l);
-    if (w.pieces > 1) {
+    if (w.split) {
         float *part = attn_part(a, w.item, h);
         if (row < w.nr) {
             if (!hh) part[2 * row] = m, part[2 * row + 1] = l;
@@ -674,17 +732,14 @@ template <typename T, typename CT, int DC, int NW> __device__ __forceinline__ vo
     for (wrong = (wrong | wrong >> 32) & 0xffffffffu; wrong; wrong &= wrong - 1)
         attn_by_formula<T>(a, w.first, w.len, w.row, w.r0 + 32 * wave + (u32)__ffsll((unsigned long long)wrong) - 1, h);
 }
-#define ATTN_MANY_K(T, TN, CT, CN, DH, NW)                                                                                   \
-    extern "C" __global__ __launch_bounds__(NW * 64, 2) void attn_many_##TN##_##CN##_##DH##_##NW(const NkAttnKvArgs a) {     \
-        attn_many<T, CT, DH, NW>(a);                                                                                         \
+#define ATTN_MANY_K(T, TN, CT, CN, DC, OCC)                                                                          \
+    extern "C" __global__ __launch_bounds__(256, OCC) void attn_many_##TN##_##CN##_##DC(const NkAttnKvArgs a) {      \
+        attn_many<T, CT, DC>(a);                                                                                     \
     }
-#define ATTN_MANY_DH(DH, NW)                                                                                                 \
-    ATTN_MANY_K(u16, bf16, u16, bf16, DH, NW) ATTN_MANY_K(u16, bf16, unsigned char, e4m3, DH, NW)                            \
-    ATTN_MANY_K(float, f32, u16, bf16, DH, NW) ATTN_MANY_K(float, f32, unsigned char, e4m3, DH, NW)
-ATTN_MANY_DH(64, 4) ATTN_MANY_DH(96, 4) ATTN_MANY_DH(128, 4)
-#ifdef W8
-ATTN_MANY_DH(96, 8) ATTN_MANY_DH(128, 8)
-#endif
+#define ATTN_MANY_DC(DC, OCC)                                                                                        \
+    ATTN_MANY_K(u16, bf16, u16, bf16, DC, OCC) ATTN_MANY_K(u16, bf16, unsigned char, e4m3, DC, OCC)                  \
+    ATTN_MANY_K(float, f32, u16, bf16, DC, OCC) ATTN_MANY_K(float, f32, unsigned char, e4m3, DC, OCC)
+ATTN_MANY_DC(64, 2) ATTN_MANY_DC(96, 2) ATTN_MANY_DC(128, 2) ATTN_MANY_DC(192, 1) ATTN_MANY_DC(256, 1)
 
 /* The pieces of split sequences added up: a wavefront per packed row, or (share) four; a lane has
  * two neighbouring sums (and two more 128 on), eight pieces' in flight. */
@@ -711,6 +766,7 @@ template <typename T> __device__ __forceinline__ void attn_join(const NkAttnKvAr
     attn_work_t w;
     attn_tile(a, it.seq, it.local, w);
     const u32 pieces = (w.steps - 1) / piece + 1, item = before + it.local * attn_pieces(a, it.seq, piece);
+    if (pieces == 1) return;
     const u64 stride = (u64)a.kv.heads * a.tile * (dh + 2);
     const bool shared = a.share;
     const u32 begin = shared ? wave : 0, by = shared ? 4 : 1, d0 = min(2 * lane, dh - 2), d1 = min(128 + 2 * lane, dh - 2);
