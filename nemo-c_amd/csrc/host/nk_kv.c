@@ -133,8 +133,9 @@ int nk_attention_kv(gpu_t *g, const nk_kv_t *c, const nk_attend_t *p) {
     if (p->max_len > 1u << 30) return bad(g, "attention_kv: at most 2^30 tokens a sequence");
     const uint32_t group = p->heads / kv.heads;
     const uint32_t window = p->window >= p->max_len ? 0 : p->window, sinks = p->sinks < p->max_len ? p->sinks : p->max_len;
-    NkAttnKvArgs a = { kv, p->q, p->o, p->seqs, NULL, p->ldq, p->ldo, p->heads, group, window, sinks, p->nseq, p->max_rows, p->max_len, p->M,
-                       0, p->max_rows, 0, 0, 0, 0, 0, 0, p->scale };
+    NkAttnKvArgs a = { .kv = kv, .q = p->q, .o = p->o, .seqs = p->seqs, .ldq = p->ldq, .ldo = p->ldo, .heads = p->heads, .group = group,
+                       .window = window, .sinks = sinks, .nseq = p->nseq, .max_rows = p->max_rows, .max_len = p->max_len, .M = p->M,
+                       .upto = p->max_rows, .inv_group = 0xffffffffu / group, .scale = p->scale };
     a.vec = aligned(p->q, 16) && aligned(p->o, 4 * size) && p->ldq % (16 / size) == 0 && p->ldo % 4 == 0;
     const uint32_t rows = p->max_rows < p->M ? p->max_rows : p->M;
     uint32_t DH = kv.dh <= 64 ? 64 : kv.dh <= 128 ? 128 : 256;
@@ -142,21 +143,28 @@ int nk_attention_kv(gpu_t *g, const nk_kv_t *c, const nk_attend_t *p) {
     const int many = packed > 64;
     const uint32_t QT = packed > 16 && (DH < 256 || p->type == NK_BF16) ? 2 : 1;
     if (many) DH = kv.dh > 64 && kv.dh <= 96 ? 96 : kv.dh > 128 && kv.dh <= 192 ? 192 : DH;
-    a.tile = many ? 128 : 16 * QT;
-    a.step = many ? 64 : 32;
+    const uint32_t tile = many ? 128 : 16 * QT, step = many ? 64 : 32;
+    a.tile = many ? 7 : 3 + QT;
+    a.step = many ? 6 : 5;
     a.least = many && p->type == NK_F32 ? 4 : 8;
+    a.first = tile / group + 1;
+    if (window) {
+        const uint64_t reach = ((uint64_t)window + tile / group + 1 + step) / step + 1 + ((uint64_t)sinks + step - 1) / step;
+        a.reach = (uint32_t)reach;
+    }
     /* tiles that there can be, and the pieces that a tile can have */
-    const uint64_t each = ((uint64_t)rows * group + a.tile - 1) / a.tile, by_rows = (uint64_t)p->M * group / a.tile + p->nseq;
+    const uint64_t each = ((uint64_t)rows * group + tile - 1) / tile, by_rows = (uint64_t)p->M * group / tile + p->nseq;
     const uint64_t tiles = p->nseq * each < by_rows ? p->nseq * each : by_rows;
-    const uint64_t pieces = ((p->max_len + a.step - 1) / a.step + a.least - 1) / a.least;
+    const uint64_t pieces = ((p->max_len + step - 1) / step + a.least - 1) / a.least;
     if (tiles > 1u << 23) return bad(g, "attention_kv: more rows than a launch covers");
     uint64_t items = tiles;
     const uint32_t wanted = packed > 16 ? many && p->type == NK_F32 ? 512 : 256 : p->nseq > 1 ? 1024 : 512, slots = (wanted + kv.heads - 1) / kv.heads;
-    if (pieces > 1 && (uint64_t)p->M * group / a.tile < slots) {
+    if (pieces > 1 && (uint64_t)p->M * group / tile < slots) {
         a.slots = slots;
+        a.per_slot = 1.0f / (float)slots;
         const uint64_t split = tiles * pieces < 2ull * a.slots ? tiles * pieces : 2ull * a.slots;
         if (items < split) items = split;
-        a.ws = gpu_scratch_ws(g, (size_t)(split * kv.heads * a.tile * (kv.dh + 2)));
+        a.ws = gpu_scratch_ws(g, (size_t)(split * kv.heads * tile * (kv.dh + 2)));
         if (!a.ws) return bad(g, "attention_kv: scratch unavailable (size it before capture)");
     }
     const char *type = p->type == NK_F32 ? "f32" : "bf16";
@@ -168,7 +176,7 @@ int nk_attention_kv(gpu_t *g, const nk_kv_t *c, const nk_attend_t *p) {
     if (gpu_launch(g, name, &a, sizeof a, (uint32_t)items * kv.heads, 1, 1, 256, 1, 1)) return -1;
     if (!a.slots) return 0;
     snprintf(name, sizeof name, "attn_join_%s", type);
-    const uint64_t most = (uint64_t)rows * group < a.tile ? (uint64_t)rows * group : a.tile, some = tiles < a.slots ? tiles : a.slots;
+    const uint64_t most = (uint64_t)rows * group < tile ? (uint64_t)rows * group : tile, some = tiles < a.slots ? tiles : a.slots;
     /* a row to a workgroup, or its wavefronts a row each and going round: some 2048 workgroups */
     a.share = some * kv.heads * most <= 2048;
     uint64_t z = 2048 / (some * kv.heads);

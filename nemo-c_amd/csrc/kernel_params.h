@@ -585,8 +585,11 @@ typedef struct {
     float *ws;        /* split sequences: per piece, head of the cache and row m, l and dh sums */
     u32 ldq, ldo, heads, group, window, sinks, nseq, max_rows, max_len, M;
     u32 over, upto;   /* sequences of more than `over` and at most `upto` rows are this launch's */
-    u32 tile, step;   /* rows (of all heads of a group) of a workgroup; tokens of a step */
+    u32 inv_group;    /* (2^32 - 1) / group: quotients by a product and a correction */
+    u32 tile, step;   /* a workgroup's packed rows and a step's tokens, as powers of two */
+    u32 reach, first; /* the most steps of a tile's window and first tokens (0: no window); rows of the first tile */
     u32 slots, least; /* workgroups per head of the cache that are wanted; the fewest steps of a piece */
+    float per_slot;   /* 1 / slots */
     u32 share;        /* attn_join: four wavefronts to a row */
     u32 vec;          /* rows are read and written 16 (bf16: 8) bytes at a time */
     float scale;

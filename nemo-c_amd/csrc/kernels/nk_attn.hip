@@ -88,57 +88,61 @@ template <int TERMS> __device__ __forceinline__ float attn_sum(float l, const fl
 typedef struct {
     u32 first, rows, len, row;  /* the sequence */
     u32 r0, nr;                 /* the tile's packed rows */
+    u32 pos_lo, pos_hi;         /* positions of the first and the last */
     u32 lo_step, sink_steps, steps; /* its steps: sink_steps from 0 on, the others from lo_step on */
     u32 from, to;               /* the piece's */
     u32 split, item;            /* whether it has other pieces; this one's number over all */
 } attn_work_t;
 
+/* packed row -> row: at most one below, which the remainder shows */
+__device__ __forceinline__ u32 attn_row(const NkAttnKvArgs &a, u32 r) {
+    const u32 q = __umulhi(r, a.inv_group);
+    return q + (r - q * a.group >= a.group);
+}
 __device__ __forceinline__ u32 attn_tiles(const NkAttnKvArgs &a, const kvseq_t &s) {
-    return s.ok && s.rows > a.over && s.rows <= a.upto ? (s.rows * a.group - 1) / a.tile + 1 : 0;
+    return s.ok && s.rows > a.over && s.rows <= a.upto ? ((s.rows * a.group - 1) >> a.tile) + 1 : 0;
 }
 /* the most steps that a tile has whose last row is the sequence's row `rows` - 1 */
 __device__ __forceinline__ u32 attn_most_steps(const NkAttnKvArgs &a, const kvseq_t &s, u32 rows) {
-    const u32 all = (s.len + rows - 1) / a.step + 1;
-    if (!a.window) return all;
-    const u64 some = ((u64)a.window + (a.tile - 1) / a.group + 2 + a.step - 1) / a.step + 1 + ((u64)a.sinks + a.step - 1) / a.step;
-    return some < all ? (u32)some : all;
+    const u32 all = ((s.len + rows - 1) >> a.step) + 1;
+    return a.reach ? min(all, a.reach) : all;
 }
 __device__ __forceinline__ void attn_steps(const NkAttnKvArgs &a, attn_work_t &w) {
-    const u32 lowest = w.len + w.r0 / a.group, last = w.len + (w.r0 + w.nr - 1) / a.group;
+    const u32 lowest = w.len + attn_row(a, w.r0), last = w.len + attn_row(a, w.r0 + w.nr - 1);
     const u32 lo = a.window && lowest >= a.window ? lowest + 1 - a.window : 0;
-    w.lo_step = lo / a.step;
-    w.sink_steps = a.window ? min((u32)(((u64)a.sinks + a.step - 1) / a.step), w.lo_step) : 0;
-    w.steps = w.sink_steps + last / a.step - w.lo_step + 1;
+    w.pos_lo = lowest;
+    w.pos_hi = last;
+    w.lo_step = lo >> a.step;
+    w.sink_steps = a.window ? min((u32)(((u64)a.sinks + (1u << a.step) - 1) >> a.step), w.lo_step) : 0;
+    w.steps = w.sink_steps + (last >> a.step) - w.lo_step + 1;
 }
 __device__ __forceinline__ kvseq_t attn_seq(const NkAttnKvArgs &a, u32 i) {
     return kvseq_load(a.seqs, i, a.M, a.max_rows, a.kv.tables, min(kv_room(a.kv), (u64)a.max_len));
 }
 /* the sequence of this lane, of the first 64 */
 __device__ __forceinline__ kvseq_t attn_mine(const NkAttnKvArgs &a) { return attn_seq(a, min(threadIdx.x & 63, a.nseq - 1)); }
-/* steps of a piece; 0: nothing is split */
+/* steps of a piece; 0: nothing is split.  All wavefronts of all workgroups come to the same. */
 __device__ __forceinline__ u32 attn_piece(const NkAttnKvArgs &a, kvseq_t s) {
     const u32 lane = threadIdx.x & 63;
     if (!a.slots) return 0;
-    u64 tiles = 0, steps = 0;
+    u32 tiles = 0;
+    float steps = 0.0f;
     for (u32 i = lane; i < a.nseq; i += 64) {
         if (i != lane) s = attn_seq(a, i);
         const u32 n = attn_tiles(a, s);
         tiles += n;
-        if (n) steps += (u64)n * (attn_most_steps(a, s, s.rows) + attn_most_steps(a, s, min(s.rows, a.tile / a.group + 1))) / 2;
+        if (n) steps += 0.5f * (float)n * (float)(attn_most_steps(a, s, s.rows) + attn_most_steps(a, s, min(s.rows, a.first)));
     }
-    auto total = [](u64 v) { return ((u64)lane_of(wave_scan((u32)(v >> 24)), 63) << 24) + lane_of(wave_scan((u32)v & 0xffffffu), 63); };
-    tiles = total(tiles);
-    if (tiles >= a.slots) return 0;
-    steps = total(steps);
-    return max((u32)((steps + a.slots - 1) / a.slots), a.least);
+    if (lane_of(wave_scan(tiles), 63) >= a.slots) return 0;
+    return max((u32)(wsum(steps) * a.per_slot) + 1, a.least);
 }
 __device__ __forceinline__ u32 attn_pieces(const NkAttnKvArgs &a, const kvseq_t &s, u32 piece) {
     return piece ? (attn_most_steps(a, s, s.rows) - 1) / piece + 1 : 1;
 }
 __device__ __forceinline__ void attn_tile(const NkAttnKvArgs &a, const kvseq_t &s, u32 tile, attn_work_t &w) {
     w.first = s.first, w.rows = s.rows, w.len = s.len, w.row = s.row;
-    w.r0 = (attn_tiles(a, s) - 1 - tile) * a.tile; /* the last rows, which see most, first */
-    w.nr = min(a.tile, s.rows * a.group - w.r0);
+    w.r0 = (attn_tiles(a, s) - 1 - tile) << a.tile; /* the last rows, which see most, first */
+    w.nr = min(1u << a.tile, s.rows * a.group - w.r0);
     attn_steps(a, w);
 }
 __device__ __forceinline__ void attn_uniform(attn_work_t &w) {
@@ -165,7 +169,7 @@ __device__ __forceinline__ bool attn_find(const NkAttnKvArgs &a, u32 id, attn_wo
 }
 /* a piece's place in the scratch: m and l of its rows, then their sums */
 __device__ __forceinline__ float *attn_part(const NkAttnKvArgs &a, u32 item, u32 h) {
-    return a.ws + ((u64)item * a.kv.heads + h) * a.tile * (a.kv.dh + 2);
+    return a.ws + (((u64)item * a.kv.heads + h) << a.tile) * (a.kv.dh + 2);
 }
 
 /* the page of a token, the same for all lanes (nothing writes the table meanwhile) */
@@ -241,15 +245,15 @@ template <typename T, typename CT, int DH, int QT, int NW> __device__ __forceinl
     attn_work_t w;
     if (!attn_find(a, blockIdx.x / kv.heads, w) || w.from >= w.to) return;
     if (threadIdx.x < ROWS) wrong[threadIdx.x] = 0;
-    const u32 pos_lo = w.len + w.r0 / a.group, pos_hi = w.len + (w.r0 + w.nr - 1) / a.group;
+    const u32 pos_lo = w.pos_lo, pos_hi = w.pos_hi;
 
     u32x4 qf[QT][NC][TERMS];
     u32 pos[QT];
 #pragma unroll
     for (int t = 0; t < QT; ++t) {
-        const u32 r = w.r0 + min(16 * t + c16, w.nr - 1), i = r / a.group;
+        const u32 r = w.r0 + min(16 * t + c16, w.nr - 1), i = attn_row(a, r);
         pos[t] = w.len + i;
-        const T *q = (const T *)a.q + (u64)(w.first + i) * a.ldq + (u64)(h * a.group + r % a.group) * dh;
+        const T *q = (const T *)a.q + (u64)(w.first + i) * a.ldq + (u64)(h * a.group + r - i * a.group) * dh;
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
             const u32 d = 64 * (c / 2) + 16 * g4 + 8 * (c % 2);
@@ -425,13 +429,13 @@ const bool see = th[b] & ((pos[t] - j < reach) | ((j < a.sinks) & (j <= pos[t]) 
             }
             if (part) {
                 if (!d) part[2 * rt] = top, part[2 * rt + 1] = sum;
-                *(floatx2 *)(part + 2 * a.tile + (u64)rt * dh + d) = v.xy;
-                *(floatx2 *)(part + 2 * a.tile + (u64)rt * dh + d + 2) = v.zw;
+                *(floatx2 *)(part + (2u << a.tile) + (u64)rt * dh + d) = v.xy;
+                *(floatx2 *)(part + (2u << a.tile) + (u64)rt * dh + d + 2) = v.zw;
                 continue;
             }
             v /= sum;
-            const u32 pr = w.r0 + rt;
-            T *out = (T *)a.o + (u64)(w.first + pr / a.group) * a.ldo + (u64)(h * a.group + pr % a.group) * dh + d;
+            const u32 pr = w.r0 + rt, pi = attn_row(a, pr);
+            T *out = (T *)a.o + (u64)(w.first + pi) * a.ldo + (u64)(h * a.group + pr - pi * a.group) * dh + d;
             if (!(fabsf(v.x) < INFINITY && fabsf(v.y) < INFINITY && fabsf(v.z) < INFINITY && fabsf(v.w) < INFINITY)) wrong[rt] = 1;
             const float e[4] = { v.x, v.y, v.z, v.w };
             if (a.vec) kv_store<4>(out, e);
@@ -497,9 +501,9 @@ template <typename T, typename CT, int DC> __device__ __forceinline__ void attn_
     const u32 wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
     attn_work_t w;
     if (!attn_find(a, blockIdx.x / kv.heads, w) || w.from >= w.to) return;
-    const u32 pos_lo = w.len + w.r0 / a.group, pos_hi = w.len + (w.r0 + w.nr - 1) / a.group;
-    const u32 row = 32 * wave + c32, pr = w.r0 + min(row, w.nr - 1), pos = w.len + pr / a.group;
-    const u64 at_head = (u64)(h * a.group + pr % a.group) * dh;
+    const u32 pos_lo = w.pos_lo, pos_hi = w.pos_hi;
+    const u32 row = 32 * wave + c32, pr = w.r0 + min(row, w.nr - 1), pi = attn_row(a, pr), pos = w.len + pi;
+    const u64 at_head = (u64)(h * a.group + pr - pi * a.group) * dh;
 
     auto token = [&](u32 u) { return (u < w.sink_steps ? u : w.lo_step + u - w.sink_steps) * ATTN_MANY; };
     auto mixk = [](u32 t) { return DH == 64 ? (t >> 1) & 7 : t & 15; };
@@ -562,7 +566,7 @@ template <typename T, typename CT, int DC> __device__ __forceinline__ void attn_
 
     u32x4 qf[NC][TERMS];
     {
-        const T *q = (const T *)a.q + (u64)(w.first + pr / a.group) * a.ldq + at_head;
+        const T *q = (const T *)a.q + (u64)(w.first + pi) * a.ldq + at_head;
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
             const u32 d = 16 * c + 8 * hh;
@@ -702,14 +706,14 @@ template <typename T, typename CT, int DC> __device__ __forceinline__ void attn_
 #pragma unroll
                 for (int i = 0; i < 16; i += 4) {
                     const u32 d = 32 * n + 2 * i + 4 * hh;
-                    if (d < dh) *(floatx4 *)(part + 2 * a.tile + (u64)row * dh + d) = (floatx4){ o[n][i], o[n][i + 1], o[n][i + 2], o[n][i + 3] };
+                    if (d < dh) *(floatx4 *)(part + (2u << a.tile) + (u64)row * dh + d) = (floatx4){ o[n][i], o[n][i + 1], o[n][i + 2], o[n][i + 3] };
                 }
         }
         return;
     }
     bool bad = false;
     if (row < w.nr) {
-        T *out = (T *)a.o + (u64)(w.first + pr / a.group) * a.ldo + at_head;
+        T *out = (T *)a.o + (u64)(w.first + pi) * a.ldo + at_head;
 #pragma unroll
         for (int n = 0; n < ND; ++n)
 #pragma unroll
@@ -767,11 +771,11 @@ template <typename T> __device__ __forceinline__ void attn_join(const NkAttnKvAr
     attn_tile(a, it.seq, it.local, w);
     const u32 pieces = (w.steps - 1) / piece + 1, item = before + it.local * attn_pieces(a, it.seq, piece);
     if (pieces == 1) return;
-    const u64 stride = (u64)a.kv.heads * a.tile * (dh + 2);
+    const u64 stride = ((u64)a.kv.heads << a.tile) * (dh + 2);
     const bool shared = a.share;
     const u32 begin = shared ? wave : 0, by = shared ? 4 : 1, d0 = min(2 * lane, dh - 2), d1 = min(128 + 2 * lane, dh - 2);
     for (u32 r = shared ? blockIdx.z : blockIdx.z * 4 + wave; r < w.nr; r += gridDim.z * (shared ? 1 : 4)) {
-        const float *part = attn_part(a, item, h), *rows = part + 2 * a.tile + (u64)r * dh;
+        const float *part = attn_part(a, item, h), *rows = part + (2u << a.tile) + (u64)r * dh;
         float top = -1e30f;
         for (u32 k = lane; k < pieces; k += 64) top = fmaxf(top, part[k * stride + 2 * r]);
         top = wmax(top);
@@ -815,8 +819,8 @@ template <typename T> __device__ __forceinline__ void attn_join(const NkAttnKvAr
                 sum += total[k];
             }
         }
-        const u32 pr = w.r0 + r;
-        T *out = (T *)a.o + (u64)(w.first + pr / a.group) * a.ldo + (u64)(h * a.group + pr % a.group) * dh;
+        const u32 pr = w.r0 + r, pi = attn_row(a, pr);
+        T *out = (T *)a.o + (u64)(w.first + pi) * a.ldo + (u64)(h * a.group + pr - pi * a.group) * dh;
         const float e[4] = { v.x / sum, v.y / sum, v1.x / sum, v1.y / sum };
         bool bad = false;
 #pragma unroll
