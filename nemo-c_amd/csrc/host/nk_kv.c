@@ -146,7 +146,7 @@ int nk_attention_kv(gpu_t *g, const nk_kv_t *c, const nk_attend_t *p) {
     const uint32_t tile = many ? 128 : 16 * QT, step = many ? 64 : 32;
     a.tile = many ? 7 : 3 + QT;
     a.step = many ? 6 : 5;
-    a.least = many && p->type == NK_F32 ? 4 : 8;
+    a.least = packed <= 16 || (many && p->type == NK_F32) ? 4 : 8;
     a.first = tile / group + 1;
     if (window) {
         const uint64_t reach = ((uint64_t)window + tile / group + 1 + step) / step + 1 + ((uint64_t)sinks + step - 1) / step;
@@ -158,10 +158,11 @@ int nk_attention_kv(gpu_t *g, const nk_kv_t *c, const nk_attend_t *p) {
     const uint64_t pieces = ((p->max_len + step - 1) / step + a.least - 1) / a.least;
     if (tiles > 1u << 23) return bad(g, "attention_kv: more rows than a launch covers");
     uint64_t items = tiles;
-    const uint32_t wanted = packed > 16 ? many && p->type == NK_F32 ? 512 : 256 : p->nseq > 1 ? 1024 : 512, slots = (wanted + kv.heads - 1) / kv.heads;
+    const uint32_t wanted = packed > 16 ? many && p->type == NK_F32 ? 512 : 256 : p->nseq > 1 ? 1536 : 512, slots = (wanted + kv.heads - 1) / kv.heads;
     if (pieces > 1 && (uint64_t)p->M * group / tile < slots) {
         a.slots = slots;
         a.per_slot = 1.0f / (float)slots;
+        a.per_cu = (float)kv.heads / (wanted == 512 && many ? 512.0f : 256.0f);
         const uint64_t split = tiles * pieces < 2ull * a.slots ? tiles * pieces : 2ull * a.slots;
         if (items < split) items = split;
         a.ws = gpu_scratch_ws(g, (size_t)(split * kv.heads * tile * (kv.dh + 2)));

@@ -589,7 +589,7 @@ typedef struct {
     u32 tile, step;   /* a workgroup's packed rows and a step's tokens, as powers of two */
     u32 reach, first; /* the most steps of a tile's window and first tokens (0: no window); rows of the first tile */
     u32 slots, least; /* workgroups per head of the cache that are wanted; the fewest steps of a piece */
-    float per_slot;   /* 1 / slots */
+    float per_slot, per_cu; /* 1 / slots; heads of the cache / 256 */
     u32 share;        /* attn_join: four wavefronts to a row */
     u32 vec;          /* rows are read and written 16 (bf16: 8) bytes at a time */
     float scale;

@@ -134,10 +134,17 @@ __device__ __forceinline__ u32 attn_piece(const NkAttnKvArgs &a, kvseq_t s) {
         if (n) steps += 0.5f * (float)n * (float)(attn_most_steps(a, s, s.rows) + attn_most_steps(a, s, min(s.rows, a.first)));
     }
     if (lane_of(wave_scan(tiles), 63) >= a.slots) return 0;
-    return max((u32)(wsum(steps) * a.per_slot) + 1, a.least);
+    /* as many as a workgroup per CU has, or, where those are many, shorter ones that even out */
+    steps = wsum(steps);
+    const float some = steps * a.per_cu;
+    return some < 24.0f ? max((u32)some + 1, a.least) : max((u32)(steps * a.per_slot) + 1, a.least);
 }
 __device__ __forceinline__ u32 attn_pieces(const NkAttnKvArgs &a, const kvseq_t &s, u32 piece) {
-    return piece ? (attn_most_steps(a, s, s.rows) - 1) / piece + 1 : 1;
+    return piece ? max((attn_most_steps(a, s, s.rows) + piece / 2) / piece, 1u) : 1;
+}
+/* a sequence's are all alike */
+__device__ __forceinline__ u32 attn_piece_of(const NkAttnKvArgs &a, const kvseq_t &s, u32 pieces) {
+    return (attn_most_steps(a, s, s.rows) - 1) / pieces + 1;
 }
 __device__ __forceinline__ void attn_tile(const NkAttnKvArgs &a, const kvseq_t &s, u32 tile, attn_work_t &w) {
     w.first = s.first, w.rows = s.rows, w.len = s.len, w.row = s.row;
@@ -161,8 +168,9 @@ __device__ __forceinline__ bool attn_find(const NkAttnKvArgs &a, u32 id, attn_wo
     const u32 pieces = attn_pieces(a, it.seq, piece);
     w.item = id;
     attn_tile(a, it.seq, it.local / pieces, w);
-    w.from = it.local % pieces * piece;
-    w.to = piece ? min(w.steps, w.from + piece) : w.steps;
+    const u32 len = pieces > 1 ? attn_piece_of(a, it.seq, pieces) : w.steps;
+    w.from = it.local % pieces * len;
+    w.to = min(w.steps, w.from + len);
     w.split = w.steps > w.to - w.from;
     attn_uniform(w); /* or the compiler keeps all that follows from it per lane */
     return true;
@@ -769,7 +777,7 @@ template <typename T> __device__ __forceinline__ void attn_join(const NkAttnKvAr
     before = lane_of(wave_scan(before), 63);
     attn_work_t w;
     attn_tile(a, it.seq, it.local, w);
-    const u32 pieces = (w.steps - 1) / piece + 1, item = before + it.local * attn_pieces(a, it.seq, piece);
+    const u32 all = attn_pieces(a, it.seq, piece), pieces = (w.steps - 1) / attn_piece_of(a, it.seq, all) + 1, item = before + it.local * all;
     if (pieces == 1) return;
     const u64 stride = ((u64)a.kv.heads << a.tile) * (dh + 2);
     const bool shared = a.share;
