@@ -79,16 +79,15 @@ int nk_kv_append(gpu_t *g, const nk_kv_t *c, const nk_append_t *p) {
         if (half % P == 0 && tail % (2 * P) == 0 && rows) break;
     }
     const uint64_t blocks = blocks_of(p->nseq, p->max_rows, p->M);
-    const uint32_t units = (p->q ? p->heads : 0) + (p->k ? 2 * kv.heads : 0);
     if (blocks > 1u << 23) return bad(g, "kv_append: more rows than a launch covers");
-    uint32_t gy = (units + 3) / 4;
-    while (gy > 1 && blocks * gy > 4096) gy = (gy + 1) / 2;
+    uint32_t gq = p->q ? (p->heads + 3) / 4 : 0, gk = p->k ? (2 * kv.heads + 3) / 4 : 0;
+    while (gq + gk > 2 && blocks * (gq + gk) > 4096) gq = (gq + 1) / 2, gk = (gk + 1) / 2;
     NkAppendArgs a = { kv, p->q, p->k, p->v, p->qo, p->freq, p->seqs, p->ldq, p->ldk, p->ldv, p->ldqo, p->heads, p->rot, p->inter != 0,
-                       p->nseq, p->max_rows, p->M, p->amp };
+                       p->nseq, p->max_rows, p->M, gq, p->amp };
     char name[32];
     snprintf(name, sizeof name, "kv_append_%sx%u_%s", p->type == NK_F32 ? "f32" : "bf16", P, cache_name(&kv));
     gpu_next_bytes(g, (double)p->M * ((p->q ? 2.0 * size * nq : 0.0) + (p->k ? 2.0 * nk * (size + (kv.ks ? 1 : 2)) : 0.0)));
-    return gpu_launch(g, name, &a, sizeof a, (uint32_t)blocks, gy, 1, 256, 1, 1);
+    return gpu_launch(g, name, &a, sizeof a, (uint32_t)blocks, gq + gk, 1, 256, 1, 1);
 }
 
 int nk_kv_read(gpu_t *g, const nk_kv_t *c, void *K, uint32_t ldk, void *V, uint32_t ldv, int type, const int *seqs, uint32_t nseq,
@@ -158,6 +157,7 @@ int nk_attention_kv(gpu_t *g, const nk_kv_t *c, const nk_attend_t *p) {
     const uint64_t pieces = ((p->max_len + step - 1) / step + a.least - 1) / a.least;
     if (tiles > 1u << 23) return bad(g, "attention_kv: more rows than a launch covers");
     uint64_t items = tiles;
+    a.pair = many && tiles * kv.heads > 256 && tiles * kv.heads <= 512;
     const uint32_t wanted = packed > 16 ? many && p->type == NK_F32 ? 512 : 256 : p->nseq > 1 ? 1536 : 512, slots = (wanted + kv.heads - 1) / kv.heads;
     if (pieces > 1 && (uint64_t)p->M * group / tile < slots) {
         a.slots = slots;

@@ -567,6 +567,7 @@ typedef struct {
     const float *freq;     /* radians per position of the rot / 2 pairs */
     const int *seqs;
     u32 ldq, ldk, ldv, ldqo, heads, rot, inter, nseq, max_rows, M;
+    u32 qgroups; /* workgroups in y that take queries, the others keys and values */
     float amp;
 } NkAppendArgs;
 
@@ -590,6 +591,7 @@ typedef struct {
     u32 reach, first; /* the most steps of a tile's window and first tokens (0: no window); rows of the first tile */
     u32 slots, least; /* workgroups per head of the cache that are wanted; the fewest steps of a piece */
     float per_slot, per_cu; /* 1 / slots; heads of the cache / 256 */
+    u32 pair;         /* the second half of a sequence's tiles least first */
     u32 share;        /* attn_join: four wavefronts to a row */
     u32 vec;          /* rows are read and written 16 (bf16: 8) bytes at a time */
     float scale;

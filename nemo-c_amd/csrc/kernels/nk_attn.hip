@@ -147,8 +147,11 @@ __device__ __forceinline__ u32 attn_piece_of(const NkAttnKvArgs &a, const kvseq_
     return (attn_most_steps(a, s, s.rows) - 1) / pieces + 1;
 }
 __device__ __forceinline__ void attn_tile(const NkAttnKvArgs &a, const kvseq_t &s, u32 tile, attn_work_t &w) {
+    const u32 n = attn_tiles(a, s), half = (n + 1) / 2;
     w.first = s.first, w.rows = s.rows, w.len = s.len, w.row = s.row;
-    w.r0 = (attn_tiles(a, s) - 1 - tile) << a.tile; /* the last rows, which see most, first */
+    /* the last rows, which see most, first; where two workgroups share a CU from the start (pair), the first half of them
+     * and then the least */
+    w.r0 = (a.pair && tile >= half ? tile - half : n - 1 - tile) << a.tile;
     w.nr = min(1u << a.tile, s.rows * a.group - w.r0);
     attn_steps(a, w);
 }

@@ -144,14 +144,18 @@ __device__ __forceinline__ float to_odd(double d) {
 #define KV_PAIRS 128 /* dh / 2 at most */
 
 /* A workgroup takes the rows of a sequence that fall into one block of 16 tokens; its wavefronts take heads, one at a
- * time: of the queries, the keys and the values.  The block's cosines and sines are computed once for all of them.
+ * time: of the queries, or (behind a.qgroups in y) of the keys and the values.  The block's cosines and sines are computed
+ * once for all of them.
  * Values go in pairs of P at a time: pair (i, i + rot / 2), or interleaved (2 i, 2 i + 1), and as they are behind the
  * rotated part.  8 bits: the block's scale is the least power of two of which 448 times reach the largest new value
  * and at least that of the tokens that the block has; where it grows, their codes are rounded again (exactly, but for
  * those that become subnormal). */
 template <typename T, int P, bool E4M3> __device__ __forceinline__ void kv_append(const NkAppendArgs &a) {
-    __shared__ float2 turn[NK_KV_BLOCK][KV_PAIRS];
-    __shared__ double2 turn64[E4M3 ? NK_KV_BLOCK : 1][E4M3 ? KV_PAIRS : 1]; /* of the keys */
+    __shared__ union {
+        float2 f[NK_KV_BLOCK][KV_PAIRS];
+        double2 d[E4M3 ? NK_KV_BLOCK : 1][E4M3 ? KV_PAIRS : 1];
+    } turn;
+    const bool queries = blockIdx.y < a.qgroups, wide = E4M3 && !queries;
     const NkKv &kv = a.kv;
     const u64 room = kv_room(kv);
     auto load = [&](u32 i) { return kvseq_load(a.seqs, i, a.M, a.max_rows, kv.tables, room); };
@@ -162,22 +166,19 @@ template <typename T, int P, bool E4M3> __device__ __forceinline__ void kv_appen
     const u32 lo = max(s.len, t0) - t0, hi = min(s.len + s.rows - t0, (u32)NK_KV_BLOCK), half = a.rot / 2;
     for (u32 i = threadIdx.x; i < (hi - lo) * half; i += 256) {
         const u32 t = lo + i / half, j = i % half;
-        if constexpr (E4M3) {
-            const double2 c = kv_turn64(t0 + t, a.freq[j], a.amp);
-            turn64[t][j] = c;
-            turn[t][j] = make_float2((float)c.x, (float)c.y);
-        } else turn[t][j] = kv_turn(t0 + t, a.freq[j], a.amp);
+        if constexpr (E4M3)
+            if (wide) turn.d[t][j] = kv_turn64(t0 + t, a.freq[j], a.amp);
+        if (!wide) turn.f[t][j] = kv_turn(t0 + t, a.freq[j], a.amp);
     }
     __syncthreads();
     const int pe = kv.table[(u64)s.row * kv.ldt + (t0 >> kv.shift)];
     const bool there = (u32)pe < kv.pages;
     const u32 lane = threadIdx.x & 63, U = kv.dh / (2 * P), rp = half / P;
     const u32 tpp = U <= 64 ? 64 / U : 1, tk0 = U <= 64 ? lane / U : 0, u0 = U > 64 ? lane : tk0 < tpp ? lane % U : U;
-    const u32 nq = a.q ? a.heads : 0, units = nq + (a.k ? 2 * kv.heads : 0);
-    for (u32 w = blockIdx.y * 4 + threadIdx.x / 64; w < units; w += gridDim.y * 4) {
-        const bool isq = w < nq, isv = !isq && w - nq >= kv.heads;
-        const u32 h = isq ? w : isv ? w - nq - kv.heads : w - nq, ld = isq ? a.ldq : isv ? a.ldv : a.ldk;
-        if (!isq && !there) continue;
+    const u32 groups = queries ? a.qgroups : gridDim.y - a.qgroups, units = queries ? a.heads : there ? 2 * kv.heads : 0;
+    for (u32 w = (queries ? blockIdx.y : blockIdx.y - a.qgroups) * 4 + threadIdx.x / 64; w < units; w += groups * 4) {
+        const bool isq = queries, isv = !isq && w >= kv.heads;
+        const u32 h = isv ? w - kv.heads : w, ld = isq ? a.ldq : isv ? a.ldv : a.ldk;
         const u64 row0 = (u64)s.first + t0 - s.len; /* of token t0, which may lie before the first row */
         const T *src = (const T *)(isq ? a.q : isv ? a.v : a.k) + (u64)h * kv.dh;
         auto places = [&](u32 u, u32 &oa, u32 &ob, u32 &j) {
@@ -186,23 +187,18 @@ template <typename T, int P, bool E4M3> __device__ __forceinline__ void kv_appen
             oa = split ? j : 2 * P * u;
             ob = split ? j + half : oa + P;
         };
-        auto get = [&](u32 t, u32 u, float (&x)[P], float (&y)[P]) {
-            u32 oa, ob, j;
-            places(u, oa, ob, j);
-            const T *r = src + (row0 + t) * ld;
-            kv_load<P>(x, r + oa);
-            kv_load<P>(y, r + ob);
+        auto turned = [&](u32 t, u32 j, float (&x)[P], float (&y)[P]) {
             if (j >= half) return;
             auto pair = [&](int i, float &p, float &q) {
                 if constexpr (E4M3)
                     if (!isq) {
-                        const double2 c = turn64[t][j + i];
+                        const double2 c = turn.d[t][j + i];
                         const double v = fma((double)p, c.x, -((double)q * c.y));
                         q = to_odd(fma((double)q, c.x, (double)p * c.y));
                         p = to_odd(v);
                         return;
                     }
-                const float2 c = turn[t][j + i];
+                const float2 c = turn.f[t][j + i];
                 const float v = fmaf(p, c.x, -(q * c.y));
                 q = fmaf(q, c.x, p * c.y);
                 p = v;
@@ -217,44 +213,71 @@ template <typename T, int P, bool E4M3> __device__ __forceinline__ void kv_appen
 #pragma unroll
                 for (int i = 0; i < P; ++i) pair(i, x[i], y[i]);
         };
-        auto each = [&](auto f) {
-            for (u32 t = lo + tk0; t < hi; t += tpp)
-                for (u32 u = u0; u < U; u += 64) {
-                    float x[P], y[P];
-                    u32 oa, ob, j;
-                    get(t, u, x, y);
-                    places(u, oa, ob, j);
-                    f(t, oa, ob, x, y);
-                }
+        /* two rounds of the lanes at a time, their loads in flight together */
+        constexpr int NB = 2;
+        const u32 wraps = U <= 64 ? 1 : (U - 1) / 64 + 1, rounds = U <= 64 ? (hi - lo - 1) / tpp + 1 : (hi - lo) * wraps;
+        float x[NB][P], y[NB][P];
+        u32 tt[NB], oa[NB], ob[NB];
+        bool in[NB];
+        auto load = [&](u32 r0) {
+            u32 j[NB];
+#pragma unroll
+            for (int i = 0; i < NB; ++i) {
+                const u32 r = r0 + i, t = U <= 64 ? lo + tk0 + r * tpp : lo + r / wraps, u = U <= 64 ? u0 : u0 + 64 * (r % wraps);
+                in[i] = t < hi && u < U;
+                tt[i] = min(t, hi - 1);
+                places(min(u, U - 1), oa[i], ob[i], j[i]);
+                if (i && r >= rounds) continue; /* the same for all lanes */
+                const T *row = src + (row0 + tt[i]) * ld;
+                kv_load<P>(x[i], row + oa[i]);
+                kv_load<P>(y[i], row + ob[i]);
+            }
+#pragma unroll
+            for (int i = 0; i < NB; ++i)
+                if (!i || r0 + i < rounds) turned(tt[i], j[i], x[i], y[i]);
+        };
+        auto each = [&](u32 r0, auto f) {
+#pragma unroll
+            for (int i = 0; i < NB; ++i)
+                if (in[i] && (!i || r0 + i < rounds)) f(tt[i], oa[i], ob[i], x[i], y[i]);
         };
         if (isq) {
             T *dst = (T *)a.qo + (u64)h * kv.dh;
-            each([&](u32 t, u32 oa, u32 ob, const float(&x)[P], const float(&y)[P]) {
-                T *r = dst + (row0 + t) * a.ldqo;
-                kv_store<P>(r + oa, x);
-                kv_store<P>(r + ob, y);
-            });
+            for (u32 r0 = 0; r0 < rounds; r0 += NB) {
+                load(r0);
+                each(r0, [&](u32 t, u32 ia, u32 ib, const float(&p)[P], const float(&q)[P]) {
+                    T *r = dst + (row0 + t) * a.ldqo;
+                    kv_store<P>(r + ia, p);
+                    kv_store<P>(r + ib, q);
+                });
+            }
             continue;
         }
         const u64 slot = (((u64)(u32)pe * kv.heads + h) << kv.shift) + (t0 & ((1u << kv.shift) - 1)); /* of the block's first token */
         if constexpr (!E4M3) {
             u16 *dst = (u16 *)(isv ? kv.v : kv.k) + slot * kv.dh;
-            each([&](u32 t, u32 oa, u32 ob, const float(&x)[P], const float(&y)[P]) {
-                kv_store<P>(dst + t * kv.dh + oa, x);
-                kv_store<P>(dst + t * kv.dh + ob, y);
-            });
+            for (u32 r0 = 0; r0 < rounds; r0 += NB) {
+                load(r0);
+                each(r0, [&](u32 t, u32 ia, u32 ib, const float(&p)[P], const float(&q)[P]) {
+                    kv_store<P>(dst + t * kv.dh + ia, p);
+                    kv_store<P>(dst + t * kv.dh + ib, q);
+                });
+            }
         } else {
-            float top = 0.0f;
-            each([&](u32 t, u32 oa, u32 ob, const float(&x)[P], const float(&y)[P]) {
-#pragma unroll
-                for (int i = 0; i < P; ++i) {
-                    top = fmaxf(top, __builtin_isinf(x[i]) ? 0.0f : fabsf(x[i]));
-                    top = fmaxf(top, __builtin_isinf(y[i]) ? 0.0f : fabsf(y[i]));
-                }
-            });
-            const u32 bits = __float_as_uint(wmax(top)), e = bits >> 23;
             unsigned char *sb = (isv ? kv.vs : kv.ks) + slot / NK_KV_BLOCK, *dst = (unsigned char *)(isv ? kv.v : kv.k) + slot * kv.dh;
             const u32 was = lo ? min((u32)*sb, 247u) : 0;
+            float top = 0.0f;
+            for (u32 r0 = 0; r0 < rounds; r0 += NB) {
+                load(r0);
+                each(r0, [&](u32 t, u32 ia, u32 ib, const float(&p)[P], const float(&q)[P]) {
+#pragma unroll
+                    for (int i = 0; i < P; ++i) {
+                        top = fmaxf(top, __builtin_isinf(p[i]) ? 0.0f : fabsf(p[i]));
+                        top = fmaxf(top, __builtin_isinf(q[i]) ? 0.0f : fabsf(q[i]));
+                    }
+                });
+            }
+            const u32 bits = __float_as_uint(wmax(top)), e = bits >> 23;
             const u32 now = max(max(e < 18 ? 10u : e - 8 + ((bits & 0x7fffffu) > 0x600000u), was), 10u);
             if (lo && now > was) {
                 const float f = scale8(max((int)(was + 127 - now), 1)); /* below 2^-18 every code becomes 0 */
@@ -265,10 +288,13 @@ template <typename T, int P, bool E4M3> __device__ __forceinline__ void kv_appen
             }
             if (now != was || !lo) *sb = (unsigned char)now;
             const float r = scale8(254 - now);
-            each([&](u32 t, u32 oa, u32 ob, const float(&x)[P], const float(&y)[P]) {
-                kv_store8<P>(dst + t * kv.dh + oa, x, r);
-                kv_store8<P>(dst + t * kv.dh + ob, y, r);
-            });
+            for (u32 r0 = 0; r0 < rounds; r0 += NB) {
+                if (rounds > NB) load(r0); /* or they are still there */
+                each(r0, [&](u32 t, u32 ia, u32 ib, const float(&p)[P], const float(&q)[P]) {
+                    kv_store8<P>(dst + t * kv.dh + ia, p, r);
+                    kv_store8<P>(dst + t * kv.dh + ib, q, r);
+                });
+            }
         }
     }
 }
