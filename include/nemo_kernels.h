@@ -381,7 +381,7 @@ int nk_ssm_scan(gpu_t *g, const nk_scan_t *a);
  * seqs (device, 16-byte aligned) has four ints per sequence: { first row, rows, tokens before them, row of the table }.  Row i
  * of it stands at position "tokens before them" + i.  No row is in two sequences; a sequence of no rows has nothing
  * done; its rows are below M and at most max_rows, its tokens within its table row, which is one of `tables` rows of ldt
- * entries: a sequence that breaks these is left out.  Rows that no sequence has are not written.  At most 65535 sequences.
+ * entries: a sequence that breaks these is left out.  Rows that no sequence has are not written.  At most 4096 sequences.
  * max_rows may be far above the longest, as in a captured graph that is replayed with other tables.
  *
  * The same table serves an append and the attention of the rows that were appended.  Sequences may share pages that

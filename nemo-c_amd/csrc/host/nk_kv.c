@@ -28,6 +28,7 @@ int nk_rope_freqs(float *freq, uint32_t rot, double base, int scaling, double fa
     return 0;
 }
 
+#define NK_KV_SEQS 4096 /* every wavefront finds its work in the table: 16 steps of it at the most */
 /* what all ask of the cache and the batch */
 static const char *cache_bad(const nk_kv_t *c, NkKv *kv, const int *seqs, uint32_t nseq, uint32_t max_rows) {
     if (c->type != NK_BF16 && c->type != NK_E4M3) return "kv: a cache of bf16 or e4m3";
@@ -37,7 +38,7 @@ static const char *cache_bad(const nk_kv_t *c, NkKv *kv, const int *seqs, uint32
     if (c->type == NK_E4M3 && (!c->ks || !c->vs)) return "kv: scales of an 8-bit cache";
     if (!c->table || !aligned(c->table, 4) || !c->ldt || !c->tables || c->tables > 0x7fffffffu) return "kv: a table of pages";
     if (!seqs || !aligned(seqs, 16)) return "kv: a 16-byte aligned table of sequences";
-    if (nseq > 65535) return "kv: at most 65535 sequences in a call";
+    if (nseq > NK_KV_SEQS) return "kv: at most 4096 sequences in a call";
     if (max_rows > 1u << 30) return "kv: at most 2^30 rows a sequence";
     uint32_t shift = 0;
     while (1u << shift < c->page) ++shift;
@@ -115,6 +116,63 @@ int nk_kv_read(gpu_t *g, const nk_kv_t *c, void *K, uint32_t ldk, void *V, uint3
     return gpu_launch(g, name, &a, sizeof a, (uint32_t)blocks, gy, 1, 256, 1, 1);
 }
 
+/* The sequences of more than `over` and at most `upto` rows. */
+static int attend(gpu_t *g, NkAttnKvArgs a, int type, uint32_t over, uint32_t upto) {
+    const uint32_t rows = upto < a.M ? upto : a.M, dh = a.kv.dh, heads = a.kv.heads;
+    const uint64_t packed = (uint64_t)rows * a.group;
+    /* Up to 64 packed rows go 16 or 32 to a workgroup whose wavefronts share the tokens, more 128 to one whose wavefronts share
+     * the rows (8 heads of 128, groups of 4, 4000 tokens: 64 packed rows 18.4 us; 32000 tokens and 256 rows 67; 8192 rows 1299
+     * and 550 us). */
+    const int many = packed > 64, f32 = type == NK_F32;
+    const uint32_t QT = packed > 16 && (dh <= 128 || !f32) ? 2 : 1, tile = many ? 128 : 16 * QT, step = many ? 64 : 32;
+    const uint32_t DH = dh <= 64 ? 64 : many && dh <= 96 ? 96 : dh <= 128 ? 128 : many && dh <= 192 ? 192 : 256;
+    a.over = over;
+    a.upto = upto;
+    a.tile = many ? 7 : 3 + QT;
+    a.step = many ? 6 : 5;
+    a.first = tile / a.group + 1;
+    if (a.window)
+        a.reach = (uint32_t)(((uint64_t)a.window + tile / a.group + 1 + step) / step + 1 + ((uint64_t)a.sinks + step - 1) / step);
+    /* tiles that there can be (and, if the rows are there, are), and the pieces that a tile can have */
+    const uint64_t by_rows = (uint64_t)a.M * a.group / tile, by_seqs = a.nseq * ((packed + tile - 1) / tile);
+    const uint64_t tiles = by_seqs < by_rows + a.nseq ? by_seqs : by_rows + a.nseq;
+    /* Steps are split where tiles are fewer than the workgroups wanted.  Sums of few rows cost little to write and add up: three
+     * rounds of workgroups, which evens out mixed lengths (64 sequences of up to 16384 tokens 241, 234 and 221 us with 512, 1024
+     * and 1536), one sequence's a single round (131071 tokens 111, 117 and 124 us); 128 rows' (66 KB and as much again to
+     * read) only below a workgroup per CU (1024 rows 32 us whole, 62 split for 1024; 2048 rows 65 and 114), of f32 rows, whose
+     * steps are three times as long, two (1000 rows 47 and 52). */
+    const uint32_t wanted = packed <= 16 ? a.nseq > 1 && upto == a.max_rows ? 1536 : 512 : many && f32 ? 512 : 256, slots = (wanted + heads - 1) / heads;
+    a.least = packed <= 16 || (many && f32) ? 4 : 8;
+    const uint64_t pieces = ((a.max_len + step - 1) / step + a.least - 1) / a.least;
+    if (tiles > 1u << 23) return bad(g, "attention_kv: more rows than a launch covers");
+    uint64_t items = tiles;
+    if (pieces > 1 && (by_rows < by_seqs ? by_rows : by_seqs) < slots) {
+        a.slots = slots;
+        a.per_slot = 1.0f / (float)slots;
+        a.per_cu = (float)heads / (many && f32 ? 512.0f : 256.0f);
+        const uint64_t split = tiles * pieces < 2ull * slots ? tiles * pieces : 2ull * slots;
+        if (items < split) items = split;
+        a.ws = gpu_scratch_ws(g, (size_t)(split * heads * tile * (dh + 2)));
+        if (!a.ws) return bad(g, "attention_kv: scratch unavailable (size it before capture)");
+    }
+    if (items * heads > 1u << 23) return bad(g, "attention_kv: more rows than a launch covers");
+    /* two workgroups a CU from the start: long tiles beside short ones (2048 rows 63 -> 60 us) */
+    a.pair = many && tiles * heads > 256 && tiles * heads <= 512;
+    char name[40];
+    if (many) snprintf(name, sizeof name, "attn_many_%s_%s_%u", f32 ? "f32" : "bf16", cache_name(&a.kv), DH);
+    else snprintf(name, sizeof name, "attn_few_%s_%s_%u_%u", f32 ? "f32" : "bf16", cache_name(&a.kv), DH, QT);
+    gpu_next_bytes(g, (f32 ? 8.0 : 4.0) * a.M * a.heads * dh);
+    if (gpu_launch(g, name, &a, sizeof a, (uint32_t)items * heads, 1, 1, 256, 1, 1)) return -1;
+    if (!a.slots) return 0;
+    /* a row to a workgroup, or its wavefronts a row each and going round: some 2048 workgroups */
+    const uint64_t most = packed < tile ? packed : tile, some = tiles < slots ? tiles : slots;
+    uint64_t z = 2048 / (some * heads);
+    a.share = some * heads * most <= 2048;
+    if (a.share) z = most;
+    else if (z > (most + 3) / 4) z = (most + 3) / 4;
+    return gpu_launch(g, f32 ? "attn_join_f32" : "attn_join_bf16", &a, sizeof a, (uint32_t)some, heads, z ? (uint32_t)z : 1, 256, 1, 1);
+}
+
 int nk_attention_kv(gpu_t *g, const nk_kv_t *c, const nk_attend_t *p) {
     if (!c || !p) return bad(g, "attention_kv: no arguments");
     if (!p->nseq || !p->max_rows || !p->M) return 0;
@@ -131,57 +189,15 @@ int nk_attention_kv(gpu_t *g, const nk_kv_t *c, const nk_attend_t *p) {
     if (!(p->scale > 0.0f) || !isfinite(p->scale)) return bad(g, "attention_kv: a scale above zero");
     if (p->max_len > 1u << 30) return bad(g, "attention_kv: at most 2^30 tokens a sequence");
     const uint32_t group = p->heads / kv.heads;
-    const uint32_t window = p->window >= p->max_len ? 0 : p->window, sinks = p->sinks < p->max_len ? p->sinks : p->max_len;
+    if ((uint64_t)(p->max_rows < p->M ? p->max_rows : p->M) * group > 1u << 30) return bad(g, "attention_kv: more rows than a launch covers");
     NkAttnKvArgs a = { .kv = kv, .q = p->q, .o = p->o, .seqs = p->seqs, .ldq = p->ldq, .ldo = p->ldo, .heads = p->heads, .group = group,
-                       .window = window, .sinks = sinks, .nseq = p->nseq, .max_rows = p->max_rows, .max_len = p->max_len, .M = p->M,
-                       .upto = p->max_rows, .inv_group = 0xffffffffu / group, .scale = p->scale };
+                       .window = p->window >= p->max_len ? 0 : p->window, .sinks = p->sinks < p->max_len ? p->sinks : p->max_len,
+                       .nseq = p->nseq, .max_rows = p->max_rows, .max_len = p->max_len, .M = p->M, .inv_group = 0xffffffffu / group,
+                       .scale = p->scale };
     a.vec = aligned(p->q, 16) && aligned(p->o, 4 * size) && p->ldq % (16 / size) == 0 && p->ldo % 4 == 0;
-    const uint32_t rows = p->max_rows < p->M ? p->max_rows : p->M;
-    uint32_t DH = kv.dh <= 64 ? 64 : kv.dh <= 128 ? 128 : 256;
-    const uint64_t packed = (uint64_t)rows * group;
-    const int many = packed > 64;
-    const uint32_t QT = packed > 16 && (DH < 256 || p->type == NK_BF16) ? 2 : 1;
-    if (many) DH = kv.dh > 64 && kv.dh <= 96 ? 96 : kv.dh > 128 && kv.dh <= 192 ? 192 : DH;
-    const uint32_t tile = many ? 128 : 16 * QT, step = many ? 64 : 32;
-    a.tile = many ? 7 : 3 + QT;
-    a.step = many ? 6 : 5;
-    a.least = packed <= 16 || (many && p->type == NK_F32) ? 4 : 8;
-    a.first = tile / group + 1;
-    if (window) {
-        const uint64_t reach = ((uint64_t)window + tile / group + 1 + step) / step + 1 + ((uint64_t)sinks + step - 1) / step;
-        a.reach = (uint32_t)reach;
-    }
-    /* tiles that there can be, and the pieces that a tile can have */
-    const uint64_t each = ((uint64_t)rows * group + tile - 1) / tile, by_rows = (uint64_t)p->M * group / tile + p->nseq;
-    const uint64_t tiles = p->nseq * each < by_rows ? p->nseq * each : by_rows;
-    const uint64_t pieces = ((p->max_len + step - 1) / step + a.least - 1) / a.least;
-    if (tiles > 1u << 23) return bad(g, "attention_kv: more rows than a launch covers");
-    uint64_t items = tiles;
-    a.pair = many && tiles * kv.heads > 256 && tiles * kv.heads <= 512;
-    const uint32_t wanted = packed > 16 ? many && p->type == NK_F32 ? 512 : 256 : p->nseq > 1 ? 1536 : 512, slots = (wanted + kv.heads - 1) / kv.heads;
-    if (pieces > 1 && (uint64_t)p->M * group / tile < slots) {
-        a.slots = slots;
-        a.per_slot = 1.0f / (float)slots;
-        a.per_cu = (float)kv.heads / (wanted == 512 && many ? 512.0f : 256.0f);
-        const uint64_t split = tiles * pieces < 2ull * a.slots ? tiles * pieces : 2ull * a.slots;
-        if (items < split) items = split;
-        a.ws = gpu_scratch_ws(g, (size_t)(split * kv.heads * tile * (kv.dh + 2)));
-        if (!a.ws) return bad(g, "attention_kv: scratch unavailable (size it before capture)");
-    }
-    const char *type = p->type == NK_F32 ? "f32" : "bf16";
-    char name[40];
-    if (many) snprintf(name, sizeof name, "attn_many_%s_%s_%u", type, cache_name(&kv), DH);
-    else snprintf(name, sizeof name, "attn_few_%s_%s_%u_%u_4", type, cache_name(&kv), DH, QT);
-    gpu_next_bytes(g, 2.0 * size * p->M * nq);
-    if (items * kv.heads > 1u << 22) return bad(g, "attention_kv: more rows than a launch covers");
-    if (gpu_launch(g, name, &a, sizeof a, (uint32_t)items * kv.heads, 1, 1, 256, 1, 1)) return -1;
-    if (!a.slots) return 0;
-    snprintf(name, sizeof name, "attn_join_%s", type);
-    const uint64_t most = (uint64_t)rows * group < tile ? (uint64_t)rows * group : tile, some = tiles < a.slots ? tiles : a.slots;
-    /* a row to a workgroup, or its wavefronts a row each and going round: some 2048 workgroups */
-    a.share = some * kv.heads * most <= 2048;
-    uint64_t z = 2048 / (some * kv.heads);
-    if (a.share) z = most;
-    else if (z > (most + 3) / 4) z = (most + 3) / 4;
-    return gpu_launch(g, name, &a, sizeof a, (uint32_t)some, kv.heads, z ? (uint32_t)z : 1, 256, 1, 1);
+    /* beside prompts, sequences of a few rows (the steps of a mixed batch) have a launch of their own */
+    const uint32_t few = group <= 16 ? 16 / group : 64 / group;
+    const int mixed = p->nseq > 1 && few && (uint64_t)(p->max_rows < p->M ? p->max_rows : p->M) * group > 64;
+    if (mixed && attend(g, a, p->type, 0, few)) return -1;
+    return attend(g, a, p->type, mixed ? few : 0, p->max_rows);
 }

@@ -127,6 +127,7 @@ __device__ __forceinline__ u32 attn_piece(const NkAttnKvArgs &a, kvseq_t s) {
     if (!a.slots) return 0;
     u32 tiles = 0;
     float steps = 0.0f;
+#pragma unroll 4
     for (u32 i = lane; i < a.nseq; i += 64) {
         if (i != lane) s = attn_seq(a, i);
         const u32 n = attn_tiles(a, s);
@@ -241,9 +242,9 @@ template <typename T> __device__ __forceinline__ void attn_by_formula(const NkAt
  * group g of a chunk pair has the values 16 g on), values through the wavefront's own LDS for their columns;
  * the next step's loads are in flight. */
 #define ATTN_STEP 32
-template <typename T, typename CT, int DH, int QT, int NW> __device__ __forceinline__ void attn_few(const NkAttnKvArgs &a) {
+template <typename T, typename CT, int DH, int QT> __device__ __forceinline__ void attn_few(const NkAttnKvArgs &a) {
     constexpr bool E4M3 = sizeof(CT) == 1;
-    constexpr int NC = DH / 32, ND = DH / 16, TERMS = sizeof(T) == 4 ? 3 : 1, ROWS = 16 * QT;
+    constexpr int NC = DH / 32, ND = DH / 16, TERMS = sizeof(T) == 4 ? 3 : 1, ROWS = 16 * QT, NW = 4;
     constexpr int LDV = DH + 16; /* u16 of a token's row in LDS: 32 bytes more, so that four tokens' are in other banks */
     constexpr int NK = E4M3 ? DH / 64 : DH / 32, NV = E4M3 ? DH / 32 : DH / 16; /* 16-byte loads of a lane: per 16 tokens; per step */
     constexpr u32 VBYTES = NW * ATTN_STEP * LDV * 2, OBYTES = NW * 16 * DH * 4;
@@ -460,24 +461,15 @@ const bool see = th[b] & ((pos[t] - j < reach) | ((j < a.sinks) & (j <= pos[t]) 
     for (u32 r = wave; r < w.nr; r += NW)
         if (wrong[r]) attn_by_formula<T>(a, w.first, w.len, w.row, w.r0 + r, h);
 }
-#ifndef OCC_B
-#define OCC_B 2
-#define OCC_E 3
-#endif
-#define ATTN_FEW(T, TN, CT, CN, DH, QT, NW, OCC)                                                                                \
-    extern "C" __global__ __launch_bounds__(NW * 64, OCC) void attn_few_##TN##_##CN##_##DH##_##QT##_##NW(const NkAttnKvArgs a) { \
-        attn_few<T, CT, DH, QT, NW>(a);                                                                                         \
+#define ATTN_FEW(T, TN, CT, CN, DH, QT)                                                                                  \
+    extern "C" __global__ __launch_bounds__(256) void attn_few_##TN##_##CN##_##DH##_##QT(const NkAttnKvArgs a) {         \
+        attn_few<T, CT, DH, QT>(a);                                                                                      \
     }
-#define ATTN_FEW_DH(DH, QT, NW)                                                                                                 \
-    ATTN_FEW(u16, bf16, u16, bf16, DH, QT, NW, 1) ATTN_FEW(u16, bf16, unsigned char, e4m3, DH, QT, NW, 1)                       \
-    ATTN_FEW(float, f32, u16, bf16, DH, QT, NW, 1) ATTN_FEW(float, f32, unsigned char, e4m3, DH, QT, NW, 1)
-ATTN_FEW_DH(64, 1, 4) ATTN_FEW_DH(256, 1, 4) ATTN_FEW_DH(64, 2, 4) ATTN_FEW_DH(128, 2, 4)
-ATTN_FEW(u16, bf16, u16, bf16, 256, 2, 4, 1) ATTN_FEW(u16, bf16, unsigned char, e4m3, 256, 2, 4, 1)
-ATTN_FEW(u16, bf16, u16, bf16, 128, 1, 4, OCC_B) ATTN_FEW(u16, bf16, unsigned char, e4m3, 128, 1, 4, OCC_E)
-ATTN_FEW(float, f32, u16, bf16, 128, 1, 4, 1) ATTN_FEW(float, f32, unsigned char, e4m3, 128, 1, 4, 1)
-ATTN_FEW_DH(64, 1, 8) ATTN_FEW_DH(256, 1, 8)
-ATTN_FEW(u16, bf16, u16, bf16, 128, 1, 8, 2) ATTN_FEW(u16, bf16, unsigned char, e4m3, 128, 1, 8, 2)
-ATTN_FEW(float, f32, u16, bf16, 128, 1, 8, 2) ATTN_FEW(float, f32, unsigned char, e4m3, 128, 1, 8, 2)
+#define ATTN_FEW_DH(DH, QT)                                                                                              \
+    ATTN_FEW(u16, bf16, u16, bf16, DH, QT) ATTN_FEW(u16, bf16, unsigned char, e4m3, DH, QT)                              \
+    ATTN_FEW(float, f32, u16, bf16, DH, QT) ATTN_FEW(float, f32, unsigned char, e4m3, DH, QT)
+ATTN_FEW_DH(64, 1) ATTN_FEW_DH(128, 1) ATTN_FEW_DH(256, 1) ATTN_FEW_DH(64, 2) ATTN_FEW_DH(128, 2)
+ATTN_FEW(u16, bf16, u16, bf16, 256, 2) ATTN_FEW(u16, bf16, unsigned char, e4m3, 256, 2)
 
 /* ---- many rows: wavefronts over the rows ----------------------------------------------------------------
  * A workgroup's 128 packed rows, 32 to a wavefront, over steps of 64 tokens whose keys and values lie in LDS for all of
@@ -772,6 +764,7 @@ template <typename T> __device__ __forceinline__ void attn_join(const NkAttnKvAr
     });
     if (!it.found) return;
     u32 before = 0; /* items of the sequences before this one */
+#pragma unroll 4
     for (u32 i = lane; i < it.i; i += 64) {
         const kvseq_t s = i == lane ? mine : load(i);
         const u32 n = attn_tiles(a, s);

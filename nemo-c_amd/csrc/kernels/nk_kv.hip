@@ -32,26 +32,49 @@ __device__ __forceinline__ u32 wave_scan(u32 v) {
 __device__ __forceinline__ u32 lane_of(u32 v, int lane) { return (u32)__builtin_amdgcn_readlane((int)v, lane); }
 
 /* The sequence that has number `id` when every sequence has count(it) of them, and its number there.  Every wavefront
- * looks by itself, a sequence a lane; `mine` is that of the first 64, load(i) any other. */
+ * looks by itself: `mine` is this lane's of the first 64, or, of more, four to a lane and 256 at a time by load(i). */
 typedef struct {
     kvseq_t seq;
     u32 i, local;
     bool found;
 } kvitem_t;
-template <typename L, typename F> __device__ __forceinline__ kvitem_t kv_find(u32 nseq, u32 id, kvseq_t mine, L load, F count) {
+__device__ __forceinline__ kvseq_t kvseq_of(const kvseq_t &s, int lane) {
+    return (kvseq_t){ lane_of(s.first, lane), lane_of(s.rows, lane), lane_of(s.len, lane), lane_of(s.row, lane), true };
+}
+template <typename L, typename F> __device__ __forceinline__ kvitem_t kv_find(u32 nseq, u32 id, const kvseq_t &mine, L load, F count) {
     const u32 lane = threadIdx.x & 63;
+    if (nseq <= 64) {
+        const u32 n = lane < nseq ? count(mine) : 0, sum = wave_scan(n);
+        const u64 past = __ballot(sum > id);
+        const int at = past ? __ffsll((unsigned long long)past) - 1 : 63;
+        return (kvitem_t){ kvseq_of(mine, at), (u32)at, id - lane_of(sum - n, at), past != 0 };
+    }
     u32 before = 0;
-    for (u32 i0 = 0;;) {
-        const u32 n = i0 + lane < nseq ? count(mine) : 0, sum = wave_scan(n);
+    for (u32 i0 = 0; i0 < nseq; i0 += 256) {
+        kvseq_t s[4];
+        u32 n[4], all = 0;
+#pragma unroll
+        for (u32 k = 0; k < 4; ++k) s[k] = load(min(i0 + 4 * lane + k, nseq - 1));
+#pragma unroll
+        for (u32 k = 0; k < 4; ++k) all += n[k] = i0 + 4 * lane + k < nseq ? count(s[k]) : 0;
+        const u32 sum = wave_scan(all);
         const u64 past = __ballot(before + sum > id);
         if (past) {
             const int at = __ffsll((unsigned long long)past) - 1;
-            const kvseq_t s = { lane_of(mine.first, at), lane_of(mine.rows, at), lane_of(mine.len, at), lane_of(mine.row, at), true };
-            return (kvitem_t){ s, i0 + (u32)at, id - before - lane_of(sum - n, at), true };
+            u32 local = id - before - lane_of(sum - all, at), k = 0;
+            kvseq_t q = kvseq_of(s[0], at);
+#pragma unroll
+            for (u32 e = 0; e < 3; ++e) {
+                const u32 here = lane_of(n[e], at);
+                if (k == e && local >= here) {
+                    local -= here;
+                    k = e + 1;
+                    q = kvseq_of(s[e + 1], at);
+                }
+            }
+            return (kvitem_t){ q, i0 + 4 * (u32)at + k, local, true };
         }
         before += lane_of(sum, 63);
-        if ((i0 += 64) >= nseq) break;
-        mine = load(min(i0 + lane, nseq - 1));
     }
     return (kvitem_t){ mine, 0, 0, false };
 }

@@ -33,7 +33,7 @@ KV = dict(type=1, heads=2, dh=64, page=32, pages=9, k=P, v=P, ks=P, vs=P, table=
 BAD_KV = [dict(type=0), dict(type=3), dict(heads=0), dict(heads=65536), dict(dh=0), dict(dh=24), dict(dh=272), dict(page=8), dict(page=48),
           dict(page=1 << 21), dict(pages=0), dict(pages=1 << 31), dict(k=None), dict(v=None), dict(k=P + 8), dict(v=P + 2),
           dict(type=2, ks=None), dict(type=2, vs=None), dict(table=None), dict(table=P + 2), dict(ldt=0), dict(tables=0)]
-BAD_BATCH = [dict(seqs=None), dict(seqs=P + 4), dict(nseq=65536), dict(max_rows=(1 << 30) + 1)]
+BAD_BATCH = [dict(seqs=None), dict(seqs=P + 4), dict(nseq=4097), dict(max_rows=(1 << 30) + 1)]
 
 
 def kv(**more):
