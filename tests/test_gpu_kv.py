@@ -646,3 +646,165 @@ def test_prompt_then_tokens(gpu, cache_type):
         close(back(out, BF16).reshape(M, heads, dh), ref, bound)
         done = [d + p for d, p in zip(done, part)]
     cache.free()
+
+
+# ---- many rows ---------------------------------------------------------------------------------------
+
+PROMPT_HEADS = [(4, 4, 128), (2, 1, 96), (6, 2, 64), (2, 1, 256), (3, 3, 192), (4, 1, 80), (20, 1, 32)]
+
+
+@pytest.mark.parametrize("window,sinks", [(0, 0), (70, 0), (100, 70)])
+@pytest.mark.parametrize("shape", range(len(PROMPT_HEADS)))
+@pytest.mark.parametrize("cache_type", [BF16, E4M3])
+@pytest.mark.parametrize("typ", [F32, BF16])
+def test_attend_prompts(gpu, window, sinks, shape, cache_type, typ):
+    """Prompts over more than one tile of 128 packed rows, tokens and chunks beside them, an empty sequence."""
+    heads, hk, dh = PROMPT_HEADS[shape]
+    rng = np.random.default_rng([17, window, shape, cache_type, typ])
+    seqs, M = sequences([150, 1, 0, 33, 4], [7 * shape, 300, 9, 100, 64], gap=shape % 2)
+    more = [dict(), dict(ld=heads * dh + 3, off=1), dict(max_rows=1000, max_len=100000)][(shape + window) % 3]
+    check_attend(gpu, rng, typ, cache_type, heads, hk, dh, (64, 16, 32)[shape % 3], seqs, M, window, sinks, **more)
+
+
+@pytest.mark.parametrize("typ", [F32, BF16])
+@pytest.mark.parametrize("cache_type", [BF16, E4M3])
+@pytest.mark.parametrize("dh", [64, 128, 192, 256])
+def test_attend_prompt_behind_many_tokens(gpu, typ, cache_type, dh):
+    """Few tiles of many rows, split along their tokens; pages that are not there among them."""
+    rng = np.random.default_rng([18, typ, cache_type, dh])
+    seqs, M = sequences([130], [2900])
+    check_attend(gpu, rng, typ, cache_type, 1, 1, dh, 16, seqs, M)
+    check_attend(gpu, rng, typ, cache_type, 1, 1, dh, 16, seqs, M, 2000, 100, drop=[(0, 3), (0, 70), (0, 100), (0, 189)])
+
+
+def test_attend_pairs_of_tiles(gpu):
+    """Sizes at which tiles go two to a CU, the long ones beside the short ones."""
+    rng = np.random.default_rng(19)
+    seqs, M = sequences([1060], [3])
+    check_attend(gpu, rng, BF16, BF16, 64, 32, 16, 64, seqs, M, 60)
+
+
+@pytest.mark.parametrize("typ", [F32, BF16])
+def test_attend_prompt_values_not_finite(gpu, typ):
+    rng = np.random.default_rng(20)
+    dh, rows = 64, 150
+    seqs = np.array([(0, rows, 0, 0)], np.int32)
+    pages = Pages(rng, BF16, 1, dh, 16, [rows])
+
+    def put(name, j, d, value):
+        getattr(pages, name)[pages.table[0, j // 16], 0, j % 16, d] = oracle.f32_to_bf16(np.array([value], np.float32))[0]
+
+    put("v", 70, 3, np.inf)
+    put("v", 75, 4, np.nan)
+    put("k", 140, 0, -np.inf)
+    q = kept(rng.standard_normal((rows, dh)), typ)
+    q[:, 0] = np.abs(q[:, 0]) + 0.1  # the logit of token 140 is -inf: it has no weight
+    q = kept(q, typ)
+    cache = Cache(gpu, pages)
+    out = back(run_attend(gpu, cache, typ, q, seqs, 1), typ)
+    cache.free()
+    k, v = (pages.tokens(x, 0, rows)[0][:, 0] for x in "kv")
+    fin = np.where(np.isfinite(v), v, 0.0)
+    for i in range(rows):
+        s = (k[:i + 1] @ q[i]) * dh ** -0.5
+        w = np.exp(s - s.max())
+        ref = w @ fin[:i + 1] / w.sum()
+        for d in range(dh):
+            if d == 3 and i >= 70:
+                assert out[i, d] == np.inf or i >= 140 and np.isinf(out[i, d])
+            elif d == 4 and i >= 75:
+                assert np.isnan(out[i, d])
+            else:
+                assert abs(out[i, d] - ref[d]) < 0.05, (i, d)  # values below 5, two roundings to bf16
+
+
+def test_attend_4096_sequences(gpu):
+    """As many sequences as a call takes, most of them one token long."""
+    rng = np.random.default_rng(21)
+    n = 4096
+    rows = (rng.random(n) < 0.7).astype(int)
+    rows[[100, 2000, 4095]] = 3, 20, 2
+    seqs, M = sequences(list(rows), list(rng.integers(0, 40, n)))
+    check_attend(gpu, rng, BF16, BF16, 1, 1, 16, 16, seqs, M)
+
+
+def test_captured_mixed_batches(gpu):
+    """A captured call replayed with other tables: prompts, steps, both, none; against the formulas and eager calls."""
+    rng = np.random.default_rng(22)
+    L = nemoasr.lib()
+    heads, hk, dh, n, M = 4, 2, 32, 4, 300
+    pages = Pages(rng, BF16, hk, dh, 16, [3000, 400, 300, 200])
+    cache = Cache(gpu, pages)
+    q = kept(rng.standard_normal((M, heads * dh)), F32)
+    dq, seqs, outs = gpu.put(bits(q, F32)), gpu.alloc(n * 16), [gpu.alloc(M * heads * dh * 4) for _ in range(2)]
+
+    def call(out):
+        a = nemoasr.Attend(type=F32, q=dq.ptr, ldq=heads * dh, o=out.ptr, ldo=heads * dh, heads=heads, window=0, sinks=0, scale=dh ** -0.5,
+                           seqs=seqs.ptr, nseq=n, max_rows=250, max_len=3000, M=M)
+        gpu.check(L.nk_attention_kv(gpu.h, C.byref(cache.kv), C.byref(a)))
+
+    graph = None
+    for table in ([(0, 200, 100, 1), (200, 1, 2990, 0), (201, 90, 0, 2), (291, 0, 0, 3)], [(0, 1, 2999, 0), (1, 1, 7, 1), (2, 1, 255, 2), (3, 1, 0, 3)],
+                  [(0, 0, 5, 0), (0, 0, 5, 1), (0, 0, 5, 2), (0, 0, 5, 3)], [(10, 250, 2750, 0), (260, 3, 100, 1), (263, 2, 9, 2), (299, 1, 199, 3)]):
+        table = np.array(table, np.int32)
+        seqs.write(table)
+        for o in outs:
+            o.write(np.full((M, heads * dh), 7.0, np.float32))
+        gpu.begin()
+        call(outs[0])
+        gpu.end()
+        if graph is None:
+            gpu.begin()
+            assert L.gpu_capture_begin(gpu.h) == 0
+            call(outs[1])
+            graph = L.gpu_capture_end(gpu.h)
+            assert graph
+            gpu.end()
+        for _ in range(2):
+            gpu.begin()
+            gpu.check(L.gpu_graph_launch(gpu.h, graph))
+            gpu.end()
+        a, b = (o.read((M, heads, dh)) for o in outs)
+        np.testing.assert_array_equal(a.view(np.uint32), b.view(np.uint32))
+        ref, bound = attend(q.reshape(M, heads, dh), pages, table, 0, 0, np.float32(dh ** -0.5), F32, np.full((M, heads, dh), 7.0))
+        close(a, ref, bound)
+    L.gpu_graph_free(graph)
+    for b in [dq, seqs] + outs:
+        b.free()
+    cache.free()
+
+
+def test_capture_needs_the_scratch(gpu):
+    """A call that is split refuses to be captured before one has sized the scratch, and is captured after it."""
+    rng = np.random.default_rng(23)
+    own = nemoasr.Gpu()
+    L = nemoasr.lib()
+    pages = Pages(rng, BF16, 8, 128, 64, [700, 700])
+    cache = Cache(own, pages)
+    q, o = own.put(np.zeros((2, 8 * 128), np.uint16)), own.alloc(2 * 8 * 128 * 2)
+    seqs = own.put(np.array([(0, 1, 600, 0), (1, 1, 5, 1)], np.int32))
+    a = nemoasr.Attend(type=BF16, q=q.ptr, ldq=1024, o=o.ptr, ldo=1024, heads=8, scale=0.1, seqs=seqs.ptr, nseq=2, max_rows=1, max_len=1 << 20, M=2)
+
+    def call():
+        return L.nk_attention_kv(own.h, C.byref(cache.kv), C.byref(a))
+
+    own.begin()
+    assert L.gpu_capture_begin(own.h) == 0
+    assert call() == -1 and "scratch unavailable" in L.gpu_last_error(own.h).decode()
+    graph = L.gpu_capture_end(own.h)
+    if graph:
+        L.gpu_graph_free(graph)
+    err = C.create_string_buffer(512)
+    L.gpu_end(own.h, err, 512)
+    own.begin()
+    own.check(call())
+    own.end()
+    own.begin()
+    assert L.gpu_capture_begin(own.h) == 0
+    own.check(call())
+    graph = L.gpu_capture_end(own.h)
+    assert graph
+    own.check(L.gpu_graph_launch(own.h, graph))
+    own.end()
+    L.gpu_graph_free(graph)
+    own.close()
