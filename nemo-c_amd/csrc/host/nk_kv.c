@@ -195,9 +195,12 @@ int nk_attention_kv(gpu_t *g, const nk_kv_t *c, const nk_attend_t *p) {
                        .nseq = p->nseq, .max_rows = p->max_rows, .max_len = p->max_len, .M = p->M, .inv_group = 0xffffffffu / group,
                        .scale = p->scale };
     a.vec = aligned(p->q, 16) && aligned(p->o, 4 * size) && p->ldq % (16 / size) == 0 && p->ldo % 4 == 0;
-    /* beside prompts, sequences of a few rows (the steps of a mixed batch) have a launch of their own */
+    /* Beside prompts, sequences of a few rows (the steps of a mixed batch) have a launch of their own, which splits them, where
+     * a step may see more than 2048 tokens: a workgroup of many rows takes 1.2 us for 64 of them, the launches some 6 us (12
+     * prompts with a window of 512 tokens 53 and 60). */
     const uint32_t few = group <= 16 ? 16 / group : 64 / group;
-    const int mixed = p->nseq > 1 && few && (uint64_t)(p->max_rows < p->M ? p->max_rows : p->M) * group > 64;
+    const uint64_t sees = a.window && (uint64_t)a.window + a.sinks < a.max_len ? (uint64_t)a.window + a.sinks : a.max_len;
+    const int mixed = p->nseq > 1 && few && sees > 2048 && (uint64_t)(p->max_rows < p->M ? p->max_rows : p->M) * group > 64;
     if (mixed && attend(g, a, p->type, 0, few)) return -1;
     return attend(g, a, p->type, mixed ? few : 0, p->max_rows);
 }

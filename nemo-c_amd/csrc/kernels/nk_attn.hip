@@ -7,8 +7,9 @@
  *
  * in one pass over the tokens, with the running maximum, sum and sums of v in 32 bits.  The products are on the matrix
  * units: keys and values are exact in bf16 (8-bit codes with their power of two too); bf16 rows are, and their
- * probabilities are rounded to bf16 (a relative 2^-9 of each, as much as the output's own rounding); f32 rows and
- * their probabilities are three bf16 terms, 24 bits.
+ * probabilities are rounded to bf16 (at most a relative 2^-8 of each, as the output is too: with both the error is 1.3 times
+ * that of the output's rounding alone, and a second term would be half as many products again); f32 rows and their
+ * probabilities are three bf16 terms, 24 bits.
  *
  * Rows whose result is not finite (an infinity or NaN was near, also in a token that only some rows see: 0 times it is
  * NaN in a product), or whose sum is zero, are computed again by the formula, row by row. */
@@ -240,7 +241,12 @@ template <typename T> __device__ __forceinline__ void attn_by_formula(const NkAt
  * A workgroup's 16 QT packed rows; its four wavefronts take every fourth step of 32 tokens, each with sums of its own that
  * are joined at the end.  Keys go from memory into fragments (a fragment's sum may take its values in any order: lane
  * group g of a chunk pair has the values 16 g on), values through the wavefront's own LDS for their columns;
- * the next step's loads are in flight. */
+ * the next step's loads are in flight.
+ *
+ * Bound by memory where there is much: 131071 tokens of 8 heads of 128 bf16 95 us (5.7 TB/s), 64 sequences of up to 16384
+ * 8-bit tokens 202 us (5.5 TB/s).  By round trips where there is little: 1000 tokens 7.5 us, of which the table 1.6, the
+ * rows' queries 0.5, page and first keys 1.5, two steps 2, joining the wavefronts and storing 1.7.  More wavefronts per SIMD
+ * (registers held to 128: 8-bit steps 230 -> 300 us) or per workgroup (eight: 112 and 240) are not faster. */
 #define ATTN_STEP 32
 template <typename T, typename CT, int DH, int QT> __device__ __forceinline__ void attn_few(const NkAttnKvArgs &a) {
     constexpr bool E4M3 = sizeof(CT) == 1;
@@ -478,7 +484,14 @@ ATTN_FEW(u16, bf16, u16, bf16, 256, 2) ATTN_FEW(u16, bf16, unsigned char, e4m3, 
  * tokens 4 hh + (0..3) and 8 on of every 16 (hh: the lane's half) are the order in which the columns of V are read.
  * A row of LDS is DH values; its 16-byte chunks are mixed by the token so that the lanes of a read spread over all
  * banks.  The maximum follows only where a logit is 2^8 times above it: 2^(x - m) may exceed 1 as well as not, and the
- * sums are rescaled once or twice a row instead of every step. */
+ * sums are rescaled once or twice a row instead of every step.
+ *
+ * 8192 rows of 32 heads on 8 of 128: 547 us, 1.0 PFLOP/s of those that count, four fifths of a large library product's rate.
+ * The matrix units are busy half of the cycles, the vector units (32 exponentials, 32 products, maxima, sums and conversions
+ * of a wavefront's step) nearly as many, at the 1.9 to 2.0 GHz that the card's power leaves; what was tried beside: the next
+ * step's K Q^T while this one's weights are computed (7 % fewer cycles at a lower clock, 573 us against 569), two
+ * workgroups' wavefronts of different priority (no change), eight wavefronts that share rows and halve the
+ * tokens (607), per-lane 64-bit addresses (610).  Heads of 64 keep three workgroups a CU. */
 typedef float floatx16 __attribute__((ext_vector_type(16)));
 __device__ __forceinline__ floatx16 attn_mfma32(u32x4 a, u32x4 b, floatx16 acc) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), acc, 0, 0, 0);

@@ -172,7 +172,13 @@ __device__ __forceinline__ float to_odd(double d) {
  * Values go in pairs of P at a time: pair (i, i + rot / 2), or interleaved (2 i, 2 i + 1), and as they are behind the
  * rotated part.  8 bits: the block's scale is the least power of two of which 448 times reach the largest new value
  * and at least that of the tokens that the block has; where it grows, their codes are rounded again (exactly, but for
- * those that become subnormal). */
+ * those that become subnormal).
+ *
+ * Bound by memory: 17.8 thousand f32 rows of 20 heads of 96 into bf16 43 us (5.8 TB/s, part of it from the caches; 57 us, 4.3
+ * TB/s, with rows from HBM).  8 bits: 8192 bf16 rows of 48 heads of 128 56 us, 3.3 TB/s: the keys' sums in 64 bits take
+ * registers (three wavefronts a SIMD; in f32 38 us, with two or three of 8 million codes a step off).  Loading the rows twice
+ * instead of keeping them is as fast with warm caches and 5 us slower without; four rounds in flight need 248
+ * registers (70 us).  One token of 64 streams 8 us: the table, the page, the rows and the stores, each a round trip. */
 template <typename T, int P, bool E4M3> __device__ __forceinline__ void kv_append(const NkAppendArgs &a) {
     __shared__ union {
         float2 f[NK_KV_BLOCK][KV_PAIRS];
@@ -219,6 +225,7 @@ template <typename T, int P, bool E4M3> __device__ __forceinline__ void kv_appen
                         const double v = fma((double)p, c.x, -((double)q * c.y));
                         q = to_odd(fma((double)q, c.x, (double)p * c.y));
                         p = to_odd(v);
+                        if (i % 2) __builtin_amdgcn_sched_barrier(0); /* two pairs' operands at a time (f32 rows: 167 registers -> 108) */
                         return;
                     }
                 const float2 c = turn.f[t][j + i];

@@ -114,6 +114,8 @@ def test_steps_of_a_mixed_batch(launches):
     """Beside prompts, sequences of up to 16 packed rows have a launch of their own; one sequence's rows, or few, have one."""
     names = [k[0] for k in attend(launches, 1, 1, 32, 8, 128, 64, 500, 8000)]
     assert [n for n in names if "join" not in n] == ["attn_few_bf16_bf16_128_1", "attn_many_bf16_bf16_128"]
+    for more in (dict(max_len=2048), dict(window=2000)):  # or none where a step sees little
+        assert [k[0] for k in attend(launches, 1, 1, 32, 8, 128, 64, 500, 8000, **more)] == ["attn_many_bf16_bf16_128"]
     assert [k[0] for k in attend(launches, 1, 1, 32, 8, 128, 1, 5000, 5000)] == ["attn_many_bf16_bf16_128"]
     assert [k[0] for k in attend(launches, 1, 1, 32, 8, 128, 64, 1, 64)] == ["attn_few_bf16_bf16_128_1", "attn_join_bf16"]
     assert np.all([k[0] == "attn_few_bf16_bf16_128_1" for k in attend(launches, 1, 1, 32, 8, 128, 64, 1, 64, 100)])
