@@ -164,10 +164,11 @@ static int attend(gpu_t *g, NkAttnKvArgs a, int type, uint32_t over, uint32_t up
     gpu_next_bytes(g, (f32 ? 8.0 : 4.0) * a.M * a.heads * dh);
     if (gpu_launch(g, name, &a, sizeof a, (uint32_t)items * heads, 1, 1, 256, 1, 1)) return -1;
     if (!a.slots) return 0;
-    /* a row to a workgroup, or its wavefronts a row each and going round: some 2048 workgroups */
+    /* a row to a workgroup, or its wavefronts a row each and going round: some 1024 workgroups, one round of them (58 x 8 heads
+     * x 4 rows a workgroup each 216 us with what they join, 207 so; 24 x 4 x 128 rows by 512, 1024 and 2048: 46.4, 42.6, 44.1) */
     const uint64_t most = packed < tile ? packed : tile, some = tiles < slots ? tiles : slots;
-    uint64_t z = 2048 / (some * heads);
-    a.share = some * heads * most <= 2048;
+    uint64_t z = 1024 / (some * heads);
+    a.share = some * heads * most <= 256;
     if (a.share) z = most;
     else if (z > (most + 3) / 4) z = (most + 3) / 4;
     return gpu_launch(g, f32 ? "attn_join_f32" : "attn_join_bf16", &a, sizeof a, (uint32_t)some, heads, z ? (uint32_t)z : 1, 256, 1, 1);

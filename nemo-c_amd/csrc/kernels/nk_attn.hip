@@ -11,8 +11,10 @@
  * that of the output's rounding alone, and a second term would be half as many products again); f32 rows and their
  * probabilities are three bf16 terms, 24 bits.
  *
- * Rows whose result is not finite (an infinity or NaN was near, also in a token that only some rows see: 0 times it is
- * NaN in a product), or whose sum is zero, are computed again by the formula, row by row. */
+ * A bf16 row whose sum of weights is NaN has a logit that is (or an infinite one): all NaN, as the formula has it.  Rows
+ * whose result is not finite otherwise (an infinity or NaN was near among the values, also of a token that only some rows
+ * see: 0 times it is NaN in a product; of an f32 row's terms the later ones are zero too), or whose sum is zero, are computed
+ * again by the formula, row by row, as far as a NaN logit. */
 #include "nk_common.h"
 
 typedef short s16x4 __attribute__((ext_vector_type(4)));
@@ -52,8 +54,9 @@ __device__ __forceinline__ floatx4 attn_mfma(u32x4 a, u32x4 b, floatx4 acc) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), acc, 0, 0, 0);
 }
 
-/* 8 f32 values as TERMS bf16 fragments: to nearest each, the first of what the values are, the next of what is left */
-template <int TERMS> __device__ __forceinline__ void attn_terms(const float (&x)[8], u32x4 (&t)[TERMS]) {
+/* 8 f32 values as TERMS bf16 fragments: to nearest each, the first of what the values are, the next of what is left.  BIG: also
+ * values that round to infinity, whose first term is the largest number */
+template <int TERMS, bool BIG = false> __device__ __forceinline__ void attn_terms(const float (&x)[8], u32x4 (&t)[TERMS]) {
     floatx2 r[4];
 #pragma unroll
     for (int p = 0; p < 4; ++p) r[p] = (floatx2){ x[2 * p], x[2 * p + 1] };
@@ -63,6 +66,10 @@ template <int TERMS> __device__ __forceinline__ void attn_terms(const float (&x)
 #pragma unroll
         for (int p = 0; p < 4; ++p) {
             w[p] = __builtin_bit_cast(u32, __builtin_convertvector(r[p], bf16x2));
+            if (BIG && TERMS > 1 && !k) {
+                if ((w[p] & 0x7fffu) == 0x7f80u && fabsf(r[p].x) < INFINITY) w[p] -= 1;
+                if ((w[p] & 0x7fff0000u) == 0x7f800000u && fabsf(r[p].y) < INFINITY) w[p] -= 0x10000u;
+            }
             if (k + 1 < TERMS) r[p] -= (floatx2){ bf_lo(w[p]), bf_hi(w[p]) };
         }
         t[k] = (u32x4){ w[0], w[1], w[2], w[3] };
@@ -199,42 +206,59 @@ __device__ __forceinline__ float ld_q(const u16 *p) { return bf2f(*p); }
 __device__ __forceinline__ void st_o(float *p, float v) { *p = v; }
 __device__ __forceinline__ void st_o(u16 *p, float v) { *p = (u16)pk_bf16(v, 0.0f); }
 
-/* Packed row r of a sequence by the formula: one wavefront, a lane's dims d = lane, lane + 64, ...; first the maximum, then
- * the sums.  No token seen: zeros. */
+/* Packed row r of a sequence by the formula: one wavefront, first the maximum, then the sums; 64 tokens at a time, a token a
+ * lane for the logits and a lane's dims d = lane, lane + 64, ... for the sums.  No token seen: zeros.  Some 0.1 us a token. */
 template <typename T> __device__ __forceinline__ void attn_by_formula(const NkAttnKvArgs &a, u32 first, u32 len, u32 row, u32 r, u32 h) {
     const NkKv &kv = a.kv;
-    const u32 lane = threadIdx.x & 63, i = r / a.group, p = len + i;
-    const u64 at = (u64)(h * a.group + r % a.group) * kv.dh;
+    const u32 lane = threadIdx.x & 63, i = attn_row(a, r), p = len + i;
+    const u64 at = (u64)(h * a.group + r - i * a.group) * kv.dh;
     const T *q = (const T *)a.q + (u64)(first + i) * a.ldq + at;
     T *o = (T *)a.o + (u64)(first + i) * a.ldo + at;
-    const u32 lo = a.window && p >= a.window ? p + 1 - a.window : 0, sinks = a.window ? min(a.sinks, lo) : 0;
+    const u32 lo = a.window && p >= a.window ? p + 1 - a.window : 0, sinks = a.window ? min(a.sinks, lo) : 0, n = sinks + p + 1 - lo;
     float m = -INFINITY, l = 0.0f, acc[4] = { 0.0f, 0.0f, 0.0f, 0.0f };
-    bool any = false;
-    for (int pass = 0; pass < 2; ++pass)
-        for (u32 k = 0; k < sinks + p + 1 - lo; ++k) {
-            const u32 j = k < sinks ? k : lo + k - sinks;
+    u64 any = 0;
+    bool nan = false;
+    for (int pass = 0; pass < 2 && !nan; ++pass)
+        for (u32 k0 = 0; k0 < n; k0 += 64) {
+            const u32 k = min(k0 + lane, n - 1), j = k < sinks ? k : lo + k - sinks;
             const int pe = kv.table[(u64)row * kv.ldt + (j >> kv.shift)];
-            if ((u32)pe >= kv.pages) continue;
-            const u64 slot = (((u64)(u32)pe * kv.heads + h) << kv.shift) + (j & ((1u << kv.shift) - 1));
+            const bool see = k0 + lane < n && (u32)pe < kv.pages;
+            const u64 seen = __ballot(see);
+            if (!seen) continue;
+            const u64 slot = (((u64)(u32)(see ? pe : 0) * kv.heads + h) << kv.shift) + (j & ((1u << kv.shift) - 1));
             float s = 0.0f;
-            for (u32 d = lane; d < kv.dh; d += 64) s = fmaf(ld_q(q + d), kv_value(kv, kv.k, kv.ks, slot, d), s);
-            s = wave_sum(s) * a.scale;
+            for (u32 d = 0; d < kv.dh; ++d) s = fmaf(ld_q(q + d), kv_value(kv, kv.k, kv.ks, slot, d), s);
+            s *= a.scale;
             if (!pass) {
-                m = !any || s > m || s != s ? s : m; /* a NaN stays */
-                any = true;
+                any |= seen;
+                nan |= __ballot(see && s != s) != 0;
+                m = fmaxf(m, wmax(see && s == s ? s : -INFINITY));
+                if (nan) break;
                 continue;
             }
-            const float e = expf(s - m);
+            const float e = see ? expf(s - m) : 0.0f;
             l += e;
+            for (u32 t0 = 0; t0 < 64; t0 += 8) {
+                float v[8][4];
 #pragma unroll
-            for (int u = 0; u < 4; ++u) {
-                const u32 d = lane + 64 * u;
-                if (d < kv.dh) acc[u] = fmaf(e, kv_value(kv, kv.v, kv.vs, slot, d), acc[u]);
+                for (u32 t = 0; t < 8; ++t) {
+                    const u64 st = (u64)lane_of((u32)(slot >> 32), (int)(t0 + t)) << 32 | lane_of((u32)slot, (int)(t0 + t));
+#pragma unroll
+                    for (int u = 0; u < 4; ++u) v[t][u] = 64 * u < (int)kv.dh ? kv_value(kv, kv.v, kv.vs, st, min(lane + 64 * u, kv.dh - 1)) : 0.0f;
+                }
+#pragma unroll
+                for (u32 t = 0; t < 8; ++t)
+                    if (seen >> (t0 + t) & 1) {
+                        const float g = __uint_as_float(lane_of(__float_as_uint(e), (int)(t0 + t)));
+#pragma unroll
+                        for (int u = 0; u < 4; ++u) acc[u] = fmaf(g, v[t][u], acc[u]);
+                    }
             }
         }
+    l = wave_sum(l);
 #pragma unroll
     for (int u = 0; u < 4; ++u)
-        if (lane + 64 * u < kv.dh) st_o(o + lane + 64 * u, any ? acc[u] / l : 0.0f);
+        if (lane + 64 * u < kv.dh) st_o(o + lane + 64 * u, !any ? 0.0f : nan ? __builtin_nanf("") : acc[u] / l);
 }
 
 /* ---- few rows: wavefronts over the tokens --------------------------------------------------------------
@@ -284,7 +308,7 @@ template <typename T, typename CT, int DH, int QT> __device__ __forceinline__ vo
             if (d >= dh)
 #pragma unroll
                 for (int e = 0; e < 8; ++e) v[e] = 0.0f;
-            attn_terms<TERMS>(v, qf[t][c]);
+            attn_terms<TERMS, true>(v, qf[t][c]);
         }
     }
 
@@ -454,7 +478,7 @@ const bool see = th[b] & ((pos[t] - j < reach) | ((j < a.sinks) & (j <= pos[t]) 
             v /= sum;
             const u32 pr = w.r0 + rt, pi = attn_row(a, pr);
             T *out = (T *)a.o + (u64)(w.first + pi) * a.ldo + (u64)(h * a.group + pr - pi * a.group) * dh + d;
-            if (!(fabsf(v.x) < INFINITY && fabsf(v.y) < INFINITY && fabsf(v.z) < INFINITY && fabsf(v.w) < INFINITY)) wrong[rt] = 1;
+            if ((TERMS > 1 || sum == sum) && !(fabsf(v.x) < INFINITY && fabsf(v.y) < INFINITY && fabsf(v.z) < INFINITY && fabsf(v.w) < INFINITY)) wrong[rt] = 1;
             const float e[4] = { v.x, v.y, v.z, v.w };
             if (a.vec) kv_store<4>(out, e);
             else
@@ -595,7 +619,7 @@ template <typename T, typename CT, int DC> __device__ __forceinline__ void attn_
             if (d >= dh)
 #pragma unroll
                 for (int e = 0; e < 8; ++e) v[e] = 0.0f;
-            attn_terms<TERMS>(v, qf[c]);
+            attn_terms<TERMS, true>(v, qf[c]);
         }
     }
     floatx16 o[ND];
@@ -740,7 +764,7 @@ template <typename T, typename CT, int DC> __device__ __forceinline__ void attn_
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
                     e[k] = o[n][i + k] / l;
-                    bad |= !(fabsf(e[k]) < INFINITY);
+                    bad |= (TERMS > 1 || l == l) && !(fabsf(e[k]) < INFINITY);
                 }
                 if (a.vec) kv_store<4>(out + d, e);
                 else
@@ -759,7 +783,9 @@ template <typename T, typename CT, int DC> __device__ __forceinline__ void attn_
 #define ATTN_MANY_DC(DC, OCC)                                                                                        \
     ATTN_MANY_K(u16, bf16, u16, bf16, DC, OCC) ATTN_MANY_K(u16, bf16, unsigned char, e4m3, DC, OCC)                  \
     ATTN_MANY_K(float, f32, u16, bf16, DC, OCC) ATTN_MANY_K(float, f32, unsigned char, e4m3, DC, OCC)
-ATTN_MANY_DC(64, 2) ATTN_MANY_DC(96, 2) ATTN_MANY_DC(128, 2) ATTN_MANY_DC(192, 1) ATTN_MANY_DC(256, 1)
+ATTN_MANY_K(u16, bf16, u16, bf16, 64, 3) ATTN_MANY_K(u16, bf16, unsigned char, e4m3, 64, 3)
+ATTN_MANY_K(float, f32, u16, bf16, 64, 2) ATTN_MANY_K(float, f32, unsigned char, e4m3, 64, 2)
+ATTN_MANY_DC(96, 2) ATTN_MANY_DC(128, 2) ATTN_MANY_DC(192, 1) ATTN_MANY_DC(256, 1)
 
 /* The pieces of split sequences added up: a wavefront per packed row, or (share) four; a lane has
  * two neighbouring sums (and two more 128 on), eight pieces' in flight. */
@@ -844,7 +870,7 @@ template <typename T> __device__ __forceinline__ void attn_join(const NkAttnKvAr
         for (u32 k = 0; k < 4; ++k) {
             const u32 d = 128 * (k / 2) + 2 * lane + k % 2;
             if (d < dh) {
-                bad |= !(fabsf(e[k]) < INFINITY);
+                bad |= (sizeof(T) == 4 || sum == sum) && !(fabsf(e[k]) < INFINITY);
                 st_o(out + d, e[k]);
             }
         }

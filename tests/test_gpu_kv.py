@@ -550,9 +550,46 @@ def test_attend_logits_far_apart(gpu):
         out = run_attend(gpu, cache, F32, q, seqs, 1)
         ref, bound = attend(q.reshape(40, 1, dh), pages, seqs, 0, 0, np.float32(dh ** -0.5), F32, np.zeros((40, 1, dh)))
         close(out.reshape(40, 1, dh), ref, bound)
-    q = np.full((40, dh), 3e38)
-    out = run_attend(gpu, cache, F32, q, seqs, 1)
-    assert np.isfinite(out[0]).all() or np.isnan(out[0]).all()
+    cache.free()
+
+
+def test_attend_largest_queries(gpu):
+    """Queries up to the largest f32, which round to infinity in bf16, against keys that keep the products in range; where
+    they are not, the formula's logits are infinite and the row NaN."""
+    rng = np.random.default_rng(25)
+    dh = 32
+    seqs = np.array([(0, 3, 20, 0)], np.int32)
+    pages = Pages(rng, BF16, 1, dh, 16, [23])
+    pages.k = oracle.f32_to_bf16(oracle.bf16_to_f32(pages.k) * np.float32(2.0 ** -120))
+    cache = Cache(gpu, pages)
+    q = np.full((3, dh), np.finfo(np.float32).max, np.float64) * np.where(rng.random((3, dh)) < 0.5, -1, 1)
+    out = run_attend(gpu, cache, F32, q, seqs, 1, scale=2.0 ** -8)
+    ref, bound = attend(kept(q, F32).reshape(3, 1, dh), pages, seqs, 0, 0, np.float32(2.0 ** -8), F32, np.zeros((3, 1, dh)))
+    close(out.reshape(3, 1, dh), ref, bound)
+    cache.free()
+    pages.k = oracle.f32_to_bf16(oracle.bf16_to_f32(pages.k) * np.float32(2.0 ** 120))
+    cache = Cache(gpu, pages)
+    assert np.isnan(run_attend(gpu, cache, F32, np.abs(q), seqs, 1)).all()
+    cache.free()
+
+
+@pytest.mark.parametrize("typ", [F32, BF16])
+@pytest.mark.parametrize("rows,start", [(1, 700), (150, 0), (3, 5000)])
+def test_attend_all_values_nan(gpu, typ, rows, start):
+    """A cache that holds nothing but NaN, and queries that are NaN: NaN rows, and at once."""
+    rng = np.random.default_rng(26)
+    seqs = np.array([(0, rows, start, 0)], np.int32)
+    pages = Pages(rng, E4M3, 2, 64, 16, [rows + start])
+    q = rng.standard_normal((rows, 256))
+    q[0, 64:128] = np.nan
+    cache = Cache(gpu, pages)
+    out = back(run_attend(gpu, cache, typ, q, seqs, 4), typ).reshape(rows, 4, 64)
+    cache.free()
+    assert np.isnan(out[0, 1]).all() and np.isfinite(out[0, [0, 2, 3]]).all() and np.isfinite(out[1:]).all()
+    pages.k[:] = 0x7f
+    pages.v[:] = 0xff
+    cache = Cache(gpu, pages)
+    assert np.isnan(back(run_attend(gpu, cache, typ, q, seqs, 4), typ)).all()
     cache.free()
 
 
