@@ -523,7 +523,7 @@ __device__ __forceinline__ floatx16 attn_mfma32(u32x4 a, u32x4 b, floatx16 acc) 
 /* dma16 (see there) from a base that all lanes share and 32 bits of a lane's own, to an LDS address; it writes where nothing
  * is read before the next wait and barrier, so that the reads around it may move */
 __device__ __forceinline__ void dma16_at(const char *base, u32 off, u32 to) {
-    asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(to));
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(to));
 }
 #define ATTN_MANY 64
 template <typename T, typename CT, int DC> __device__ __forceinline__ void attn_many(const NkAttnKvArgs &a) {

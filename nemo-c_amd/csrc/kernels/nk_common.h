@@ -222,10 +222,12 @@ typedef __attribute__((address_space(3))) char lds_char_t;
 /* 16 bytes per lane from global memory straight into LDS: lane i writes LDS bytes
  * [lds + 16 i, +16) of the wavefront-uniform base `lds`.  Issued as inline assembly, so the
  * compiler does not track these loads: a kernel waits for them itself (wait_vm_lgkm) before the
- * barrier that publishes the data, and drains them all before it can end. */
+ * barrier that publishes the data, and drains them all before it can end.  A load to
+ * LDS comes one wait state behind a write of m0 at the earliest, which is left to the program: the
+ * compiler sees to it in its own code, not in an assembly block (s_nop). */
 __device__ __forceinline__ void dma16(const void *g, lds_char_t *lds) {
     const u32 base = __builtin_amdgcn_readfirstlane((u32)(size_t)lds);
-    asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(g), "s"(base) : "memory");
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(g), "s"(base) : "memory");
 }
 
 /* s_waitcnt vmcnt(N) lgkmcnt(0) */

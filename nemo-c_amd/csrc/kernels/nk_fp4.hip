@@ -209,12 +209,12 @@ extern "C" __global__ __launch_bounds__(256) void gemm_fp4_glu(const NkGemm4Args
 /* 16 bytes per lane from global memory at base + off into LDS bytes [lds + 16 i, +16), as dma16 */
 __device__ __forceinline__ void dma16_at(const unsigned char *base, u32 off, lds_char_t *lds) {
     const u32 m = __builtin_amdgcn_readfirstlane((u32)(size_t)lds);
-    asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(m) : "memory");
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(m) : "memory");
 }
 /* and 4 bytes per lane into [lds + 4 i, +4) */
 __device__ __forceinline__ void dma4_at(const unsigned char *base, u32 off, lds_char_t *lds) {
     const u32 m = __builtin_amdgcn_readfirstlane((u32)(size_t)lds);
-    asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dword %0, %1" ::"v"(off), "s"(base), "s"(m) : "memory");
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dword %0, %1" ::"v"(off), "s"(base), "s"(m) : "memory");
 }
 __device__ __forceinline__ const unsigned char *uniform_ptr(const unsigned char *p) {
     const u32 lo = __builtin_amdgcn_readfirstlane((u32)(u64)p), hi = __builtin_amdgcn_readfirstlane((u32)((u64)p >> 32));
