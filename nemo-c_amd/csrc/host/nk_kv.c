@@ -146,11 +146,12 @@ static int attend(gpu_t *g, NkAttnKvArgs a, int type, uint32_t over, uint32_t up
     const uint64_t pieces = ((a.max_len + step - 1) / step + a.least - 1) / a.least;
     if (tiles > 1u << 23) return bad(g, "attention_kv: more rows than a launch covers");
     uint64_t items = tiles;
-    if (pieces > 1 && (by_rows < by_seqs ? by_rows : by_seqs) < slots) {
+    if (pieces > 1 && slots > 1 && (by_rows < by_seqs ? by_rows : by_seqs) < slots) {
         a.slots = slots;
         a.per_slot = 1.0f / (float)slots;
         a.per_cu = (float)heads / (many && f32 ? 512.0f : 256.0f);
-        const uint64_t split = tiles * pieces < 2ull * slots ? tiles * pieces : 2ull * slots;
+        const uint64_t split = nk_attn_items_bound(tiles, pieces, slots, packed <= tile);
+        a.items = (uint32_t)split;
         if (items < split) items = split;
         a.ws = gpu_scratch_ws(g, (size_t)(split * heads * tile * (dh + 2)));
         if (!a.ws) return bad(g, "attention_kv: scratch unavailable (size it before capture)");

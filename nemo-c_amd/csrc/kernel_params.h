@@ -590,11 +590,87 @@ typedef struct {
     u32 tile, step;   /* a workgroup's packed rows and a step's tokens, as powers of two */
     u32 reach, first; /* the most steps of a tile's window and first tokens (0: no window); rows of the first tile */
     u32 slots, least; /* workgroups per head of the cache that are wanted; the fewest steps of a piece */
-    float per_slot, per_cu; /* 1 / slots; heads of the cache / 256 */
+    u32 items;        /* pieces per head of the cache that the grid and the scratch are made for */
+    float per_slot, per_cu; /* 1 / slots; heads of the cache / 256, or / 512 (many f32 rows): the workgroups of a first round */
     u32 pair;         /* the second half of a sequence's tiles least first */
     u32 share;        /* attn_join: four wavefronts to a row */
     u32 vec;          /* rows are read and written 16 (bf16: 8) bytes at a time */
     float scale;
 } NkAttnKvArgs;
+
+/* ---- the attention's plan -------------------------------------------------------------------------
+ * A sequence's packed rows (row * group + head of the group) go in tiles of 2^tile; a tile's tokens in steps of 2^step: the
+ * steps of the first tokens that stay visible, then those from the first row's window to the last row.  Where all tiles are
+ * fewer than the workgroups wanted, their steps are split into pieces.  The kernels come to the plan by themselves, from the
+ * table; the host knows bounds of it alone and makes the grid and the scratch by nk_attn_items_bound. */
+#ifdef __HIPCC__
+#define NK_PLAN static __device__ __forceinline__
+#else
+#define NK_PLAN static inline
+#endif
+NK_PLAN u32 nk_lower(u32 a, u32 b) { return a < b ? a : b; }
+NK_PLAN u32 nk_higher(u32 a, u32 b) { return a > b ? a : b; }
+/* packed row -> row: at most one below, which the remainder shows */
+NK_PLAN u32 nk_attn_row(const NkAttnKvArgs *a, u32 r) {
+    const u32 q = (u32)((unsigned long long)r * a->inv_group >> 32);
+    return q + (r - q * a->group >= a->group);
+}
+/* tiles of a sequence that fits */
+NK_PLAN u32 nk_attn_tiles(const NkAttnKvArgs *a, u32 rows) {
+    return rows > a->over && rows <= a->upto ? ((rows * a->group - 1) >> a->tile) + 1 : 0;
+}
+/* the most steps that a tile has whose last row is the sequence's row `rows` - 1 */
+NK_PLAN u32 nk_attn_most_steps(const NkAttnKvArgs *a, u32 len, u32 rows) {
+    const u32 all = ((len + rows - 1) >> a->step) + 1;
+    return a->reach ? nk_lower(all, a->reach) : all;
+}
+/* about the steps of a sequence's n tiles: the mean of the first one's and the last one's of each */
+NK_PLAN float nk_attn_all_steps(const NkAttnKvArgs *a, u32 n, u32 len, u32 rows) {
+    return n ? 0.5f * (float)n * (float)(nk_attn_most_steps(a, len, rows) + nk_attn_most_steps(a, len, nk_lower(rows, a->first))) : 0.0f;
+}
+/* steps of a piece, by the sums over all sequences; 0: nothing is split.  As many pieces as a workgroup per CU has, or, where
+ * those are many, shorter ones that even out; never shorter than steps * per_slot. */
+NK_PLAN u32 nk_attn_piece(const NkAttnKvArgs *a, u32 tiles, float steps) {
+    if (tiles >= a->slots) return 0;
+    const float some = steps * a->per_cu;
+    return nk_higher(some < 24.0f ? (u32)some + 1 : (u32)(steps * a->per_slot) + 1, a->least);
+}
+/* pieces of each tile of a sequence, by the longest: a shorter tile's last ones may be empty */
+NK_PLAN u32 nk_attn_pieces(const NkAttnKvArgs *a, u32 len, u32 rows, u32 piece) {
+    return piece ? nk_higher((nk_attn_most_steps(a, len, rows) + piece / 2) / piece, 1) : 1;
+}
+/* steps of a piece of a sequence */
+NK_PLAN u32 nk_attn_piece_of(const NkAttnKvArgs *a, u32 len, u32 rows, u32 pieces) {
+    return (nk_attn_most_steps(a, len, rows) - 1) / pieces + 1;
+}
+/* The pieces per head that a split call can have.  With n tiles of a sequence, `most` steps at the most in each and P steps
+ * to a piece: n max(1, (most + P / 2) / P) <= n most / P + n.  P > steps / slots, and `steps` is at least half the sum of n most
+ * (the first tile's steps count half, and there may be next to none), or all of it where no sequence has a second tile.  So
+ * the sum over the sequences stays at or below 2 slots + tiles, or slots + tiles (tiles < slots, and f32 sums of
+ * `steps` are off by 10^-5 at the most: less than one piece).  Nor does a tile have more than pieces of `least` steps. */
+static inline unsigned long long nk_attn_items_bound(unsigned long long tiles, unsigned long long pieces, u32 slots, int one_tile) {
+    const unsigned long long by_steps = (one_tile ? 1ull : 2ull) * slots + (tiles < slots ? tiles : slots);
+    return tiles * pieces < by_steps ? tiles * pieces : by_steps;
+}
+typedef struct {
+    u32 r0, nr;         /* a tile's packed rows */
+    u32 pos_lo, pos_hi; /* positions of the first and the last */
+    u32 lo_step, sink_steps, steps; /* its steps: sink_steps from 0 on, the others from lo_step on */
+} nk_attn_tile_t;
+/* The last rows, which see most, first; where two workgroups share a CU from the start (pair), the first half of them
+ * and then the least. */
+NK_PLAN nk_attn_tile_t nk_attn_tile(const NkAttnKvArgs *a, u32 len, u32 rows, u32 tile) {
+    const u32 n = nk_attn_tiles(a, rows), half = (n + 1) / 2;
+    nk_attn_tile_t t;
+    t.r0 = (a->pair && tile >= half ? tile - half : n - 1 - tile) << a->tile;
+    t.nr = nk_lower(1u << a->tile, rows * a->group - t.r0);
+    t.pos_lo = len + nk_attn_row(a, t.r0);
+    t.pos_hi = len + nk_attn_row(a, t.r0 + t.nr - 1);
+    const u32 lo = a->window && t.pos_lo >= a->window ? t.pos_lo + 1 - a->window : 0;
+    t.lo_step = lo >> a->step;
+    t.sink_steps = a->window ? nk_lower((u32)(((unsigned long long)a->sinks + (1u << a->step) - 1) >> a->step), t.lo_step) : 0;
+    t.steps = t.sink_steps + (t.pos_hi >> a->step) - t.lo_step + 1;
+    return t;
+}
 
 #endif

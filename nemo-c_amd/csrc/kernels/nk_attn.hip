@@ -88,42 +88,17 @@ template <int TERMS> __device__ __forceinline__ float attn_sum(float l, const fl
 }
 
 /* ---- who does what ------------------------------------------------------------------------------------
- * A sequence's packed rows go in tiles of a.tile; a tile's tokens in steps of a.step: the steps of the first tokens that
- * stay visible (`sinks`), then those from the first row's window to the last row.  Where all tiles are fewer than the
- * workgroups wanted, their steps are split into pieces of equal length, by all the work that there is (the lengths are
- * known here alone); a piece's sums go to the scratch, and attn_join adds them up.  Items are numbered over all
- * sequences. */
+ * The plan (kernel_params.h) of the table: pieces of equal length, by all the work that there is (the lengths are known here
+ * alone); a piece's sums go to the scratch, and attn_join adds them up.  Items are numbered over all sequences. */
 typedef struct {
     u32 first, rows, len, row;  /* the sequence */
-    u32 r0, nr;                 /* the tile's packed rows */
-    u32 pos_lo, pos_hi;         /* positions of the first and the last */
-    u32 lo_step, sink_steps, steps; /* its steps: sink_steps from 0 on, the others from lo_step on */
+    u32 r0, nr, pos_lo, pos_hi, lo_step, sink_steps, steps; /* the tile, as nk_attn_tile_t */
     u32 from, to;               /* the piece's */
     u32 split, item;            /* whether it has other pieces; this one's number over all */
 } attn_work_t;
 
-/* packed row -> row: at most one below, which the remainder shows */
-__device__ __forceinline__ u32 attn_row(const NkAttnKvArgs &a, u32 r) {
-    const u32 q = __umulhi(r, a.inv_group);
-    return q + (r - q * a.group >= a.group);
-}
-__device__ __forceinline__ u32 attn_tiles(const NkAttnKvArgs &a, const kvseq_t &s) {
-    return s.ok && s.rows > a.over && s.rows <= a.upto ? ((s.rows * a.group - 1) >> a.tile) + 1 : 0;
-}
-/* the most steps that a tile has whose last row is the sequence's row `rows` - 1 */
-__device__ __forceinline__ u32 attn_most_steps(const NkAttnKvArgs &a, const kvseq_t &s, u32 rows) {
-    const u32 all = ((s.len + rows - 1) >> a.step) + 1;
-    return a.reach ? min(all, a.reach) : all;
-}
-__device__ __forceinline__ void attn_steps(const NkAttnKvArgs &a, attn_work_t &w) {
-    const u32 lowest = w.len + attn_row(a, w.r0), last = w.len + attn_row(a, w.r0 + w.nr - 1);
-    const u32 lo = a.window && lowest >= a.window ? lowest + 1 - a.window : 0;
-    w.pos_lo = lowest;
-    w.pos_hi = last;
-    w.lo_step = lo >> a.step;
-    w.sink_steps = a.window ? min((u32)(((u64)a.sinks + (1u << a.step) - 1) >> a.step), w.lo_step) : 0;
-    w.steps = w.sink_steps + (last >> a.step) - w.lo_step + 1;
-}
+__device__ __forceinline__ u32 attn_row(const NkAttnKvArgs &a, u32 r) { return nk_attn_row(&a, r); }
+__device__ __forceinline__ u32 attn_tiles(const NkAttnKvArgs &a, const kvseq_t &s) { return s.ok ? nk_attn_tiles(&a, s.rows) : 0; }
 __device__ __forceinline__ kvseq_t attn_seq(const NkAttnKvArgs &a, u32 i) {
     return kvseq_load(a.seqs, i, a.M, a.max_rows, a.kv.tables, min(kv_room(a.kv), (u64)a.max_len));
 }
@@ -140,29 +115,19 @@ __device__ __forceinline__ u32 attn_piece(const NkAttnKvArgs &a, kvseq_t s) {
         if (i != lane) s = attn_seq(a, i);
         const u32 n = attn_tiles(a, s);
         tiles += n;
-        if (n) steps += 0.5f * (float)n * (float)(attn_most_steps(a, s, s.rows) + attn_most_steps(a, s, min(s.rows, a.first)));
+        steps += nk_attn_all_steps(&a, n, s.len, s.rows);
     }
-    if (lane_of(wave_scan(tiles), 63) >= a.slots) return 0;
-    /* as many as a workgroup per CU has, or, where those are many, shorter ones that even out */
-    steps = wsum(steps);
-    const float some = steps * a.per_cu;
-    return some < 24.0f ? max((u32)some + 1, a.least) : max((u32)(steps * a.per_slot) + 1, a.least);
+    tiles = lane_of(wave_scan(tiles), 63);
+    return tiles < a.slots ? nk_attn_piece(&a, tiles, wsum(steps)) : 0;
 }
-__device__ __forceinline__ u32 attn_pieces(const NkAttnKvArgs &a, const kvseq_t &s, u32 piece) {
-    return piece ? max((attn_most_steps(a, s, s.rows) + piece / 2) / piece, 1u) : 1;
-}
+__device__ __forceinline__ u32 attn_pieces(const NkAttnKvArgs &a, const kvseq_t &s, u32 piece) { return nk_attn_pieces(&a, s.len, s.rows, piece); }
 /* a sequence's are all alike */
-__device__ __forceinline__ u32 attn_piece_of(const NkAttnKvArgs &a, const kvseq_t &s, u32 pieces) {
-    return (attn_most_steps(a, s, s.rows) - 1) / pieces + 1;
-}
+__device__ __forceinline__ u32 attn_piece_of(const NkAttnKvArgs &a, const kvseq_t &s, u32 pieces) { return nk_attn_piece_of(&a, s.len, s.rows, pieces); }
 __device__ __forceinline__ void attn_tile(const NkAttnKvArgs &a, const kvseq_t &s, u32 tile, attn_work_t &w) {
-    const u32 n = attn_tiles(a, s), half = (n + 1) / 2;
+    const nk_attn_tile_t t = nk_attn_tile(&a, s.len, s.rows, tile);
     w.first = s.first, w.rows = s.rows, w.len = s.len, w.row = s.row;
-    /* the last rows, which see most, first; where two workgroups share a CU from the start (pair), the first half of them
-     * and then the least */
-    w.r0 = (a.pair && tile >= half ? tile - half : n - 1 - tile) << a.tile;
-    w.nr = min(1u << a.tile, s.rows * a.group - w.r0);
-    attn_steps(a, w);
+    w.r0 = t.r0, w.nr = t.nr, w.pos_lo = t.pos_lo, w.pos_hi = t.pos_hi;
+    w.lo_step = t.lo_step, w.sink_steps = t.sink_steps, w.steps = t.steps;
 }
 __device__ __forceinline__ void attn_uniform(attn_work_t &w) {
     u32 *p = &w.first;
@@ -813,7 +778,7 @@ template <typename T> __device__ __forceinline__ void attn_join(const NkAttnKvAr
     attn_work_t w;
     attn_tile(a, it.seq, it.local, w);
     const u32 all = attn_pieces(a, it.seq, piece), pieces = (w.steps - 1) / attn_piece_of(a, it.seq, all) + 1, item = before + it.local * all;
-    if (pieces == 1) return;
+    if (pieces == 1 || item + pieces > a.items) return; /* items: of a table that has a row twice, or the scratch holds them */
     const u64 stride = ((u64)a.kv.heads << a.tile) * (dh + 2);
     const bool shared = a.share;
     const u32 begin = shared ? wave : 0, by = shared ? 4 : 1, d0 = min(2 * lane, dh - 2), d1 = min(128 + 2 * lane, dh - 2);
