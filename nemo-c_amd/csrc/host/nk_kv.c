@@ -131,6 +131,7 @@ static int attend(gpu_t *g, NkAttnKvArgs a, int type, uint32_t over, uint32_t up
     a.tile = many ? 7 : 3 + QT;
     a.step = many ? 6 : 5;
     a.first = tile / a.group + 1;
+    a.pad = dh < DH;
     if (a.window)
         a.reach = (uint32_t)(((uint64_t)a.window + tile / a.group + 1 + step) / step + 1 + ((uint64_t)a.sinks + step - 1) / step);
     /* tiles that there can be (and, if the rows are there, are), and the pieces that a tile can have */

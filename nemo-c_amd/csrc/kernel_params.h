@@ -595,6 +595,7 @@ typedef struct {
     u32 pair;         /* the second half of a sequence's tiles least first */
     u32 share;        /* attn_join: four wavefronts to a row */
     u32 vec;          /* rows are read and written 16 (bf16: 8) bytes at a time */
+    u32 pad;          /* a fragment is wider than a head */
     float scale;
 } NkAttnKvArgs;
 

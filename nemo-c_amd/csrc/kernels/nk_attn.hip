@@ -11,10 +11,12 @@
  * that of the output's rounding alone, and a second term would be half as many products again); f32 rows and their
  * probabilities are three bf16 terms, 24 bits.
  *
- * A bf16 row whose sum of weights is NaN has a logit that is (or an infinite one): all NaN, as the formula has it.  Rows
- * whose result is not finite otherwise (an infinity or NaN was near among the values, also of a token that only some rows
- * see: 0 times it is NaN in a product; of an f32 row's terms the later ones are zero too), or whose sum is zero, are computed
- * again by the formula, row by row, as far as a NaN logit. */
+ * A bf16 row whose sum of weights is NaN has a logit that is (or an infinite one): all NaN, as the formula has it, where its
+ * head fills the fragments.  Where it does not (pad), their rest is keys' last values again, times zeros of the row: NaN
+ * of an infinite one, whose logit may be -inf and have no weight.  Such rows, and those whose result is not finite
+ * otherwise (an infinity or NaN was near among the values, also of a token that only some rows see: 0 times it is NaN in a
+ * product; of an f32 row's terms the later ones are zero too), or whose sum is zero, are computed again by the formula, row
+ * by row, as far as a NaN logit. */
 #include "nk_common.h"
 
 typedef short s16x4 __attribute__((ext_vector_type(4)));
@@ -443,7 +445,7 @@ const bool see = th[b] & ((pos[t] - j < reach) | ((j < a.sinks) & (j <= pos[t]) 
             v /= sum;
             const u32 pr = w.r0 + rt, pi = attn_row(a, pr);
             T *out = (T *)a.o + (u64)(w.first + pi) * a.ldo + (u64)(h * a.group + pr - pi * a.group) * dh + d;
-            if ((TERMS > 1 || sum == sum) && !(fabsf(v.x) < INFINITY && fabsf(v.y) < INFINITY && fabsf(v.z) < INFINITY && fabsf(v.w) < INFINITY)) wrong[rt] = 1;
+            if ((TERMS > 1 || a.pad || sum == sum) && !(fabsf(v.x) < INFINITY && fabsf(v.y) < INFINITY && fabsf(v.z) < INFINITY && fabsf(v.w) < INFINITY)) wrong[rt] = 1;
             const float e[4] = { v.x, v.y, v.z, v.w };
             if (a.vec) kv_store<4>(out, e);
             else
@@ -729,7 +731,7 @@ template <typename T, typename CT, int DC> __device__ __forceinline__ void attn_
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
                     e[k] = o[n][i + k] / l;
-                    bad |= (TERMS > 1 || l == l) && !(fabsf(e[k]) < INFINITY);
+                    bad |= (TERMS > 1 || a.pad || l == l) && !(fabsf(e[k]) < INFINITY);
                 }
                 if (a.vec) kv_store<4>(out + d, e);
                 else
@@ -835,7 +837,7 @@ template <typename T> __device__ __forceinline__ void attn_join(const NkAttnKvAr
         for (u32 k = 0; k < 4; ++k) {
             const u32 d = 128 * (k / 2) + 2 * lane + k % 2;
             if (d < dh) {
-                bad |= (sizeof(T) == 4 || sum == sum) && !(fabsf(e[k]) < INFINITY);
+                bad |= (sizeof(T) == 4 || a.pad || sum == sum) && !(fabsf(e[k]) < INFINITY);
                 st_o(out + d, e[k]);
             }
         }
