@@ -116,8 +116,15 @@ int nk_kv_read(gpu_t *g, const nk_kv_t *c, void *K, uint32_t ldk, void *V, uint3
     return gpu_launch(g, name, &a, sizeof a, (uint32_t)blocks, gy, 1, 256, 1, 1);
 }
 
-/* The sequences of more than `over` and at most `upto` rows. */
-static int attend(gpu_t *g, NkAttnKvArgs a, int type, uint32_t over, uint32_t upto) {
+/* A launch over the sequences of more than `over` and at most `upto` rows, and the join behind it. */
+typedef struct {
+    NkAttnKvArgs a;
+    char name[40];
+    int f32;
+    uint32_t x, join_x, join_z; /* workgroups; join_x 0: nothing is split */
+    uint64_t floats;            /* of scratch */
+} attend_t;
+static const char *attend_plan(attend_t *l, NkAttnKvArgs a, int type, uint32_t over, uint32_t upto) {
     const uint32_t rows = upto < a.M ? upto : a.M, dh = a.kv.dh, heads = a.kv.heads;
     const uint64_t packed = (uint64_t)rows * a.group;
     /* Up to 64 packed rows go 16 or 32 to a workgroup whose wavefronts share the tokens, more 128 to one whose wavefronts share
@@ -145,7 +152,7 @@ static int attend(gpu_t *g, NkAttnKvArgs a, int type, uint32_t over, uint32_t up
     const uint32_t wanted = packed <= 16 ? a.nseq > 1 && upto == a.max_rows ? 1536 : 512 : many && f32 ? 512 : 256, slots = (wanted + heads - 1) / heads;
     a.least = packed <= 16 || (many && f32) ? 4 : 8;
     const uint64_t pieces = ((a.max_len + step - 1) / step + a.least - 1) / a.least;
-    if (tiles > 1u << 23) return bad(g, "attention_kv: more rows than a launch covers");
+    if (tiles > 1u << 23) return "attention_kv: more rows than a launch covers";
     uint64_t items = tiles;
     if (pieces > 1 && slots > 1 && (by_rows < by_seqs ? by_rows : by_seqs) < slots) {
         a.slots = slots;
@@ -154,26 +161,35 @@ static int attend(gpu_t *g, NkAttnKvArgs a, int type, uint32_t over, uint32_t up
         const uint64_t split = nk_attn_items_bound(tiles, pieces, slots, packed <= tile);
         a.items = (uint32_t)split;
         if (items < split) items = split;
-        a.ws = gpu_scratch_ws(g, (size_t)(split * heads * tile * (dh + 2)));
-        if (!a.ws) return bad(g, "attention_kv: scratch unavailable (size it before capture)");
     }
-    if (items * heads > 1u << 23) return bad(g, "attention_kv: more rows than a launch covers");
+    if (items * heads > 1u << 23) return "attention_kv: more rows than a launch covers";
     /* two workgroups a CU from the start: long tiles beside short ones (2048 rows 63 -> 60 us) */
     a.pair = many && tiles * heads > 256 && tiles * heads <= 512;
-    char name[40];
-    if (many) snprintf(name, sizeof name, "attn_many_%s_%s_%u", f32 ? "f32" : "bf16", cache_name(&a.kv), DH);
-    else snprintf(name, sizeof name, "attn_few_%s_%s_%u_%u", f32 ? "f32" : "bf16", cache_name(&a.kv), DH, QT);
-    gpu_next_bytes(g, (f32 ? 8.0 : 4.0) * a.M * a.heads * dh);
-    if (gpu_launch(g, name, &a, sizeof a, (uint32_t)items * heads, 1, 1, 256, 1, 1)) return -1;
-    if (!a.slots) return 0;
-    /* a row to a workgroup, or its wavefronts a row each and going round: some 1024 workgroups, one round of them (58 x 8 heads
-     * x 4 rows a workgroup each 216 us with what they join, 207 so; 24 x 4 x 128 rows by 512, 1024 and 2048: 46.4, 42.6, 44.1) */
-    const uint64_t most = packed < tile ? packed : tile, some = tiles < slots ? tiles : slots;
-    uint64_t z = 1024 / (some * heads);
-    a.share = some * heads * most <= 256;
-    if (a.share) z = most;
-    else if (z > (most + 3) / 4) z = (most + 3) / 4;
-    return gpu_launch(g, f32 ? "attn_join_f32" : "attn_join_bf16", &a, sizeof a, (uint32_t)some, heads, z ? (uint32_t)z : 1, 256, 1, 1);
+    *l = (attend_t){ .f32 = f32, .x = (uint32_t)items * heads, .floats = (uint64_t)a.items * heads * tile * (dh + 2) };
+    if (many) snprintf(l->name, sizeof l->name, "attn_many_%s_%s_%u", f32 ? "f32" : "bf16", cache_name(&a.kv), DH);
+    else snprintf(l->name, sizeof l->name, "attn_few_%s_%s_%u_%u", f32 ? "f32" : "bf16", cache_name(&a.kv), DH, QT);
+    if (a.slots) {
+        /* a row to a workgroup, or its wavefronts a row each and going round: some 1024 workgroups, one round of them (58 x 8
+         * heads x 4 rows a workgroup each 216 us with what they join, 207 so; 24 x 4 x 128 rows by 512, 1024 and 2048: 46.4,
+         * 42.6, 44.1) */
+        const uint64_t most = packed < tile ? packed : tile, some = tiles < slots ? tiles : slots;
+        uint64_t z = 1024 / (some * heads);
+        a.share = some * heads * most <= 256;
+        if (a.share) z = most;
+        else if (z > (most + 3) / 4) z = (most + 3) / 4;
+        l->join_x = (uint32_t)some;
+        l->join_z = z ? (uint32_t)z : 1;
+    }
+    l->a = a;
+    return NULL;
+}
+
+static int attend(gpu_t *g, const attend_t *l) {
+    const NkAttnKvArgs *a = &l->a;
+    gpu_next_bytes(g, (l->f32 ? 8.0 : 4.0) * a->M * a->heads * a->kv.dh);
+    if (gpu_launch(g, l->name, a, sizeof *a, l->x, 1, 1, 256, 1, 1)) return -1;
+    if (!l->join_x) return 0;
+    return gpu_launch(g, l->f32 ? "attn_join_f32" : "attn_join_bf16", a, sizeof *a, l->join_x, a->kv.heads, l->join_z, 256, 1, 1);
 }
 
 int nk_attention_kv(gpu_t *g, const nk_kv_t *c, const nk_attend_t *p) {
@@ -204,6 +220,17 @@ int nk_attention_kv(gpu_t *g, const nk_kv_t *c, const nk_attend_t *p) {
     const uint32_t few = group <= 16 ? 16 / group : 64 / group;
     const uint64_t sees = a.window && (uint64_t)a.window + a.sinks < a.max_len ? (uint64_t)a.window + a.sinks : a.max_len;
     const int mixed = p->nseq > 1 && few && sees > 2048 && (uint64_t)(p->max_rows < p->M ? p->max_rows : p->M) * group > 64;
-    if (mixed && attend(g, a, p->type, 0, few)) return -1;
-    return attend(g, a, p->type, mixed ? few : 0, p->max_rows);
+    attend_t l[2];
+    const int n = mixed ? 2 : 1;
+    if (mixed && (why = attend_plan(&l[0], a, p->type, 0, few))) return bad(g, why);
+    if ((why = attend_plan(&l[n - 1], a, p->type, mixed ? few : 0, p->max_rows))) return bad(g, why);
+    /* one after the other on the context's stream, they share its scratch */
+    const uint64_t floats = mixed && l[0].floats > l[1].floats ? l[0].floats : l[n - 1].floats;
+    float *ws = floats ? gpu_scratch_ws(g, (size_t)floats) : NULL;
+    if (floats && !ws) return bad(g, "attention_kv: scratch unavailable (size it before capture)");
+    for (int i = 0; i < n; ++i) {
+        l[i].a.ws = ws;
+        if (attend(g, &l[i])) return -1;
+    }
+    return 0;
 }

@@ -1,12 +1,15 @@
 """The attention's plan against the launches, without a GPU: the launcher and the planning that the kernels do of the table
 (kernel_params.h), compiled together for the host.  Of many prompts and batches every tile is planned once, every step of a
 tile lies in one piece, no piece lies beyond the grid or the scratch, and the joining launch covers the tiles that are split."""
+import ctypes as C
 import os
 import shutil
 import subprocess
 
 import pytest
 
+import nemoasr
+import test_kv_launches
 from conftest import REPO
 
 HOST = os.path.join(REPO, "nemo-c_amd", "csrc", "host")
@@ -196,3 +199,25 @@ def test_pieces_lie_in_the_grid_and_the_scratch(program, what):
     tiles, split, plans, share, refused = (int(w) for w in r.stdout.split() if w.isdigit())
     assert split > 100000 and plans > 10000  # tiles that are split were among them
     assert tiles > 10 ** 7 and refused < 5000 and share > 200  # and calls of more than two pieces a slot
+
+
+def test_refused_calls_launch_nothing(tmp_path, monkeypatch):
+    """A mixed batch whose prompts are refused, for their number or for want of scratch, is refused as a whole: the launch of its
+    few-row sequences does not come first."""
+    if not shutil.which("gcc"):
+        pytest.skip("gcc not present")
+    stubs = test_kv_launches.STUBS.replace("{ return scratch; }", "{ return n < 1u << 21 ? scratch : 0; }").replace("error", "why")  # libc has an `error`
+    monkeypatch.setattr(test_kv_launches, "STUBS", stubs)
+    rec, P = test_kv_launches.Recorder(tmp_path), test_kv_launches.P
+
+    def call(**more):
+        rec.n.value = 0
+        a = dict(type=1, q=P, ldq=1024, o=2 * P, ldo=1024, heads=8, scale=0.1, seqs=P, nseq=2, max_rows=130, max_len=40000, M=131)
+        rc = rec.L.nk_attention_kv(None, test_kv_launches.cache(1, 8, 128), C.byref(nemoasr.Attend(**dict(a, **more))))
+        return rc, rec.n.value, (C.c_char * 256).in_dll(rec.L, "why").value
+
+    assert call(max_rows=100, M=101, max_len=2100)[:2] == (0, 4)  # steps and prompts, joined each
+    rc, n, why = call(max_rows=1 << 30, M=(1 << 30) + 1)
+    assert (rc, n) == (-1, 0) and b"more rows" in why
+    rc, n, why = call()
+    assert (rc, n) == (-1, 0) and b"scratch" in why
