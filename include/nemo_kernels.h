@@ -408,7 +408,8 @@ int nk_rope_freqs(float *freq, uint32_t rot, double base, int scaling, double fa
  * amp; the rest is as it was.  Sums in f32, rounded once.
  * NK_E4M3: a block's scale is the least power of two of which 448 times reach its largest new value, and at least what the
  * block's older tokens have; where that grows their codes are rounded again.  Values are rounded to the nearest, ties to
- * the even code; an infinity becomes NaN. */
+ * the even code; an infinity becomes NaN.  What rounds beyond the largest value of a type (8 bits: to 2^128) reads back as an
+ * infinity, as in any rounding. */
 typedef struct {
     int type;
     uint32_t ldq, ldk, ldv, ldqo;
@@ -430,7 +431,8 @@ int nk_kv_read(gpu_t *g, const nk_kv_t *kv, void *K, uint32_t ldk, void *V, uint
  * (not overlapping q): softmax of scale q.k over the tokens that a row sees, in f32.  A row at position p sees token j
  * where j <= p, its page is there and, with a window (0: none), j > p - window or j < sinks; a row that sees none
  * gets zeros.  scale > 0.  max_len is at least the longest sequence's tokens, its rows among them (one that has more is left
- * out), and may be far above.  bf16 rows: probabilities are rounded to bf16; f32 rows keep 24 bits.  Infinities and NaN
+ * out), and may be far above.  bf16 rows: probabilities are rounded to bf16; f32 rows keep 24 bits.  q.k, and scale q.k times
+ * log2(e), beyond the largest f32 count as infinite.  Infinities and NaN
  * count in the rows that see them alone, where they give what the formula gives.  Few rows behind many tokens are split along
  * the tokens: the parts lie in the context's scratch (no residual update may be pending; a capture needs the scratch sized by
  * a call with its arguments before it). */

@@ -129,7 +129,7 @@ static const char *attend_plan(attend_t *l, NkAttnKvArgs a, int type, uint32_t o
     const uint64_t packed = (uint64_t)rows * a.group;
     /* Up to 64 packed rows go 16 or 32 to a workgroup whose wavefronts share the tokens, more 128 to one whose wavefronts share
      * the rows (8 heads of 128, groups of 4, 4000 tokens: 64 packed rows 18.4 us; 32000 tokens and 256 rows 67; 8192 rows 1299
-     * and 550 us). */
+     * and 566 us). */
     const int many = packed > 64, f32 = type == NK_F32;
     const uint32_t QT = packed > 16 && (dh <= 128 || !f32) ? 2 : 1, tile = many ? 128 : 16 * QT, step = many ? 64 : 32;
     const uint32_t DH = dh <= 64 ? 64 : many && dh <= 96 ? 96 : dh <= 128 ? 128 : many && dh <= 192 ? 192 : 256;

@@ -234,8 +234,8 @@ template <typename T> __device__ __forceinline__ void attn_by_formula(const NkAt
  * group g of a chunk pair has the values 16 g on), values through the wavefront's own LDS for their columns;
  * the next step's loads are in flight.
  *
- * Bound by memory where there is much: 131071 tokens of 8 heads of 128 bf16 94 us (5.7 TB/s), 64 sequences of up to 16384
- * 8-bit tokens 200 us (5.5 TB/s).  By round trips where there is little: 1000 tokens 7.5 us, of which the table 1.6, the
+ * Bound by memory where there is much: 131071 tokens of 8 heads of 128 bf16 96 us (5.6 TB/s), 64 sequences of up to 16384
+ * 8-bit tokens 203 us (5.4 TB/s).  By round trips where there is little: 1000 tokens 7.7 us, of which the table 1.6, the
  * rows' queries 0.5, page and first keys 1.5, two steps 2, joining the wavefronts and storing 1.7.  More wavefronts per SIMD
  * (registers held to 128: 8-bit steps 230 -> 300 us) or per workgroup (eight: 112 and 240) are not faster. */
 #define ATTN_STEP 32
@@ -382,7 +382,7 @@ template <typename T, typename CT, int DH, int QT> __device__ __forceinline__ vo
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         const u32 j = t0 + 16 * b + 4 * g4 + i;
-const bool see = th[b] & ((pos[t] - j < reach) | ((j < a.sinks) & (j <= pos[t]) & (reach < 1u << 31)));
+                        const bool see = th[b] & ((pos[t] - j < reach) | ((j < a.sinks) & (j <= pos[t]) & (reach < 1u << 31)));
                         s[t][b][i] = see ? s[t][b][i] : -INFINITY;
                     }
             }
@@ -477,9 +477,10 @@ ATTN_FEW(u16, bf16, u16, bf16, 256, 2) ATTN_FEW(u16, bf16, unsigned char, e4m3, 
  * banks.  The maximum follows only where a logit is 2^8 times above it: 2^(x - m) may exceed 1 as well as not, and the
  * sums are rescaled once or twice a row instead of every step.
  *
- * 8192 rows of 32 heads on 8 of 128: 547 to 569 us, 1.0 PFLOP/s of those that count, four fifths of a large library product's rate.
- * The matrix units are busy half of the cycles, the vector units (32 exponentials, 32 products, maxima, sums and conversions
- * of a wavefront's step) nearly as many, at the 1.9 to 2.0 GHz that the card's power leaves; what was tried beside: the next
+ * 8192 rows of 32 heads on 8 of 128: 561 to 575 us calls one behind another, 0.96 to 0.98 PFLOP/s of those that count, under the
+ * profiler 608 in the median (0.90): 74 to 80 % of a large library product's rate.  The matrix units are busy 47 % of the
+ * cycles, the vector units (206 instructions of a wavefront's step: 32 exponentials, 32 products, maxima, sums, conversions)
+ * nearly as many, at the 1.8 to 2.0 GHz that the card's power leaves; what was tried beside: the next
  * step's K Q^T while this one's weights are computed (7 % fewer cycles at a lower clock, 573 us against 569), two
  * workgroups' wavefronts of different priority (no change), eight wavefronts that share rows and halve the
  * tokens (607), per-lane 64-bit addresses (610).  Heads of 64 keep three workgroups a CU. */
